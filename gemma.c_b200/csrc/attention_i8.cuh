@@ -1,0 +1,121 @@
+// attention_i8.cuh -- what the kernels of attention over the 8-bit KV cache
+// share: the launch arguments, which positions a query row sees, and the
+// three-digit form of the queries.
+//
+//   s[t]  = asc * ks[t] * sum_d q[d] * kc[t][d]          (kc, vc int8 codes)
+//   p[t]  = exp(cap(s[t]) - m)
+//   o     = sum_t p[t] * vs[t] * vc[t] / sum_t p[t]
+//
+// The codes stay integers up to the matrix products: a query row is scaled to
+// 24-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
+// products with int8 keys are int8 x int8 sums, exact in int32, and the
+// rounding of q is 2^-24 of the row's largest element -- what fp32 holds of
+// that element itself.
+//
+// Rows: the query heads of one kv head share its keys, so a row is (i, g):
+// token or sequence i, head h0 + g of the group, row index i * G + g.
+#pragma once
+
+#include "gcu_internal.cuh"
+
+namespace gcu {
+namespace attn8 {
+
+constexpr int kMaxGroup = 8;        // query heads per kv head
+constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1): the largest three signed digits
+constexpr float kLog2e = 1.4426950408889634f;
+
+enum Mode {
+  PREFILL,  // row i is token spos + i of one sequence, keys at cache positions
+  OWN,      // row i is sequence i, its own cache
+  PREFIX    // row i is sequence i, the cache that all sequences share
+};
+
+struct Args {
+  const float *xq;  // row (i, h) at xq + i*q_i + h*q_h
+  long q_i, q_h;
+  float *xo;  // row (i, h) at xo + i*o_i + h*hdim
+  long o_i;
+  gcu_kv_i8 kv;
+  Mode mode;
+  int n_heads, ni;  // ni: tokens or sequences
+  int spos, slide, mask;
+  int plen, max_len;
+  const int *len;  // device lengths of the sequences' own caches, or null: max_len
+  float asc, sc_att;
+  // Key ranges are cut into `splits` chunks; a launch writes slots [slot0,
+  // slot0 + splits) of `slots` per row: unnormalised sums part[slot][row][hdim]
+  // and (m, l) stat[slot][row] with row = i*n_heads + h, weights 2^(log2e*s - m).
+  // slots == 1: the rows go straight to xo.
+  int chunk, splits, slot0, slots;
+  float *part;
+  float2 *stat;
+  unsigned int *err;
+};
+
+// query heads [head0(hk), head0(hk + 1)) belong to kv head hk (h * nkv / n_heads)
+__host__ __device__ __forceinline__ int head0(int hk, int n_heads, int nkv) {
+  return (hk * n_heads + nkv - 1) / nkv;
+}
+
+// own length of sequence i; -1: skipped
+__device__ __forceinline__ int seq_len(const Args &a, int i) {
+  if (!a.len) return a.max_len;
+  const int n = __ldg(a.len + i);
+  return n < 0 || n > a.max_len ? -1 : n;
+}
+
+// cache positions [lo, hi) that row i sees (lo >= hi: none)
+__device__ __forceinline__ void row_window(const Args &a, int i, int &lo, int &hi) {
+  if (a.mode == PREFILL) {
+    const int pos = a.spos + i;
+    lo = a.mask && a.slide > 0 ? max(0, pos + 1 - a.slide) : 0;
+    hi = a.mask ? pos + 1 : a.spos + a.ni;
+    return;
+  }
+  const int n = seq_len(a, i);
+  if (n < 0) {
+    lo = hi = 0;
+    return;
+  }
+  // of plen + n positions the last `slide`
+  const long skip = a.slide > 0 ? (long)a.plen + n - a.slide : 0;
+  if (a.mode == OWN) {
+    lo = (int)max(0l, skip - a.plen);
+    hi = n;
+  } else {
+    lo = (int)min((long)a.plen, max(0l, skip));
+    hi = a.plen;
+  }
+}
+
+// whether row i's output is written at all
+__device__ __forceinline__ bool row_live(const Args &a, int i) { return a.mode == PREFILL || seq_len(a, i) >= 0; }
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// digits of q * inv (|q * inv| <= kQMax): v = 65536 d2 + 256 d1 + d0
+__device__ __forceinline__ void digits(float q, float inv, int &d2, int &d1, int &d0) {
+  int v = __float2int_rn(__fmul_rn(q, inv));
+  v = v > 8355711 ? 8355711 : v < -8355711 ? -8355711 : v;
+  d0 = (int)(int8_t)v;
+  v = (v - d0) >> 8;
+  d1 = (int)(int8_t)v;
+  d2 = (v - d1) >> 8;
+}
+
+int launch_rows(const Args &a, cudaStream_t st);
+int launch_merge(const Args &a, cudaStream_t st);
+
+}  // namespace attn8
+}  // namespace gcu

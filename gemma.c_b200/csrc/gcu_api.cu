@@ -139,6 +139,13 @@ static unsigned int take_error_code(bool read_symbol) {
   return code;
 }
 
+// the message of a nonzero device error code; returns 1
+static int report_error_code(unsigned int code) {
+  if (code == DEV_BAD_LENGTH)
+    return set_error("a sequence length outside its 8-bit cache: that sequence was skipped (code %u)", code);
+  return set_error("device-side wait gave up (code %u)", code);
+}
+
 int num_sms() { return device_info().sms; }
 
 bool pdl_enabled() {
@@ -438,7 +445,7 @@ static int sync_and_check(ThreadCtx *c, cudaStream_t st) {
   (void)c;
   GCU_CUDA(cudaStreamSynchronize(st));
   const unsigned int code = take_error_code(false);
-  if (code) return set_error("device-side wait gave up (code %u)", code);
+  if (code) return report_error_code(code);
   return 0;
 }
 static int sync_and_check(ThreadCtx *c) { return sync_and_check(c, c->stream); }
@@ -488,10 +495,7 @@ GCU_EXPORT int gcu_init(int device) {
 GCU_EXPORT int gcu_check_device(void) {
   GCU_CUDA(cudaDeviceSynchronize());
   const unsigned int code = take_error_code(true);
-  if (code) {
-    set_error("device-side wait gave up (code %u)", code);
-    return 1;
-  }
+  if (code) return report_error_code(code);
   return 0;
 }
 

@@ -65,6 +65,7 @@ enum DevErr : unsigned int {
   DEV_TIMEOUT_SPLIT = 7,  // a split-K CTA waited too long for the other splits
   DEV_TIMEOUT_SELFTEST = 8,  // gcu_selftest_bounded_wait's wait (nothing ever completes it)
   DEV_TIMEOUT_CHAIN = 9,     // a chain launch's grid-wide hand-off between two steps
+  DEV_BAD_LENGTH = 10,       // a sequence length outside its 8-bit cache (that sequence was skipped)
 };
 unsigned int *dev_error_word();  // device address of the error word
 // Bit mask of the device error codes the host has observed since start-up
@@ -197,6 +198,10 @@ int launch_gemm_tc_jobs(const int8_t *src, long sstr, const float *ssc, int m,
 // split-K workspace and tile counters (device memory owned by the runtime)
 int gemm_workspace(size_t bytes, void **ws, int **counters, int ncounters,
                    cudaStream_t st);
+
+// 8-bit KV cache (k_cache_i8.cu): checks a descriptor's sizes, strides and
+// alignment; sets the error and returns 1 when it cannot be used.
+int check_kv_i8(const char *what, const gcu_kv_i8 *kv, int nseq = 0);
 
 // Shared with the chain kernel (k_chain.cu): TMA tensor maps of the GEMM's
 // operand layouts (int8 [rows][k], box 128 B x box_rows, 128-byte swizzle;

@@ -42,6 +42,14 @@ class QTensor(ctypes.Structure):
                 ("k", ctypes.c_int), ("kind", ctypes.c_int), ("layer", ctypes.c_int)]
 
 
+class _KvI8(ctypes.Structure):
+    """gcu_kv_i8: the buffers and strides of an 8-bit KV cache."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p),
+                ("seq_stride", ctypes.c_long), ("kv_stride", ctypes.c_long), ("sc_seq_stride", ctypes.c_long),
+                ("sc_stride", ctypes.c_long), ("nseq", ctypes.c_int), ("nkv", ctypes.c_int), ("clen", ctypes.c_int),
+                ("hdim", ctypes.c_int)]
+
+
 # gcu_qt_kind
 QT_KINDS = ("lm_head", "wq", "wk", "wv", "wo", "w1", "w2", "w3",
             "vwq", "vwk", "vwv", "vwo", "vw1", "vw2", "vproj")
@@ -108,6 +116,19 @@ SIGNATURES = {
                                           ctypes.c_float, _int, _int, _int, _int, _int, _vp]),
     "gcu_dev_qkv_norm_rope_cache": (_int, [_vp, _vp, ctypes.c_long, _vp, _vp, ctypes.c_long, _vp, _vp, ctypes.c_float,
                                            _vp, ctypes.c_float, _int, _int, _int, _int, _int, _vp]),
+    "gcu_dev_qkv_norm_rope_cache_i8": (_int, [_vp, _vp, ctypes.c_long, _vp, _vp, _vp, ctypes.c_float, _vp,
+                                              ctypes.c_float, _int, _int, _int, _vp]),
+    "gcu_dev_qkv_norm_rope_cache_i8_seqs": (_int, [_vp, _vp, ctypes.c_long, _vp, _vp, _vp, _vp, ctypes.c_float, _vp,
+                                                   ctypes.c_float, _int, _vp]),
+    "gcu_dev_cache_i8_read": (_int, [_vp, _vp, ctypes.c_long, ctypes.c_long, _vp, _int, _int, _vp]),
+    "gcu_attention_decode_i8_work": (ctypes.c_size_t, [_vp, _int, _vp, _int, _int, _int]),
+    "gcu_dev_attention_decode_i8": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _int, _int, _int, ctypes.c_float,
+                                           ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
+    "gcu_attention_prefill_i8_work": (ctypes.c_size_t, [_vp, _int, _int, _int, _int, _int]),
+    "gcu_dev_attention_prefill_i8": (_int, [_vp, _int, _vp, _vp, _int, _int, _int, _int, ctypes.c_float, _int, _vp,
+                                            ctypes.c_size_t, _vp]),
+    "gcu_dev_sample": (_int, [_vp, _vp, _vp, ctypes.c_long, _vp, ctypes.c_float, _int, ctypes.c_float, ctypes.c_float,
+                              _int, _int, _vp]),
     "gcu_dev_patch_embed": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _int, _int, _int, _vp]),
     "gcu_dev_vision_pool_quantize": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_float, _int, _int, _int,
                                             _vp]),
@@ -618,3 +639,190 @@ def dev_qkv_norm_rope_cache(xq, qkv, kc, vc, freqs, spos, n_heads, q_scale=1.0, 
                                              nk.data_ptr() if nk is not None else None, eps, freqs.data_ptr(),
                                              q_scale, n_heads, nkv, hdim, spos, ntok, _stream(stream)),
            "dev_qkv_norm_rope_cache")
+
+
+# --------------------------------------------------------------------------
+# 8-bit KV cache, attention over it, sampling
+# --------------------------------------------------------------------------
+
+def _want(what, ok, *msg):
+    if not ok:
+        raise GcuError(f"{what}: " + " ".join(str(m) for m in msg))
+
+
+def _rows(what, name, t, dtype, shape):
+    """t is a contiguous CUDA tensor of this dtype and shape on the current device."""
+    import torch
+    _want(what, t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(), name, "must be a contiguous",
+          dtype, "tensor of", tuple(shape), "not", t.dtype, tuple(t.shape))
+    _want(what, t.is_cuda and t.device.index == torch.cuda.current_device(), name, "is on", t.device,
+          "and the current device is another")
+
+
+def _work(nbytes, device, stream):
+    """Scratch of one call.  It comes from torch's allocator, so it is the
+    call's own: in a captured graph it lives in the graph's pool."""
+    if not nbytes:
+        return None, 0, None
+    import torch
+    w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if stream is not None:
+        w.record_stream(stream)
+    return w.data_ptr(), nbytes, w
+
+
+class KvCacheI8:
+    """An 8-bit KV cache (gcu_kv_i8): int8 codes k, v (nseq, nkv, clen, hdim) and
+    fp32 scales ks, vs (nseq, nkv, clen), one scale per (sequence, kv head,
+    position).  The tensors may be views with strides (k and v alike, ks and
+    vs alike); a position's hdim codes and a head's positions are contiguous."""
+
+    def __init__(self, k, v, ks, vs):
+        import torch
+        what = "KvCacheI8"
+        _want(what, k.dim() == 4 and ks.dim() == 3, "k, v (nseq, nkv, clen, hdim) and ks, vs (nseq, nkv, clen) expected")
+        for t, like, dt in ((k, k, torch.int8), (v, k, torch.int8), (ks, ks, torch.float32), (vs, ks, torch.float32)):
+            _want(what, t.dtype == dt and t.shape == like.shape and t.stride() == like.stride() and
+                  t.device == k.device, "k and v (int8), ks and vs (float32) must be alike in shape, strides and device")
+        _want(what, ks.shape == k.shape[:3], "scales", tuple(ks.shape), "of codes", tuple(k.shape))
+        _want(what, k.stride(3) == 1 and k.stride(2) == k.shape[3] and ks.stride(2) == 1,
+              "a head's positions must be contiguous")
+        self.k, self.v, self.ks, self.vs = k, v, ks, vs
+        self.nseq, self.nkv, self.clen, self.hdim = k.shape
+        self.device = k.device
+        self.c = _KvI8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.stride(0), k.stride(1),
+                       ks.stride(0), ks.stride(1), *k.shape)
+        self.ref = ctypes.byref(self.c)
+
+    @classmethod
+    def empty(cls, nseq, nkv, clen, hdim, device="cuda"):
+        """A cache of zero codes with scale 1."""
+        import torch
+        codes = torch.zeros((2, nseq, nkv, clen, hdim), dtype=torch.int8, device=device)
+        scales = torch.ones((2, nseq, nkv, clen), dtype=torch.float32, device=device)
+        return cls(codes[0], codes[1], scales[0], scales[1])
+
+    def seq(self, b):
+        """The cache of sequence b alone (a view)."""
+        return KvCacheI8(self.k[b:b + 1], self.v[b:b + 1], self.ks[b:b + 1], self.vs[b:b + 1])
+
+    def check(self, what):
+        import torch
+        _want(what, self.k.is_cuda and self.device.index == torch.cuda.current_device(), "cache is on", self.device,
+              "and the current device is another")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
+    """dev_qkv_norm_rope_cache into an 8-bit cache of one sequence: qkv (ntok, >=
+    (n_heads+2*nkv)*hdim) rows, rotated queries to xq (n_heads, ntok, hdim),
+    codes and scales to kv (KvCacheI8) at [spos, spos+ntok); freqs (ntok, hdim)."""
+    import torch
+    what = "dev_qkv_norm_rope_cache_i8"
+    n_heads, ntok, _ = xq.shape
+    kv.check(what)
+    _check_write(what, xq, (n_heads, ntok, kv.hdim), qkv, kv, freqs, nq, nk, ntok, n_heads)
+    _check(lib().gcu_dev_qkv_norm_rope_cache_i8(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref, _ptr(nq), _ptr(nk),
+                                                eps, freqs.data_ptr(), q_scale, n_heads, spos, ntok, _stream(stream)),
+           what)
+
+
+def dev_qkv_norm_rope_cache_i8_seqs(xq, qkv, kv, length, freqs, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
+    """One token of each of kv.nseq sequences: row b of qkv to position length[b] - 1
+    of sequence b (length int32 (nseq,) counts the new token; below 1: skipped),
+    queries to xq (nseq, n_heads, hdim); freqs (nseq, hdim)."""
+    import torch
+    what = "dev_qkv_norm_rope_cache_i8_seqs"
+    n_heads = xq.shape[1]
+    kv.check(what)
+    _check_write(what, xq, (kv.nseq, n_heads, kv.hdim), qkv, kv, freqs, nq, nk, kv.nseq, n_heads)
+    _rows(what, "length", length, torch.int32, (kv.nseq,))
+    _check(lib().gcu_dev_qkv_norm_rope_cache_i8_seqs(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref,
+                                                     length.data_ptr(), _ptr(nq), _ptr(nk), eps, freqs.data_ptr(),
+                                                     q_scale, n_heads, _stream(stream)), what)
+
+
+def _check_write(what, xq, shape, qkv, kv, freqs, nq, nk, rows, n_heads):
+    import torch
+    _rows(what, "xq", xq, torch.float32, shape)
+    _want(what, qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.shape[0] == rows and qkv.stride(1) == 1 and
+          qkv.shape[1] >= (n_heads + 2 * kv.nkv) * kv.hdim and qkv.device == kv.device,
+          "qkv must be float32 rows of the fused q|k|v projection, one per token, not", qkv.dtype, tuple(qkv.shape))
+    _rows(what, "freqs", freqs, torch.float32, (rows, kv.hdim))
+    for name, w in (("nq", nq), ("nk", nk)):
+        if w is not None:
+            _rows(what, name, w, torch.float32, (kv.hdim,))
+
+
+def dev_cache_i8_read(k, v, kv, spos, stream=None):
+    """Positions [spos, spos+ntok) of kv as fp32 rows in k, v (nseq, nkv, ntok, hdim),
+    views of a longer fp32 cache among them."""
+    import torch
+    what = "dev_cache_i8_read"
+    kv.check(what)
+    for name, t in (("k", k), ("v", v)):
+        _want(what, t.dtype == torch.float32 and t.dim() == 4 and t.shape == k.shape and t.stride() == k.stride() and
+              tuple(t.shape[:2]) == (kv.nseq, kv.nkv) and t.shape[3] == kv.hdim and t.stride(3) == 1 and
+              (t.stride(2) == kv.hdim or t.shape[2] < 2) and t.device == kv.device,
+              name, "must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, k and v alike")
+    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), kv.ref, spos, k.shape[2],
+                                       _stream(stream)), what)
+
+
+def dev_attention_decode_i8(xo, xq, kv, length, max_len, asc, sc_att=0.0, slide=0, prefix=None, plen=0, stream=None):
+    """One token of each of kv.nseq sequences: xq, xo (nseq, n_heads, hdim).  Sequence b
+    sees the plen positions of prefix (a KvCacheI8 of one sequence, shared) and
+    the first length[b] of its own cache (int32 (nseq,); None: max_len each), of
+    these the last `slide` when slide > 0.  length[b] < 0: skipped."""
+    import torch
+    what = "dev_attention_decode_i8"
+    kv.check(what)
+    n_heads = xq.shape[1]
+    _rows(what, "xq", xq, torch.float32, (kv.nseq, n_heads, kv.hdim))
+    _rows(what, "xo", xo, torch.float32, (kv.nseq, n_heads, kv.hdim))
+    if length is not None:
+        _rows(what, "length", length, torch.int32, (kv.nseq,))
+    if prefix is not None:
+        prefix.check(what)
+    pref = prefix.ref if prefix is not None else None
+    l = lib()
+    work = _work(l.gcu_attention_decode_i8_work(pref, plen, kv.ref, max_len, n_heads, slide), kv.device, stream)
+    _check(l.gcu_dev_attention_decode_i8(xo.data_ptr(), xq.data_ptr(), pref, plen, kv.ref, _ptr(length), max_len, n_heads,
+                                         slide, asc, sc_att, work[0], work[1], _stream(stream)), what)
+
+
+def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, stream=None):
+    """dev_attention_prefill over an 8-bit cache of one sequence: xq (n_heads, ntok, hdim)
+    rotated and scaled, kv holding the chunk at [spos, spos+ntok); writes xo
+    rows (ntok, >= n_heads*hdim)."""
+    import torch
+    what = "dev_attention_prefill_i8"
+    kv.check(what)
+    n_heads, ntok, _ = xq.shape
+    _rows(what, "xq", xq, torch.float32, (n_heads, ntok, kv.hdim))
+    _want(what, xo.dtype == torch.float32 and xo.dim() == 2 and xo.shape[0] == ntok and xo.stride(1) == 1 and
+          xo.shape[1] >= n_heads * kv.hdim and xo.device == kv.device, "xo must be float32 (ntok, >= n_heads*hdim) rows")
+    l = lib()
+    work = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, int(mask)), kv.device, stream)
+    _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0), xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
+                                          sc_att, int(mask), work[0], work[1], _stream(stream)), what)
+
+
+def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
+    """The next token of each row of logits (m, nvocab): token int32 (m,), from u (m,)
+    float32 random numbers in [0, 1); prob (m,) float32 (optional) receives the
+    tokens' shares of the kept weights.  See gcu_dev_sample in include/gcu.h."""
+    import torch
+    what = "dev_sample"
+    _want(what, logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1 and logits.is_cuda and
+          logits.device.index == torch.cuda.current_device(), "logits must be float32 (m, nvocab) rows on the current device")
+    m, n = logits.shape
+    _rows(what, "token", token, torch.int32, (m,))
+    _rows(what, "u", u, torch.float32, (m,))
+    if prob is not None:
+        _rows(what, "prob", prob, torch.float32, (m,))
+    _check(lib().gcu_dev_sample(token.data_ptr(), _ptr(prob), logits.data_ptr(), logits.stride(0) if m > 1 else 0,
+                                u.data_ptr(), temperature, top_k, top_p, min_p, m, n, _stream(stream)), what)

@@ -352,6 +352,96 @@ int gcu_dev_attention_prefill(float *xo, int xostr, const float *xq, const float
                               const float *v_cache, long kv_stride, int n_heads, int nkv, int hdim,
                               int spos, int ntok, int slide, float sc_att, int mask, void *stream);
 
+/* ---- 8-bit KV cache: written, read back, attended to --------------------------
+ * No counterpart in the reference, whose cache is fp32.  A cache holds int8
+ * codes and one fp32 scale per (sequence, kv head, position) row, K and V
+ * each, quantized as gcu_quantize_acts quantizes a row: a quarter of the fp32
+ * cache's memory and traffic.  Sequence b's kv head h, position t is at
+ * codes k + b*seq_stride + h*kv_stride + t*hdim, scale ks + b*sc_seq_stride +
+ * h*sc_stride + t (v, vs alike), 0 <= t < clen.  Strides count elements
+ * (codes / floats); k and v 16-byte aligned, seq_stride and kv_stride
+ * multiples of 16; hdim 64, 128 or 256. */
+typedef struct {
+  int8_t *k, *v;
+  float *ks, *vs;
+  long seq_stride, kv_stride, sc_seq_stride, sc_stride;
+  int nseq, nkv, clen, hdim;
+} gcu_kv_i8;
+
+/* gcu_dev_qkv_norm_rope_cache into an 8-bit cache of one sequence (kv->nseq
+ * 1): row t of qkv (row stride ld floats, a multiple of 4) holds the token's
+ * query heads, then its key heads, then its value heads; the rotated queries
+ * (times q_scale) go to xq [n_heads][ntok][hdim], the codes and scales of the
+ * rotated keys and of the values to positions [spos, spos+ntok).  nq / nk:
+ * QK-norm weights [hdim] or NULL; freqs [ntok][hdim] (cos, sin interleaved).
+ * The norm's sum of squares is taken in 64 bits and every fp32 step after it
+ * is rounded by itself (no fused multiply-adds), so the codes follow from the
+ * formulas alone.  16-byte aligned qkv, xq and freqs. */
+int gcu_dev_qkv_norm_rope_cache_i8(float *xq, const float *qkv, long ld, const gcu_kv_i8 *kv,
+                                   const float *nq, const float *nk, float eps, const float *freqs,
+                                   float q_scale, int n_heads, int spos, int ntok, void *stream);
+/* The same for one token of each of kv->nseq sequences: row b of qkv to
+ * position len[b] - 1 of sequence b's cache, its queries to xq
+ * [nseq][n_heads][hdim]; freqs [nseq][hdim].  len (device int32) counts the new
+ * token.  A sequence with len[b] < 1 is left as it is, its xq row too; one
+ * with len[b] > clen is left as well and reported by gcu_check_device. */
+int gcu_dev_qkv_norm_rope_cache_i8_seqs(float *xq, const float *qkv, long ld, const gcu_kv_i8 *kv,
+                                        const int *len, const float *nq, const float *nk, float eps,
+                                        const float *freqs, float q_scale, int n_heads, void *stream);
+/* Positions [spos, spos+ntok) of every sequence and kv head as fp32 rows
+ * (code * scale): sequence b, kv head h, position spos+t goes to
+ * k + b*out_seq_stride + h*out_stride + t*hdim, and v alike (an fp32 cache
+ * in gemma.c's layout takes them at its own strides).  16-byte aligned k and
+ * v, strides multiples of 4 floats. */
+int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stride, const gcu_kv_i8 *kv,
+                          int spos, int ntok, void *stream);
+
+/* One decode step of one layer for own->nseq sequences over 8-bit caches:
+ * xq, xo [nseq][n_heads][hdim].  Sequence b sees the plen positions of
+ * `prefix` (a cache of one sequence that all of them share, read once for
+ * all; NULL with plen 0: none) and then the first len[b] positions of its own
+ * cache, of these plen + len[b] positions the last `slide` when slide > 0.
+ * len: device int32 [nseq], 0 <= len[b] <= max_len <= clen, or NULL when
+ * every sequence has max_len.  Scores are scaled by asc, then soft-capped by
+ * sc_att (0 = off).  A sequence that sees nothing gets zeros; one with len[b]
+ * < 0 is skipped, its xo row left as it is; one with len[b] > max_len is
+ * skipped too and reported by gcu_check_device.  At most 8 query heads per
+ * kv head.  work: device scratch of at least
+ * gcu_attention_decode_i8_work(...) bytes, 16-byte aligned, not shared with
+ * work that may run at the same time (0 bytes: may be NULL). */
+size_t gcu_attention_decode_i8_work(const gcu_kv_i8 *prefix, int plen, const gcu_kv_i8 *own, int max_len,
+                                    int n_heads, int slide);
+int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu_kv_i8 *prefix, int plen,
+                                const gcu_kv_i8 *own, const int *len, int max_len, int n_heads, int slide,
+                                float asc, float sc_att, void *work, size_t work_bytes, void *stream);
+/* gcu_dev_attention_prefill over an 8-bit cache of one sequence (kv->nseq 1):
+ * a chunk of ntok tokens at [spos, spos+ntok) whose keys and values are
+ * already in the cache; xq [n_heads][ntok][hdim], rotated and scaled; token i
+ * of head h goes to xo + i*xostr + h*hdim (xostr 0 = n_heads*hdim).  mask,
+ * slide and sc_att as there; work as above. */
+size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide, int mask);
+int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,
+                                 int spos, int ntok, int slide, float sc_att, int mask, void *work,
+                                 size_t work_bytes, void *stream);
+
+/* ---- sampling -----------------------------------------------------------------
+ * The next token of each of m rows of logits (nvocab floats at row stride
+ * ld, 0 = nvocab) from one given random number u[i] in [0, 1) per row
+ * (gemma.c samples on the host, gemma.c:5769).  With w_j = exp((x_j - max) /
+ * temperature): keep the top_k largest logits (0 = all; of equal ones the
+ * lowest indices), of those in descending order the shortest run whose
+ * weights reach top_p of their sum (top_p >= 1 = all), of those the ones with
+ * w_j >= min_p (0 = all); the token is the first kept index, in index order,
+ * whose running sum of weights passes u times their total.  temperature 0:
+ * the largest logit, of equal ones the lowest index.  NaN logits count as
+ * -inf, and a logit of -inf is never kept; a row with nothing else gives token
+ * -1 and prob 0.  +inf logits share all the weight.  token [m]; prob [m] (may
+ * be NULL): the token's share of the kept weights.  Weights and sums are
+ * held in 64 bits, fixed point: a weight is rounded to a multiple of
+ * 2^-(63 - log2 nvocab) of the largest.  nvocab <= 2^20. */
+int gcu_dev_sample(int *token, float *prob, const float *logits, long ld, const float *u, float temperature,
+                   int top_k, float top_p, float min_p, int m, int nvocab, void *stream);
+
 /* ---- SigLIP head (fp32) around the vision tower's matmuls ------------------
  * gemma.c:4411-4466: the patch embedding, Conv2d(3, dim, kernel = stride =
  * psize, bias) of the (img_px, img_px, 3) image img, then the int8 position
