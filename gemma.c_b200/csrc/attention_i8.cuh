@@ -114,7 +114,11 @@ __device__ __forceinline__ void digits(float q, float inv, int &d2, int &d1, int
   d2 = (v - d1) >> 8;
 }
 
+// k_attention_i8.cu: up to 8 rows per CTA on the CUDA cores; k_attention_i8_tc.cu:
+// 128 rows per CTA on the tensor cores, kTcKeys keys at a time
 int launch_rows(const Args &a, cudaStream_t st);
+int launch_tc(const Args &a, cudaStream_t st);
+constexpr int kTcRows = 128, kTcKeys = 64;
 int launch_merge(const Args &a, cudaStream_t st);
 
 }  // namespace attn8

@@ -209,6 +209,10 @@ int check_kv_i8(const char *what, const gcu_kv_i8 *kv, int nseq = 0);
 // tiles, K split) over the cost model of the GEMM launcher.
 int gemm_tmap_i8(CUtensorMap *m, const int8_t *base, int k, int rows, long stride, int box_rows);
 int gemm_tmap_f32(CUtensorMap *m, float *base, int n, int rows, long stride_elems);
+// int8 [heads][rows][hdim] of a KV cache (k_attention_i8_tc.cu): box min(hdim,
+// 128) B x box_rows of one head, swizzled over its inner bytes (64 or 128)
+int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, int hdim, int rows, int heads, long head_stride,
+                       int box_rows);
 int gemm_plan_one_cta(int m, int k, const int *n, int njobs, int sms, int *bn, int *mb,
                       int *splits);
 int gemm_split_for(int tiles, int k, int sms);
@@ -371,6 +375,14 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap *m,
       "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap *m, uint64_t *bar, void *dst, int x, int y, int z,
+                                            uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "l"(policy)
+      : "memory");
+}
 // L2 prefetch of one tile through a tensor map (no data reaches the CTA)
 __device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap *m, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(m), "r"(x),
@@ -531,6 +543,28 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc,
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit floats -> fp32, one CTA.  A: row = lane,
+// two consecutive K elements per 32-bit column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Registers of a warpgroup (128 threads, all of them call it): give some back, or
+// take from those given back.  The shares may not add up to more than the
+// launch's.
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
 // arrive on `bar` once all tcgen05 operations issued so far have completed
 __device__ __forceinline__ void mma_commit(uint64_t *bar) {
   asm volatile(
@@ -555,6 +589,28 @@ __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32])
       : "r"(taddr)
       : "memory");
 }
+// 32 lanes x 16 columns
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// 16 registers per thread -> 32 lanes x 16 columns
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
@@ -573,6 +629,26 @@ __device__ __forceinline__ uint64_t smem_desc_k128(uint32_t saddr) {
   return d;
 }
 
+// The same for any swizzled tile: lbo / sbo in bytes, swizzle 128 or 64.
+// K-major: 8-row atoms (8 x swizzle bytes) sbo apart, lbo unused.  MN-major
+// (swizzle 128, 16-bit elements): atoms of 64 MN elements x 8 K rows, lbo
+// apart along MN and sbo along K.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo, int swizzle) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
+  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)(swizzle == 128 ? 2 : 4) << 61;
+  return d;
+}
+
+// Instruction descriptor, kind::f16: D = fp32, A = B = fp16, A K-major, B
+// MN-major, shape M x N.
+__host__ __device__ constexpr uint32_t idesc_f16_bt(int M, int N) {
+  return (1u << 4) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
 // Instruction descriptor, kind::i8: D = s32, A = B = signed int8, both
 // K-major, shape M x N.
 __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
@@ -580,6 +656,19 @@ __host__ __device__ constexpr uint32_t idesc_i8(int M, int N) {
          ((uint32_t)(M >> 4) << 24);
 }
 
+// named barrier that also tells every thread whether `flag` is set in any
+__device__ __forceinline__ bool named_bar_or(int id, int nthreads, bool flag) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(nthreads), "r"((uint32_t)flag)
+      : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

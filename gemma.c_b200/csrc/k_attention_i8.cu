@@ -452,32 +452,45 @@ namespace {
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
-// Chunks of a range of n positions for `units` independent row groups: enough
-// CTAs to fill the SMs twice, 32 to kMaxChunk positions each.
-void split_range(int n, long units, int &chunk, int &splits) {
+// How one launch covers its key ranges: which kernel, and chunks of the range.
+struct Plan {
+  bool tc;
+  int chunk, splits;
+};
+
+// ni x G rows per kv head over at most n positions each.  More rows than one
+// CTA of k_rows takes go to the tensor cores.
+Plan plan_rows(const gcu_kv_i8 &kv, Mode mode, long ni, int G, int n) {
+  Plan p{mode != OWN && ni * G > kMaxGroup, 1, 0};
   if (n < 1) n = 1;
-  const long target = 2 * num_sms();
-  long want = std::max(1l, (target + units - 1) / units);
-  want = std::min(want, ((long)n + 31) / 32);
-  want = std::max(want, ((long)n + kMaxChunk - 1) / kMaxChunk);
-  chunk = (int)((n + want - 1) / want);
-  splits = (n + chunk - 1) / chunk;
+  if (p.tc) {
+    // one CTA per SM: as many chunks as make one wave of them
+    const long units = (ni * G + kTcRows - 1) / kTcRows * kv.nkv, nk = kTcKeys;
+    const long tiles = (n + nk - 1) / nk, want = std::min(tiles, std::max(1l, num_sms() / units));
+    p.chunk = (int)((tiles + want - 1) / want * nk);
+  } else {
+    // enough CTAs to fill the SMs twice, 32 to kMaxChunk positions each
+    const long units = mode == OWN ? ni * kv.nkv : (ni * G + kMaxGroup - 1) / kMaxGroup * kv.nkv;
+    long want = std::max(1l, (2l * num_sms() + units - 1) / units);
+    want = std::min(want, ((long)n + 31) / 32);
+    want = std::max(want, ((long)n + kMaxChunk - 1) / kMaxChunk);
+    p.chunk = (int)((n + want - 1) / want);
+  }
+  p.splits = (int)(((long)n + p.chunk - 1) / p.chunk);
+  return p;
 }
 
 int visible(int n, int slide) { return slide > 0 ? std::min(n, slide) : n; }
 
 struct DecodePlan {
-  int own_chunk, own_splits, pre_chunk, pre_splits;
-  int slots() const { return own_splits + pre_splits; }
+  Plan own, pre;
+  int slots() const { return own.splits + pre.splits; }
 };
 
 DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads, int slide) {
-  DecodePlan p{1, 0, 1, 0};
   const int G = max_group(n_heads, own.nkv);
-  split_range(visible(max_len, slide), (long)own.nkv * own.nseq, p.own_chunk, p.own_splits);
-  if (plen > 0)
-    split_range(visible(plen, slide), (long)own.nkv * (((long)own.nseq * G + kMaxGroup - 1) / kMaxGroup),
-                p.pre_chunk, p.pre_splits);
+  DecodePlan p{plan_rows(own, OWN, own.nseq, G, visible(max_len, slide)), Plan{false, 1, 0}};
+  if (plen > 0) p.pre = plan_rows(own, PREFIX, own.nseq, G, visible(plen, slide));
   return p;
 }
 
@@ -537,16 +550,16 @@ GCU_EXPORT int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long qrow = (long)n_heads * own->hdim;
   Args a{xq, qrow, own->hdim, xo, qrow, *own, OWN, n_heads, own->nseq, 0, slide, 1, plen, max_len, len, asc, sc_att,
-         p.own_chunk, p.own_splits, p.pre_splits, p.slots(), nullptr, nullptr, dev_error_word()};
+         p.own.chunk, p.own.splits, p.pre.splits, p.slots(), nullptr, nullptr, dev_error_word()};
   use_work(a, work, rows);
   if (plen > 0) {
     Args b = a;
     b.mode = PREFIX;
     b.kv = *prefix;
-    b.chunk = p.pre_chunk;
-    b.splits = p.pre_splits;
+    b.chunk = p.pre.chunk;
+    b.splits = p.pre.splits;
     b.slot0 = 0;
-    if (launch_rows(b, st)) return 1;
+    if (p.pre.tc ? launch_tc(b, st) : launch_rows(b, st)) return 1;
   }
   if (launch_rows(a, st)) return 1;
   return a.slots > 1 ? launch_merge(a, st) : 0;
@@ -554,16 +567,10 @@ GCU_EXPORT int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu
 
 namespace {
 
-struct PrefillPlan {
-  int chunk, splits;
-};
-
-PrefillPlan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, int slide, int mask) {
-  PrefillPlan p;
-  const long rows = (long)ntok * max_group(n_heads, kv.nkv);
-  const int n = mask && slide > 0 ? std::min(spos + ntok, slide + kMaxGroup) : spos + ntok;
-  split_range(n, (rows + kMaxGroup - 1) / kMaxGroup * kv.nkv, p.chunk, p.splits);
-  return p;
+Plan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, int slide, int mask) {
+  // a window's width, and the tokens of one CTA's rows past its first
+  const long n = mask && slide > 0 ? std::min((long)spos + ntok, (long)slide + kTcRows) : (long)spos + ntok;
+  return plan_rows(kv, PREFILL, ntok, max_group(n_heads, kv.nkv), (int)n);
 }
 
 }  // namespace
@@ -586,13 +593,13 @@ GCU_EXPORT int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *x
   if (xostr == 0) xostr = n_heads * kv->hdim;
   if (!aligned16(xo) || !aligned16(xq) || xostr % 4 || xostr < n_heads * kv->hdim)
     return set_error("%s: buffers must be 16-byte aligned, xostr a multiple of 4 floats, at least n_heads*hdim", what);
-  const PrefillPlan p = plan_prefill(*kv, n_heads, spos, ntok, slide, mask);
+  const Plan p = plan_prefill(*kv, n_heads, spos, ntok, slide, mask);
   const long rows = (long)ntok * n_heads;
   if (check_work(what, slot_bytes(p.splits, rows, kv->hdim), work, work_bytes)) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Args a{xq, kv->hdim, (long)ntok * kv->hdim, xo, xostr, *kv, PREFILL, n_heads, ntok, spos, slide, mask ? 1 : 0, 0, 0,
          nullptr, 1.0f, sc_att, p.chunk, p.splits, 0, p.splits, nullptr, nullptr, dev_error_word()};
   use_work(a, work, rows);
-  if (launch_rows(a, st)) return 1;
+  if (p.tc ? launch_tc(a, st) : launch_rows(a, st)) return 1;
   return a.slots > 1 ? launch_merge(a, st) : 0;
 }

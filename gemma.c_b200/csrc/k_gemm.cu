@@ -1264,6 +1264,24 @@ int gemm_tmap_i8(CUtensorMap *m, const int8_t *base, int k, int rows, long strid
   return make_map_i8(m, base, k, rows, stride, box_rows);
 }
 
+int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, int hdim, int rows, int heads, long head_stride,
+                       int box_rows) {
+  if (get_encode()) return 1;
+  const cuuint32_t inner = hdim < 128 ? (cuuint32_t)hdim : 128u;
+  cuuint64_t dims[3] = {(cuuint64_t)hdim, (cuuint64_t)rows, (cuuint64_t)heads};
+  cuuint64_t strides[2] = {(cuuint64_t)hdim, (cuuint64_t)(heads > 1 ? head_stride : (long)rows * hdim)};
+  cuuint32_t box[3] = {inner, (cuuint32_t)box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t *>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        inner < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error("tensor map (int8 %d heads of %d x %d, stride %ld) failed: %d", heads, rows, hdim, head_stride,
+                     (int)r);
+  return 0;
+}
+
 int gemm_tmap_f32(CUtensorMap *m, float *base, int n, int rows, long stride_elems) {
   if (get_encode()) return 1;
   return make_map_f32(m, base, n, rows, stride_elems);
