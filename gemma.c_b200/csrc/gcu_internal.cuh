@@ -543,15 +543,42 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t adesc,
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// D[tmem] (+)= A[tmem] * B[smem], 16-bit floats -> fp32, one CTA.  A: row = lane,
-// two consecutive K elements per 32-bit column.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// One thread of a converged warp (the same in every call).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+// A shared-memory matrix descriptor in two words (desc_lo, desc_hi below): the
+// second is a constant and the first moves with the address, so that a warp
+// that computes them uniformly spends one addition per product.
+struct Desc {
+  uint32_t lo, hi;
+};
+// mma_i8 with such descriptors
+__device__ __forceinline__ void mma_i8(uint32_t d_tmem, Desc a, Desc b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], x, y, %5, p;\n\t}" ::"r"(d_tmem),
+      "r"(a.lo), "r"(a.hi), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem], 16-bit floats -> fp32, one CTA.  A: row = lane,
+// two consecutive K elements per 32-bit column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, Desc b, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b.lo), "r"(b.hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 // Registers of a warpgroup (128 threads, all of them call it): give some back, or
@@ -608,6 +635,13 @@ __device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 32 lanes x 8 columns
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -632,15 +666,10 @@ __device__ __forceinline__ uint64_t smem_desc_k128(uint32_t saddr) {
 // The same for any swizzled tile: lbo / sbo in bytes, swizzle 128 or 64.
 // K-major: 8-row atoms (8 x swizzle bytes) sbo apart, lbo unused.  MN-major
 // (swizzle 128, 16-bit elements): atoms of 64 MN elements x 8 K rows, lbo
-// apart along MN and sbo along K.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo, int swizzle) {
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)((lbo >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)((sbo >> 4) & 0x3FFF) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)(swizzle == 128 ? 2 : 4) << 61;
-  return d;
+// apart along MN and sbo along K.  Moving by n bytes adds n >> 4 to lo.
+__device__ __forceinline__ Desc smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo, int swizzle) {
+  return Desc{((saddr >> 4) & 0x3FFF) | ((lbo >> 4) & 0x3FFF) << 16,
+              ((sbo >> 4) & 0x3FFF) | 1u << 14 | (swizzle == 128 ? 2u : 4u) << 29};
 }
 
 // Instruction descriptor, kind::f16: D = fp32, A = B = fp16, A K-major, B

@@ -23,11 +23,16 @@
 // nearest, and the next tile starts T afresh.  The same happens when a row's m
 // moves, so the rescaling is a multiplication of registers.
 //
-// Warpgroups 0 and 1: softmax (two threads per row, half a tile's columns and half
-// the output columns each; the row's sums take HD/2 registers of each, which
-// the third warpgroup gives up).  Warps 8, 9: V codes to fp16 in the MN-major
-// layout that the product reads; 10: loads; 11: products.  While the softmax of
-// tile j runs, the tensor cores compute S of tile j + 1 and T of tile j - 1.
+// Warps 0-7 and 8-15: two groups of softmax threads, for even and odd tiles, so
+// that one's loads and barriers hide behind the other's arithmetic.  In a group
+// two threads share a row, half a tile's columns each; of the row's output
+// columns each of its four threads holds a quarter in HD/4 registers (some of
+// which the last warpgroup gives up).  The groups agree on m through shared
+// memory, tile by tile (a "decision").  A group also turns its tile's V codes
+// into fp16, in the MN-major layout that the product reads, before its scores
+// arrive.  Warp 16: products, issued by one thread of a warp that computes
+// the descriptors uniformly; 17: loads.  While the softmax of tile j runs, the
+// tensor cores compute S of tile j + 1 and T of tile j - 1.
 // Every wait is bounded; a role that gives up sets the CTA's abort flag, which
 // ends the others' waits.
 #include "attention_i8.cuh"
@@ -41,11 +46,10 @@ namespace gcu {
 namespace attn8 {
 namespace {
 
-constexpr int kSoftmax = 256;   // warps 0-7
-constexpr int kConvert = 64;    // warps 8, 9
-constexpr int kLoadWarp = 10, kMmaWarp = 11;
-constexpr int kThreads = 384;
-constexpr int kRegsSoftmax = 224, kRegsOther = 56;  // 2 * 224 + 56 = 3 * 168
+constexpr int kGroup = 256, kSoftmax = 2 * kGroup;  // warps 0-7, 8-15
+constexpr int kMmaWarp = 16, kLoadWarp = 17;
+constexpr int kThreads = 640;  // setmaxnreg counts whole warpgroups: two warps of the last one idle
+constexpr int kRegsSoftmax = 112, kRegsOther = 32;  // 4 * 112 + 32 = 5 * 96
 constexpr int kRows = 128;
 constexpr int NK = 64;     // keys per tile
 constexpr int kFlush = 4;  // tiles per T
@@ -73,12 +77,14 @@ struct Cfg {
   static constexpr int V16_OFF = K_OFF + 2 * K_BYTES;
   static constexpr int V8_OFF = V16_OFF + 2 * V16_BYTES;
   static constexpr int SC_OFF = V8_OFF + NV8 * V8_BYTES;      // scales [4][3][NK]: ks, log2 vs, 1 / vs
-  static constexpr int MAX_OFF = SC_OFF + 4 * 3 * NK * 4;     // [2][2][128] row maxima (at the end: sums)
-  static constexpr int RF_OFF = MAX_OFF + 2 * 2 * kRows * 4;  // [128] score factors
+  static constexpr int REF_OFF = SC_OFF + 4 * 3 * NK * 4;     // [128] reference points
+  static constexpr int MAX_OFF = REF_OFF + kRows * 4;         // [2][2][128] row maxima (at the end: sums)
+  static constexpr int RF_OFF = MAX_OFF + 4 * kRows * 4;  // [128] score factors
   static constexpr int SMEM = RF_OFF + kRows * 4 + 1024;
   // TMEM columns: S of three digits, T, P (two parts, two keys per column)
-  static constexpr int S_COL = 0, T_COL = 3 * NK, P_COL = T_COL + HD;
   static constexpr int HALF = NK / 2;  // score columns per softmax thread
+  static constexpr int OC = HD / 4;    // output columns per softmax thread
+  static constexpr int S_COL = 0, T_COL = 3 * NK, P_COL = T_COL + HD;
   static_assert(SMEM <= 232448 - 512, "shared memory budget");
   static_assert(P_COL + NK <= 512, "TMEM budget");
 };
@@ -90,9 +96,12 @@ struct alignas(64) TcArgs {
 };
 
 struct Bars {
-  uint64_t kfull[2], kempty[2], v8full[2], v8empty[2], v16full[2], v16empty[2], sfull, sfree, pfull, pvdone, drain;
+  uint64_t kfull[2], kempty[2], v8full[2], v8empty[2], v16full[2], dec[2], sfull[2], pvdone[2], sfree, pfull, tfree, drain;
 };
 
+// Every wait is on the phase after the last one that its waiter knows complete
+// (a parity cannot tell two phases apart): what the two softmax groups take in
+// turn has one barrier per tile parity.
 struct Waiter {
   volatile int *abort;
   unsigned int *err;
@@ -140,13 +149,13 @@ __device__ __forceinline__ void put_scale(float *sc, int i, float v) {
   if (i < NK) {
     sc[i] = v;
   } else if (i < 2 * NK) {
-    v = v < kVsMin ? kVsMin : v > kVsMax ? kVsMax : v;  // NaN stays
-    sc[i] = log2f(v);
-    sc[i + NK] = 1.0f / v;
+    v = v < kVsMin ? kVsMin : v > kVsMax ? kVsMax : v;
+    sc[i] = log2f(v);                   // NaN makes the weights NaN where the key is seen
+    sc[i + NK] = v == v ? 1.0f / v : 1.0f;  // finite: times the zero weight of a key that is not
   }
 }
 
-template <int HD>
+template <int HD, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcArgs p) {
   using C = Cfg<HD>;
   extern __shared__ uint8_t smem_raw[];
@@ -166,14 +175,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       ptx::mbar_init(&bars.kfull[s], 1);
       ptx::mbar_init(&bars.kempty[s], 1);
       ptx::mbar_init(&bars.v8full[s], 1);
-      ptx::mbar_init(&bars.v8empty[s], kConvert);
-      ptx::mbar_init(&bars.v16full[s], kConvert);
-      ptx::mbar_init(&bars.v16empty[s], 1);
+      ptx::mbar_init(&bars.v8empty[s], kGroup);
+      ptx::mbar_init(&bars.v16full[s], kGroup);
     }
-    ptx::mbar_init(&bars.sfull, 1);
-    ptx::mbar_init(&bars.sfree, kSoftmax);
-    ptx::mbar_init(&bars.pfull, kSoftmax);
-    ptx::mbar_init(&bars.pvdone, 1);
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&bars.dec[s], kGroup);
+      ptx::mbar_init(&bars.sfull[s], 1);
+      ptx::mbar_init(&bars.pvdone[s], 1);
+    }
+    ptx::mbar_init(&bars.sfree, kGroup);
+    ptx::mbar_init(&bars.pfull, kGroup);
+    ptx::mbar_init(&bars.tfree, 2 * kGroup);
     ptx::mbar_init(&bars.drain, 1);
     ptx::fence_mbar_init();
     s_abort = 0;
@@ -223,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   };
   auto load_v = [&](int j, uint64_t pol) {
     const uint32_t bytes = (uint32_t)min(NK, n - j * NK) * HD;
-    uint64_t *bar = &bars.v8full[j % C::NV8];
+    uint64_t *bar = &bars.v8full[j & 1];
     ptx::mbar_arrive_expect_tx(bar, bytes);
     ptx::bulk_load(smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES, vh + (long)(kbeg + j * NK) * HD, bytes, bar, pol);
   };
@@ -312,189 +324,209 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       // every load issued must have landed before the CTA may exit
       for (int j = max(0, nk - 2); j < nk; ++j)
         ptx::mbar_wait(&bars.kfull[j & 1], (j >> 1) & 1, a.err, DEV_TIMEOUT_DRAIN);
-      for (int j = max(0, nv - C::NV8); j < nv; ++j)
-        ptx::mbar_wait(&bars.v8full[j % C::NV8], (j / C::NV8) & 1, a.err, DEV_TIMEOUT_DRAIN);
+      for (int j = max(0, nv - 2); j < nv; ++j)
+        ptx::mbar_wait(&bars.v8full[j & 1], (j >> 1) & 1, a.err, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ products
-    if (lane == 0 && nt > 0) {
+    const int tiles = __shfl_sync(0xffffffffu, nt, 0);
+    if (tiles > 0) {
       constexpr uint32_t id_s = ptx::idesc_i8(kRows, NK), id_o = ptx::idesc_f16_bt(kRows, HD);
-      const uint32_t q0 = ptx::smem_u32(smem + C::Q_OFF), k0 = ptx::smem_u32(smem + C::K_OFF);
-      const uint32_t v0 = ptx::smem_u32(smem + C::V16_OFF);
+      const ptx::Desc dq = ptx::smem_desc(ptx::smem_u32(smem + C::Q_OFF), 16, 8 * C::SW, C::SW);
+      const ptx::Desc dk = ptx::smem_desc(ptx::smem_u32(smem + C::K_OFF), 16, 8 * C::SW, C::SW);
+      const ptx::Desc dv = ptx::smem_desc(ptx::smem_u32(smem + C::V16_OFF), C::V16_BLOCK, 1024, 128);
       auto scores = [&](int j) {
-#pragma unroll
-        for (int d = 0; d < 3; ++d)
+        if (ptx::elect_one()) {
+          const uint32_t k_lo = dk.lo + (j & 1) * (C::K_BYTES >> 4);
 #pragma unroll
           for (int b = 0; b < C::KB; ++b)
 #pragma unroll
             for (int s = 0; s < C::SW / 32; ++s)
-              ptx::mma_i8(tmem + C::S_COL + d * NK,
-                          ptx::smem_desc(q0 + (d * C::KB + b) * C::Q_BLOCK + 32 * s, 16, 8 * C::SW, C::SW),
-                          ptx::smem_desc(k0 + (j & 1) * C::K_BYTES + b * C::K_BLOCK + 32 * s, 16, 8 * C::SW, C::SW), id_s,
-                          b + s > 0 ? 1u : 0u);
-        ptx::mma_commit(&bars.kempty[j & 1]);
-        ptx::mma_commit(&bars.sfull);
+#pragma unroll
+              for (int d = 0; d < 3; ++d)
+                ptx::mma_i8(tmem + C::S_COL + d * NK,
+                            ptx::Desc{dq.lo + (((d * C::KB + b) * C::Q_BLOCK + 32 * s) >> 4), dq.hi},
+                            ptx::Desc{k_lo + ((b * C::K_BLOCK + 32 * s) >> 4), dk.hi}, id_s, b + s > 0 ? 1u : 0u);
+          ptx::mma_commit(&bars.kempty[j & 1]);
+          ptx::mma_commit(&bars.sfull[j & 1]);
+        }
+        __syncwarp();
       };
       bool ok = wait(&bars.kfull[0], 0, DEV_TIMEOUT_FULL);
+      if (__any_sync(0xffffffffu, !ok)) ok = false;
       if (ok) {
         ptx::tc_fence_after();
         scores(0);
       }
-      for (int j = 0; j < nt && ok; ++j) {
-        if (j + 1 < nt) {
+      int taken = 0;
+      for (int j = 0; j < tiles && ok; ++j) {
+        if (j + 1 < tiles) {
           ok = wait(&bars.kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, DEV_TIMEOUT_FULL) &&
                wait(&bars.sfree, j & 1, DEV_TIMEOUT_TMEM);
-          if (!ok) break;
+          if (__any_sync(0xffffffffu, !ok)) break;
           ptx::tc_fence_after();
           scores(j + 1);
         }
         ok = wait(&bars.v16full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && wait(&bars.pfull, j & 1, DEV_TIMEOUT_TMEM);
-        if (!ok) break;
+        const bool fresh = __shfl_sync(0xffffffffu, *(volatile int *)&s_fresh[j & 1], 0);
+        if (fresh && j > 0)  // T's sums have been taken
+          ok = ok && wait(&bars.tfree, taken++ & 1, DEV_TIMEOUT_TMEM);
+        if (__any_sync(0xffffffffu, !ok)) break;
         ptx::tc_fence_after();
-        const uint32_t keep = *(volatile int *)&s_fresh[j & 1] ? 0u : 1u;
+        if (ptx::elect_one()) {
+          const uint32_t v_lo = dv.lo + (j & 1) * (C::V16_BYTES >> 4);
 #pragma unroll
-        for (int part = 0; part < 2; ++part)
+          for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int s = 0; s < NK / 16; ++s)
-            ptx::mma_f16_ts(tmem + C::T_COL, tmem + C::P_COL + part * (NK / 2) + 8 * s,
-                            ptx::smem_desc(v0 + (j & 1) * C::V16_BYTES + s * 2048, C::V16_BLOCK, 1024, 128), id_o,
-                            part + s > 0 ? 1u : keep);
-        ptx::mma_commit(&bars.v16empty[j & 1]);
-        ptx::mma_commit(&bars.pvdone);
+            for (int s = 0; s < NK / 16; ++s)
+              ptx::mma_f16_ts(tmem + C::T_COL, tmem + C::P_COL + part * (NK / 2) + 8 * s,
+                              ptx::Desc{v_lo + ((s * 2048) >> 4), dv.hi}, id_o, part + s > 0 || !fresh ? 1u : 0u);
+          ptx::mma_commit(&bars.pvdone[j & 1]);
+        }
+        __syncwarp();
       }
       // all products complete before TMEM is freed
-      ptx::mma_commit(&bars.drain);
+      if (ptx::elect_one()) ptx::mma_commit(&bars.drain);
+      __syncwarp();
       ptx::mbar_wait(&bars.drain, 0, a.err, DEV_TIMEOUT_DRAIN);
     }
-  } else if (warp >= kSoftmax / 32) {
-    // ------------------------------------------------------------ V codes to fp16
-    const int t = threadIdx.x - kSoftmax;
-    constexpr int L = HD / 8, KS = kConvert / L;  // threads per key (8 columns each), keys at a time
-    const int c = t % L, key0 = t / L;
-    for (int j = 0; j < nt; ++j) {
-      if (!wait(&bars.v8full[j % C::NV8], (j / C::NV8) & 1, DEV_TIMEOUT_FULL)) break;
-      if (j > 1 && !wait(&bars.v16empty[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM)) break;
-      const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
-      uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
-      // keys past the range hold an earlier tile's codes, which weigh nothing
-#pragma unroll 8
-      for (int k = 0; k < NK; k += KS) {
-        const int key = key0 + k;
-        const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
-        const uint2 x = to_half4(w.x), y = to_half4(w.y);
-        *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
-      }
-      ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
-      ptx::mbar_arrive(&bars.v16full[j & 1]);
-    }
-  } else {
+  } else if (warp < kSoftmax / 32) {
     // ------------------------------------------------------------ softmax
     ptx::regs_inc<kRegsSoftmax>();
-    const int half = warp >> 2, row = (warp & 3) * 32 + lane, tid = threadIdx.x;
+    const int grp = warp >> 3, half = (warp >> 2) & 1, quarter = warp >> 2;
+    const int row = threadIdx.x & (kRows - 1), tid = threadIdx.x & (kGroup - 1);
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     float *sc = reinterpret_cast<float *>(smem + C::SC_OFF);
-    float *smax = reinterpret_cast<float *>(smem + C::MAX_OFF);
+    volatile float *refs = reinterpret_cast<float *>(smem + C::REF_OFF);
+    volatile float *smax = reinterpret_cast<float *>(smem + C::MAX_OFF);
+    volatile int *freshp = s_fresh;
     const bool live = row < nrows;
-    const int i = live ? (first + row) / G : 0, h = live ? h0 + (first + row) % G : h0;
     int lo = 0, hi = 0;
-    if (live) row_window(a, i, lo, hi);
-    const float rf_nat = nt > 0 ? s_rf[row] : 0.0f;
-    const bool capped = a.sc_att != 0.0f;
-    const float rf = capped ? kLog2e : rf_nat * kLog2e;
-    const float *sc_src = (tid < NK ? a.kv.ks : a.kv.vs) + hk * a.kv.sc_stride + kbeg;
+    if (live) row_window(a, (first + row) / G, lo, hi);
+    const float rf_nat = nt > 0 ? s_rf[row] : 0.0f, rf = CAP ? kLog2e : rf_nat * kLog2e;
+    // scales of the other group's next tile: thread tid of ks (tid < NK) or vs
     auto fetch_scale = [&](int j) {
-      const int t = j * NK + tid % NK;
-      return tid < 2 * NK && t < n ? __ldg(sc_src + t) : 1.0f;
+      const int t = j * NK + (tid & (NK - 1));
+      return tid < 2 * NK && t < n ? __ldg((tid < NK ? a.kv.ks : a.kv.vs) + hk * a.kv.sc_stride + kbeg + t) : 1.0f;
     };
-    float next = fetch_scale(1);
+    float next = fetch_scale(grp + 1);
     float m = -INFINITY, l = 0.0f;
-    float acc[HD / 2];  // the row's sums, output columns [half * HD/2, +HD/2)
+    float acc[C::OC];  // the row's sums, output columns [quarter * OC, +OC)
 #pragma unroll
-    for (int c = 0; c < HD / 2; ++c) acc[c] = 0.0f;
-    // add T (complete) to the row's sums
-    auto flush = [&]() {
+    for (int c = 0; c < C::OC; ++c) acc[c] = 0.0f;
+    // add T (complete) to the row's sums, then scale them
+    auto flush = [&](float f) {
       ptx::tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < HD / 2; c += 32) {
-        uint32_t t[32];
-        ptx::tmem_ld_32x32(lanes + C::T_COL + half * (HD / 2) + c, t);
+      for (int c = 0; c < C::OC; c += 16) {
+        uint32_t t[16];
+        ptx::tmem_ld_32x16(lanes + C::T_COL + quarter * C::OC + c, t);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) acc[c + e] += __uint_as_float(t[e]);
+        for (int e = 0; e < 16; ++e) acc[c + e] = (acc[c + e] + __uint_as_float(t[e])) * f;
       }
       ptx::tc_fence_before();
     };
     bool ok = true;
-    for (int j = 0; j < nt; ++j) {
+    // take over the decision of tile j (the other group's): its reference point,
+    // and T's sums when its product starts T afresh
+    auto follow = [&](int j) {
+      ok = wait(&bars.dec[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      const float to = refs[row];
+      const float f = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
+      l *= f;
+      m = to;
+      if (j > 0 && freshp[j & 1]) {
+        ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+        flush(f);
+        ptx::mbar_arrive(&bars.tfree);
+      }
+    };
+    int j = grp;
+    for (; j < nt; j += 2) {
+      // V codes of this tile to fp16; 8 columns of a key per thread.  Keys past
+      // the range hold an earlier tile's codes, which weigh nothing.
+      ok = wait(&bars.v8full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && ok;
+      if (j > 1) ok = wait(&bars.pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      {
+        constexpr int L = HD / 8, KS = kGroup / L;
+        const int c = tid % L, key0 = tid / L;
+        const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
+        uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
+#pragma unroll
+        for (int k = 0; k < NK; k += KS) {
+          const int key = key0 + k;
+          const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
+          const uint2 x = to_half4(w.x), y = to_half4(w.y);
+          *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
+        ptx::mbar_arrive(&bars.v16full[j & 1]);
+      }
       const float *ks = sc + (j & 3) * 3 * NK + half * C::HALF, *lvs = ks + NK, *rvs = ks + 2 * NK;
-      ok = ok && wait(&bars.sfull, j & 1, DEV_TIMEOUT_TMEM);
+      if (j > 0) follow(j - 1);
+      ok = wait(&bars.sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       ptx::tc_fence_after();
       // exponents: the score in log2 units plus log2 of the value row's scale
       float x[C::HALF];
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 16) {
-        uint32_t s2[16], s1[16], s0[16];
+      for (int c = 0; c < C::HALF; c += 8) {
+        uint32_t s2[8], s1[8], s0[8];
         const uint32_t at = lanes + C::S_COL + half * C::HALF + c;
-        ptx::tmem_ld_32x16(at, s0);
-        ptx::tmem_ld_32x16(at + NK, s1);
-        ptx::tmem_ld_32x16(at + 2 * NK, s2);
+        ptx::tmem_ld_32x8(at, s0);
+        ptx::tmem_ld_32x8(at + NK, s1);
+        ptx::tmem_ld_32x8(at + 2 * NK, s2);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
+        for (int e = 0; e < 8; e += 4) {
           const float4 k = *reinterpret_cast<const float4 *>(ks + c + e);
-          float2 u = digit_sum2(s2 + e, s1 + e, s0 + e), v = digit_sum2(s2 + e + 2, s1 + e + 2, s0 + e + 2);
-          u = __fmul2_rn(u, make_float2(k.x, k.y));
-          v = __fmul2_rn(v, make_float2(k.z, k.w));
-          x[c + e] = u.x;
-          x[c + e + 1] = u.y;
-          x[c + e + 2] = v.x;
-          x[c + e + 3] = v.y;
+          const float4 v = *reinterpret_cast<const float4 *>(lvs + c + e);
+          float2 y = __fmul2_rn(digit_sum2(s2 + e, s1 + e, s0 + e), make_float2(k.x, k.y));
+          float2 z = __fmul2_rn(digit_sum2(s2 + e + 2, s1 + e + 2, s0 + e + 2), make_float2(k.z, k.w));
+          if constexpr (CAP) {
+            y = make_float2(tanhf(y.x * rf_nat / a.sc_att) * a.sc_att, tanhf(y.y * rf_nat / a.sc_att) * a.sc_att);
+            z = make_float2(tanhf(z.x * rf_nat / a.sc_att) * a.sc_att, tanhf(z.y * rf_nat / a.sc_att) * a.sc_att);
+          }
+          y = __ffma2_rn(y, make_float2(rf, rf), make_float2(v.x, v.y));
+          z = __ffma2_rn(z, make_float2(rf, rf), make_float2(v.z, v.w));
+          x[c + e] = y.x;
+          x[c + e + 1] = y.y;
+          x[c + e + 2] = z.x;
+          x[c + e + 3] = z.y;
         }
       }
       ptx::tc_fence_before();
       ptx::mbar_arrive(&bars.sfree);
-      if (capped) {
-#pragma unroll
-        for (int c = 0; c < C::HALF; ++c) x[c] = tanhf(x[c] * rf_nat / a.sc_att) * a.sc_att;
-      }
-#pragma unroll
-      for (int c = 0; c < C::HALF; c += 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(lvs + c);
-        const float2 r2 = make_float2(rf, rf);
-        const float2 y = __ffma2_rn(make_float2(x[c], x[c + 1]), r2, make_float2(v.x, v.y));
-        const float2 z = __ffma2_rn(make_float2(x[c + 2], x[c + 3]), r2, make_float2(v.z, v.w));
-        x[c] = y.x;
-        x[c + 1] = y.y;
-        x[c + 2] = z.x;
-        x[c + 3] = z.y;
-      }
       // a tile that some row does not see in full
       const int t0 = kbeg + j * NK;
-      const bool masked = t0 < all_lo || t0 + NK > min(all_hi, kend);
-      if (masked) {
+      if (t0 < all_lo || t0 + NK > min(all_hi, kend)) {
         const int cl = lo - t0 - half * C::HALF, ch = min(hi, kend) - t0 - half * C::HALF;
 #pragma unroll
         for (int c = 0; c < C::HALF; ++c)
           if (c < cl || c >= ch) x[c] = -INFINITY;
       }
-      float mx = -INFINITY;
+      float top = -INFINITY, top2 = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < C::HALF; ++c) mx = fmaxf(mx, x[c]);
-      float *sm = smax + (j & 1) * 2 * kRows;
-      sm[half * kRows + row] = mx;
-      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
-      next = fetch_scale(j + 2);
-      float f = 1.0f;
-      bool fresh = j % kFlush == 0;
-      if (ptx::named_bar_or(1, kSoftmax, mx > m + kSlack || (m == -INFINITY && mx > m) || !ok)) {
-        if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
-        const float to = fmaxf(m, fmaxf(sm[row], sm[kRows + row]));
-        f = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
-        l *= f;
-        m = to;
-        fresh = true;
+      for (int c = 0; c < C::HALF; c += 4) {
+        top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
+        top2 = fmaxf(fmaxf(top2, x[c + 2]), x[c + 3]);
       }
+      top = fmaxf(top, top2);
+      smax[(grp * 2 + half) * kRows + row] = top;
+      // the other group reads these scales after this tile's decision
+      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
+      next = fetch_scale(j + 3);
+      const bool moved = ptx::named_bar_or(1 + grp, kGroup, top > m + kSlack || (m == -INFINITY && top > m) || !ok);
+      if (moved && ptx::named_bar_or(1 + grp, kGroup, !ok)) break;
+      const float to = moved ? fmaxf(m, fmaxf(top, smax[(grp * 2 + (half ^ 1)) * kRows + row])) : m;
+      const bool fresh = moved || j % kFlush == 0;
+      if (half == 0) refs[row] = to;
+      if (tid == 0) freshp[j & 1] = fresh;
+      ptx::mbar_arrive(&bars.dec[j & 1]);
+      const float f = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
+      l *= f;
+      m = to;
       const float ref = m == -INFINITY ? 0.0f : m - kTop;
       uint32_t ph[C::HALF / 2], pl[C::HALF / 2];
       float2 lt = make_float2(0.0f, 0.0f);
@@ -505,15 +537,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         for (int e = 0; e < 4; e += 2) {
           const float2 d = __fadd2_rn(make_float2(x[c + e], x[c + e + 1]), make_float2(-ref, -ref));
           const float2 w = make_float2(ex2(d.x), ex2(d.y));
-          float2 q = e ? make_float2(r.z, r.w) : make_float2(r.x, r.y);
-          if (masked) {  // a key that is not seen weighs nothing, whatever its scales
-            q.x = x[c + e] == -INFINITY ? 0.0f : q.x;
-            q.y = x[c + e + 1] == -INFINITY ? 0.0f : q.y;
-          }
-          lt = __ffma2_rn(w, q, lt);
+          lt = __ffma2_rn(w, e ? make_float2(r.z, r.w) : make_float2(r.x, r.y), lt);
           const __half2 hi2 = __floats2half2_rn(w.x, w.y);
           const float2 back = __half22float2(hi2);
-          const __half2 lo2 = __floats2half2_rn(w.x - back.x, w.y - back.y);
+          const float2 rest = __fadd2_rn(w, make_float2(-back.x, -back.y));
+          const __half2 lo2 = __floats2half2_rn(rest.x, rest.y);
           ph[(c + e) / 2] = *reinterpret_cast<const uint32_t *>(&hi2);
           pl[(c + e) / 2] = *reinterpret_cast<const uint32_t *>(&lo2);
         }
@@ -521,39 +549,40 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       l += lt.x + lt.y;
       // P and T are free once the previous tile's product is done
       if (j > 0) {
-        ok = wait(&bars.pvdone, (j - 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+        ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
         if (fresh) {
-          flush();
-          if (f != 1.0f) {
-#pragma unroll
-            for (int c = 0; c < HD / 2; ++c) acc[c] *= f;
-          }
+          flush(f);
+          ptx::mbar_arrive(&bars.tfree);
         }
       }
+      ptx::tc_fence_after();
       ptx::tmem_st_32x16(lanes + C::P_COL + half * (C::HALF / 2), ph);
       ptx::tmem_st_32x16(lanes + C::P_COL + NK / 2 + half * (C::HALF / 2), pl);
-      if (tid == 0) *(volatile int *)&s_fresh[j & 1] = fresh;
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       ptx::mbar_arrive(&bars.pfull);
     }
+    // the group without the last tile follows its decision too (j is the tile
+    // after it); then both take what is left in T
+    if (j == nt && nt > 0) follow(nt - 1);
     if (nt > 0) {
-      ok = wait(&bars.pvdone, (nt - 1) & 1, DEV_TIMEOUT_TMEM) && ok;
-      flush();
+      ok = wait(&bars.pvdone[(nt - 1) & 1], ((nt - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      flush(1.0f);
     }
-    // the row's sum over both halves
-    ptx::named_bar_sync(1, kSoftmax);
-    smax[half * kRows + row] = l;
-    ptx::named_bar_sync(1, kSoftmax);
-    l = smax[row] + smax[kRows + row];
+    // the row's sum over its four threads, which end with the same m
+    ptx::named_bar_sync(3, kSoftmax);
+    smax[quarter * kRows + row] = l;
+    ptx::named_bar_sync(3, kSoftmax);
+    l = (smax[row] + smax[kRows + row]) + (smax[2 * kRows + row] + smax[3 * kRows + row]);
+    const int i = live ? (first + row) / G : 0, h = live ? h0 + (first + row) % G : h0;
     const size_t at = ((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h;
-    float *out = (a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD : a.part + at * HD) + half * (HD / 2);
+    float *out = (a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD : a.part + at * HD) + quarter * C::OC;
     const float d = a.slots > 1 || l == 0.0f ? 1.0f : l;  // a row that sees nothing: zeros
     if (live && ok && (a.slots > 1 || row_live(a, i))) {
 #pragma unroll
-      for (int c = 0; c < HD / 2; c += 4)
+      for (int c = 0; c < C::OC; c += 4)
         *reinterpret_cast<float4 *>(out + c) = make_float4(acc[c] / d, acc[c + 1] / d, acc[c + 2] / d, acc[c + 3] / d);
-      if (a.slots > 1 && half == 0) a.stat[at] = make_float2(m == -INFINITY ? m : m - kTop, l);
+      if (a.slots > 1 && quarter == 0) a.stat[at] = make_float2(m == -INFINITY ? m : m - kTop, l);
     }
   }
   __syncthreads();
@@ -561,13 +590,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, 512);
 }
 
-template <int HD>
+template <int HD, bool CAP>
 int launch_tc_hd(const Args &a, cudaStream_t st) {
   using C = Cfg<HD>;
   TcArgs p;
   p.a = a;
   const int gmax = (a.n_heads + a.kv.nkv - 1) / a.kv.nkv;
   p.tiles = (int)(((long)a.ni * gmax + kRows - 1) / kRows);
+  if ((long)p.tiles * a.splits > 0x7fffffffL) return set_error("attention_i8: %d x %d CTAs", p.tiles, a.splits);
   if (gemm_tmap_heads_i8(&p.tmK, a.kv.k, HD, a.kv.clen, a.kv.nkv, a.kv.kv_stride, NK)) return 1;
   {
     // the shared-memory opt-in is per device: once for each device this runs on
@@ -577,19 +607,25 @@ int launch_tc_hd(const Args &a, cudaStream_t st) {
     GCU_CUDA(cudaGetDevice(&dev));
     std::lock_guard<std::mutex> lk(mu);
     if (!(done & (1ull << (dev & 63)))) {
-      GCU_CUDA(cudaFuncSetAttribute(k_tc<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+      GCU_CUDA(cudaFuncSetAttribute(k_tc<HD, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
       done |= 1ull << (dev & 63);
     }
   }
-  if ((long)p.tiles * a.splits > 0x7fffffffL) return set_error("attention_i8: %d x %d CTAs", p.tiles, a.splits);
-  GCU_CUDA(launch_k(k_tc<HD>, dim3((unsigned)(p.tiles * a.splits), a.kv.nkv), dim3(kThreads), C::SMEM, st, p));
+  GCU_CUDA(launch_k(k_tc<HD, CAP>, dim3((unsigned)(p.tiles * a.splits), a.kv.nkv), dim3(kThreads), C::SMEM, st, p));
   return 0;
+}
+
+template <bool CAP>
+int launch_tc_cap(const Args &a, cudaStream_t st) {
+  return a.kv.hdim == 256   ? launch_tc_hd<256, CAP>(a, st)
+         : a.kv.hdim == 128 ? launch_tc_hd<128, CAP>(a, st)
+                            : launch_tc_hd<64, CAP>(a, st);
 }
 
 }  // namespace
 
 int launch_tc(const Args &a, cudaStream_t st) {
-  return a.kv.hdim == 256 ? launch_tc_hd<256>(a, st) : a.kv.hdim == 128 ? launch_tc_hd<128>(a, st) : launch_tc_hd<64>(a, st);
+  return a.sc_att != 0.0f ? launch_tc_cap<true>(a, st) : launch_tc_cap<false>(a, st);
 }
 
 }  // namespace attn8

@@ -90,6 +90,27 @@ def test_decode_many_rows_of_one_prefix():
     check(run_decode(xq, handle(own), lens, 9, prefix=handle(pre), plen=1500), want, tol)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("plen", [63, 129, 700, 705])
+def test_decode_long_chunks(hd, plen):
+    """More query tiles than SMs: each walks the whole prefix; scores grow along it in half the rows."""
+    rng = np.random.default_rng(plen)
+    nseq = 150 * 128 // 8
+    pre = list(R.cache(rng, 1, 1, plen, hd))
+    pre[2][0, 0] *= np.linspace(0.5, 6, plen, dtype=np.float32)
+    xq = rng.standard_normal((nseq, 8, hd), dtype=np.float32)
+    xq[::2] *= np.float32(3)
+    own = gcu.KvCacheI8.empty(nseq, 1, 1, hd)
+    lens = dev(np.zeros(nseq, np.int32))
+    xo = torch.full(xq.shape, 9.0, device="cuda")
+    gcu.dev_attention_decode_i8(xo, dev(xq), own, lens, 1, hd ** -0.5, 0.0, 0, handle(pre), plen)
+    some = np.r_[0:40, 1000:1016, nseq - 24:nseq]
+    want, tol = R.decode(xq[some], tuple(np.zeros((len(some), 1, 1, hd), np.int8) if i < 2 else
+                                         np.ones((len(some), 1, 1), np.float32) for i in range(4)),
+                         [0] * len(some), hd ** -0.5, 0.0, 0, tuple(pre), plen)
+    check(xo[torch.from_numpy(some).cuda()], want, tol)
+
+
 def test_decode_sees_nothing():
     rng = np.random.default_rng(3)
     own = R.cache(rng, 3, 1, 8, 64)
