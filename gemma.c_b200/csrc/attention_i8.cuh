@@ -114,11 +114,64 @@ __device__ __forceinline__ void digits(float q, float inv, int &d2, int &d1, int
   d2 = (v - d1) >> 8;
 }
 
-// k_attention_i8.cu: up to 8 rows per CTA on the CUDA cores; k_attention_i8_tc.cu:
-// 128 rows per CTA on the tensor cores, kTcKeys keys at a time
-int launch_rows(const Args &a, cudaStream_t st);
+// 65536 s2 + 256 s1 + s0 in fp32, two columns at a time.  |s| < 2^22 goes into the
+// mantissa of 1.5 * 2^23 by an integer addition (a conversion instruction runs
+// at a fraction of the rate); the offsets leave with the next step.  256 s1 + s0
+// is rounded at 2^31.6 at most, to 2^8, where the largest possible product of one
+// query and key element alone is 127 * 8355711 = 2^30.
+__device__ __forceinline__ float2 magic2(const uint32_t *s) {
+  return make_float2(__uint_as_float(s[0] + 0x4B400000u), __uint_as_float(s[1] + 0x4B400000u));
+}
+// 256 s1 + s0 + 12582912
+__device__ __forceinline__ float2 low_digits(const uint32_t *s1, const uint32_t *s0) {
+  constexpr float off = -12582912.0f * 256.0f;
+  return __fadd2_rn(magic2(s0), __ffma2_rn(magic2(s1), make_float2(256.0f, 256.0f), make_float2(off, off)));
+}
+__device__ __forceinline__ float2 high_digit(const uint32_t *s2, float2 low) {
+  constexpr float off = -12582912.0f * 65537.0f;  // the low digits' offset too
+  return __fadd2_rn(low, __ffma2_rn(magic2(s2), make_float2(65536.0f, 65536.0f), make_float2(off, off)));
+}
+
+// A value row's scale as it goes into the exponent and out of the sum of weights.
+// Taken as at least 2^-100 and at most 2^100: reciprocals and sums stay finite.
+// NaN makes the weights NaN where the key is seen; where it is not, 1 / vs is
+// finite against the zero weight.
+__device__ __forceinline__ void value_scale(float v, float &log2_vs, float &inv_vs) {
+  constexpr float lo = 7.888609e-31f, hi = 1.2676506e30f;
+  v = v < lo ? lo : v > hi ? hi : v;
+  log2_vs = log2f(v);
+  inv_vs = v == v ? 1.0f / v : 1.0f;
+}
+
+// The roles of a CTA wait with a limit.  Every wait is on the phase after the last
+// one that its waiter knows complete (a parity cannot tell two phases apart): what
+// two groups take in turn has one barrier per tile parity.
+struct Waiter {
+  volatile int *abort;
+  unsigned int *err;
+  // false once any role of the CTA has given up
+  __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity, unsigned int code) const {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = ptx::globaltimer();
+    while (!*abort) {
+      for (int i = 0; i < 64; ++i)
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+      if (ptx::globaltimer() - t0 > 2000000000ull) {
+        ptx::record_err(err, code);
+        *abort = 1;
+      }
+    }
+    return false;
+  }
+};
+
+// k_attention_i8_tc.cu: 128 rows per CTA, kTcKeys keys at a time
 int launch_tc(const Args &a, cudaStream_t st);
 constexpr int kTcRows = 128, kTcKeys = 64;
+// k_attention_i8_kt.cu: 16 or 32 rows per CTA, kKtKeys keys at a time; one launch
+// for one or two sets of rows (a shared prefix, the sequences' own caches)
+int launch_kt(const Args *sets, int n, int rows, cudaStream_t st);
+constexpr int kKtKeys = 128;
 int launch_merge(const Args &a, cudaStream_t st);
 
 }  // namespace attn8

@@ -209,10 +209,9 @@ int check_kv_i8(const char *what, const gcu_kv_i8 *kv, int nseq = 0);
 // tiles, K split) over the cost model of the GEMM launcher.
 int gemm_tmap_i8(CUtensorMap *m, const int8_t *base, int k, int rows, long stride, int box_rows);
 int gemm_tmap_f32(CUtensorMap *m, float *base, int n, int rows, long stride_elems);
-// int8 [heads][rows][hdim] of a KV cache (k_attention_i8_tc.cu): box min(hdim,
-// 128) B x box_rows of one head, swizzled over its inner bytes (64 or 128)
-int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, int hdim, int rows, int heads, long head_stride,
-                       int box_rows);
+// the codes `base` (kv.k or kv.v) of an 8-bit cache, [nseq][nkv][clen][hdim]:
+// box min(hdim, 128) B x box_rows of one head, swizzled over its inner bytes
+int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, const gcu_kv_i8 &kv, int box_rows);
 int gemm_plan_one_cta(int m, int k, const int *n, int njobs, int sms, int *bn, int *mb,
                       int *splits);
 int gemm_split_for(int tiles, int k, int sms);
@@ -375,12 +374,12 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap *m,
       "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
       : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(const CUtensorMap *m, uint64_t *bar, void *dst, int x, int y, int z,
+__device__ __forceinline__ void tma_load_4d(const CUtensorMap *m, uint64_t *bar, void *dst, int x, int y, int z, int w,
                                             uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::"
-      "bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
-      "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "l"(policy)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_u32(dst)),
+      "l"(m), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(policy)
       : "memory");
 }
 // L2 prefetch of one tile through a tensor map (no data reaches the CTA)
@@ -670,6 +669,12 @@ __device__ __forceinline__ uint64_t smem_desc_k128(uint32_t saddr) {
 __device__ __forceinline__ Desc smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo, int swizzle) {
   return Desc{((saddr >> 4) & 0x3FFF) | ((lbo >> 4) & 0x3FFF) << 16,
               ((sbo >> 4) & 0x3FFF) | 1u << 14 | (swizzle == 128 ? 2u : 4u) << 29};
+}
+
+// Instruction descriptor, kind::i8: D = s32, A = signed, B = unsigned int8, both
+// MN-major, shape M x N.
+__host__ __device__ constexpr uint32_t idesc_i8u_mn(int M, int N) {
+  return (2u << 4) | (1u << 7) | (1u << 15) | (1u << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
 // Instruction descriptor, kind::f16: D = fp32, A = B = fp16, A K-major, B

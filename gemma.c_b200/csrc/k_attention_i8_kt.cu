@@ -1,0 +1,528 @@
+// k_attention_i8_kt.cu -- decode attention over the 8-bit KV cache: few query rows
+// per kv head (the heads of one token, or of the tokens of several sequences
+// that share a prefix), many keys.  Bound by HBM: the codes are read once, as
+// they lie, and go from TMA into the tensor cores without a conversion.
+//
+// With few rows the keys take the long side of the products:
+//   S^T  [128 keys x 3R]    = K [128 x hdim] * Q^T, the R rows' three digits side
+//                             by side (kind::i8, exact)
+//   O^T  [hdim x 4R]       += V^T [hdim x 128 keys] * W, the R rows' weights as four
+//                             unsigned digits (kind::i8 with both operands
+//                             MN-major: V's tile as it lies is V^T)
+// Weights are 32-bit fixed point, W = round(2^(s + log2 vs - m)), m placed so that
+// the row's largest weight so far is 2^24 at least and 2^31.5 at most; rounding
+// is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 65536
+// keys fits), so nothing is lost however long the range, and only moves to fp32
+// registers when a row's m has to move.
+//
+// Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
+// against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM.
+//
+// Warps 0-7: softmax, thread = (key, half of the rows); 8: products; 9: loads.
+#include "attention_i8.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+namespace gcu {
+namespace attn8 {
+namespace {
+
+constexpr int kSoftmax = 256, kMmaWarp = 8, kLoadWarp = 9, kThreads = 320;
+constexpr int kKeys = kKtKeys;
+constexpr float kTop = 24.0f, kSlack = 7.5f;  // log2 of the weight at m, and how far it may pass
+
+template <int HD, int R>
+struct Cfg {
+  static constexpr int SW = HD == 64 ? 64 : 128;  // bytes of a Q / K / V swizzle row
+  static constexpr int KB = HD / SW;              // blocks of SW bytes
+  static constexpr int NS = 3 * R, NP = 4 * R;    // columns of S^T and of W
+  static constexpr int MB = HD == 256 ? 2 : 1;    // 128-row blocks of O^T (hdim 64: rows 64-127 repeat)
+  static constexpr int Q_BLOCK = NS * SW;
+  static constexpr int Q_BYTES = KB * Q_BLOCK;
+  static constexpr int T_BLOCK = kKeys * SW;
+  static constexpr int T_BYTES = KB * T_BLOCK;  // a K or V tile
+  static constexpr int P_ROW = NP;              // bytes of a key: 64 or 128
+  static constexpr int P_BYTES = kKeys * P_ROW;
+  static constexpr int Q_PAD = (Q_BYTES + 1023) / 1024 * 1024;
+  static constexpr int FIXED = Q_PAD + 2 * P_BYTES + 1024 + 6 * 1024;
+  static constexpr int FIT = (232448 - FIXED) / (2 * T_BYTES);
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;  // of K and of V
+  static constexpr int Q_OFF = 0;
+  static constexpr int P_OFF = Q_PAD;
+  static constexpr int K_OFF = P_OFF + 2 * P_BYTES;
+  static constexpr int V_OFF = K_OFF + STAGES * T_BYTES;
+  static constexpr int SMEM = V_OFF + STAGES * T_BYTES + 1024;
+  static constexpr int S_COL = 0, O_COL = 2 * NS;
+  static constexpr int COLS = O_COL + MB * NP <= 256 ? 256 : 512;
+  static constexpr int RH = R / 2;                  // rows per softmax thread
+  static constexpr int OR = HD == 256 ? R : R / 2;  // output rows per thread (of one column)
+  static_assert(STAGES >= 2 && O_COL + MB * NP <= 512, "budget");
+};
+
+struct alignas(64) KtArgs {
+  CUtensorMap k[2], v[2];
+  Args a[2];
+  int groups[2];  // row groups of each set
+  int first1;     // blocks of set 0
+};
+
+template <int HD, int R, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtArgs p) {
+  using C = Cfg<HD, R>;
+  constexpr int ST = C::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_abort, s_fresh[2], s_range[4], s_lo[R], s_hi[R];
+  __shared__ float s_rf[R], s_m[R], s_f[R], s_red[8][R / 2];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int set = (int)blockIdx.x >= p.first1;
+  const Args &a = p.a[set];
+  const int block = (int)blockIdx.x - (set ? p.first1 : 0);
+  const int split = block % a.splits, group = block / a.splits, hk = blockIdx.y;
+  const int h0 = head0(hk, a.n_heads, a.kv.nkv), G = head0(hk + 1, a.n_heads, a.kv.nkv) - h0;
+  // rows of this CTA: OWN one sequence's group, else R of the (i, g) rows
+  const int first = a.mode == OWN ? group * G : group * R;
+  const int nr = max(0, a.mode == OWN ? G : min(R, a.ni * G - first));
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      ptx::mbar_init(&kfull[s], 1);
+      ptx::mbar_init(&kempty[s], 1);
+      ptx::mbar_init(&vfull[s], 1);
+      ptx::mbar_init(&vempty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&sfull[s], 1);
+      ptx::mbar_init(&sfree[s], kSoftmax);
+      ptx::mbar_init(&pfull[s], kSoftmax);
+      ptx::mbar_init(&pvdone[s], 1);
+    }
+    ptx::mbar_init(&drain, 1);
+    ptx::fence_mbar_init();
+    s_abort = 0;
+    s_range[0] = s_range[3] = 0x7fffffff;
+    s_range[1] = s_range[2] = 0;
+    ptx::prefetch_tmap(&p.k[set]);
+    ptx::prefetch_tmap(&p.v[set]);
+  }
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(&s_tmem, C::COLS);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  // the next kernel may start now: this CTA holds its TMEM
+  ptx::griddep_launch();
+  ptx::griddep_wait();
+
+  // the rows' windows: the CTA's key range, and the keys that every row sees
+  if (a.mode == OWN && a.len && threadIdx.x == 0 && split == 0 && hk == 0 && __ldg(a.len + group) > a.max_len)
+    ptx::record_err(a.err, DEV_BAD_LENGTH);
+  if (threadIdx.x < R) {
+    int lo = 0, hi = 0;
+    if ((int)threadIdx.x < nr) {
+      row_window(a, (first + threadIdx.x) / G, lo, hi);
+      if (lo < hi) {
+        atomicMin(&s_range[0], lo);
+        atomicMax(&s_range[1], hi);
+      }
+      atomicMax(&s_range[2], lo);
+      atomicMin(&s_range[3], hi);
+    }
+    s_lo[threadIdx.x] = lo;
+    s_hi[threadIdx.x] = hi;
+    s_m[threadIdx.x] = -INFINITY;
+  }
+  __syncthreads();
+  const int all_lo = s_range[2], all_hi = s_range[3];
+  const long c0 = (long)s_range[0] + (long)split * a.chunk;
+  const int n = (int)max(0l, min((long)s_range[1], c0 + a.chunk) - c0);
+  const int kbeg = (int)min(c0, 0x7fffffffl), kend = kbeg + n;
+  const int nt = __shfl_sync(0xffffffffu, (n + kKeys - 1) / kKeys, 0);
+  const int seq = a.mode == OWN ? group : 0;
+  Waiter wait{&s_abort, a.err};
+
+  const uint64_t pol = ptx::policy_evict_first();
+  auto load = [&](const CUtensorMap *m, uint64_t *full, int off, int j) {
+    const int st = j % ST;
+    ptx::mbar_arrive_expect_tx(&full[st], C::T_BYTES);
+#pragma unroll
+    for (int b = 0; b < C::KB; ++b)
+      ptx::tma_load_4d(m, &full[st], smem + off + st * C::T_BYTES + b * C::T_BLOCK, b * C::SW, kbeg + j * kKeys, hk, seq,
+                       pol);
+  };
+  if (warp == kLoadWarp && lane == 0)
+    for (int j = 0; j < min(ST, nt); ++j) {
+      load(&p.k[set], kfull, C::K_OFF, j);
+      load(&p.v[set], vfull, C::V_OFF, j);
+    }
+
+  // the query rows' digits, row n = d * R + r; rows past the end are zeros
+  if (nt > 0) {
+    constexpr int E = HD / 32;
+    for (int r = warp; r < R; r += kThreads / 32) {
+      float v[E], amax = 0.0f;
+      const float *src =
+          a.xq + (long)((first + r) / G) * a.q_i + (long)(h0 + (first + r) % G) * a.q_h + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[e] = r < nr ? __ldg(src + e) : 0.0f;
+        amax = max_nan(amax, fabsf(v[e]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      const float inv = amax > 0.0f ? kQMax / amax : 0.0f;
+      uint32_t w[3][(E + 3) / 4] = {};
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        int d2, d1, d0;
+        digits(v[e], inv, d2, d1, d0);
+        w[0][e / 4] |= (uint32_t)(d0 & 0xff) << (8 * (e % 4));
+        w[1][e / 4] |= (uint32_t)(d1 & 0xff) << (8 * (e % 4));
+        w[2][e / 4] |= (uint32_t)(d2 & 0xff) << (8 * (e % 4));
+      }
+      const int col = lane * E, in = col % C::SW;
+#pragma unroll
+      for (int d = 0; d < 3; ++d) {
+        const int row = d * R + r, sw = C::SW == 128 ? row & 7 : (row >> 1) & 3;
+        uint8_t *q = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + row * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint2 *>(q) = make_uint2(w[d][0], w[d][1]);
+        } else if constexpr (E == 4) {
+          *reinterpret_cast<uint32_t *>(q) = w[d][0];
+        } else {
+          *reinterpret_cast<uint16_t *>(q) = (uint16_t)w[d][0];
+        }
+      }
+      if (lane == 0) s_rf[r] = amax / kQMax * a.asc;
+    }
+  }
+  ptx::fence_proxy_async_smem();
+  __syncthreads();
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      int nk = min(ST, nt), nv = nk;  // tiles issued
+      for (int j = nk; j < nt; ++j) {
+        if (!wait(&kempty[j % ST], ((j - ST) / ST) & 1, DEV_TIMEOUT_EMPTY)) break;
+        load(&p.k[set], kfull, C::K_OFF, j);
+        ++nk;
+        if (!wait(&vempty[j % ST], ((j - ST) / ST) & 1, DEV_TIMEOUT_EMPTY)) break;
+        load(&p.v[set], vfull, C::V_OFF, j);
+        ++nv;
+      }
+      // every load issued must have landed before the CTA may exit
+      for (int j = max(0, nk - ST); j < nk; ++j)
+        ptx::mbar_wait(&kfull[j % ST], (j / ST) & 1, a.err, DEV_TIMEOUT_DRAIN);
+      for (int j = max(0, nv - ST); j < nv; ++j)
+        ptx::mbar_wait(&vfull[j % ST], (j / ST) & 1, a.err, DEV_TIMEOUT_DRAIN);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ products
+    if (nt > 0) {
+      constexpr uint32_t id_s = ptx::idesc_i8(128, C::NS), id_o = ptx::idesc_i8u_mn(128, C::NP);
+      const ptx::Desc dq = ptx::smem_desc(ptx::smem_u32(smem + C::Q_OFF), 16, 8 * C::SW, C::SW);
+      const ptx::Desc dk = ptx::smem_desc(ptx::smem_u32(smem + C::K_OFF), 16, 8 * C::SW, C::SW);
+      // V^T: atoms of SW columns x 8 keys; hdim 64 repeats its one atom along M (lbo 0)
+      const ptx::Desc dv = ptx::smem_desc(ptx::smem_u32(smem + C::V_OFF), 0, 8 * C::SW, C::SW);
+      const ptx::Desc dp = ptx::smem_desc(ptx::smem_u32(smem + C::P_OFF), 0, 8 * C::P_ROW, C::P_ROW);
+      auto scores = [&](int j) {
+        if (ptx::elect_one()) {
+          const uint32_t k_lo = dk.lo + (j % ST) * (C::T_BYTES >> 4);
+#pragma unroll
+          for (int b = 0; b < C::KB; ++b)
+#pragma unroll
+            for (int s = 0; s < C::SW / 32; ++s)
+              ptx::mma_i8(tmem + C::S_COL + (j & 1) * C::NS,
+                          ptx::Desc{k_lo + ((b * C::T_BLOCK + 32 * s) >> 4), dk.hi},
+                          ptx::Desc{dq.lo + ((b * C::Q_BLOCK + 32 * s) >> 4), dq.hi}, id_s, b + s > 0 ? 1u : 0u);
+          ptx::mma_commit(&kempty[j % ST]);
+          ptx::mma_commit(&sfull[j & 1]);
+        }
+        __syncwarp();
+      };
+      bool ok = wait(&kfull[0], 0, DEV_TIMEOUT_FULL);
+      if (__any_sync(0xffffffffu, !ok)) ok = false;
+      if (ok) {
+        ptx::tc_fence_after();
+        scores(0);
+      }
+      for (int j = 0; j < nt && ok; ++j) {
+        if (j + 1 < nt) {
+          ok = wait(&kfull[(j + 1) % ST], ((j + 1) / ST) & 1, DEV_TIMEOUT_FULL) &&
+               (j < 1 || wait(&sfree[(j + 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM));
+          if (__any_sync(0xffffffffu, !ok)) break;
+          ptx::tc_fence_after();
+          scores(j + 1);
+        }
+        ok = wait(&vfull[j % ST], (j / ST) & 1, DEV_TIMEOUT_FULL) && wait(&pfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM);
+        const bool fresh = __shfl_sync(0xffffffffu, *(volatile int *)&s_fresh[j & 1], 0);
+        if (__any_sync(0xffffffffu, !ok)) break;
+        ptx::tc_fence_after();
+        if (ptx::elect_one()) {
+          const uint32_t v_lo = dv.lo + (j % ST) * (C::T_BYTES >> 4), p_lo = dp.lo + (j & 1) * (C::P_BYTES >> 4);
+#pragma unroll
+          for (int s = 0; s < kKeys / 32; ++s)
+#pragma unroll
+            for (int b = 0; b < C::MB; ++b)
+              ptx::mma_i8(tmem + C::O_COL + b * C::NP, ptx::Desc{v_lo + ((b * C::T_BLOCK + s * 32 * C::SW) >> 4), dv.hi},
+                          ptx::Desc{p_lo + ((s * 32 * C::P_ROW) >> 4), dp.hi}, id_o, s > 0 || !fresh ? 1u : 0u);
+          ptx::mma_commit(&vempty[j % ST]);
+          ptx::mma_commit(&pvdone[j & 1]);
+        }
+        __syncwarp();
+      }
+      // all products complete before TMEM is freed
+      if (ptx::elect_one()) ptx::mma_commit(&drain);
+      __syncwarp();
+      ptx::mbar_wait(&drain, 0, a.err, DEV_TIMEOUT_DRAIN);
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    constexpr int RH = C::RH;
+    const int half = warp >> 2, key = threadIdx.x & (kKeys - 1), r0 = half * RH;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const float *ksrc = a.kv.ks + seq * a.kv.sc_seq_stride + hk * a.kv.sc_stride;
+    const float *vsrc = a.kv.vs + seq * a.kv.sc_seq_stride + hk * a.kv.sc_stride;
+    auto fetch = [&](const float *src, int j) {
+      const int t = j * kKeys + key;
+      return t < n ? __ldg(src + kbeg + t) : 1.0f;
+    };
+    float rf[RH], l[RH];
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      rf[r] = nt > 0 ? s_rf[r0 + r] : 0.0f;
+      l[r] = 0.0f;
+    }
+    // the output column of this thread: lane of O^T's block (hdim 256: block = half;
+    // else the halves take half of the rows each)
+    const int ocol = (C::MB == 2 ? half * 128 : 0) + (warp & 3) * 32 + lane, orow = C::MB == 2 ? 0 : r0;
+    float acc[C::OR];
+#pragma unroll
+    for (int r = 0; r < C::OR; ++r) acc[r] = 0.0f;
+    const uint32_t olane = lanes + C::O_COL + (C::MB == 2 ? half * C::NP : 0) + orow;
+    // add O^T's digit sums (complete) to the column's sums, then scale them
+    auto flush = [&]() {
+      ptx::tc_fence_after();
+#pragma unroll
+      for (int r = 0; r < C::OR; r += 8) {
+        uint32_t d3[8], d2[8], d1[8], d0[8];
+        ptx::tmem_ld_32x8(olane + r, d0);
+        ptx::tmem_ld_32x8(olane + R + r, d1);
+        ptx::tmem_ld_32x8(olane + 2 * R + r, d2);
+        ptx::tmem_ld_32x8(olane + 3 * R + r, d3);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v = (float)(int)d3[e] * 16777216.0f + (float)(int)d2[e] * 65536.0f;
+          v += (float)(int)d1[e] * 256.0f + (float)(int)d0[e];
+          acc[r + e] += v;
+        }
+      }
+      ptx::tc_fence_before();
+    };
+    float ks = fetch(ksrc, 0), vs = fetch(vsrc, 0);
+    bool ok = true;
+    for (int j = 0; j < nt; ++j) {
+      const float ks_next = fetch(ksrc, j + 1), vs_next = fetch(vsrc, j + 1);
+      float lvs, rvs;
+      value_scale(vs, lvs, rvs);
+      ok = wait(&sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      ptx::tc_fence_after();
+      // exponents: the score in log2 units plus log2 of the value row's scale
+      float x[RH];
+#pragma unroll
+      for (int c = 0; c < RH; c += 8) {
+        uint32_t s2[8], s1[8], s0[8];
+        const uint32_t at = lanes + C::S_COL + (j & 1) * C::NS + r0 + c;
+        ptx::tmem_ld_32x8(at, s0);
+        ptx::tmem_ld_32x8(at + R, s1);
+        ptx::tmem_ld_32x8(at + 2 * R, s2);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 y = high_digit(s2 + e, low_digits(s1 + e, s0 + e));
+          float s[2] = {y.x * ks * rf[c + e], y.y * ks * rf[c + e + 1]};
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (CAP) s[q] = tanhf(s[q] / a.sc_att) * a.sc_att;
+            x[c + e + q] = __fmaf_rn(s[q], kLog2e, lvs);
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      ptx::mbar_arrive(&sfree[j & 1]);
+      const int t0 = kbeg + j * kKeys;
+      if (t0 < all_lo || t0 + kKeys > min(all_hi, kend)) {  // a tile that some row does not see in full
+        const int t = t0 + key;
+#pragma unroll
+        for (int r = 0; r < RH; ++r)
+          if (t < s_lo[r0 + r] || t >= min(s_hi[r0 + r], kend)) x[r] = -INFINITY;
+      }
+      bool over = !ok;
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        const float m = s_m[r0 + r];
+        over |= x[r] > m + kSlack || (m == -INFINITY && x[r] > m);
+      }
+      bool fresh = j == 0;
+      if (ptx::named_bar_or(1, kSoftmax, over)) {
+        // some row's weights would run over: move every row's m to its largest
+        // exponent so far, and take O^T's sums at the old one
+        if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
+#pragma unroll
+        for (int r = 0; r < RH; ++r) {
+          float top = x[r];
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          if (lane == 0) s_red[warp][r] = top;
+        }
+        ptx::named_bar_sync(1, kSoftmax);
+        if (threadIdx.x < R) {
+          const int hh = threadIdx.x / RH, r = threadIdx.x % RH;
+          const float m = s_m[threadIdx.x];
+          float to = m;
+          for (int w = 0; w < 4; ++w) to = fmaxf(to, s_red[hh * 4 + w][r]);
+          s_f[threadIdx.x] = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
+          s_m[threadIdx.x] = to;
+        }
+        ptx::named_bar_sync(1, kSoftmax);
+        if (j > 0) {
+          ok = wait(&pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+          if (!fresh) flush();
+        }
+#pragma unroll
+        for (int r = 0; r < C::OR; ++r) acc[r] *= s_f[orow + r];
+#pragma unroll
+        for (int r = 0; r < RH; ++r) l[r] *= s_f[r0 + r];
+        fresh = true;
+      }
+      // this buffer's last reader is the product of tile j - 2
+      if (j > 1) ok = wait(&pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      uint32_t w[RH];
+#pragma unroll
+      for (int r = 0; r < RH; ++r) {
+        const float m = s_m[r0 + r];
+        const float v = ex2(x[r] - (m == -INFINITY ? 0.0f : m - kTop));
+        l[r] = __fmaf_rn(v, rvs, l[r]);
+        w[r] = __float2uint_rn(v);
+      }
+      uint8_t *dst = smem + C::P_OFF + (j & 1) * C::P_BYTES + key * C::P_ROW;
+      const int sw = C::P_ROW == 128 ? key & 7 : (key >> 1) & 3;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) {
+        const int col = d * R + r0;
+        uint32_t b[RH / 4];
+#pragma unroll
+        for (int e = 0; e < RH / 4; ++e) {
+          const uint32_t lo = __byte_perm(w[4 * e], w[4 * e + 1], d | (d + 4) << 4);
+          const uint32_t hi = __byte_perm(w[4 * e + 2], w[4 * e + 3], d | (d + 4) << 4);
+          b[e] = __byte_perm(lo, hi, 0x5410);
+        }
+        uint8_t *q = dst + (((col >> 4) ^ sw) << 4) + (col & 15);
+        if constexpr (RH == 16) {
+          *reinterpret_cast<uint4 *>(q) = make_uint4(b[0], b[1], b[2], b[3]);
+        } else {
+          *reinterpret_cast<uint2 *>(q) = make_uint2(b[0], b[1]);
+        }
+      }
+      if (threadIdx.x == 0) *(volatile int *)&s_fresh[j & 1] = fresh;
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(&pfull[j & 1]);
+      ks = ks_next;
+      vs = vs_next;
+    }
+    // the rows' sums of weights, over the keys' threads
+#pragma unroll
+    for (int r = 0; r < RH; ++r) {
+      float v = l[r];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (lane == 0) s_red[warp][r] = v;
+    }
+    ptx::named_bar_sync(1, kSoftmax);
+    if (nt > 0) {
+      ok = wait(&pvdone[(nt - 1) & 1], ((nt - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      flush();
+    }
+    if (ok && ocol < HD) {
+#pragma unroll
+      for (int r = 0; r < C::OR; ++r) {
+        const int rr = orow + r;
+        if (rr >= nr) break;
+        const int hh = rr / RH, i = (first + rr) / G, h = h0 + (first + rr) % G;
+        const float sum = (s_red[hh * 4][rr % RH] + s_red[hh * 4 + 1][rr % RH]) +
+                          (s_red[hh * 4 + 2][rr % RH] + s_red[hh * 4 + 3][rr % RH]);
+        if (a.slots == 1) {  // a row that sees nothing: zeros
+          if (row_live(a, i)) a.xo[(long)i * a.o_i + (long)h * HD + ocol] = acc[r] / (sum == 0.0f ? 1.0f : sum);
+        } else {
+          const size_t at = ((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h;
+          const float m = s_m[rr];
+          a.part[at * HD + ocol] = acc[r];
+          if (ocol == 0) a.stat[at] = make_float2(m == -INFINITY ? m : m - kTop, sum);
+        }
+      }
+    }
+    ptx::tc_fence_before();
+  }
+  __syncthreads();
+  ptx::tc_fence_after();
+  if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, C::COLS);
+}
+
+template <int HD, int R, bool CAP>
+int launch_kt_r(const Args *sets, int n, cudaStream_t st) {
+  using C = Cfg<HD, R>;
+  KtArgs p;
+  long blocks = 0;
+  for (int s = 0; s < 2; ++s) {
+    const Args &a = sets[s < n ? s : 0];
+    const int G = (a.n_heads + a.kv.nkv - 1) / a.kv.nkv;
+    p.a[s] = a;
+    if (s == 1) p.first1 = (int)(n > 1 ? blocks : 0x7fffffff);
+    if (s >= n) continue;
+    blocks += (a.mode == OWN ? (long)a.ni : ((long)a.ni * G + R - 1) / R) * a.splits;
+    if (blocks > 0x7fffffffL - 1) return set_error("attention_i8: %ld CTAs", blocks);
+    if (gemm_tmap_heads_i8(&p.k[s], a.kv.k, a.kv, kKeys) || gemm_tmap_heads_i8(&p.v[s], a.kv.v, a.kv, kKeys)) return 1;
+  }
+  {
+    // the shared-memory opt-in is per device: once for each device this runs on
+    static std::mutex mu;
+    static unsigned long long done = 0;
+    int dev = 0;
+    GCU_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    if (!(done & (1ull << (dev & 63)))) {
+      GCU_CUDA(cudaFuncSetAttribute(k_kt<HD, R, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+      done |= 1ull << (dev & 63);
+    }
+  }
+  GCU_CUDA(launch_k(k_kt<HD, R, CAP>, dim3((unsigned)blocks, sets[0].kv.nkv), dim3(kThreads), C::SMEM, st, p));
+  return 0;
+}
+
+template <int HD, int R>
+int launch_kt_cap(const Args *sets, int n, cudaStream_t st) {
+  return sets[0].sc_att != 0.0f ? launch_kt_r<HD, R, true>(sets, n, st) : launch_kt_r<HD, R, false>(sets, n, st);
+}
+
+}  // namespace
+
+int launch_kt(const Args *sets, int n, int rows, cudaStream_t st) {
+  const int hd = sets[0].kv.hdim;
+  if (rows == 16)
+    return hd == 256   ? launch_kt_cap<256, 16>(sets, n, st)
+           : hd == 128 ? launch_kt_cap<128, 16>(sets, n, st)
+                       : launch_kt_cap<64, 16>(sets, n, st);
+  return hd == 256   ? launch_kt_cap<256, 32>(sets, n, st)
+         : hd == 128 ? launch_kt_cap<128, 32>(sets, n, st)
+                     : launch_kt_cap<64, 32>(sets, n, st);
+}
+
+}  // namespace attn8
+}  // namespace gcu

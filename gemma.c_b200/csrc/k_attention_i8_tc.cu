@@ -56,9 +56,6 @@ constexpr int kFlush = 4;  // tiles per T
 // Weights run up to 2^kTop at the reference point and may pass it by 2^kSlack:
 // 2^15 stays below fp16's 65504.
 constexpr float kTop = 10.0f, kSlack = 5.0f;
-// Scales of V rows are taken as at least 2^-100 and at most 2^100: their
-// reciprocals and sums stay finite.
-constexpr float kVsMin = 7.888609e-31f, kVsMax = 1.2676506e30f;
 
 template <int HD>
 struct Cfg {
@@ -99,28 +96,6 @@ struct Bars {
   uint64_t kfull[2], kempty[2], v8full[2], v8empty[2], v16full[2], dec[2], sfull[2], pvdone[2], sfree, pfull, tfree, drain;
 };
 
-// Every wait is on the phase after the last one that its waiter knows complete
-// (a parity cannot tell two phases apart): what the two softmax groups take in
-// turn has one barrier per tile parity.
-struct Waiter {
-  volatile int *abort;
-  unsigned int *err;
-  // false once any role of the CTA has given up
-  __device__ __forceinline__ bool operator()(uint64_t *bar, uint32_t parity, unsigned int code) const {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = ptx::globaltimer();
-    while (!*abort) {
-      for (int i = 0; i < 64; ++i)
-        if (ptx::mbar_try_wait(bar, parity)) return true;
-      if (ptx::globaltimer() - t0 > 2000000000ull) {
-        ptx::record_err(err, code);
-        *abort = 1;
-      }
-    }
-    return false;
-  }
-};
-
 // four codes of a word as two fp16 pairs: byte ^ 0x80 into the mantissa of 1024,
 // less 1152; exact
 __device__ __forceinline__ uint2 to_half4(uint32_t w) {
@@ -132,26 +107,12 @@ __device__ __forceinline__ uint2 to_half4(uint32_t w) {
   return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
 }
 
-// 65536 s2 + 256 s1 + s0 in fp32.  |s| < 2^22 goes into the mantissa of 1.5 *
-// 2^23 by an integer addition (a conversion instruction runs at a quarter of
-// the rate); the three offsets leave together in the first step, whose result
-// is 2^31.6 or more: an error of 2^8 at most, where the largest possible
-// product of one query and key element alone is 127 * 8355711 = 2^30.
-__device__ __forceinline__ float2 digit_sum2(const uint32_t *s2, const uint32_t *s1, const uint32_t *s0) {
-  constexpr float offsets = 12582912.0f * 65793.0f;
-  auto in = [](const uint32_t *s) { return make_float2(__uint_as_float(s[0] + 0x4B400000u), __uint_as_float(s[1] + 0x4B400000u)); };
-  const float2 t = __ffma2_rn(in(s2), make_float2(65536.0f, 65536.0f), make_float2(-offsets, -offsets));
-  return __fadd2_rn(in(s0), __ffma2_rn(in(s1), make_float2(256.0f, 256.0f), t));
-}
-
 // thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK]
 __device__ __forceinline__ void put_scale(float *sc, int i, float v) {
   if (i < NK) {
     sc[i] = v;
   } else if (i < 2 * NK) {
-    v = v < kVsMin ? kVsMin : v > kVsMax ? kVsMax : v;
-    sc[i] = log2f(v);                   // NaN makes the weights NaN where the key is seen
-    sc[i + NK] = v == v ? 1.0f / v : 1.0f;  // finite: times the zero weight of a key that is not
+    value_scale(v, sc[i], sc[i + NK]);
   }
 }
 
@@ -230,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     ptx::mbar_arrive_expect_tx(bar, C::K_BYTES);
 #pragma unroll
     for (int b = 0; b < C::KB; ++b)
-      ptx::tma_load_3d(&p.tmK, bar, smem + C::K_OFF + (j & 1) * C::K_BYTES + b * C::K_BLOCK, b * C::SW, kbeg + j * NK, hk,
-                       pol);
+      ptx::tma_load_4d(&p.tmK, bar, smem + C::K_OFF + (j & 1) * C::K_BYTES + b * C::K_BLOCK, b * C::SW, kbeg + j * NK, hk,
+                       0, pol);
   };
   auto load_v = [&](int j, uint64_t pol) {
     const uint32_t bytes = (uint32_t)min(NK, n - j * NK) * HD;
@@ -472,18 +433,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       float x[C::HALF];
 #pragma unroll
       for (int c = 0; c < C::HALF; c += 8) {
-        uint32_t s2[8], s1[8], s0[8];
+        uint32_t s1[8], s0[8];
         const uint32_t at = lanes + C::S_COL + half * C::HALF + c;
         ptx::tmem_ld_32x8(at, s0);
         ptx::tmem_ld_32x8(at + NK, s1);
-        ptx::tmem_ld_32x8(at + 2 * NK, s2);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const float2 u = low_digits(s1 + e, s0 + e);
+          x[c + e] = u.x;
+          x[c + e + 1] = u.y;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < C::HALF; c += 8) {
+        uint32_t s2[8];
+        ptx::tmem_ld_32x8(lanes + C::S_COL + 2 * NK + half * C::HALF + c, s2);
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
           const float4 k = *reinterpret_cast<const float4 *>(ks + c + e);
           const float4 v = *reinterpret_cast<const float4 *>(lvs + c + e);
-          float2 y = __fmul2_rn(digit_sum2(s2 + e, s1 + e, s0 + e), make_float2(k.x, k.y));
-          float2 z = __fmul2_rn(digit_sum2(s2 + e + 2, s1 + e + 2, s0 + e + 2), make_float2(k.z, k.w));
+          float2 y = __fmul2_rn(high_digit(s2 + e, make_float2(x[c + e], x[c + e + 1])), make_float2(k.x, k.y));
+          float2 z = __fmul2_rn(high_digit(s2 + e + 2, make_float2(x[c + e + 2], x[c + e + 3])), make_float2(k.z, k.w));
           if constexpr (CAP) {
             y = make_float2(tanhf(y.x * rf_nat / a.sc_att) * a.sc_att, tanhf(y.y * rf_nat / a.sc_att) * a.sc_att);
             z = make_float2(tanhf(z.x * rf_nat / a.sc_att) * a.sc_att, tanhf(z.y * rf_nat / a.sc_att) * a.sc_att);
@@ -598,7 +570,7 @@ int launch_tc_hd(const Args &a, cudaStream_t st) {
   const int gmax = (a.n_heads + a.kv.nkv - 1) / a.kv.nkv;
   p.tiles = (int)(((long)a.ni * gmax + kRows - 1) / kRows);
   if ((long)p.tiles * a.splits > 0x7fffffffL) return set_error("attention_i8: %d x %d CTAs", p.tiles, a.splits);
-  if (gemm_tmap_heads_i8(&p.tmK, a.kv.k, HD, a.kv.clen, a.kv.nkv, a.kv.kv_stride, NK)) return 1;
+  if (gemm_tmap_heads_i8(&p.tmK, a.kv.k, a.kv, NK)) return 1;
   {
     // the shared-memory opt-in is per device: once for each device this runs on
     static std::mutex mu;

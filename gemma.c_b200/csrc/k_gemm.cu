@@ -1264,21 +1264,22 @@ int gemm_tmap_i8(CUtensorMap *m, const int8_t *base, int k, int rows, long strid
   return make_map_i8(m, base, k, rows, stride, box_rows);
 }
 
-int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, int hdim, int rows, int heads, long head_stride,
-                       int box_rows) {
+int gemm_tmap_heads_i8(CUtensorMap *m, const int8_t *base, const gcu_kv_i8 &kv, int box_rows) {
   if (get_encode()) return 1;
-  const cuuint32_t inner = hdim < 128 ? (cuuint32_t)hdim : 128u;
-  cuuint64_t dims[3] = {(cuuint64_t)hdim, (cuuint64_t)rows, (cuuint64_t)heads};
-  cuuint64_t strides[2] = {(cuuint64_t)hdim, (cuuint64_t)(heads > 1 ? head_stride : (long)rows * hdim)};
-  cuuint32_t box[3] = {inner, (cuuint32_t)box_rows, 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<int8_t *>(base), dims, strides, box, estr,
+  const cuuint32_t inner = kv.hdim < 128 ? (cuuint32_t)kv.hdim : 128u;
+  // a stride along a dimension of one is never taken; it only has to be legal
+  const long head = kv.nkv > 1 ? kv.kv_stride : (long)kv.clen * kv.hdim;
+  const long seq = kv.nseq > 1 ? kv.seq_stride : head * kv.nkv;
+  cuuint64_t dims[4] = {(cuuint64_t)kv.hdim, (cuuint64_t)kv.clen, (cuuint64_t)kv.nkv, (cuuint64_t)kv.nseq};
+  cuuint64_t strides[3] = {(cuuint64_t)kv.hdim, (cuuint64_t)head, (cuuint64_t)seq};
+  cuuint32_t box[4] = {inner, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = g_encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t *>(base), dims, strides, box, estr,
                         CU_TENSOR_MAP_INTERLEAVE_NONE,
                         inner < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
-    return set_error("tensor map (int8 %d heads of %d x %d, stride %ld) failed: %d", heads, rows, hdim, head_stride,
-                     (int)r);
+    return set_error("tensor map (int8 cache %d x %d x %d x %d) failed: %d", kv.nseq, kv.nkv, kv.clen, kv.hdim, (int)r);
   return 0;
 }
 
