@@ -106,18 +106,32 @@ struct DecodePlan {
   int slots() const { return own.splits + pre.splits; }
 };
 
-// One CTA per SM over both sets: the sequences' own ranges first, the prefix
-// takes the SMs they leave (at least half).
+// Splits of the prefix: a CTA costs about kSetup tiles' time before and after its
+// tiles, and CTAs run one per SM, the prefix's first.  Of the splits that give
+// at most one wave of prefix CTAs the one whose last CTA ends first.
+constexpr long kSetup = 3;
+
 DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads, int slide) {
-  const long G = max_group(n_heads, own.nkv), sms = num_sms();
+  const long G = max_group(n_heads, own.nkv), sms = std::max(1, num_sms());
   DecodePlan p;
   p.rows = plen > 0 && own.nseq * G > 16 ? 32 : 16;
   const long units = (long)own.nkv * own.nseq;
   p.own = plan_range(visible(max_len, slide), units, plen > 0 ? sms / 2 : sms, kKtKeys);
   p.pre = Plan{1, 0};
-  if (plen > 0)
-    p.pre = plan_range(visible(plen, slide), (own.nseq * G + p.rows - 1) / p.rows * own.nkv,
-                       std::max(sms / 2, sms - units * p.own.splits), kKtKeys);
+  if (plen > 0) {
+    const long n = visible(plen, slide), tiles = (n + kKtKeys - 1) / kKtKeys;
+    const long pre = (own.nseq * G + p.rows - 1) / p.rows * own.nkv;
+    const long own_ctas = units * p.own.splits, own_time = kSetup + p.own.chunk / kKtKeys;
+    long best = -1, ctas = pre;
+    for (long s = 1; s <= std::max(1l, std::min(tiles, sms / pre)); ++s) {
+      const long time = kSetup + (tiles + s - 1) / s, idle = sms - std::min(sms, s * pre);
+      // own CTAs that fit beside the prefix's, the others after them
+      const long beside = std::min(own_ctas, idle * (time / own_time));
+      const long end = time + (own_ctas - beside + sms - 1) / sms * own_time;
+      if (best < 0 || end < best) best = end, ctas = s * pre;
+    }
+    p.pre = plan_range(n, pre, ctas, kKtKeys);
+  }
   return p;
 }
 

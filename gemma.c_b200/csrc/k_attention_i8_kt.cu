@@ -18,7 +18,7 @@
 // Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
 // against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM.
 //
-// Warps 0-7: softmax, thread = (key, half of the rows); 8: products; 9: loads.
+// Warps 0-15: softmax, thread = (key, a quarter of the rows); 16: products; 17: loads.
 #include "attention_i8.cuh"
 
 #include <algorithm>
@@ -28,7 +28,7 @@ namespace gcu {
 namespace attn8 {
 namespace {
 
-constexpr int kSoftmax = 256, kMmaWarp = 8, kLoadWarp = 9, kThreads = 320;
+constexpr int kSoftmax = 512, kMmaWarp = 16, kLoadWarp = 17, kThreads = 576;
 constexpr int kKeys = kKtKeys;
 constexpr float kTop = 24.0f, kSlack = 7.5f;  // log2 of the weight at m, and how far it may pass
 
@@ -55,8 +55,8 @@ struct Cfg {
   static constexpr int SMEM = V_OFF + STAGES * T_BYTES + 1024;
   static constexpr int S_COL = 0, O_COL = 2 * NS;
   static constexpr int COLS = O_COL + MB * NP <= 256 ? 256 : 512;
-  static constexpr int RH = R / 2;                  // rows per softmax thread
-  static constexpr int OR = HD == 256 ? R : R / 2;  // output rows per thread (of one column)
+  static constexpr int RQ = R / 4;                      // rows per softmax thread
+  static constexpr int OR = HD == 256 ? R / 2 : R / 4;  // output rows per thread (of one column)
   static_assert(STAGES >= 2 && O_COL + MB * NP <= 512, "budget");
 };
 
@@ -74,8 +74,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_fresh[2], s_range[4], s_lo[R], s_hi[R];
-  __shared__ float s_rf[R], s_m[R], s_f[R], s_red[8][R / 2];
+  __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R];
+  __shared__ float s_rf[R], s_m[R], s_f[R], s_red[16][R / 4];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int set = (int)blockIdx.x >= p.first1;
@@ -86,13 +86,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   // rows of this CTA: OWN one sequence's group, else R of the (i, g) rows
   const int first = a.mode == OWN ? group * G : group * R;
   const int nr = max(0, a.mode == OWN ? G : min(R, a.ni * G - first));
-  if (threadIdx.x == 0) {
+  // The loads start before anything else: their warp sets up their barriers.
+  if (warp == kLoadWarp && lane == 0) {
+    ptx::prefetch_tmap(&p.k[set]);
+    ptx::prefetch_tmap(&p.v[set]);
     for (int s = 0; s < ST; ++s) {
       ptx::mbar_init(&kfull[s], 1);
       ptx::mbar_init(&kempty[s], 1);
       ptx::mbar_init(&vfull[s], 1);
       ptx::mbar_init(&vempty[s], 1);
     }
+    ptx::fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&sfull[s], 1);
       ptx::mbar_init(&sfree[s], kSoftmax);
@@ -102,49 +108,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     ptx::mbar_init(&drain, 1);
     ptx::fence_mbar_init();
     s_abort = 0;
-    s_range[0] = s_range[3] = 0x7fffffff;
-    s_range[1] = s_range[2] = 0;
-    ptx::prefetch_tmap(&p.k[set]);
-    ptx::prefetch_tmap(&p.v[set]);
   }
-  if (warp == kMmaWarp) {
-    ptx::tmem_alloc(&s_tmem, C::COLS);
-    ptx::tmem_relinquish();
-  }
-  ptx::tc_fence_before();
-  __syncthreads();
-  ptx::tc_fence_after();
-  const uint32_t tmem = s_tmem;
-  // the next kernel may start now: this CTA holds its TMEM
-  ptx::griddep_launch();
   ptx::griddep_wait();
 
-  // the rows' windows: the CTA's key range, and the keys that every row sees
-  if (a.mode == OWN && a.len && threadIdx.x == 0 && split == 0 && hk == 0 && __ldg(a.len + group) > a.max_len)
-    ptx::record_err(a.err, DEV_BAD_LENGTH);
+  // The rows' windows, lane r of every warp: the CTA's key range, and the keys that
+  // every row sees.
+  int lo = 0, hi = 0;
+  if (lane < nr) row_window(a, (first + lane) / G, lo, hi);
   if (threadIdx.x < R) {
-    int lo = 0, hi = 0;
-    if ((int)threadIdx.x < nr) {
-      row_window(a, (first + threadIdx.x) / G, lo, hi);
-      if (lo < hi) {
-        atomicMin(&s_range[0], lo);
-        atomicMax(&s_range[1], hi);
-      }
-      atomicMax(&s_range[2], lo);
-      atomicMin(&s_range[3], hi);
-    }
     s_lo[threadIdx.x] = lo;
     s_hi[threadIdx.x] = hi;
     s_m[threadIdx.x] = -INFINITY;
   }
-  __syncthreads();
-  const int all_lo = s_range[2], all_hi = s_range[3];
-  const long c0 = (long)s_range[0] + (long)split * a.chunk;
-  const int n = (int)max(0l, min((long)s_range[1], c0 + a.chunk) - c0);
-  const int kbeg = (int)min(c0, 0x7fffffffl), kend = kbeg + n;
-  const int nt = __shfl_sync(0xffffffffu, (n + kKeys - 1) / kKeys, 0);
+  const int any_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : 0x7fffffff);
+  const int any_hi = __reduce_max_sync(0xffffffffu, lo < hi ? hi : 0);
+  const int all_lo = __reduce_max_sync(0xffffffffu, lo);
+  const int all_hi = __reduce_min_sync(0xffffffffu, lane < nr ? hi : 0x7fffffff);
+  const long c0 = (long)any_lo + (long)split * a.chunk;
+  const int n = (int)max(0l, min((long)any_hi, c0 + a.chunk) - c0);
+  const int kbeg = (int)min(c0, 0x7fffffffl), kend = kbeg + n, nt = (n + kKeys - 1) / kKeys;
   const int seq = a.mode == OWN ? group : 0;
   Waiter wait{&s_abort, a.err};
+  if (a.mode == OWN && a.len && threadIdx.x == 0 && split == 0 && hk == 0 && __ldg(a.len + group) > a.max_len)
+    ptx::record_err(a.err, DEV_BAD_LENGTH);
 
   const uint64_t pol = ptx::policy_evict_first();
   auto load = [&](const CUtensorMap *m, uint64_t *full, int off, int j) {
@@ -161,6 +147,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       load(&p.v[set], vfull, C::V_OFF, j);
     }
 
+  if (warp == kMmaWarp) {
+    ptx::tmem_alloc(&s_tmem, C::COLS);
+    ptx::tmem_relinquish();
+  }
   // the query rows' digits, row n = d * R + r; rows past the end are zeros
   if (nt > 0) {
     constexpr int E = HD / 32;
@@ -202,7 +192,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     }
   }
   ptx::fence_proxy_async_smem();
+  ptx::tc_fence_before();
   __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  // the next kernel may start now: this CTA holds its TMEM
+  ptx::griddep_launch();
 
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------ loads
@@ -284,8 +279,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     }
   } else {
     // ------------------------------------------------------------ softmax
-    constexpr int RH = C::RH;
-    const int half = warp >> 2, key = threadIdx.x & (kKeys - 1), r0 = half * RH;
+    constexpr int RQ = C::RQ;
+    const int quarter = warp >> 2, key = threadIdx.x & (kKeys - 1), r0 = quarter * RQ;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const float *ksrc = a.kv.ks + seq * a.kv.sc_seq_stride + hk * a.kv.sc_stride;
     const float *vsrc = a.kv.vs + seq * a.kv.sc_seq_stride + hk * a.kv.sc_stride;
@@ -293,32 +288,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       const int t = j * kKeys + key;
       return t < n ? __ldg(src + kbeg + t) : 1.0f;
     };
-    float rf[RH], l[RH];
+    float rf[RQ], l[RQ];
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
+    for (int r = 0; r < RQ; ++r) {
       rf[r] = nt > 0 ? s_rf[r0 + r] : 0.0f;
       l[r] = 0.0f;
     }
-    // the output column of this thread: lane of O^T's block (hdim 256: block = half;
-    // else the halves take half of the rows each)
-    const int ocol = (C::MB == 2 ? half * 128 : 0) + (warp & 3) * 32 + lane, orow = C::MB == 2 ? 0 : r0;
+    // the output column of this thread, a lane of O^T, and its rows of it (hdim 256:
+    // two blocks of columns, half of the rows each; else a quarter)
+    const int oblock = C::MB == 2 ? quarter & 1 : 0, ocol = oblock * 128 + (warp & 3) * 32 + lane;
+    const int orow = C::MB == 2 ? (quarter >> 1) * C::OR : r0;
     float acc[C::OR];
 #pragma unroll
     for (int r = 0; r < C::OR; ++r) acc[r] = 0.0f;
-    const uint32_t olane = lanes + C::O_COL + (C::MB == 2 ? half * C::NP : 0) + orow;
+    const uint32_t olane = lanes + C::O_COL + oblock * C::NP + orow;
     // add O^T's digit sums (complete) to the column's sums, then scale them
     auto flush = [&]() {
       ptx::tc_fence_after();
 #pragma unroll
-      for (int r = 0; r < C::OR; r += 8) {
-        uint32_t d3[8], d2[8], d1[8], d0[8];
-        ptx::tmem_ld_32x8(olane + r, d0);
-        ptx::tmem_ld_32x8(olane + R + r, d1);
-        ptx::tmem_ld_32x8(olane + 2 * R + r, d2);
-        ptx::tmem_ld_32x8(olane + 3 * R + r, d3);
+      for (int r = 0; r < C::OR; r += 4) {
+        uint32_t d3[4], d2[4], d1[4], d0[4];
+        ptx::tmem_ld_32x4(olane + r, d0);
+        ptx::tmem_ld_32x4(olane + R + r, d1);
+        ptx::tmem_ld_32x4(olane + 2 * R + r, d2);
+        ptx::tmem_ld_32x4(olane + 3 * R + r, d3);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 4; ++e) {
           float v = (float)(int)d3[e] * 16777216.0f + (float)(int)d2[e] * 65536.0f;
           v += (float)(int)d1[e] * 256.0f + (float)(int)d0[e];
           acc[r + e] += v;
@@ -335,17 +331,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       ok = wait(&sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       ptx::tc_fence_after();
       // exponents: the score in log2 units plus log2 of the value row's scale
-      float x[RH];
+      float x[RQ];
 #pragma unroll
-      for (int c = 0; c < RH; c += 8) {
-        uint32_t s2[8], s1[8], s0[8];
+      for (int c = 0; c < RQ; c += 4) {
+        uint32_t s2[4], s1[4], s0[4];
         const uint32_t at = lanes + C::S_COL + (j & 1) * C::NS + r0 + c;
-        ptx::tmem_ld_32x8(at, s0);
-        ptx::tmem_ld_32x8(at + R, s1);
-        ptx::tmem_ld_32x8(at + 2 * R, s2);
+        ptx::tmem_ld_32x4(at, s0);
+        ptx::tmem_ld_32x4(at + R, s1);
+        ptx::tmem_ld_32x4(at + 2 * R, s2);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
+        for (int e = 0; e < 4; e += 2) {
           const float2 y = high_digit(s2 + e, low_digits(s1 + e, s0 + e));
           float s[2] = {y.x * ks * rf[c + e], y.y * ks * rf[c + e + 1]};
 #pragma unroll
@@ -361,12 +357,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       if (t0 < all_lo || t0 + kKeys > min(all_hi, kend)) {  // a tile that some row does not see in full
         const int t = t0 + key;
 #pragma unroll
-        for (int r = 0; r < RH; ++r)
+        for (int r = 0; r < RQ; ++r)
           if (t < s_lo[r0 + r] || t >= min(s_hi[r0 + r], kend)) x[r] = -INFINITY;
       }
       bool over = !ok;
 #pragma unroll
-      for (int r = 0; r < RH; ++r) {
+      for (int r = 0; r < RQ; ++r) {
         const float m = s_m[r0 + r];
         over |= x[r] > m + kSlack || (m == -INFINITY && x[r] > m);
       }
@@ -376,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         // exponent so far, and take O^T's sums at the old one
         if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
 #pragma unroll
-        for (int r = 0; r < RH; ++r) {
+        for (int r = 0; r < RQ; ++r) {
           float top = x[r];
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -384,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         }
         ptx::named_bar_sync(1, kSoftmax);
         if (threadIdx.x < R) {
-          const int hh = threadIdx.x / RH, r = threadIdx.x % RH;
+          const int hh = threadIdx.x / RQ, r = threadIdx.x % RQ;
           const float m = s_m[threadIdx.x];
           float to = m;
           for (int w = 0; w < 4; ++w) to = fmaxf(to, s_red[hh * 4 + w][r]);
@@ -399,14 +395,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
         for (int r = 0; r < C::OR; ++r) acc[r] *= s_f[orow + r];
 #pragma unroll
-        for (int r = 0; r < RH; ++r) l[r] *= s_f[r0 + r];
+        for (int r = 0; r < RQ; ++r) l[r] *= s_f[r0 + r];
         fresh = true;
       }
       // this buffer's last reader is the product of tile j - 2
       if (j > 1) ok = wait(&pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
-      uint32_t w[RH];
+      uint32_t w[RQ];
 #pragma unroll
-      for (int r = 0; r < RH; ++r) {
+      for (int r = 0; r < RQ; ++r) {
         const float m = s_m[r0 + r];
         const float v = ex2(x[r] - (m == -INFINITY ? 0.0f : m - kTop));
         l[r] = __fmaf_rn(v, rvs, l[r]);
@@ -417,18 +413,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
       for (int d = 0; d < 4; ++d) {
         const int col = d * R + r0;
-        uint32_t b[RH / 4];
+        uint32_t b[RQ / 4];
 #pragma unroll
-        for (int e = 0; e < RH / 4; ++e) {
+        for (int e = 0; e < RQ / 4; ++e) {
           const uint32_t lo = __byte_perm(w[4 * e], w[4 * e + 1], d | (d + 4) << 4);
           const uint32_t hi = __byte_perm(w[4 * e + 2], w[4 * e + 3], d | (d + 4) << 4);
           b[e] = __byte_perm(lo, hi, 0x5410);
         }
         uint8_t *q = dst + (((col >> 4) ^ sw) << 4) + (col & 15);
-        if constexpr (RH == 16) {
-          *reinterpret_cast<uint4 *>(q) = make_uint4(b[0], b[1], b[2], b[3]);
-        } else {
+        if constexpr (RQ == 8) {
           *reinterpret_cast<uint2 *>(q) = make_uint2(b[0], b[1]);
+        } else {
+          *reinterpret_cast<uint32_t *>(q) = b[0];
         }
       }
       if (threadIdx.x == 0) *(volatile int *)&s_fresh[j & 1] = fresh;
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     }
     // the rows' sums of weights, over the keys' threads
 #pragma unroll
-    for (int r = 0; r < RH; ++r) {
+    for (int r = 0; r < RQ; ++r) {
       float v = l[r];
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -455,9 +451,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       for (int r = 0; r < C::OR; ++r) {
         const int rr = orow + r;
         if (rr >= nr) break;
-        const int hh = rr / RH, i = (first + rr) / G, h = h0 + (first + rr) % G;
-        const float sum = (s_red[hh * 4][rr % RH] + s_red[hh * 4 + 1][rr % RH]) +
-                          (s_red[hh * 4 + 2][rr % RH] + s_red[hh * 4 + 3][rr % RH]);
+        const int hh = rr / RQ, i = (first + rr) / G, h = h0 + (first + rr) % G;
+        const float sum = (s_red[hh * 4][rr % RQ] + s_red[hh * 4 + 1][rr % RQ]) +
+                          (s_red[hh * 4 + 2][rr % RQ] + s_red[hh * 4 + 3][rr % RQ]);
         if (a.slots == 1) {  // a row that sees nothing: zeros
           if (row_live(a, i)) a.xo[(long)i * a.o_i + (long)h * HD + ocol] = acc[r] / (sum == 0.0f ? 1.0f : sum);
         } else {
