@@ -3,26 +3,30 @@
 //   w_j = exp((x_j - max) / T);  top-k, top-p, min-p;  the first kept index whose
 //   running sum of weights passes u * total.
 //
-// Weights are 64-bit fixed point, round(w * 2^b) with the largest b at which n
-// equal logits' sum fits (45 for 262144 logits): their sums are whole numbers,
-// the same in every order, so the token does not depend on how the row is
-// split.  A weight below 2^-(b + 1) of the largest is zero.
+// Weights are 64-bit fixed point, round(w * 2^b) with the largest b up to 51 at
+// which n equal logits' sum fits (45 for 262144 logits): their sums are whole
+// numbers, the same in every order, so the token does not depend on how the row
+// is split.  A weight below 2^-(b + 1) of the largest is zero.
 //
 // Top-k and top-p both keep the logits down to a cut in the order (value
-// descending, index ascending), so each is one search for a cut (key, index):
-// a histogram over (max - x) / T in steps of 1/64 (counts, and for top-p the
-// weights) finds the step that holds the cut, and the step's few elements are
-// gathered and sorted.  A step with too many elements is split by its float
-// keys until they fit or are all equal, and then the cut is an index.
+// descending, index ascending).  A histogram over (max - x) / T in steps of 1/64
+// (counts, and for top-p the weights) finds the step that holds the cut.  When all
+// that lies above its end is a short list, that list is gathered and sorted, and
+// one CTA ends the search on it; otherwise the step's few elements are gathered
+// and sorted for the cut (key, index), and all CTAs sum what it keeps.  A step with
+// too many elements is split by its float keys until they fit or are all equal,
+// and then the cut is an index.
 //
-// One cluster per row: every CTA scans its contiguous slice (which stays in
-// its L1 after the first pass), the histograms and lists meet in distributed
-// shared memory, and the whole search is one launch with one read of HBM.
-// Latency-bound for a few rows: each pass is a scan of 16 K logits and a
-// cluster barrier.
+// One cluster of eight CTAs per row: every CTA keeps its contiguous slice in shared
+// memory (rows up to 262144; longer ones are read again from L2), histograms and
+// lists meet in distributed shared memory, and the whole search is one launch
+// with one read of HBM.  Bound by latency for a few rows, each pass a scan of 32 K
+// logits and a cluster barrier, and by the 64-bit weights for many.
 #include "gcu_internal.cuh"
 
 #include <cooperative_groups.h>
+
+#include <mutex>
 
 #define GCU_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -31,12 +35,14 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCluster = 16;
+constexpr int kCluster = 8;
 constexpr int kBins = 2048;
 constexpr float kBinsPerNat = 64.0f;
-constexpr int kCap = 1024;  // elements that are sorted
+constexpr int kCap = 1024;                // elements that are sorted
+constexpr int kKeep = 1024;               // logits per warp held in shared memory
+constexpr int kTable = 64;                // entries of the 2^(j/64) table
 
 typedef unsigned long long u64;
 
@@ -63,47 +69,75 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 constexpr uint32_t kNegInf = 0x007fffffu;  // key_of(-inf); keys up to it are never kept
 
 struct Shared {
-  unsigned int count[kBins];
-  unsigned int mass_lo[kBins], mass_hi[kBins];
-  u64 sum_count[kBins];  // rank 0: the row's histograms
+  double table[kTable];
+  unsigned int count[kBins], mass_lo[kBins], mass_hi[kBins];  // of this CTA's slice
+  unsigned int sum_count[kBins];                              // of the row
   u64 sum_mass[kBins];
   u64 list[kCap];  // rank 0: gathered (~key, index), sorted ascending
   u64 weight[kCap];
-  u64 warp_sum[kWarps + 1];
-  u64 cta_sum;
-  unsigned int nlist, kmax, klo, khi;
-  // rank 0's answers
-  int bin;
-  u64 before, nbin;
+  unsigned int order[kCap];
+  u64 warp_sum[kWarps], totals[kCluster];
+  float maxes[kCluster];
+  u64 cta_sum, before;
+  unsigned int nlist, klo, khi;
+  int bin, above, argmax, cut_idx;
   uint32_t cut_key;
-  int cut_idx;
-  int argmax;
+  u64 need;
+  float values[kWarps * kKeep];
 };
 
-struct Row {
-  const float *x;
-  int w0, w1;  // this warp's contiguous elements
-  float max;
-  bool inf;  // the largest logit is +inf
-  double inv_t, one;
-  float inv_tf;
+// 2^t * one, rounded to a whole number, for t <= 0: table-driven (Tang's method): t
+// = k/64 + r, 2^(j/64) from the table, 2^r by its Taylor series to r^5 (|r| <=
+// 1/128: the rest is below 2^-57), and the sum with 2^52 leaves the whole number
+// in the low bits.
+__device__ __forceinline__ u64 fixed_exp2(const double *table, double t, double one) {
+  if (t < -64.0) return 0;
+  constexpr double shift = 6755399441055744.0 / 64.0;  // 1.5 * 2^52 / 64: rounds to 64ths
+  const double z = t + shift;
+  const int k = __double2loint(z);
+  const double r = t - (z - shift);
+  double p = 1.3333558146428443e-3;  // ln(2)^i / i!, i = 5 .. 1
+  p = fma(p, r, 9.6181291076284772e-3);
+  p = fma(p, r, 5.5504108664821580e-2);
+  p = fma(p, r, 2.4022650695910071e-1);
+  p = fma(p, r, 6.9314718055994531e-1);
+  double w = table[k & (kTable - 1)];
+  w = fma(w * r, p, w);
+  w = __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
+  const double f = fma(w, one, 4503599627370496.0);
+  return (u64)__double_as_longlong(f) & 0xfffffffffffffull;
+}
 
-  // w as a 64-bit float, of the largest
-  __device__ __forceinline__ double weight(float v) const {
-    if (inf) return v == max ? 1.0 : 0.0;
-    return exp(((double)v - (double)max) * inv_t);
+struct Row {
+  const float *x;       // the row
+  const float *held;    // this warp's slice in shared memory, or null
+  const double *table;
+  int w0, w1;           // this warp's contiguous elements
+  float max;
+  bool inf;             // the largest logit is +inf
+  double max_d, scale;  // log2(e) / T
+  double one;
+  float bin_scale;
+
+  __device__ __forceinline__ u64 weight(float v) const {
+    if (inf) return v == max ? (u64)one : 0;
+    return fixed_exp2(table, ((double)v - max_d) * scale, one);
   }
-  __device__ __forceinline__ u64 fixed(float v) const { return __double2ull_rn(weight(v) * one); }
   // steps of 1/64 below the largest; monotone in v
   __device__ __forceinline__ int bin(float v) const {
     if (inf) return v == max ? 0 : kBins - 1;
-    const float t = (max - v) * inv_tf * kBinsPerNat;
+    const float t = (max - v) * bin_scale;
     return t < (float)(kBins - 1) ? (int)t : kBins - 1;
   }
-  // f(index, value) over the warp's elements, 32 consecutive ones at a time
-  // (every lane calls f; index >= w1 for lanes past the end, with -inf)
+  // f(index, value) over the warp's elements, 32 consecutive ones at a time (every
+  // lane calls f; index >= w1 for lanes past the end, with -inf); NaN as -inf, -0
+  // as +0
   template <typename F>
   __device__ __forceinline__ void each(int lane, F f) const {
+    if (held) {
+      for (int i = lane; i - lane < w1 - w0; i += 32) f(w0 + i, held[i]);
+      return;
+    }
     for (int b = w0; b < w1; b += 128) {
       float v[4];
 #pragma unroll
@@ -113,7 +147,7 @@ struct Row {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (b + 32 * j < w1) f(b + 32 * j + lane, v[j]);
+        if (b + 32 * j < w1) f(b + 32 * j + lane, v[j] == v[j] ? v[j] + 0.0f : -INFINITY);
     }
   }
 };
@@ -126,232 +160,310 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {  // inclusive
   }
   return v;
 }
-
-// A cut: kept are the elements with (key > cut.key) or (key == cut.key and
-// index <= cut.idx).
-struct Cut {
-  uint32_t key = kNegInf + 1;
-  int idx = 0x7fffffff;
-  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= idx); }
-};
-
-// exclusive prefix over the warps of each one's `v` (lane 0's), in warp order;
-// the CTA's total in cta_sum
-__device__ __forceinline__ u64 cta_prefix(Shared &s, u64 v, int warp, int lane) {
-  __syncthreads();
-  if (lane == 0) s.warp_sum[warp] = v;
-  __syncthreads();
-  u64 p = 0, t = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) p += s.warp_sum[w];
-    t += s.warp_sum[w];
-  }
-  if (threadIdx.x == 0) s.cta_sum = t;
-  return p;
-}
-
 __device__ __forceinline__ u64 warp_total(u64 v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// The search for one cut among the elements that `c` keeps: the first element,
-// in (value descending, index ascending) order, at which the running count
-// (MASS false) reaches k, or the running weight (MASS) reaches share of the
-// total.  c is left as it is when the elements never reach it.
-template <bool MASS>
-__device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c, u64 k, double share) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Shared &s0 = *cl.map_shared_rank(&s, 0);
-  const int rank = cl.block_rank();
-  uint32_t klo = 0, khi = 0xffffffffu;  // keys of the current range; level 0: all of them, in linear bins
-  uint32_t step = 0;
-  u64 before = 0;
-  double target = (double)k;
-  for (int level = 0;; ++level) {
-    for (int b = tid; b < kBins; b += kThreads) {
-      s.count[b] = 0;
-      if (MASS) s.mass_lo[b] = s.mass_hi[b] = 0;
-    }
-    __syncthreads();
-    auto bin_of = [&](uint32_t key, float v) { return level == 0 ? r.bin(v) : (int)((khi - key) / step); };
-    auto in_range = [&](uint32_t key) { return key >= klo && key <= khi; };
-    r.each(lane, [&](int i, float v) {
-      const uint32_t key = key_of(v);
-      if (i < r.w1 && c.keeps(key, i) && in_range(key)) {
-        const int b = bin_of(key, v);
-        atomicAdd(&s.count[b], 1u);
-        if (MASS) {
-          const u64 w = r.fixed(v);
-          const unsigned int lo = (unsigned int)w, old = atomicAdd(&s.mass_lo[b], lo);
-          atomicAdd(&s.mass_hi[b], (unsigned int)(w >> 32) + (old + lo < old ? 1u : 0u));
+// exclusive prefix over the warps of each one's `v` (lane 0's), in warp order;
+// the CTA's total in s.cta_sum after the next barrier
+__device__ __forceinline__ u64 cta_prefix(Shared &s, u64 v, int warp, int lane) {
+  __syncthreads();
+  if (lane == 0) s.warp_sum[warp] = v;
+  __syncthreads();
+  const u64 mine = s.warp_sum[lane], incl = warp_scan(mine, lane);
+  if (threadIdx.x == kThreads - 1) s.cta_sum = incl;
+  const u64 p = __shfl_sync(0xffffffffu, incl - mine, warp);
+  __syncthreads();
+  return p;
+}
+// inclusive prefix over the CTA's threads
+__device__ __forceinline__ u64 cta_scan(Shared &s, u64 v, int warp, int lane) {
+  const u64 incl = warp_scan(v, lane);
+  return incl + cta_prefix(s, __shfl_sync(0xffffffffu, incl, 31), warp, lane);
+}
+
+// A cut: kept are the elements with (key > key) or (key == key and index <= idx).
+struct Cut {
+  uint32_t key = kNegInf + 1;
+  int idx = 0x7fffffff;
+  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= idx); }
+};
+
+// ascending bitonic sort of the power-of-two n2 <= 2 * kThreads elements
+template <typename T>
+__device__ void sort(T *a, int n2) {
+  __syncthreads();
+  for (int size = 2; size <= n2; size <<= 1)
+    for (int d = size >> 1; d > 0; d >>= 1) {
+      for (int i = threadIdx.x; i < n2 / 2; i += kThreads) {
+        const int p = 2 * i - (i & (d - 1)), q = p + d;
+        const T x = a[p], y = a[q];
+        if ((x > y) == ((p & size) == 0)) {
+          a[p] = y;
+          a[q] = x;
         }
       }
-    });
-    cl.sync();
-    // each CTA sums a share of the bins over the cluster into rank 0
-    for (int b = rank * (kBins / kCluster) + tid; b < (rank + 1) * (kBins / kCluster); b += kThreads) {
-      u64 n = 0, w = 0;
-      for (int p = 0; p < kCluster; ++p) {
-        const Shared &o = *cl.map_shared_rank(&s, p);
-        n += o.count[b];
-        if (MASS) w += ((u64)o.mass_hi[b] << 32) + o.mass_lo[b];
-      }
-      s0.sum_count[b] = n;
-      s0.sum_mass[b] = w;
-    }
-    cl.sync();
-    if (rank == 0) {
-      // prefix sums over the bins, four per thread, and the bin that holds the cut
-      if (tid == 0) {
-        s.bin = -1;
-        s.nlist = 0;
-        s.klo = 0xffffffffu;
-        s.khi = 0;
-      }
-      u64 v[kBins / kThreads], t = 0;
-#pragma unroll
-      for (int j = 0; j < kBins / kThreads; ++j) {
-        v[j] = MASS ? s.sum_mass[tid * (kBins / kThreads) + j] : s.sum_count[tid * (kBins / kThreads) + j];
-        t += v[j];
-      }
-      const u64 incl = warp_scan(t, lane);
-      const u64 base = cta_prefix(s, __shfl_sync(0xffffffffu, incl, 31), warp, lane);
       __syncthreads();
-      if (MASS && level == 0) target = share * (double)s.cta_sum;
-      u64 run = before + base + incl - t;
-#pragma unroll
-      for (int j = 0; j < kBins / kThreads; ++j) {
-        // the first bin at which the running sum reaches the target; rounding
-        // leaves no bin behind: the sums only grow
-        if (v[j] && (double)run < target && (double)(run + v[j]) >= target) {
-          s.bin = tid * (kBins / kThreads) + j;
-          s.before = run;
-          s.nbin = s.sum_count[s.bin];
-        }
-        run += v[j];
+    }
+}
+__device__ __forceinline__ int pow2_at_least(int v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+__device__ __forceinline__ float list_value(u64 e) { return value_of(~(uint32_t)(e >> 32)); }
+
+// The row's histograms over the elements that are in range and kept, in every
+// CTA's sum_count and (MASS) sum_mass; bin_of maps an element to its bin.
+template <bool MASS, typename B>
+__device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, const Cut &c, uint32_t klo, uint32_t khi,
+                          B bin_of) {
+  const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
+  for (int b = tid; b < kBins; b += kThreads) {
+    s.count[b] = 0;
+    if (MASS) s.mass_lo[b] = s.mass_hi[b] = 0;
+  }
+  __syncthreads();
+  r.each(lane, [&](int i, float v) {
+    const uint32_t key = key_of(v);
+    if (i < r.w1 && c.keeps(key, i) && key >= klo && key <= khi) {
+      const int b = bin_of(key, v);
+      atomicAdd(&s.count[b], 1u);
+      if (MASS) {
+        const u64 w = r.weight(v);
+        const unsigned int lo = (unsigned int)w, old = atomicAdd(&s.mass_lo[b], lo);
+        const unsigned int hi = (unsigned int)(w >> 32) + (old + lo < old ? 1u : 0u);
+        if (hi) atomicAdd(&s.mass_hi[b], hi);
       }
     }
+  });
+  cl.sync();
+  // each CTA sums its share of the bins over the cluster and hands it to all
+  constexpr int kShare = kBins / kCluster;
+  if (tid < kShare) {
+    const int b = rank * kShare + tid;
+    unsigned int n = 0;
+    u64 w = 0;
+#pragma unroll
+    for (int p = 0; p < kCluster; ++p) {
+      const Shared &o = *cl.map_shared_rank(&s, p);
+      n += o.count[b];
+      if (MASS) w += ((u64)o.mass_hi[b] << 32) + o.mass_lo[b];
+    }
+#pragma unroll
+    for (int p = 0; p < kCluster; ++p) {
+      Shared &o = *cl.map_shared_rank(&s, p);
+      o.sum_count[b] = n;
+      if (MASS) o.sum_mass[b] = w;
+    }
+  }
+  cl.sync();
+}
+
+// The first bin at which the running sum (of counts, or MASS of weights), which
+// starts at `before`, reaches the target: s.bin (-1: none), the sum before it
+// (s.before) and how many elements lie in the bins up to it (s.above).  The same
+// in every CTA.
+template <bool MASS>
+__device__ void find_bin(Shared &s, u64 before, double target, int warp, int lane) {
+  constexpr int J = kBins / kThreads;
+  const int tid = threadIdx.x;
+  if (tid == 0) s.bin = -1;
+  u64 v[J], t = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    v[j] = MASS ? s.sum_mass[tid * J + j] : s.sum_count[tid * J + j];
+    t += v[j];
+  }
+  u64 run = before + cta_scan(s, t, warp, lane) - t;
+#pragma unroll
+  for (int j = 0; j < J; ++j) {
+    // sums of whole numbers only grow, also rounded to doubles: one bin at most
+    if (v[j] && (double)run < target && (double)(run + v[j]) >= target) {
+      s.bin = tid * J + j;
+      s.before = run;
+    }
+    run += v[j];
+  }
+  __syncthreads();
+  const int bin = s.bin;
+  u64 n = 0;
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+    if (tid * J + j <= bin) n += s.sum_count[tid * J + j];
+  n = cta_scan(s, n, warp, lane);
+  if (tid == kThreads - 1) s.above = (int)n;
+  __syncthreads();
+}
+
+// elements that pass `in` to rank 0's list (at most kCap of them)
+template <typename P>
+__device__ void gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
+  Shared &s0 = *cl.map_shared_rank(&s, 0);
+  r.each(threadIdx.x & 31, [&](int i, float v) {
+    const uint32_t key = key_of(v);
+    if (i < r.w1 && in(key, i, v)) {
+      const unsigned int at = atomicAdd(&s0.nlist, 1u);
+      if (at < kCap) s0.list[at] = ((u64)~key << 32) | (unsigned int)i;
+    }
+  });
+  cl.sync();
+}
+
+// rank 0: the first element of the sorted list at which the running sum reaches
+// the target; its place in s.cut_idx, or nl when there is none
+template <bool MASS>
+__device__ int cut_list(Shared &s, int nl, u64 before, double target, int warp, int lane) {
+  const int tid = threadIdx.x;
+  if (tid == 0) s.cut_idx = nl;
+  const u64 v = tid >= nl ? 0 : MASS ? s.weight[tid] : 1;
+  const u64 run = before + cta_scan(s, v, warp, lane) - v;
+  if (v && (double)run < target && (double)(run + v) >= target) s.cut_idx = tid;
+  __syncthreads();
+  return s.cut_idx;
+}
+
+// rank 0: sorts its list of nl elements and fills in their weights
+__device__ void sort_list(Shared &s, const Row &r, int nl) {
+  const int tid = threadIdx.x, n2 = pow2_at_least(nl);
+  if (tid >= nl && tid < n2) s.list[tid] = ~0ull;
+  sort(s.list, n2);
+  if (tid < nl) s.weight[tid] = r.weight(list_value(s.list[tid]));
+  __syncthreads();
+}
+
+// The search for one cut among the elements that `c` keeps, whatever its size.
+// Starts from find_bin's answer over the linear bins.  c is left as it is when the
+// elements never reach the target.
+template <bool MASS>
+__device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c, double target) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank();
+  Shared &s0 = *cl.map_shared_rank(&s, 0);
+  uint32_t klo = 0, khi = 0xffffffffu, step = 0;  // level 0: linear bins; then keys
+  for (int level = 0; s.bin >= 0; ++level) {
+    const int bin = s.bin;
+    const u64 before = s.before;
+    auto here = [&](uint32_t key, int i, float v) {
+      return c.keeps(key, i) && key >= klo && key <= khi &&
+             (level == 0 ? r.bin(v) : (int)((khi - key) / step)) == bin;
+    };
+    const unsigned int nbin = s.sum_count[bin];
+    if (tid == 0) {
+      s.nlist = 0;
+      s.klo = 0xffffffffu;
+      s.khi = 0;
+    }
     cl.sync();
-    const int bin = s0.bin;
-    if (bin < 0) {
-      cl.sync();  // rank 0's answer has been read by all
+    if (nbin <= kCap) {
+      gather(cl, s, r, here);
+      if (rank == 0) {
+        sort_list(s, r, (int)nbin);
+        const int at = cut_list<MASS>(s, (int)nbin, before, target, warp, lane);
+        __syncthreads();
+        if (tid < kCluster) {
+          Shared &o = *cl.map_shared_rank(&s, tid);
+          o.cut_key = ~(uint32_t)(s.list[at] >> 32);
+          o.need = (u64)(uint32_t)s.list[at];
+        }
+      }
+      cl.sync();
+      c.key = s.cut_key;
+      c.idx = (int)s.need;
       return;
     }
-    before = s0.before;
-    const u64 nbin = s0.nbin;
-    const bool fits = nbin <= kCap;
-    // gather the bin's elements, or find its key range
+    // the bin's range of keys
     unsigned int lo = 0xffffffffu, hi = 0;
     r.each(lane, [&](int i, float v) {
       const uint32_t key = key_of(v);
-      if (i < r.w1 && c.keeps(key, i) && in_range(key) && bin_of(key, v) == bin) {
-        if (fits) {
-          const unsigned int at = atomicAdd(&s0.nlist, 1u);
-          if (at < kCap) s0.list[at] = ((u64)~key << 32) | (unsigned int)i;
-        } else {
-          lo = min(lo, key);
-          hi = max(hi, key);
-        }
+      if (i < r.w1 && here(key, i, v)) {
+        lo = min(lo, key);
+        hi = max(hi, key);
       }
     });
-    if (!fits) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      }
-      if (lane == 0) {
-        atomicMin(&s0.klo, lo);
-        atomicMax(&s0.khi, hi);
-      }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) {
+      atomicMin(&s0.klo, lo);
+      atomicMax(&s0.khi, hi);
     }
     cl.sync();
-    if (fits) {
-      if (rank == 0) {
-        const int nl = (int)nbin;
-        int n2 = 1;
-        while (n2 < nl) n2 <<= 1;
-        for (int i = nl + tid; i < n2; i += kThreads) s.list[i] = ~0ull;
-        __syncthreads();
-        for (int size = 2; size <= n2; size <<= 1)
-          for (int d = size >> 1; d > 0; d >>= 1) {
-            for (int i = tid; i < n2 / 2; i += kThreads) {
-              const int p = 2 * i - (i & (d - 1)), q = p + d;
-              const u64 x = s.list[p], y = s.list[q];
-              if ((x > y) == ((p & size) == 0)) {
-                s.list[p] = y;
-                s.list[q] = x;
-              }
-            }
-            __syncthreads();
-          }
-        constexpr int J = kCap / kThreads;
-        u64 v[J], t = 0;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int i = tid * J + j;
-          v[j] = i >= nl ? 0 : MASS ? r.fixed(value_of(~(uint32_t)(s.list[i] >> 32))) : 1;
-          t += v[j];
-        }
-        const u64 incl = warp_scan(t, lane);
-        u64 run = before + cta_prefix(s, __shfl_sync(0xffffffffu, incl, 31), warp, lane) + incl - t;
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          if (v[j] && (double)run < target && (double)(run + v[j]) >= target) {
-            s.cut_key = ~(uint32_t)(s.list[tid * J + j] >> 32);
-            s.cut_idx = (int)(uint32_t)s.list[tid * J + j];
-          }
-          run += v[j];
-        }
-      }
-      cl.sync();
-      c.key = s0.cut_key;
-      c.idx = s0.cut_idx;
-      cl.sync();
-      return;
-    }
     klo = s0.klo;
     khi = s0.khi;
     if (klo == khi) {
       // all equal: the cut is the index of one of them, counted in index order
-      if (rank == 0 && tid == 0) {
-        u64 need;
-        if (MASS) {
-          const u64 w = r.fixed(value_of(klo));
-          need = (u64)((target - (double)before) / (double)w);
-          while (need && (double)(before + need * w) >= target) --need;
-          while ((double)(before + need * w) < target) ++need;
-        } else {
-          need = k - before;
-        }
-        s.nbin = need;
-        s.cut_idx = 0x7fffffff;
+      u64 need;
+      if (MASS) {
+        const u64 w = r.weight(value_of(klo));
+        need = (u64)((target - (double)before) / (double)w);
+        while (need && (double)(before + need * w) >= target) --need;
+        while ((double)(before + need * w) < target) ++need;
+      } else {
+        need = (u64)target - before;
       }
       u64 mine = 0;
       r.each(lane, [&](int i, float v) { mine += i < r.w1 && c.keeps(key_of(v), i) && key_of(v) == klo; });
       mine = warp_total(mine);
       u64 p = cta_prefix(s, mine, warp, lane);
+      if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
       cl.sync();
-      const u64 need = s0.nbin;
-      for (int q = 0; q < rank; ++q) p += cl.map_shared_rank(&s, q)->cta_sum;
+      for (int q = 0; q < rank; ++q) p += s.totals[q];
       if (p < need && need <= p + mine) {  // this warp holds it
         r.each(lane, [&](int i, float v) {
           const bool hit = i < r.w1 && c.keeps(key_of(v), i) && key_of(v) == klo;
           const unsigned int b = __ballot_sync(0xffffffffu, hit);
-          if (hit && p + __popc(b & ((2u << lane) - 1)) == need) s0.cut_idx = i;
+          if (hit && p + __popc(b & ((2u << lane) - 1)) == need)
+            for (int q = 0; q < kCluster; ++q) cl.map_shared_rank(&s, q)->cut_idx = i;
           p += __popc(b);
         });
       }
       cl.sync();
       c.key = klo;
-      c.idx = s0.cut_idx;
-      cl.sync();
+      c.idx = s.cut_idx;
       return;
     }
     step = (khi - klo) / kBins + 1;
-    cl.sync();  // rank 0's range has been read by all
+    histogram<MASS>(cl, s, r, c, klo, khi, [&](uint32_t key, float) { return (int)((khi - key) / step); });
+    find_bin<MASS>(s, before, target, warp, lane);
+  }
+}
+
+// rank 0: the whole choice on its sorted list of nl elements, which holds all that
+// may be kept; all_mass: the sum that top-p's share is of (0: what top-k keeps)
+__device__ void choose_from_list(Shared &s, const SampleArgs &a, const Row &r, int row, int nl, u64 all_mass) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  sort_list(s, r, nl);
+  if (a.top_k > 0) nl = min(nl, a.top_k);
+  if (a.top_p < 1.0f) {
+    if (!all_mass) {
+      const u64 t = cta_scan(s, tid < nl ? s.weight[tid] : 0, warp, lane);
+      if (tid == kThreads - 1) s.need = t;
+      __syncthreads();
+      all_mass = s.need;
+    }
+    nl = min(nl, cut_list<true>(s, nl, 0, (double)a.top_p * (double)all_mass, warp, lane) + 1);
+  }
+  // in index order (index, place), what min-p drops without weight
+  const int n2 = pow2_at_least(nl);
+  if (tid < n2) s.order[tid] = tid < nl ? (unsigned int)s.list[tid] << 10 | tid : 0xffffffffu;
+  sort(s.order, n2);
+  u64 w = 0;
+  if (tid < nl) {
+    w = s.weight[s.order[tid] & (kCap - 1)];
+    if ((double)w < (double)a.min_p * r.one) w = 0;
+  }
+  const u64 incl = cta_scan(s, w, warp, lane);
+  if (tid == kThreads - 1) s.need = incl;
+  __syncthreads();
+  const u64 total = s.need;
+  const float uf = __ldg(a.u + row);
+  const double u = uf > 0.0f ? (double)uf : 0.0;  // NaN and below: 0
+  u64 target = (u64)(u * (double)total);
+  if (u >= 1.0 || target >= total) target = total - 1;
+  if (incl > target && incl - w <= target) {
+    a.token[row] = (int)(s.order[tid] >> 10);
+    if (a.prob) a.prob[row] = (float)((double)w / (double)total);
   }
 }
 
@@ -362,72 +474,131 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), row = blockIdx.x / kCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Shared &s0 = *cl.map_shared_rank(&s, 0);
   // contiguous slices of CTAs and warps, in index order, multiples of 32
   const int per_warp = ((a.n + kCluster * kWarps - 1) / (kCluster * kWarps) + 31) & ~31;
   Row r;
   r.x = a.logits + (long)row * a.ld;
   r.w0 = min(a.n, (rank * kWarps + warp) * per_warp);
   r.w1 = min(a.n, r.w0 + per_warp);
-  if (tid == 0) {
-    s.kmax = 0;
-    s.argmax = 0x7fffffff;
-    s.cut_idx = -1;
-  }
+  r.held = nullptr;
+  r.table = s.table;
+  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid == 0) s.nlist = 0;
   ptx::griddep_wait();
+  float top = -INFINITY;
+  if (per_warp <= kKeep) {
+    float *hold = s.values + warp * kKeep;
+    for (int b = lane; b - lane < r.w1 - r.w0; b += 256) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = r.w0 + b + 32 * j;
+        v[j] = i < r.w1 ? __ldg(r.x + i) : -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] = v[j] == v[j] ? v[j] + 0.0f : -INFINITY;
+        top = fmaxf(top, v[j]);
+        if (b + 32 * j < kKeep) hold[b + 32 * j] = v[j];
+      }
+    }
+    __syncwarp();
+    r.held = hold;
+  } else {
+    r.each(lane, [&](int, float v) { top = fmaxf(top, v); });
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  float *warp_max = reinterpret_cast<float *>(s.warp_sum);
+  if (lane == 0) warp_max[warp] = top;
+  __syncthreads();
+  top = warp_max[lane];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (tid < kCluster) cl.map_shared_rank(&s, tid)->maxes[rank] = top;
   cl.sync();
-  uint32_t km = 0;
-  r.each(lane, [&](int, float v) { km = max(km, key_of(v)); });
-  km = __reduce_max_sync(0xffffffffu, km);
-  if (lane == 0) atomicMax(&s0.kmax, km);
-  cl.sync();
-  const uint32_t kmax = s0.kmax;
-  if (kmax <= kNegInf) {  // nothing to choose from
+  r.max = s.maxes[0];
+  for (int p = 1; p < kCluster; ++p) r.max = fmaxf(r.max, s.maxes[p]);
+  if (r.max == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
       a.token[row] = -1;
       if (a.prob) a.prob[row] = 0.0f;
     }
-    cl.sync();
     return;
   }
-  r.max = value_of(kmax);
-  r.inf = r.max == INFINITY;
   if (a.temperature == 0.0f) {
+    // the first CTA whose slice has the largest logit knows that it is the first
+    bool mine = s.maxes[rank] == r.max;
+    for (int p = 0; p < rank; ++p) mine &= s.maxes[p] != r.max;
+    if (!mine) return;
     int at = 0x7fffffff;
     r.each(lane, [&](int i, float v) {
-      if (i < r.w1 && key_of(v) == kmax) at = min(at, i);
+      if (i < r.w1 && v == r.max) at = min(at, i);
     });
     at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == 0) atomicMin(&s0.argmax, at);
-    cl.sync();
-    if (rank == 0 && tid == 0) {
-      a.token[row] = s.argmax;
+    __syncthreads();
+    int *warp_at = reinterpret_cast<int *>(s.warp_sum);
+    if (lane == 0) warp_at[warp] = at;
+    __syncthreads();
+    at = __reduce_min_sync(0xffffffffu, warp_at[lane]);
+    if (tid == 0) {
+      a.token[row] = at;
       if (a.prob) a.prob[row] = 1.0f;
     }
     return;
   }
+  r.inf = r.max == INFINITY;
+  r.max_d = (double)r.max;
+  r.scale = 1.4426950408889634 / (double)a.temperature;
+  r.bin_scale = kBinsPerNat / a.temperature;
   r.one = a.one;
-  r.inv_t = 1.0 / (double)a.temperature;
-  r.inv_tf = 1.0f / a.temperature;
   Cut c;
-  if (a.top_k > 0 && a.top_k < a.n) find_cut<false>(cl, s, r, c, (u64)a.top_k, 0.0);
-  if (a.top_p < 1.0f) find_cut<true>(cl, s, r, c, 0, (double)a.top_p);
-  const double min_p = (double)a.min_p;
+  const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
+  auto linear = [&](uint32_t, float v) { return r.bin(v); };
+  if (by_k) {
+    histogram<false>(cl, s, r, c, 0, 0xffffffffu, linear);
+    find_bin<false>(s, 0, (double)a.top_k, warp, lane);
+    const int bin = s.bin;
+    if (bin >= 0 && s.above <= kCap) {
+      const int nl = s.above;
+      gather(cl, s, r, [&](uint32_t key, int i, float v) { return key > kNegInf && r.bin(v) <= bin; });
+      if (rank == 0) choose_from_list(s, a, r, row, nl, 0);
+      return;
+    }
+    find_cut<false>(cl, s, r, c, (double)a.top_k);
+  }
+  if (by_p) {
+    histogram<true>(cl, s, r, c, 0, 0xffffffffu, linear);
+    u64 all = s.sum_mass[tid * 2] + s.sum_mass[tid * 2 + 1];
+    all = cta_scan(s, all, warp, lane);
+    all = s.cta_sum;
+    const double target = (double)a.top_p * (double)all;
+    find_bin<true>(s, 0, target, warp, lane);
+    const int bin = s.bin;
+    if (!by_k && bin >= 0 && s.above <= kCap) {
+      const int nl = s.above;
+      gather(cl, s, r, [&](uint32_t key, int i, float v) { return key > kNegInf && r.bin(v) <= bin; });
+      if (rank == 0) choose_from_list(s, a, r, row, nl, all);
+      return;
+    }
+    find_cut<true>(cl, s, r, c, target);
+  }
+  const double least = (double)a.min_p * r.one;
   auto kept = [&](int i, float v) -> u64 {
     if (i >= r.w1 || !c.keeps(key_of(v), i)) return 0;
-    const double w = r.weight(v);
-    return w >= min_p ? __double2ull_rn(w * r.one) : 0;
+    const u64 w = r.weight(v);
+    return (double)w >= least ? w : 0;
   };
   u64 mine = 0;
   r.each(lane, [&](int i, float v) { mine += kept(i, v); });
   mine = warp_total(mine);
   u64 p = cta_prefix(s, mine, warp, lane);
+  if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
   cl.sync();
   u64 total = 0;
   for (int q = 0; q < kCluster; ++q) {
-    const u64 t = cl.map_shared_rank(&s, q)->cta_sum;
-    if (q < rank) p += t;
-    total += t;
+    if (q < rank) p += s.totals[q];
+    total += s.totals[q];
   }
   const float uf = __ldg(a.u + row);
   const double u = uf > 0.0f ? (double)uf : 0.0;  // NaN and below: 0
@@ -435,6 +606,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   if (u >= 1.0 || target >= total) target = total - 1;
   if (p <= target && target < p + mine) {  // this warp holds the token
     r.each(lane, [&](int i, float v) {
+      if (p > target) return;  // found (the same in every lane)
       const u64 w = kept(i, v), incl = warp_scan(w, lane);
       const u64 run = p + incl;
       if (run > target && run - w <= target) {
@@ -444,7 +616,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
       p += __shfl_sync(0xffffffffu, incl, 31);
     });
   }
-  cl.sync();  // no CTA leaves while another may read its sums
 }
 
 }  // namespace
@@ -466,11 +637,22 @@ GCU_EXPORT int gcu_dev_sample(int *token, float *prob, const float *logits, long
                      temperature, top_k, top_p, min_p);
   // largest weight exponent: (max - x) / T must not leave fp32 as 0 / 0
   if (temperature > 0.0f && temperature < 1e-30f) temperature = 1e-30f;
-  double one = 9223372036854775808.0;  // 2^63
+  double one = 9223372036854775808.0;  // 2^63, halved until nvocab of them fit
   for (long n = 1; n < nvocab; n <<= 1) one *= 0.5;
+  one = one > 2251799813685248.0 ? 2251799813685248.0 : one;  // and 2^51 at most, a whole number of a double
   SampleArgs a{token, prob, logits, ld, u, temperature, top_p, min_p, top_k, m, nvocab, one};
-  GCU_CUDA(cudaFuncSetAttribute(k_sample, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  GCU_CUDA(cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+  {
+    // the shared-memory opt-in is per device: once for each device this runs on
+    static std::mutex mu;
+    static unsigned long long done = 0;
+    int dev = 0;
+    GCU_CUDA(cudaGetDevice(&dev));
+    std::lock_guard<std::mutex> lk(mu);
+    if (!(done & (1ull << (dev & 63)))) {
+      GCU_CUDA(cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+      done |= 1ull << (dev & 63);
+    }
+  }
   GCU_CUDA(launch_k(k_sample, dim3((unsigned)m * kCluster), dim3(kThreads), sizeof(Shared),
                     static_cast<cudaStream_t>(stream), a));
   return 0;

@@ -438,7 +438,7 @@ int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gc
  * -1 and prob 0.  +inf logits share all the weight.  token [m]; prob [m] (may
  * be NULL): the token's share of the kept weights.  Weights and sums are
  * held in 64 bits, fixed point: a weight is rounded to a multiple of
- * 2^-(63 - log2 nvocab) of the largest.  nvocab <= 2^20. */
+ * 2^-min(51, 63 - log2 nvocab) of the largest.  nvocab <= 2^20. */
 int gcu_dev_sample(int *token, float *prob, const float *logits, long ld, const float *u, float temperature,
                    int top_k, float top_p, float min_p, int m, int nvocab, void *stream);
 
