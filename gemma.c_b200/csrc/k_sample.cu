@@ -9,7 +9,7 @@
 // is split.  A weight below 2^-(b + 1) of the largest is zero.
 //
 // Top-k and top-p both keep the logits down to a cut in the order (value
-// descending, index ascending).  A histogram over (max - x) / T in steps of 1/64
+// descending, index ascending).  A histogram over (max - x) / T in steps of 1/128
 // (counts, and for top-p the weights) finds the step that holds the cut.  When all
 // that lies above its end is a short list, that list is gathered and sorted, and
 // one CTA ends the search on it; otherwise the step's few elements are gathered
@@ -39,10 +39,10 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
 constexpr int kBins = 2048;
-constexpr float kBinsPerNat = 64.0f;
+constexpr float kBinsPerNat = 128.0f;
 constexpr int kCap = 1024;                // elements that are sorted
 constexpr int kKeep = 1024;               // logits per warp held in shared memory
-constexpr int kTable = 64;                // entries of the 2^(j/64) table
+constexpr int kTable = 32;                // entries of the 2^(j/32) table, one per lane
 
 typedef unsigned long long u64;
 
@@ -66,89 +66,95 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
-constexpr uint32_t kNegInf = 0x007fffffu;  // key_of(-inf); keys up to it are never kept
 
 struct Shared {
-  double table[kTable];
-  unsigned int count[kBins], mass_lo[kBins], mass_hi[kBins];  // of this CTA's slice
-  unsigned int sum_count[kBins];                              // of the row
-  u64 sum_mass[kBins];
-  u64 list[kCap];  // rank 0: gathered (~key, index), sorted ascending
+  unsigned int lo[kBins], hi[kBins];  // histogram of this CTA's slice
+  u64 sum[kBins];                     // of the row
+  u64 found[kCap];                    // what this CTA gathers: (~key, index)
+  u64 list[kCap];                     // rank 0: all that is gathered, sorted ascending
   u64 weight[kCap];
   unsigned int order[kCap];
   u64 warp_sum[kWarps], totals[kCluster];
   float maxes[kCluster];
   u64 cta_sum, before;
-  unsigned int nlist, klo, khi;
-  int bin, above, argmax, cut_idx;
+  u64 upto;
+  unsigned int nfound, klo, khi;
+  int bin, cut_idx;
   uint32_t cut_key;
   u64 need;
   float values[kWarps * kKeep];
 };
 
-// 2^t * one, rounded to a whole number, for t <= 0: table-driven (Tang's method): t
-// = k/64 + r, 2^(j/64) from the table, 2^r by its Taylor series to r^5 (|r| <=
-// 1/128: the rest is below 2^-57), and the sum with 2^52 leaves the whole number
-// in the low bits.
-__device__ __forceinline__ u64 fixed_exp2(const double *table, double t, double one) {
-  if (t < -64.0) return 0;
-  constexpr double shift = 6755399441055744.0 / 64.0;  // 1.5 * 2^52 / 64: rounds to 64ths
-  const double z = t + shift;
-  const int k = __double2loint(z);
-  const double r = t - (z - shift);
-  double p = 1.3333558146428443e-3;  // ln(2)^i / i!, i = 5 .. 1
-  p = fma(p, r, 9.6181291076284772e-3);
-  p = fma(p, r, 5.5504108664821580e-2);
-  p = fma(p, r, 2.4022650695910071e-1);
-  p = fma(p, r, 6.9314718055994531e-1);
-  double w = table[k & (kTable - 1)];
-  w = fma(w * r, p, w);
-  w = __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
-  const double f = fma(w, one, 4503599627370496.0);
-  return (u64)__double_as_longlong(f) & 0xfffffffffffffull;
-}
-
 struct Row {
   const float *x;       // the row
   const float *held;    // this warp's slice in shared memory, or null
-  const double *table;
+  double table;         // 2^(lane/32)
   int w0, w1;           // this warp's contiguous elements
   float max;
-  bool inf;             // the largest logit is +inf
-  double max_d, scale;  // log2(e) / T
+  bool inf;             // the largest logit is +inf: those count as 0, all others as -inf
+  double max_d, scale;  // scale: log2(e) / T
+  float least;          // logits below it weigh nothing
   double one;
   float bin_scale;
 
+  // one * 2^((v - max) * log2(e) / T), rounded to a whole number, to 2^-39 of itself;
+  // the whole warp calls it.  t = k/32 + r; 2^r by its Taylor series to r^4 (|r| <=
+  // 1/64: the rest is below 2^-39); 2^(j/32) from the table (Tang's method), which
+  // the lanes hold: two shuffles cost half of a gather from shared memory; the sum
+  // with 2^52 leaves the whole number in the low bits.
   __device__ __forceinline__ u64 weight(float v) const {
-    if (inf) return v == max ? (u64)one : 0;
-    return fixed_exp2(table, ((double)v - max_d) * scale, one);
+    constexpr double shift = 6755399441055744.0 / kTable;  // 1.5 * 2^52 / 32: rounds to 32nds
+    const double t = ((double)v - max_d) * scale, z = t + shift;
+    const int k = __double2loint(z);
+    const double r = t - (z - shift);
+    double p = 9.6181291076284772e-3;  // ln(2)^i / i!, i = 4 .. 1
+    p = fma(p, r, 5.5504108664821580e-2);
+    p = fma(p, r, 2.4022650695910071e-1);
+    p = fma(p, r, 6.9314718055994531e-1);
+    const double w = __shfl_sync(0xffffffffu, table, k & (kTable - 1));
+    // one * 2^n through its exponent (2^42 * 2^-64 stays normal)
+    const double s = __hiloint2double(__double2hiint(one) + ((k >> 5) << 20), __double2loint(one));
+    const u64 f = (u64)__double_as_longlong(fma(fma(w * r, p, w), s, 4503599627370496.0)) & 0xfffffffffffffull;
+    return v < least ? 0 : f;
   }
-  // steps of 1/64 below the largest; monotone in v
+  // steps of 1/128 below the largest; monotone in v
   __device__ __forceinline__ int bin(float v) const {
-    if (inf) return v == max ? 0 : kBins - 1;
-    const float t = (max - v) * bin_scale;
-    return t < (float)(kBins - 1) ? (int)t : kBins - 1;
+    return min((int)((max - v) * bin_scale), kBins - 1);
   }
-  // f(index, value) over the warp's elements, 32 consecutive ones at a time (every
-  // lane calls f; index >= w1 for lanes past the end, with -inf); NaN as -inf, -0
-  // as +0
+  // a logit as it counts: NaN as -inf, -0 as +0
+  __device__ __forceinline__ float counted(float v) const {
+    if (inf) return v == INFINITY ? 0.0f : -INFINITY;
+    return v == v ? v + 0.0f : -INFINITY;
+  }
+  // The warp's elements, 4 x 32 consecutive ones at a time, lane l's j-th at index +
+  // 32 j + l: f(index, values), every lane; past the end -inf.  Four at a time so
+  // that their arithmetic overlaps.
   template <typename F>
-  __device__ __forceinline__ void each(int lane, F f) const {
-    if (held) {
-      for (int i = lane; i - lane < w1 - w0; i += 32) f(w0 + i, held[i]);
-      return;
-    }
+  __device__ __forceinline__ void each4(int lane, F f) const {
     for (int b = w0; b < w1; b += 128) {
       float v[4];
+      if (held) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int i = b + 32 * j + lane;
-        v[j] = i < w1 ? __ldg(x + i) : -INFINITY;
+        for (int j = 0; j < 4; ++j) v[j] = held[b - w0 + 32 * j + lane];
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int i = b + 32 * j + lane;
+          v[j] = i < w1 ? __ldg(x + i) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = counted(v[j]);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (b + 32 * j < w1) f(b + 32 * j + lane, v[j] == v[j] ? v[j] + 0.0f : -INFINITY);
+      f(b + lane, v);
     }
+  }
+  // f(index, value), one at a time
+  template <typename F>
+  __device__ __forceinline__ void each(int lane, F f) const {
+    each4(lane, [&](int i, const float (&v)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + 32 * j, v[j]);
+    });
   }
 };
 
@@ -184,29 +190,38 @@ __device__ __forceinline__ u64 cta_scan(Shared &s, u64 v, int warp, int lane) {
   return incl + cta_prefix(s, __shfl_sync(0xffffffffu, incl, 31), warp, lane);
 }
 
-// A cut: kept are the elements with (key > key) or (key == key and index <= idx).
+// A cut: kept are the elements with (v > value) or (v == value and index <= idx); at
+// first all but -inf.
 struct Cut {
-  uint32_t key = kNegInf + 1;
-  int idx = 0x7fffffff;
-  __device__ __forceinline__ bool keeps(uint32_t k, int i) const { return k > key || (k == key && i <= idx); }
+  float value = -INFINITY;
+  int idx = -1;
+  __device__ __forceinline__ bool keeps(float v, int i) const { return v > value || (v == value && i <= idx); }
 };
 
-// ascending bitonic sort of the power-of-two n2 <= 2 * kThreads elements
+// ascending bitonic sort of the power-of-two n2 <= kThreads elements, one per
+// thread; partners within a warp by shuffles
 template <typename T>
 __device__ void sort(T *a, int n2) {
+  const int tid = threadIdx.x;
   __syncthreads();
+  T x = tid < n2 ? a[tid] : T(0);
   for (int size = 2; size <= n2; size <<= 1)
     for (int d = size >> 1; d > 0; d >>= 1) {
-      for (int i = threadIdx.x; i < n2 / 2; i += kThreads) {
-        const int p = 2 * i - (i & (d - 1)), q = p + d;
-        const T x = a[p], y = a[q];
-        if ((x > y) == ((p & size) == 0)) {
-          a[p] = y;
-          a[q] = x;
-        }
+      T y;
+      if (d >= 32) {
+        __syncthreads();
+        if (tid < n2) a[tid] = x;
+        __syncthreads();
+        y = tid < n2 ? a[tid ^ d] : T(0);
+      } else {
+        y = __shfl_xor_sync(0xffffffffu, x, d);
       }
-      __syncthreads();
+      // the lower of a pair keeps the smaller in an ascending block
+      if (((tid & d) == 0) == ((tid & size) == 0) ? y < x : y > x) x = y;
     }
+  __syncthreads();
+  if (tid < n2) a[tid] = x;
+  __syncthreads();
 }
 __device__ __forceinline__ int pow2_at_least(int v) {
   int p = 1;
@@ -215,27 +230,28 @@ __device__ __forceinline__ int pow2_at_least(int v) {
 }
 __device__ __forceinline__ float list_value(u64 e) { return value_of(~(uint32_t)(e >> 32)); }
 
-// The row's histograms over the elements that are in range and kept, in every
-// CTA's sum_count and (MASS) sum_mass; bin_of maps an element to its bin.
+// The row's histogram of the elements that bin_of(index, value) gives a bin (not
+// -1), of their number or (MASS) their weights, in every CTA's sum.
 template <bool MASS, typename B>
-__device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, const Cut &c, uint32_t klo, uint32_t khi,
-                          B bin_of) {
+__device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, B bin_of) {
   const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
   for (int b = tid; b < kBins; b += kThreads) {
-    s.count[b] = 0;
-    if (MASS) s.mass_lo[b] = s.mass_hi[b] = 0;
+    s.lo[b] = 0;
+    if (MASS) s.hi[b] = 0;
   }
   __syncthreads();
-  r.each(lane, [&](int i, float v) {
-    const uint32_t key = key_of(v);
-    if (i < r.w1 && c.keeps(key, i) && key >= klo && key <= khi) {
-      const int b = bin_of(key, v);
-      atomicAdd(&s.count[b], 1u);
-      if (MASS) {
-        const u64 w = r.weight(v);
-        const unsigned int lo = (unsigned int)w, old = atomicAdd(&s.mass_lo[b], lo);
-        const unsigned int hi = (unsigned int)(w >> 32) + (old + lo < old ? 1u : 0u);
-        if (hi) atomicAdd(&s.mass_hi[b], hi);
+  r.each4(lane, [&](int i, const float (&v)[4]) {
+    u64 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = MASS ? r.weight(v[j]) : 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = bin_of(i + 32 * j, v[j]);
+      if (b < 0 || (MASS && w[j] == 0)) continue;
+      const unsigned int lo = MASS ? (unsigned int)w[j] : 1u, old = atomicAdd(&s.lo[b], lo);
+      if (MASS) {  // 64-bit additions in shared memory are a compare-and-swap loop: two of 32 bits
+        const unsigned int hi = (unsigned int)(w[j] >> 32) + (old + lo < old ? 1u : 0u);
+        if (hi) atomicAdd(&s.hi[b], hi);
       }
     }
   });
@@ -244,29 +260,22 @@ __device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, const 
   constexpr int kShare = kBins / kCluster;
   if (tid < kShare) {
     const int b = rank * kShare + tid;
-    unsigned int n = 0;
-    u64 w = 0;
+    u64 n = 0;
 #pragma unroll
     for (int p = 0; p < kCluster; ++p) {
       const Shared &o = *cl.map_shared_rank(&s, p);
-      n += o.count[b];
-      if (MASS) w += ((u64)o.mass_hi[b] << 32) + o.mass_lo[b];
+      n += o.lo[b];
+      if (MASS) n += (u64)o.hi[b] << 32;
     }
 #pragma unroll
-    for (int p = 0; p < kCluster; ++p) {
-      Shared &o = *cl.map_shared_rank(&s, p);
-      o.sum_count[b] = n;
-      if (MASS) o.sum_mass[b] = w;
-    }
+    for (int p = 0; p < kCluster; ++p) cl.map_shared_rank(&s, p)->sum[b] = n;
   }
   cl.sync();
 }
 
-// The first bin at which the running sum (of counts, or MASS of weights), which
-// starts at `before`, reaches the target: s.bin (-1: none), the sum before it
-// (s.before) and how many elements lie in the bins up to it (s.above).  The same
-// in every CTA.
-template <bool MASS>
+// The first bin of the row's histogram at which the running sum, which starts at
+// `before`, reaches the target: s.bin (-1: none), the sum before it and with it
+// (s.before, s.upto).  The same in every CTA.
 __device__ void find_bin(Shared &s, u64 before, double target, int warp, int lane) {
   constexpr int J = kBins / kThreads;
   const int tid = threadIdx.x;
@@ -274,7 +283,7 @@ __device__ void find_bin(Shared &s, u64 before, double target, int warp, int lan
   u64 v[J], t = 0;
 #pragma unroll
   for (int j = 0; j < J; ++j) {
-    v[j] = MASS ? s.sum_mass[tid * J + j] : s.sum_count[tid * J + j];
+    v[j] = s.sum[tid * J + j];
     t += v[j];
   }
   u64 run = before + cta_scan(s, t, warp, lane) - t;
@@ -284,32 +293,40 @@ __device__ void find_bin(Shared &s, u64 before, double target, int warp, int lan
     if (v[j] && (double)run < target && (double)(run + v[j]) >= target) {
       s.bin = tid * J + j;
       s.before = run;
+      s.upto = run + v[j];
     }
     run += v[j];
   }
   __syncthreads();
-  const int bin = s.bin;
-  u64 n = 0;
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-    if (tid * J + j <= bin) n += s.sum_count[tid * J + j];
-  n = cta_scan(s, n, warp, lane);
-  if (tid == kThreads - 1) s.above = (int)n;
-  __syncthreads();
 }
 
-// elements that pass `in` to rank 0's list (at most kCap of them)
+// Elements that pass `in`, to rank 0's list; their number, in every CTA.  More than
+// kCap: the list is not made.
 template <typename P>
-__device__ void gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
-  Shared &s0 = *cl.map_shared_rank(&s, 0);
-  r.each(threadIdx.x & 31, [&](int i, float v) {
-    const uint32_t key = key_of(v);
-    if (i < r.w1 && in(key, i, v)) {
-      const unsigned int at = atomicAdd(&s0.nlist, 1u);
-      if (at < kCap) s0.list[at] = ((u64)~key << 32) | (unsigned int)i;
-    }
+__device__ int gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
+  const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
+  if (tid == 0) s.nfound = 0;
+  __syncthreads();
+  r.each(lane, [&](int i, float v) {
+    const bool hit = in(i, v);
+    const unsigned int b = __ballot_sync(0xffffffffu, hit);
+    if (!b) return;  // the whole warp
+    unsigned int at = 0;
+    if (lane == 0) at = atomicAdd(&s.nfound, (unsigned int)__popc(b));
+    at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
+    if (hit && at < kCap) s.found[at] = ((u64)~key_of(v) << 32) | (unsigned int)i;
   });
+  __syncthreads();
+  if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.nfound;
   cl.sync();
+  u64 before = 0, all = 0;
+  for (int q = 0; q < kCluster; ++q) {
+    if (q < rank) before += s.totals[q];
+    all += s.totals[q];
+  }
+  if (all <= kCap && tid < (int)s.nfound) cl.map_shared_rank(&s, 0)->list[before + tid] = s.found[tid];
+  cl.sync();
+  return all <= kCap ? (int)all : kCap + 1;
 }
 
 // rank 0: the first element of the sorted list at which the running sum reaches
@@ -330,7 +347,8 @@ __device__ void sort_list(Shared &s, const Row &r, int nl) {
   const int tid = threadIdx.x, n2 = pow2_at_least(nl);
   if (tid >= nl && tid < n2) s.list[tid] = ~0ull;
   sort(s.list, n2);
-  if (tid < nl) s.weight[tid] = r.weight(list_value(s.list[tid]));
+  const u64 w = r.weight(tid < nl ? list_value(s.list[tid]) : r.max);
+  if (tid < nl) s.weight[tid] = w;
   __syncthreads();
 }
 
@@ -342,26 +360,19 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank();
   Shared &s0 = *cl.map_shared_rank(&s, 0);
   uint32_t klo = 0, khi = 0xffffffffu, step = 0;  // level 0: linear bins; then keys
+  auto key_bin = [&](int i, float v) {
+    const uint32_t key = key_of(v);
+    return c.keeps(v, i) && key >= klo && key <= khi ? (int)((khi - key) / step) : -1;
+  };
   for (int level = 0; s.bin >= 0; ++level) {
     const int bin = s.bin;
     const u64 before = s.before;
-    auto here = [&](uint32_t key, int i, float v) {
-      return c.keeps(key, i) && key >= klo && key <= khi &&
-             (level == 0 ? r.bin(v) : (int)((khi - key) / step)) == bin;
-    };
-    const unsigned int nbin = s.sum_count[bin];
-    if (tid == 0) {
-      s.nlist = 0;
-      s.klo = 0xffffffffu;
-      s.khi = 0;
-    }
-    cl.sync();
+    auto here = [&](int i, float v) { return level == 0 ? c.keeps(v, i) && r.bin(v) == bin : key_bin(i, v) == bin; };
+    const int nbin = gather(cl, s, r, here);
     if (nbin <= kCap) {
-      gather(cl, s, r, here);
       if (rank == 0) {
-        sort_list(s, r, (int)nbin);
-        const int at = cut_list<MASS>(s, (int)nbin, before, target, warp, lane);
-        __syncthreads();
+        sort_list(s, r, nbin);
+        const int at = cut_list<MASS>(s, nbin, before, target, warp, lane);
         if (tid < kCluster) {
           Shared &o = *cl.map_shared_rank(&s, tid);
           o.cut_key = ~(uint32_t)(s.list[at] >> 32);
@@ -369,17 +380,16 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
         }
       }
       cl.sync();
-      c.key = s.cut_key;
+      c.value = value_of(s.cut_key);
       c.idx = (int)s.need;
       return;
     }
     // the bin's range of keys
     unsigned int lo = 0xffffffffu, hi = 0;
     r.each(lane, [&](int i, float v) {
-      const uint32_t key = key_of(v);
-      if (i < r.w1 && here(key, i, v)) {
-        lo = min(lo, key);
-        hi = max(hi, key);
+      if (here(i, v)) {
+        lo = min(lo, key_of(v));
+        hi = max(hi, key_of(v));
       }
     });
     lo = __reduce_min_sync(0xffffffffu, lo);
@@ -391,11 +401,17 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
     cl.sync();
     klo = s0.klo;
     khi = s0.khi;
+    cl.sync();  // read by all
+    if (tid == 0) {
+      s.klo = 0xffffffffu;
+      s.khi = 0;
+    }
     if (klo == khi) {
       // all equal: the cut is the index of one of them, counted in index order
+      const float tie = value_of(klo);
       u64 need;
       if (MASS) {
-        const u64 w = r.weight(value_of(klo));
+        const u64 w = r.weight(tie);
         need = (u64)((target - (double)before) / (double)w);
         while (need && (double)(before + need * w) >= target) --need;
         while ((double)(before + need * w) < target) ++need;
@@ -403,7 +419,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
         need = (u64)target - before;
       }
       u64 mine = 0;
-      r.each(lane, [&](int i, float v) { mine += i < r.w1 && c.keeps(key_of(v), i) && key_of(v) == klo; });
+      r.each(lane, [&](int i, float v) { mine += c.keeps(v, i) && v == tie; });
       mine = warp_total(mine);
       u64 p = cta_prefix(s, mine, warp, lane);
       if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
@@ -411,7 +427,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
       for (int q = 0; q < rank; ++q) p += s.totals[q];
       if (p < need && need <= p + mine) {  // this warp holds it
         r.each(lane, [&](int i, float v) {
-          const bool hit = i < r.w1 && c.keeps(key_of(v), i) && key_of(v) == klo;
+          const bool hit = c.keeps(v, i) && v == tie;
           const unsigned int b = __ballot_sync(0xffffffffu, hit);
           if (hit && p + __popc(b & ((2u << lane) - 1)) == need)
             for (int q = 0; q < kCluster; ++q) cl.map_shared_rank(&s, q)->cut_idx = i;
@@ -419,13 +435,13 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
         });
       }
       cl.sync();
-      c.key = klo;
+      c.value = tie;
       c.idx = s.cut_idx;
       return;
     }
     step = (khi - klo) / kBins + 1;
-    histogram<MASS>(cl, s, r, c, klo, khi, [&](uint32_t key, float) { return (int)((khi - key) / step); });
-    find_bin<MASS>(s, before, target, warp, lane);
+    histogram<MASS>(cl, s, r, key_bin);
+    find_bin(s, before, target, warp, lane);
   }
 }
 
@@ -474,16 +490,19 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   cg::cluster_group cl = cg::this_cluster();
   const int rank = cl.block_rank(), row = blockIdx.x / kCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // contiguous slices of CTAs and warps, in index order, multiples of 32
-  const int per_warp = ((a.n + kCluster * kWarps - 1) / (kCluster * kWarps) + 31) & ~31;
+  // contiguous slices of CTAs and warps, in index order, multiples of 128
+  const int per_warp = ((a.n + kCluster * kWarps - 1) / (kCluster * kWarps) + 127) & ~127;
   Row r;
   r.x = a.logits + (long)row * a.ld;
   r.w0 = min(a.n, (rank * kWarps + warp) * per_warp);
   r.w1 = min(a.n, r.w0 + per_warp);
   r.held = nullptr;
-  r.table = s.table;
-  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
-  if (tid == 0) s.nlist = 0;
+  r.inf = false;
+  r.table = exp2((double)lane / kTable);
+  if (tid == 0) {
+    s.klo = 0xffffffffu;
+    s.khi = 0;
+  }
   ptx::griddep_wait();
   float top = -INFINITY;
   if (per_warp <= kKeep) {
@@ -497,7 +516,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        v[j] = v[j] == v[j] ? v[j] + 0.0f : -INFINITY;
+        v[j] = r.counted(v[j]);
         top = fmaxf(top, v[j]);
         if (b + 32 * j < kKeep) hold[b + 32 * j] = v[j];
       }
@@ -533,7 +552,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
     if (!mine) return;
     int at = 0x7fffffff;
     r.each(lane, [&](int i, float v) {
-      if (i < r.w1 && v == r.max) at = min(at, i);
+      if (v == r.max) at = min(at, i);
     });
     at = __reduce_min_sync(0xffffffffu, at);
     __syncthreads();
@@ -547,37 +566,50 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
     }
     return;
   }
-  r.inf = r.max == INFINITY;
-  r.max_d = (double)r.max;
+  if (r.max == INFINITY) {
+    r.inf = true;
+    r.max = 0.0f;
+    float *hold = s.values + warp * kKeep;
+    if (r.held)
+      for (int i = lane; i < kKeep; i += 32) hold[i] = r.counted(hold[i]);
+    __syncwarp();
+  }
   r.scale = 1.4426950408889634 / (double)a.temperature;
+  r.max_d = (double)r.max;
+  r.least = (float)(r.max_d - 63.0 / r.scale);
   r.bin_scale = kBinsPerNat / a.temperature;
   r.one = a.one;
   Cut c;
   const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
-  auto linear = [&](uint32_t, float v) { return r.bin(v); };
+  // all that lies up to the end of the bin, as one list
+  auto list_upto = [&](int bin) {
+    return gather(cl, s, r, [&](int, float v) { return v > -INFINITY && r.bin(v) <= bin; });
+  };
   if (by_k) {
-    histogram<false>(cl, s, r, c, 0, 0xffffffffu, linear);
-    find_bin<false>(s, 0, (double)a.top_k, warp, lane);
-    const int bin = s.bin;
-    if (bin >= 0 && s.above <= kCap) {
-      const int nl = s.above;
-      gather(cl, s, r, [&](uint32_t key, int i, float v) { return key > kNegInf && r.bin(v) <= bin; });
+    histogram<false>(cl, s, r, [&](int, float v) { return v > -INFINITY ? r.bin(v) : -1; });
+    find_bin(s, 0, (double)a.top_k, warp, lane);
+    if (s.bin >= 0 && s.upto <= kCap) {
+      const int nl = list_upto(s.bin);
       if (rank == 0) choose_from_list(s, a, r, row, nl, 0);
       return;
     }
     find_cut<false>(cl, s, r, c, (double)a.top_k);
   }
   if (by_p) {
-    histogram<true>(cl, s, r, c, 0, 0xffffffffu, linear);
-    u64 all = s.sum_mass[tid * 2] + s.sum_mass[tid * 2 + 1];
-    all = cta_scan(s, all, warp, lane);
+    if (by_k) {
+      histogram<true>(cl, s, r, [&](int i, float v) { return c.keeps(v, i) ? r.bin(v) : -1; });
+    } else {
+      histogram<true>(cl, s, r, [&](int, float v) { return r.bin(v); });
+    }
+    u64 all = s.sum[tid * 2] + s.sum[tid * 2 + 1];
+    cta_scan(s, all, warp, lane);
     all = s.cta_sum;
     const double target = (double)a.top_p * (double)all;
-    find_bin<true>(s, 0, target, warp, lane);
-    const int bin = s.bin;
-    if (!by_k && bin >= 0 && s.above <= kCap) {
-      const int nl = s.above;
-      gather(cl, s, r, [&](uint32_t key, int i, float v) { return key > kNegInf && r.bin(v) <= bin; });
+    find_bin(s, 0, target, warp, lane);
+    // every element up to the end of the bin weighs at least this: a bound on their number
+    const double edge = exp2(-(double)(s.bin + 2) / kBinsPerNat * 1.4426950408889634) * r.one;
+    if (!by_k && s.bin >= 0 && s.bin < kBins - 1 && (double)s.upto <= kCap * edge) {
+      const int nl = list_upto(s.bin);
       if (rank == 0) choose_from_list(s, a, r, row, nl, all);
       return;
     }
@@ -585,12 +617,33 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   }
   const double least = (double)a.min_p * r.one;
   auto kept = [&](int i, float v) -> u64 {
-    if (i >= r.w1 || !c.keeps(key_of(v), i)) return 0;
     const u64 w = r.weight(v);
-    return (double)w >= least ? w : 0;
+    return c.keeps(v, i) && (double)w >= least ? w : 0;
   };
   u64 mine = 0;
-  r.each(lane, [&](int i, float v) { mine += kept(i, v); });
+  if (r.held) {
+    // what the cuts keep, often few, moves to the front of the warp's slice
+    float *hold = s.values + warp * kKeep;
+    int n = 0;
+    r.each4(lane, [&](int i, const float (&v)[4]) {
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = c.keeps(v[j], i + 32 * j);
+        const unsigned int b = __ballot_sync(0xffffffffu, in);
+        if (in) hold[n + __popc(b & ((1u << lane) - 1))] = v[j];
+        n += __popc(b);
+      }
+      __syncwarp();
+    });
+#pragma unroll 4
+    for (int b = 0; b < n; b += 32) {
+      const u64 w = r.weight(b + lane < n ? hold[b + lane] : -INFINITY);
+      mine += (double)w >= least ? w : 0;
+    }
+  } else {
+    r.each(lane, [&](int i, float v) { mine += kept(i, v); });
+  }
   mine = warp_total(mine);
   u64 p = cta_prefix(s, mine, warp, lane);
   if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
@@ -604,17 +657,27 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   const double u = uf > 0.0f ? (double)uf : 0.0;  // NaN and below: 0
   u64 target = (u64)(u * (double)total);
   if (u >= 1.0 || target >= total) target = total - 1;
-  if (p <= target && target < p + mine) {  // this warp holds the token
-    r.each(lane, [&](int i, float v) {
-      if (p > target) return;  // found (the same in every lane)
-      const u64 w = kept(i, v), incl = warp_scan(w, lane);
-      const u64 run = p + incl;
-      if (run > target && run - w <= target) {
-        a.token[row] = i;
-        if (a.prob) a.prob[row] = (float)((double)w / (double)total);
-      }
-      p += __shfl_sync(0xffffffffu, incl, 31);
-    });
+  // the warp that holds the token hands its elements to the whole CTA
+  __syncthreads();
+  if (tid == 0) s.bin = -1;
+  __syncthreads();
+  if (lane == 0 && p <= target && target < p + mine) {
+    s.bin = warp;
+    s.before = p;
+  }
+  __syncthreads();
+  if (s.bin < 0) return;
+  u64 before = s.before;
+  const int first = min(a.n, (rank * kWarps + s.bin) * per_warp), last = min(a.n, first + per_warp);
+  for (int b = first; b < last && before <= target; b += kThreads) {
+    const int i = b + tid;
+    const float v = i < last ? r.counted(__ldg(r.x + i)) : -INFINITY;
+    const u64 w = kept(i, v), run = before + cta_scan(s, w, warp, lane);
+    if (run > target && run - w <= target) {
+      a.token[row] = i;
+      if (a.prob) a.prob[row] = (float)((double)w / (double)total);
+    }
+    before += s.cta_sum;
   }
 }
 
