@@ -322,9 +322,10 @@ def gemm_int8(mat, matsc, src, ssc, dst=None, dstr=0, mstr=0, sstr=0, m=None, n=
 # --------------------------------------------------------------------------
 
 def _stream(stream=None) -> int:
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def dev_quantize_acts(dst, dsc, src, m, n, sstr=0, stream=None):
@@ -650,13 +651,21 @@ def _want(what, ok, *msg):
         raise GcuError(f"{what}: " + " ".join(str(m) for m in msg))
 
 
-def _rows(what, name, t, dtype, shape):
-    """t is a contiguous CUDA tensor of this dtype and shape on the current device."""
+def _device(what, t):
+    """The current device's index, which t has to be on."""
     import torch
-    _want(what, t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(), name, "must be a contiguous",
-          dtype, "tensor of", tuple(shape), "not", t.dtype, tuple(t.shape))
-    _want(what, t.is_cuda and t.device.index == torch.cuda.current_device(), name, "is on", t.device,
-          "and the current device is another")
+    d = torch._C._cuda_getDevice() if t.is_cuda else -2
+    if t.get_device() != d:
+        raise GcuError(f"{what}: a tensor is on {t.device} and the current device is another")
+    return d
+
+
+def _rows(what, name, t, dtype, shape, dev):
+    """t is a contiguous tensor of this dtype and shape (a tuple) on CUDA device dev."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+        return
+    raise GcuError(f"{what}: {name} must be a contiguous {dtype} tensor of {shape} on the current device, "
+                   f"not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def _work(nbytes, device, stream):
@@ -667,7 +676,7 @@ def _work(nbytes, device, stream):
     import torch
     w = torch.empty(nbytes, dtype=torch.uint8, device=device)
     if stream is not None:
-        w.record_stream(stream)
+        w.record_stream(stream)  # the block is not handed out again before the call is done
     return w.data_ptr(), nbytes, w
 
 
@@ -706,24 +715,33 @@ class KvCacheI8:
         """The cache of sequence b alone (a view)."""
         return KvCacheI8(self.k[b:b + 1], self.v[b:b + 1], self.ks[b:b + 1], self.vs[b:b + 1])
 
-    def check(self, what):
-        import torch
-        _want(what, self.k.is_cuda and self.device.index == torch.cuda.current_device(), "cache is on", self.device,
-              "and the current device is another")
-
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
+
+
+def _check_write(what, xq, shape, qkv, kv, freqs, nq, nk, rows, n_heads):
+    import torch
+    dev, f32 = _device(what, kv.k), torch.float32
+    _rows(what, "xq", xq, f32, shape, dev)
+    if not (qkv.dtype is f32 and qkv.dim() == 2 and qkv.shape[0] == rows and qkv.stride(1) == 1 and
+            qkv.shape[1] >= (n_heads + 2 * kv.nkv) * kv.hdim and qkv.get_device() == dev):
+        raise GcuError(f"{what}: qkv must be float32 rows of the fused q|k|v projection, one per token, "
+                       f"not {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
+    _rows(what, "freqs", freqs, f32, (rows, kv.hdim), dev)
+    if nq is not None:
+        _rows(what, "nq", nq, f32, (kv.hdim,), dev)
+    if nk is not None:
+        _rows(what, "nk", nk, f32, (kv.hdim,), dev)
+    return dev
 
 
 def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
     """dev_qkv_norm_rope_cache into an 8-bit cache of one sequence: qkv (ntok, >=
     (n_heads+2*nkv)*hdim) rows, rotated queries to xq (n_heads, ntok, hdim),
     codes and scales to kv (KvCacheI8) at [spos, spos+ntok); freqs (ntok, hdim)."""
-    import torch
     what = "dev_qkv_norm_rope_cache_i8"
-    n_heads, ntok, _ = xq.shape
-    kv.check(what)
+    n_heads, ntok = xq.shape[0], xq.shape[1]
     _check_write(what, xq, (n_heads, ntok, kv.hdim), qkv, kv, freqs, nq, nk, ntok, n_heads)
     _check(lib().gcu_dev_qkv_norm_rope_cache_i8(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref, _ptr(nq), _ptr(nk),
                                                 eps, freqs.data_ptr(), q_scale, n_heads, spos, ntok, _stream(stream)),
@@ -737,24 +755,11 @@ def dev_qkv_norm_rope_cache_i8_seqs(xq, qkv, kv, length, freqs, q_scale=1.0, nq=
     import torch
     what = "dev_qkv_norm_rope_cache_i8_seqs"
     n_heads = xq.shape[1]
-    kv.check(what)
-    _check_write(what, xq, (kv.nseq, n_heads, kv.hdim), qkv, kv, freqs, nq, nk, kv.nseq, n_heads)
-    _rows(what, "length", length, torch.int32, (kv.nseq,))
+    dev = _check_write(what, xq, (kv.nseq, n_heads, kv.hdim), qkv, kv, freqs, nq, nk, kv.nseq, n_heads)
+    _rows(what, "length", length, torch.int32, (kv.nseq,), dev)
     _check(lib().gcu_dev_qkv_norm_rope_cache_i8_seqs(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref,
                                                      length.data_ptr(), _ptr(nq), _ptr(nk), eps, freqs.data_ptr(),
                                                      q_scale, n_heads, _stream(stream)), what)
-
-
-def _check_write(what, xq, shape, qkv, kv, freqs, nq, nk, rows, n_heads):
-    import torch
-    _rows(what, "xq", xq, torch.float32, shape)
-    _want(what, qkv.dtype == torch.float32 and qkv.dim() == 2 and qkv.shape[0] == rows and qkv.stride(1) == 1 and
-          qkv.shape[1] >= (n_heads + 2 * kv.nkv) * kv.hdim and qkv.device == kv.device,
-          "qkv must be float32 rows of the fused q|k|v projection, one per token, not", qkv.dtype, tuple(qkv.shape))
-    _rows(what, "freqs", freqs, torch.float32, (rows, kv.hdim))
-    for name, w in (("nq", nq), ("nk", nk)):
-        if w is not None:
-            _rows(what, name, w, torch.float32, (kv.hdim,))
 
 
 def dev_cache_i8_read(k, v, kv, spos, stream=None):
@@ -762,13 +767,14 @@ def dev_cache_i8_read(k, v, kv, spos, stream=None):
     views of a longer fp32 cache among them."""
     import torch
     what = "dev_cache_i8_read"
-    kv.check(what)
-    for name, t in (("k", k), ("v", v)):
-        _want(what, t.dtype == torch.float32 and t.dim() == 4 and t.shape == k.shape and t.stride() == k.stride() and
-              tuple(t.shape[:2]) == (kv.nseq, kv.nkv) and t.shape[3] == kv.hdim and t.stride(3) == 1 and
-              (t.stride(2) == kv.hdim or t.shape[2] < 2) and t.device == kv.device,
-              name, "must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, k and v alike")
-    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), kv.ref, spos, k.shape[2],
+    dev = _device(what, kv.k)
+    st = k.stride()
+    if not (k.dtype is torch.float32 and v.dtype is torch.float32 and k.dim() == 4 and v.shape == k.shape and
+            v.stride() == st and k.shape[0] == kv.nseq and k.shape[1] == kv.nkv and k.shape[3] == kv.hdim and
+            st[3] == 1 and (st[2] == kv.hdim or k.shape[2] < 2) and k.get_device() == dev and v.get_device() == dev):
+        raise GcuError(f"{what}: k and v must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, alike, on the "
+                       f"cache's device, not {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
+    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0], st[1], kv.ref, spos, k.shape[2],
                                        _stream(stream)), what)
 
 
@@ -779,19 +785,20 @@ def dev_attention_decode_i8(xo, xq, kv, length, max_len, asc, sc_att=0.0, slide=
     these the last `slide` when slide > 0.  length[b] < 0: skipped."""
     import torch
     what = "dev_attention_decode_i8"
-    kv.check(what)
-    n_heads = xq.shape[1]
-    _rows(what, "xq", xq, torch.float32, (kv.nseq, n_heads, kv.hdim))
-    _rows(what, "xo", xo, torch.float32, (kv.nseq, n_heads, kv.hdim))
+    dev, n_heads = _device(what, kv.k), xq.shape[1]
+    shape = (kv.nseq, n_heads, kv.hdim)
+    _rows(what, "xq", xq, torch.float32, shape, dev)
+    _rows(what, "xo", xo, torch.float32, shape, dev)
     if length is not None:
-        _rows(what, "length", length, torch.int32, (kv.nseq,))
+        _rows(what, "length", length, torch.int32, (kv.nseq,), dev)
+    pref = None
     if prefix is not None:
-        prefix.check(what)
-    pref = prefix.ref if prefix is not None else None
+        _device(what, prefix.k)
+        pref = prefix.ref
     l = lib()
-    work = _work(l.gcu_attention_decode_i8_work(pref, plen, kv.ref, max_len, n_heads, slide), kv.device, stream)
+    work, nbytes, keep = _work(l.gcu_attention_decode_i8_work(pref, plen, kv.ref, max_len, n_heads, slide), kv.device, stream)
     _check(l.gcu_dev_attention_decode_i8(xo.data_ptr(), xq.data_ptr(), pref, plen, kv.ref, _ptr(length), max_len, n_heads,
-                                         slide, asc, sc_att, work[0], work[1], _stream(stream)), what)
+                                         slide, asc, sc_att, work, nbytes, _stream(stream)), what)
 
 
 def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, stream=None):
@@ -800,15 +807,16 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
     rows (ntok, >= n_heads*hdim)."""
     import torch
     what = "dev_attention_prefill_i8"
-    kv.check(what)
-    n_heads, ntok, _ = xq.shape
-    _rows(what, "xq", xq, torch.float32, (n_heads, ntok, kv.hdim))
-    _want(what, xo.dtype == torch.float32 and xo.dim() == 2 and xo.shape[0] == ntok and xo.stride(1) == 1 and
-          xo.shape[1] >= n_heads * kv.hdim and xo.device == kv.device, "xo must be float32 (ntok, >= n_heads*hdim) rows")
+    dev, n_heads, ntok = _device(what, kv.k), xq.shape[0], xq.shape[1]
+    _rows(what, "xq", xq, torch.float32, (n_heads, ntok, kv.hdim), dev)
+    if not (xo.dtype is torch.float32 and xo.dim() == 2 and xo.shape[0] == ntok and xo.stride(1) == 1 and
+            xo.shape[1] >= n_heads * kv.hdim and xo.get_device() == dev):
+        raise GcuError(f"{what}: xo must be float32 (ntok, >= n_heads*hdim) rows, not {xo.dtype} {tuple(xo.shape)}")
     l = lib()
-    work = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, int(mask)), kv.device, stream)
+    work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, int(mask)), kv.device,
+                               stream)
     _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0), xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
-                                          sc_att, int(mask), work[0], work[1], _stream(stream)), what)
+                                          sc_att, int(mask), work, nbytes, _stream(stream)), what)
 
 
 def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
@@ -817,12 +825,13 @@ def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     tokens' shares of the kept weights.  See gcu_dev_sample in include/gcu.h."""
     import torch
     what = "dev_sample"
-    _want(what, logits.dtype == torch.float32 and logits.dim() == 2 and logits.stride(1) == 1 and logits.is_cuda and
-          logits.device.index == torch.cuda.current_device(), "logits must be float32 (m, nvocab) rows on the current device")
+    dev = _device(what, logits)
+    if not (logits.dtype is torch.float32 and logits.dim() == 2 and logits.stride(1) == 1):
+        raise GcuError(f"{what}: logits must be float32 (m, nvocab) rows, not {logits.dtype} {tuple(logits.shape)}")
     m, n = logits.shape
-    _rows(what, "token", token, torch.int32, (m,))
-    _rows(what, "u", u, torch.float32, (m,))
+    _rows(what, "token", token, torch.int32, (m,), dev)
+    _rows(what, "u", u, torch.float32, (m,), dev)
     if prob is not None:
-        _rows(what, "prob", prob, torch.float32, (m,))
+        _rows(what, "prob", prob, torch.float32, (m,), dev)
     _check(lib().gcu_dev_sample(token.data_ptr(), _ptr(prob), logits.data_ptr(), logits.stride(0) if m > 1 else 0,
                                 u.data_ptr(), temperature, top_k, top_p, min_p, m, n, _stream(stream)), what)

@@ -145,7 +145,20 @@ def test_binding_refuses_wrong_tensors():
     with pytest.raises(gcu.GcuError, match="contiguous"):
         t = torch.zeros((1, 16, 2, 64), dtype=torch.int8).transpose(1, 2)
         gcu.KvCacheI8(t, t, s, s)
-    assert gcu.KvCacheI8.empty(3, 2, 8, 64, device="cpu").seq(1).nseq == 1
+    kv = gcu.KvCacheI8.empty(3, 2, 8, 64, device="cpu")
+    assert kv.seq(1).nseq == 1
+    # tensors that are on no CUDA device, or not on the current one, never reach the library
+    x = torch.zeros((3, 4, 64))
+    with pytest.raises(gcu.GcuError, match="device"):
+        gcu.dev_attention_decode_i8(x, x, kv, None, 8, 1.0)
+    with pytest.raises(gcu.GcuError, match="device"):
+        gcu.dev_attention_prefill_i8(torch.zeros((4, 256)), torch.zeros((4, 4, 64)), kv.seq(0), 0)
+    with pytest.raises(gcu.GcuError, match="device"):
+        gcu.dev_cache_i8_read(torch.zeros((3, 2, 4, 64)), torch.zeros((3, 2, 4, 64)), kv, 0)
+    with pytest.raises(gcu.GcuError, match="device"):
+        gcu.dev_sample(torch.zeros(1, dtype=torch.int32), torch.zeros((1, 8)), torch.zeros(1))
+    with pytest.raises(gcu.GcuError, match="device"):
+        gcu.dev_qkv_norm_rope_cache_i8(torch.zeros((4, 1, 64)), torch.zeros((1, 512)), kv.seq(0), torch.zeros((1, 64)), 0)
 
 
 def test_plain_forms():
