@@ -7,10 +7,11 @@
 //   o     = sum_t p[t] * vs[t] * vc[t] / sum_t p[t]
 //
 // The codes stay integers up to the matrix products: a query row is scaled to
-// 24-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
-// products with int8 keys are int8 x int8 sums, exact in int32, and the
-// rounding of q is 2^-24 of the row's largest element -- what fp32 holds of
-// that element itself.
+// 23-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
+// products with int8 keys are int8 x int8 sums, exact in int32, and q is rounded by
+// 2^-23 of the row's largest element at most -- twice what fp32 rounds that element
+// by, and three instructions an element, as the integer comes out of a floating
+// point addition.
 //
 // Rows: the query heads of one kv head share its keys, so a row is (i, g):
 // token or sequence i, head h0 + g of the group, row index i * G + g.
@@ -22,7 +23,7 @@ namespace gcu {
 namespace attn8 {
 
 constexpr int kMaxGroup = 8;        // query heads per kv head
-constexpr float kQMax = 8355711.0f;  // 127 * (65536 + 256 + 1): the largest three signed digits
+constexpr float kQMax = 4194000.0f;  // below 2^22: q * inv + 1.5 * 2^23 holds it as an integer
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode {
@@ -92,6 +93,16 @@ __device__ __forceinline__ void row_window(const Args &a, int i, int &lo, int &h
 // whether row i's output is written at all
 __device__ __forceinline__ bool row_live(const Args &a, int i) { return a.mode == PREFILL || seq_len(a, i) >= 0; }
 
+// Rows first, first + 1, ... of a kv head as (i, g): one division, and a multiplication
+// for each row after that (exact for up to 248 rows and G <= 8).
+struct RowSplit {
+  int i0, g0, G;
+  uint32_t inv;
+  __device__ __forceinline__ RowSplit(int first, int G_) : i0(first / G_), g0(first % G_), G(G_), inv(65536u / G_ + 1) {}
+  __device__ __forceinline__ int i(int r) const { return i0 + (int)((uint32_t)(g0 + r) * inv >> 16); }
+  __device__ __forceinline__ int g(int r) const { return g0 + r - (i(r) - i0) * G; }
+};
+
 // max that keeps a NaN
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -104,21 +115,64 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// digits of q * inv (|q * inv| <= kQMax): v = 65536 d2 + 256 d1 + d0
-__device__ __forceinline__ void digits(float q, float inv, int &d2, int &d1, int &d0) {
-  int v = __float2int_rn(__fmul_rn(q, inv));
-  v = v > 8355711 ? 8355711 : v < -8355711 ? -8355711 : v;
-  d0 = (int)(int8_t)v;
-  v = (v - d0) >> 8;
-  d1 = (int)(int8_t)v;
-  d2 = (v - d1) >> 8;
+// E consecutive floats of a query row (zeros unless `have`)
+template <int E>
+__device__ __forceinline__ void load_floats(float (&v)[E], const float *src, bool have) {
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 f = have ? __ldg(reinterpret_cast<const float4 *>(src + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      v[e] = f.x;
+      v[e + 1] = f.y;
+      v[e + 2] = f.z;
+      v[e + 3] = f.w;
+    }
+  } else {
+    const float2 f = have ? __ldg(reinterpret_cast<const float2 *>(src)) : make_float2(0.f, 0.f);
+    v[0] = f.x;
+    v[1] = f.y;
+  }
+}
+// a warp's row: its largest |element| (NaN if there is one) and the digits of this
+// lane's elements, packed bytes of d0, d1, d2
+template <int E>
+__device__ __forceinline__ void row_digits(const float (&v)[E], uint32_t (&w)[3][(E + 3) / 4], float &amax) {
+  amax = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) amax = max_nan(amax, fabsf(v[e]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float inv = amax > 0.0f ? kQMax / amax : 0.0f;
+  // n + 0x808080 has the digits, each plus 128, as its bytes
+  uint32_t u[(E + 3) / 4 * 4] = {};
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    u[e] = __float_as_uint(__fmaf_rn(v[e], inv, 12582912.0f)) - 0x4B400000u + 0x808080u;
+#pragma unroll
+  for (int i = 0; i < (E + 3) / 4; ++i) {
+    const uint32_t *x = u + 4 * i;
+    const uint32_t a = __byte_perm(x[0], x[1], 0x5140), b = __byte_perm(x[2], x[3], 0x5140);
+    w[0][i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+    w[1][i] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+    w[2][i] = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410) ^ 0x80808080u;
+  }
+}
+template <int E>
+__device__ __forceinline__ void put_digits(uint8_t *dst, const uint32_t (&w)[(E + 3) / 4]) {
+  if constexpr (E == 8) {
+    *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+  } else if constexpr (E == 4) {
+    *reinterpret_cast<uint32_t *>(dst) = w[0];
+  } else {
+    *reinterpret_cast<uint16_t *>(dst) = (uint16_t)w[0];
+  }
 }
 
 // 65536 s2 + 256 s1 + s0 in fp32, two columns at a time.  |s| < 2^22 goes into the
 // mantissa of 1.5 * 2^23 by an integer addition (a conversion instruction runs
 // at a fraction of the rate); the offsets leave with the next step.  256 s1 + s0
 // is rounded at 2^31.6 at most, to 2^8, where the largest possible product of one
-// query and key element alone is 127 * 8355711 = 2^30.
+// query and key element alone is 127 * 2^22 = 2^29.
 __device__ __forceinline__ float2 magic2(const uint32_t *s) {
   return make_float2(__uint_as_float(s[0] + 0x4B400000u), __uint_as_float(s[1] + 0x4B400000u));
 }

@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   // rows of this CTA: OWN one sequence's group, else R of the (i, g) rows
   const int first = a.mode == OWN ? group * G : group * R;
   const int nr = max(0, a.mode == OWN ? G : min(R, a.ni * G - first));
+  const RowSplit rows(first, G);
   // The loads start before anything else: their warp sets up their barriers.
   if (warp == kLoadWarp && lane == 0) {
     ptx::prefetch_tmap(&p.k[set]);
@@ -114,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   // The rows' windows, lane r of every warp: the CTA's key range, and the keys that
   // every row sees.
   int lo = 0, hi = 0;
-  if (lane < nr) row_window(a, (first + lane) / G, lo, hi);
+  if (lane < nr) row_window(a, rows.i(lane), lo, hi);
   if (threadIdx.x < R) {
     s_lo[threadIdx.x] = lo;
     s_hi[threadIdx.x] = hi;
@@ -155,38 +156,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   if (nt > 0) {
     constexpr int E = HD / 32;
     for (int r = warp; r < R; r += kThreads / 32) {
-      float v[E], amax = 0.0f;
-      const float *src =
-          a.xq + (long)((first + r) / G) * a.q_i + (long)(h0 + (first + r) % G) * a.q_h + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[e] = r < nr ? __ldg(src + e) : 0.0f;
-        amax = max_nan(amax, fabsf(v[e]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const float inv = amax > 0.0f ? kQMax / amax : 0.0f;
-      uint32_t w[3][(E + 3) / 4] = {};
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        int d2, d1, d0;
-        digits(v[e], inv, d2, d1, d0);
-        w[0][e / 4] |= (uint32_t)(d0 & 0xff) << (8 * (e % 4));
-        w[1][e / 4] |= (uint32_t)(d1 & 0xff) << (8 * (e % 4));
-        w[2][e / 4] |= (uint32_t)(d2 & 0xff) << (8 * (e % 4));
-      }
+      float v[E], amax;
+      uint32_t w[3][(E + 3) / 4];
+      load_floats<E>(v, a.xq + (long)rows.i(r) * a.q_i + (long)(h0 + rows.g(r)) * a.q_h + lane * E, r < nr);
+      row_digits<E>(v, w, amax);
       const int col = lane * E, in = col % C::SW;
 #pragma unroll
       for (int d = 0; d < 3; ++d) {
         const int row = d * R + r, sw = C::SW == 128 ? row & 7 : (row >> 1) & 3;
         uint8_t *q = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + row * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
-        if constexpr (E == 8) {
-          *reinterpret_cast<uint2 *>(q) = make_uint2(w[d][0], w[d][1]);
-        } else if constexpr (E == 4) {
-          *reinterpret_cast<uint32_t *>(q) = w[d][0];
-        } else {
-          *reinterpret_cast<uint16_t *>(q) = (uint16_t)w[d][0];
-        }
+        put_digits<E>(q, w[d]);
       }
       if (lane == 0) s_rf[r] = amax / kQMax * a.asc;
     }
@@ -451,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       for (int r = 0; r < C::OR; ++r) {
         const int rr = orow + r;
         if (rr >= nr) break;
-        const int hh = rr / RQ, i = (first + rr) / G, h = h0 + (first + rr) % G;
+        const int hh = rr / RQ, i = rows.i(rr), h = h0 + rows.g(rr);
         const float sum = (s_red[hh * 4][rr % RQ] + s_red[hh * 4 + 1][rr % RQ]) +
                           (s_red[hh * 4 + 2][rr % RQ] + s_red[hh * 4 + 3][rr % RQ]);
         if (a.slots == 1) {  // a row that sees nothing: zeros

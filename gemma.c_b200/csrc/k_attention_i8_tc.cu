@@ -29,8 +29,8 @@
 // columns each of its four threads holds a quarter in HD/4 registers (some of
 // which the last warpgroup gives up).  The groups agree on m through shared
 // memory, tile by tile (a "decision").  A group also turns its tile's V codes
-// into fp16, in the MN-major layout that the product reads, before its scores
-// arrive.  Warp 16: products, issued by one thread of a warp that computes
+// into fp16, in the MN-major layout that the product reads, when its weights are
+// formed: the buffer's last product is done by then.  Warp 16: products, issued by one thread of a warp that computes
 // the descriptors uniformly; 17: loads.  While the softmax of tile j runs, the
 // tensor cores compute S of tile j + 1 and T of tile j - 1.
 // Every wait is bounded; a role that gives up sets the CTA's abort flag, which
@@ -82,6 +82,7 @@ struct Cfg {
   static constexpr int HALF = NK / 2;  // score columns per softmax thread
   static constexpr int OC = HD / 4;    // output columns per softmax thread
   static constexpr int S_COL = 0, T_COL = 3 * NK, P_COL = T_COL + HD;
+  static_assert(V16_OFF - Q_OFF >= kRows * HD * 4, "the output's stage");
   static_assert(SMEM <= 232448 - 512, "shared memory budget");
   static_assert(P_COL + NK <= 512, "TMEM budget");
 };
@@ -131,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   // heavy tiles first: the last query rows of a prompt see the most keys
   const int tile = p.tiles - 1 - (int)(blockIdx.x / a.splits), split = blockIdx.x % a.splits;
   const int first = tile * kRows, nrows = min(kRows, a.ni * G - first);
+  const RowSplit rows(first, G);
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&bars.kfull[s], 1);
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   // the rows' windows: the CTA's key range, and the keys that every row sees
   if ((int)threadIdx.x < nrows) {
     int lo, hi;
-    row_window(a, (first + threadIdx.x) / G, lo, hi);
+    row_window(a, rows.i(threadIdx.x), lo, hi);
     if (lo < hi) {
       atomicMin(&s_range[0], lo);
       atomicMax(&s_range[1], hi);
@@ -210,43 +212,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   // the query rows' digits, a warp per row; rows past the end are zeros
   float *s_rf = reinterpret_cast<float *>(smem + C::RF_OFF);
   if (nt > 0) {
-    constexpr int E = HD / 32;
-    for (int r = warp; r < kRows; r += kThreads / 32) {
-      float v[E], amax = 0.0f;
-      const int i = (first + r) / G, g = (first + r) % G;
-      const float *src = a.xq + (long)i * a.q_i + (long)(h0 + g) * a.q_h + lane * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[e] = r < nrows ? __ldg(src + e) : 0.0f;
-        amax = max_nan(amax, fabsf(v[e]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      const float inv = amax > 0.0f ? kQMax / amax : 0.0f;
-      uint32_t w[3][(E + 3) / 4] = {};
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        int d2, d1, d0;
-        digits(v[e], inv, d2, d1, d0);
-        w[0][e / 4] |= (uint32_t)(d0 & 0xff) << (8 * (e % 4));
-        w[1][e / 4] |= (uint32_t)(d1 & 0xff) << (8 * (e % 4));
-        w[2][e / 4] |= (uint32_t)(d2 & 0xff) << (8 * (e % 4));
-      }
+    // a row ahead in flight; one copy of the code, which every CTA fetches anew
+    constexpr int E = HD / 32, W = kThreads / 32;
+    auto load_row = [&](float (&v)[E], int r) {
+      load_floats<E>(v, a.xq + (long)rows.i(r) * a.q_i + (long)(h0 + rows.g(r)) * a.q_h + lane * E, r < nrows);
+    };
+    float v[E], ahead[E];
+    load_row(v, warp);
+#pragma unroll 1
+    for (int r = warp; r < kRows; r += W) {
+      load_row(ahead, r + W);
+      float amax;
+      uint32_t w[3][(E + 3) / 4];
+      row_digits<E>(v, w, amax);
       const int col = lane * E, in = col % C::SW;
       const int sw = C::SW == 128 ? r & 7 : (r >> 1) & 3;
       uint8_t *dst = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + r * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
 #pragma unroll
-      for (int d = 0; d < 3; ++d) {
-        uint8_t *q = dst + d * C::KB * C::Q_BLOCK;
-        if constexpr (E == 8) {
-          *reinterpret_cast<uint2 *>(q) = make_uint2(w[d][0], w[d][1]);
-        } else if constexpr (E == 4) {
-          *reinterpret_cast<uint32_t *>(q) = w[d][0];
-        } else {
-          *reinterpret_cast<uint16_t *>(q) = (uint16_t)w[d][0];
-        }
-      }
+      for (int d = 0; d < 3; ++d) put_digits<E>(dst + d * C::KB * C::Q_BLOCK, w[d]);
       if (lane == 0) s_rf[r] = amax / kQMax * a.asc;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = ahead[e];
     }
     // tile 0's scales
     if ((int)threadIdx.x < 2 * NK) {
@@ -313,27 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         }
         __syncwarp();
       };
-      bool ok = wait(&bars.kfull[0], 0, DEV_TIMEOUT_FULL);
-      if (__any_sync(0xffffffffu, !ok)) ok = false;
-      if (ok) {
-        ptx::tc_fence_after();
-        scores(0);
-      }
-      int taken = 0;
-      for (int j = 0; j < tiles && ok; ++j) {
-        if (j + 1 < tiles) {
-          ok = wait(&bars.kfull[(j + 1) & 1], ((j + 1) >> 1) & 1, DEV_TIMEOUT_FULL) &&
-               wait(&bars.sfree, j & 1, DEV_TIMEOUT_TMEM);
-          if (__any_sync(0xffffffffu, !ok)) break;
-          ptx::tc_fence_after();
-          scores(j + 1);
-        }
-        ok = wait(&bars.v16full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && wait(&bars.pfull, j & 1, DEV_TIMEOUT_TMEM);
-        const bool fresh = __shfl_sync(0xffffffffu, *(volatile int *)&s_fresh[j & 1], 0);
-        if (fresh && j > 0)  // T's sums have been taken
-          ok = ok && wait(&bars.tfree, taken++ & 1, DEV_TIMEOUT_TMEM);
-        if (__any_sync(0xffffffffu, !ok)) break;
-        ptx::tc_fence_after();
+      auto values = [&](int j, bool fresh) {
         if (ptx::elect_one()) {
           const uint32_t v_lo = dv.lo + (j & 1) * (C::V16_BYTES >> 4);
 #pragma unroll
@@ -345,6 +311,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
           ptx::mma_commit(&bars.pvdone[j & 1]);
         }
         __syncwarp();
+      };
+      // The two products of a tile wait for different things: T of tile jt for its
+      // weights, S of tile js for its keys and for S of tile js - 1 to have been read.
+      // Whichever can go goes, T first.
+      uint64_t t0 = ptx::globaltimer();
+      for (int js = 0, jt = 0, taken = 0; jt < tiles;) {
+        bool go = false;
+        if (jt < js && __all_sync(0xffffffffu, ptx::mbar_test(&bars.pfull, jt & 1) &&
+                                                   ptx::mbar_test(&bars.v16full[jt & 1], (jt >> 1) & 1))) {
+          const bool fresh = __shfl_sync(0xffffffffu, *(volatile int *)&s_fresh[jt & 1], 0), taking = fresh && jt > 0;
+          if (!taking || __all_sync(0xffffffffu, ptx::mbar_test(&bars.tfree, taken & 1))) {
+            ptx::tc_fence_after();
+            values(jt++, fresh);
+            taken += taking;
+            go = true;
+          }
+        }
+        if (js < tiles && __all_sync(0xffffffffu, ptx::mbar_test(&bars.kfull[js & 1], (js >> 1) & 1) &&
+                                                      (js == 0 || ptx::mbar_test(&bars.sfree, (js - 1) & 1)))) {
+          ptx::tc_fence_after();
+          scores(js++);
+          go = true;
+        }
+        if (go) {
+          t0 = ptx::globaltimer();
+        } else if (*wait.abort || ptx::globaltimer() - t0 > 2000000000ull) {
+          if (lane == 0 && !*wait.abort) {
+            ptx::record_err(a.err, DEV_TIMEOUT_TMEM);
+            *wait.abort = 1;
+          }
+          break;
+        }
       }
       // all products complete before TMEM is freed
       if (ptx::elect_one()) ptx::mma_commit(&bars.drain);
@@ -363,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     volatile int *freshp = s_fresh;
     const bool live = row < nrows;
     int lo = 0, hi = 0;
-    if (live) row_window(a, (first + row) / G, lo, hi);
+    if (live) row_window(a, rows.i(row), lo, hi);
     const float rf_nat = nt > 0 ? s_rf[row] : 0.0f, rf = CAP ? kLog2e : rf_nat * kLog2e;
     // scales of the other group's next tile: thread tid of ks (tid < NK) or vs
     auto fetch_scale = [&](int j) {
@@ -405,26 +403,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     };
     int j = grp;
     for (; j < nt; j += 2) {
-      // V codes of this tile to fp16; 8 columns of a key per thread.  Keys past
-      // the range hold an earlier tile's codes, which weigh nothing.
-      ok = wait(&bars.v8full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && ok;
-      if (j > 1) ok = wait(&bars.pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
-      {
-        constexpr int L = HD / 8, KS = kGroup / L;
-        const int c = tid % L, key0 = tid / L;
-        const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
-        uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
-#pragma unroll
-        for (int k = 0; k < NK; k += KS) {
-          const int key = key0 + k;
-          const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
-          const uint2 x = to_half4(w.x), y = to_half4(w.y);
-          *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
-        }
-        ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
-        ptx::mbar_arrive(&bars.v16full[j & 1]);
-      }
       const float *ks = sc + (j & 3) * 3 * NK + half * C::HALF, *lvs = ks + NK, *rvs = ks + 2 * NK;
       if (j > 0) follow(j - 1);
       ok = wait(&bars.sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
@@ -519,6 +497,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         }
       }
       l += lt.x + lt.y;
+      // V codes of this tile to fp16; 8 columns of a key per thread.  Keys past
+      // the range hold an earlier tile's codes, which weigh nothing.
+      ok = wait(&bars.v8full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && ok;
+      if (j > 1) ok = wait(&bars.pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      {
+        constexpr int L = HD / 8, KS = kGroup / L;
+        const int c = tid % L, key0 = tid / L;
+        const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
+        uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
+#pragma unroll
+        for (int k = 0; k < NK; k += KS) {
+          const int key = key0 + k;
+          const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
+          const uint2 x = to_half4(w.x), y = to_half4(w.y);
+          *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
+        ptx::mbar_arrive(&bars.v16full[j & 1]);
+      }
       // P and T are free once the previous tile's product is done
       if (j > 0) {
         ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
@@ -546,15 +544,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     smax[quarter * kRows + row] = l;
     ptx::named_bar_sync(3, kSoftmax);
     l = (smax[row] + smax[kRows + row]) + (smax[2 * kRows + row] + smax[3 * kRows + row]);
-    const int i = live ? (first + row) / G : 0, h = live ? h0 + (first + row) % G : h0;
-    const size_t at = ((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h;
-    float *out = (a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD : a.part + at * HD) + quarter * C::OC;
-    const float d = a.slots > 1 || l == 0.0f ? 1.0f : l;  // a row that sees nothing: zeros
-    if (live && ok && (a.slots > 1 || row_live(a, i))) {
+    // Rows go out through shared memory (the queries' and keys' is free now: every
+    // product that reads them is done), a warp per row, 512 bytes at a time.
+    const float d = a.slots > 1 || l == 0.0f ? 1.0f : 1.0f / l;  // a row that sees nothing: zeros
+    float4 *stage = reinterpret_cast<float4 *>(smem);
 #pragma unroll
-      for (int c = 0; c < C::OC; c += 4)
-        *reinterpret_cast<float4 *>(out + c) = make_float4(acc[c] / d, acc[c + 1] / d, acc[c + 2] / d, acc[c + 3] / d);
-      if (a.slots > 1 && quarter == 0) a.stat[at] = make_float2(m == -INFINITY ? m : m - kTop, l);
+    for (int c = 0; c < C::OC; c += 4)
+      stage[row * (HD / 4) + ((quarter * C::OC + c) / 4 ^ (row & 7))] =
+          make_float4(acc[c] * d, acc[c + 1] * d, acc[c + 2] * d, acc[c + 3] * d);
+    if (live && ok && a.slots > 1 && quarter == 0)
+      a.stat[((size_t)(a.slot0 + split) * a.ni + rows.i(row)) * a.n_heads + h0 + rows.g(row)] =
+          make_float2(m == -INFINITY ? m : m - kTop, l);
+    ptx::named_bar_sync(3, kSoftmax);
+    for (int r = warp; r < nrows && ok; r += kSoftmax / 32) {
+      const int i = rows.i(r), h = h0 + rows.g(r);
+      float *out = a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD
+                                : a.part + (((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h) * HD;
+      if (a.slots == 1 && !row_live(a, i)) continue;
+#pragma unroll
+      for (int c = lane; c < HD / 4; c += 32) reinterpret_cast<float4 *>(out)[c] = stage[r * (HD / 4) + (c ^ (r & 7))];
     }
   }
   __syncthreads();

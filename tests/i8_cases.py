@@ -103,7 +103,7 @@ def prefill(xq, kv, spos, slide, cap, mask):
 def tolerance(score, n, vmax):
     """Largest error of an output element for scores up to |score| over n keys and
     values up to vmax.  A score is a handful of fp32 steps of its own size (the
-    query's 24-bit form, the digits' sum, the scales, log2 e, the shift by the
+    query's 23-bit form, the digits' sum, the scales, log2 e, the shift by the
     maximum): 8 half steps of 2^-24, which the exponential turns into a relative
     error of the weight; it enters the sum and, against it, the weights' total.
     The weights are multiplied as two bf16 parts: 2^-9 * 2^-9 each way, 2^-17 in
