@@ -115,6 +115,21 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// tanh to 2^-22 of itself, without a branch: below 0.6 y + y^3 p(y^2), p a least-squares
+// fit of (tanh(y)/y - 1)/y^2 at 400 Chebyshev nodes of [0, 0.36] with relative
+// weights (2^-23.7 measured over 200001 points); above, 1 - 2/(1 + e^2|y|).  tanhf's
+// branches cost the capped 1023-token prompt three quarters of its time (262 us).
+__device__ __forceinline__ float tanh_fast(float y) {
+  const float a = fabsf(y), z = y * y;
+  float p = __fmaf_rn(z, -5.893945228e-3f, 2.079461701e-2f);
+  p = __fmaf_rn(p, z, -5.378329381e-2f);
+  p = __fmaf_rn(p, z, 1.333191544e-1f);
+  p = __fmaf_rn(p, z, -3.333329856e-1f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(a * (2.0f * kLog2e)) + 1.0f));
+  return a < 0.6f ? __fmaf_rn(y * z, p, y) : copysignf(__fmaf_rn(-2.0f, r, 1.0f), y);
+}
+
 // E consecutive floats of a query row (zeros unless `have`)
 template <int E>
 __device__ __forceinline__ void load_floats(float (&v)[E], const float *src, bool have) {

@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       const int t = j * kKeys + key;
       return t < n ? __ldg(src + kbeg + t) : 1.0f;
     };
+    const float inv_cap = CAP ? 1.0f / a.sc_att : 0.0f, unit = CAP ? a.sc_att * kLog2e : kLog2e;
     float rf[RQ], l[RQ];
 #pragma unroll
     for (int r = 0; r < RQ; ++r) {
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
           float s[2] = {y.x * ks * rf[c + e], y.y * ks * rf[c + e + 1]};
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            if (CAP) s[q] = tanhf(s[q] / a.sc_att) * a.sc_att;
-            x[c + e + q] = __fmaf_rn(s[q], kLog2e, lvs);
+            if (CAP) s[q] = tanh_fast(s[q] * inv_cap);
+            x[c + e + q] = __fmaf_rn(s[q], unit, lvs);
           }
         }
       }

@@ -362,7 +362,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     const bool live = row < nrows;
     int lo = 0, hi = 0;
     if (live) row_window(a, rows.i(row), lo, hi);
-    const float rf_nat = nt > 0 ? s_rf[row] : 0.0f, rf = CAP ? kLog2e : rf_nat * kLog2e;
+    // scores from digit sums: natural units over the cap, then times the cap, or log2 units
+    float rf_nat = nt > 0 ? s_rf[row] : 0.0f, rf = rf_nat * kLog2e;
+    if (CAP) {
+      rf_nat /= a.sc_att;
+      rf = a.sc_att * kLog2e;
+    }
     // scales of the other group's next tile: thread tid of ks (tid < NK) or vs
     auto fetch_scale = [&](int j) {
       const int t = j * NK + (tid & (NK - 1));
@@ -435,8 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
           float2 y = __fmul2_rn(high_digit(s2 + e, make_float2(x[c + e], x[c + e + 1])), make_float2(k.x, k.y));
           float2 z = __fmul2_rn(high_digit(s2 + e + 2, make_float2(x[c + e + 2], x[c + e + 3])), make_float2(k.z, k.w));
           if constexpr (CAP) {
-            y = make_float2(tanhf(y.x * rf_nat / a.sc_att) * a.sc_att, tanhf(y.y * rf_nat / a.sc_att) * a.sc_att);
-            z = make_float2(tanhf(z.x * rf_nat / a.sc_att) * a.sc_att, tanhf(z.y * rf_nat / a.sc_att) * a.sc_att);
+            y = make_float2(tanh_fast(y.x * rf_nat), tanh_fast(y.y * rf_nat));
+            z = make_float2(tanh_fast(z.x * rf_nat), tanh_fast(z.y * rf_nat));
           }
           y = __ffma2_rn(y, make_float2(rf, rf), make_float2(v.x, v.y));
           z = __ffma2_rn(z, make_float2(rf, rf), make_float2(v.z, v.w));
