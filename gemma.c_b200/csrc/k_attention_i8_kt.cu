@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R];
   __shared__ float s_rf[R], s_m[R], s_f[R], s_red[16][R / 4];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // aligned by an offset: the accesses stay in the shared address space
+  uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int set = (int)blockIdx.x >= p.first1;
   const Args &a = p.a[set];

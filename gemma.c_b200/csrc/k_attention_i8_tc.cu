@@ -29,8 +29,8 @@
 // columns each of its four threads holds a quarter in HD/4 registers (some of
 // which the last warpgroup gives up).  The groups agree on m through shared
 // memory, tile by tile (a "decision").  A group also turns its tile's V codes
-// into fp16, in the MN-major layout that the product reads, when its weights are
-// formed: the buffer's last product is done by then.  Warp 16: products, issued by one thread of a warp that computes
+// into fp16, in the MN-major layout that the product reads, while its scores are
+// formed.  Warp 16: products, issued by one thread of a warp that computes
 // the descriptors uniformly; 17: loads.  While the softmax of tile j runs, the
 // tensor cores compute S of tile j + 1 and T of tile j - 1.
 // Every wait is bounded; a role that gives up sets the CTA's abort flag, which
@@ -81,6 +81,7 @@ struct Cfg {
   // TMEM columns: S of three digits, T, P (two parts, two keys per column)
   static constexpr int HALF = NK / 2;  // score columns per softmax thread
   static constexpr int OC = HD / 4;    // output columns per softmax thread
+  static constexpr int RB = HD == 256 ? 8 : 16;  // score columns read at a time (registers)
   static constexpr int S_COL = 0, T_COL = 3 * NK, P_COL = T_COL + HD;
   static_assert(V16_OFF - Q_OFF >= kRows * HD * 4, "the output's stage");
   static_assert(SMEM <= 232448 - 512, "shared memory budget");
@@ -108,6 +109,9 @@ __device__ __forceinline__ uint2 to_half4(uint32_t w) {
   return make_uint2(*reinterpret_cast<const uint32_t *>(&x), *reinterpret_cast<const uint32_t *>(&y));
 }
 
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[8]) { ptx::tmem_ld_32x8(at, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[16]) { ptx::tmem_ld_32x16(at, r); }
+
 // thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK]
 __device__ __forceinline__ void put_scale(float *sc, int i, float v) {
   if (i < NK) {
@@ -124,7 +128,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   __shared__ Bars bars;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_fresh[2], s_range[4];  // first key, end, last start of a window, first end
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // aligned by an offset: the accesses stay in the shared address space
+  uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const Args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int hk = blockIdx.y;
@@ -406,35 +411,65 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         ptx::mbar_arrive(&bars.tfree);
       }
     };
+    // V codes of tile j to fp16; 8 columns of a key per thread.  Keys past the range
+    // hold an earlier tile's codes, which weigh nothing.  At hdim 256 it fits into the
+    // wait for the scores (8192 tokens 1264 -> 1239 us); with shorter score products
+    // that wait is short, and it goes between the weights and the wait for the
+    // previous product (hdim 128 1000 -> 897 us).
+    auto convert = [&](int j) {
+      ok = wait(&bars.v8full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && ok;
+      if (j > 1) ok = wait(&bars.pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
+      {
+        constexpr int L = HD / 8, KS = kGroup / L;
+        const int c = tid % L, key0 = tid / L;
+        const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
+        uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
+#pragma unroll
+        for (int k = 0; k < NK; k += KS) {
+          const int key = key0 + k;
+          const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
+          const uint2 x = to_half4(w.x), y = to_half4(w.y);
+          *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
+        }
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
+        ptx::mbar_arrive(&bars.v16full[j & 1]);
+      }
+    };
     int j = grp;
     for (; j < nt; j += 2) {
       const float *ks = sc + (j & 3) * 3 * NK + half * C::HALF, *lvs = ks + NK, *rvs = ks + 2 * NK;
       if (j > 0) follow(j - 1);
+      // while the scores are formed: the scales of the other group's next tile, which it
+      // reads after this tile's decision, and the values
+      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
+      next = fetch_scale(j + 3);
+      if (HD == 256) convert(j);
       ok = wait(&bars.sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       ptx::tc_fence_after();
       // exponents: the score in log2 units plus log2 of the value row's scale
       float x[C::HALF];
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 8) {
-        uint32_t s1[8], s0[8];
+      for (int c = 0; c < C::HALF; c += C::RB) {
+        uint32_t s1[C::RB], s0[C::RB];
         const uint32_t at = lanes + C::S_COL + half * C::HALF + c;
-        ptx::tmem_ld_32x8(at, s0);
-        ptx::tmem_ld_32x8(at + NK, s1);
+        tmem_ld(at, s0);
+        tmem_ld(at + NK, s1);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
+        for (int e = 0; e < C::RB; e += 2) {
           const float2 u = low_digits(s1 + e, s0 + e);
           x[c + e] = u.x;
           x[c + e + 1] = u.y;
         }
       }
 #pragma unroll
-      for (int c = 0; c < C::HALF; c += 8) {
-        uint32_t s2[8];
-        ptx::tmem_ld_32x8(lanes + C::S_COL + 2 * NK + half * C::HALF + c, s2);
+      for (int c = 0; c < C::HALF; c += C::RB) {
+        uint32_t s2[C::RB];
+        tmem_ld(lanes + C::S_COL + 2 * NK + half * C::HALF + c, s2);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
+        for (int e = 0; e < C::RB; e += 4) {
           const float4 k = *reinterpret_cast<const float4 *>(ks + c + e);
           const float4 v = *reinterpret_cast<const float4 *>(lvs + c + e);
           float2 y = __fmul2_rn(high_digit(s2 + e, make_float2(x[c + e], x[c + e + 1])), make_float2(k.x, k.y));
@@ -469,9 +504,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       }
       top = fmaxf(top, top2);
       smax[(grp * 2 + half) * kRows + row] = top;
-      // the other group reads these scales after this tile's decision
-      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
-      next = fetch_scale(j + 3);
       const bool moved = ptx::named_bar_or(1 + grp, kGroup, top > m + kSlack || (m == -INFINITY && top > m) || !ok);
       if (moved && ptx::named_bar_or(1 + grp, kGroup, !ok)) break;
       const float to = moved ? fmaxf(m, fmaxf(top, smax[(grp * 2 + (half ^ 1)) * kRows + row])) : m;
@@ -502,26 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         }
       }
       l += lt.x + lt.y;
-      // V codes of this tile to fp16; 8 columns of a key per thread.  Keys past
-      // the range hold an earlier tile's codes, which weigh nothing.
-      ok = wait(&bars.v8full[j & 1], (j >> 1) & 1, DEV_TIMEOUT_FULL) && ok;
-      if (j > 1) ok = wait(&bars.pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
-      {
-        constexpr int L = HD / 8, KS = kGroup / L;
-        const int c = tid % L, key0 = tid / L;
-        const uint8_t *src = smem + C::V8_OFF + (j % C::NV8) * C::V8_BYTES + c * 8;
-        uint8_t *dst = smem + C::V16_OFF + (j & 1) * C::V16_BYTES + (c >> 3) * C::V16_BLOCK;
-#pragma unroll
-        for (int k = 0; k < NK; k += KS) {
-          const int key = key0 + k;
-          const uint2 w = *reinterpret_cast<const uint2 *>(src + key * HD);
-          const uint2 x = to_half4(w.x), y = to_half4(w.y);
-          *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
-        }
-        ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
-        ptx::mbar_arrive(&bars.v16full[j & 1]);
-      }
+      if (HD != 256) convert(j);
       // P and T are free once the previous tile's product is done
       if (j > 0) {
         ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
