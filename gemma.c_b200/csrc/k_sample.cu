@@ -87,7 +87,8 @@ struct Shared {
 
 struct Row {
   const float *x;       // the row
-  const float *held;    // this warp's slice in shared memory, or null
+  const float *held;    // this warp's slice in shared memory
+  bool holds;           // whether it is there
   double table;         // 2^(lane/32)
   int w0, w1;           // this warp's contiguous elements
   float max;
@@ -133,7 +134,7 @@ struct Row {
   __device__ __forceinline__ void each4(int lane, F f) const {
     for (int b = w0; b < w1; b += 128) {
       float v[4];
-      if (held) {
+      if (holds) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = held[b - w0 + 32 * j + lane];
       } else {
@@ -496,7 +497,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   r.x = a.logits + (long)row * a.ld;
   r.w0 = min(a.n, (rank * kWarps + warp) * per_warp);
   r.w1 = min(a.n, r.w0 + per_warp);
-  r.held = nullptr;
+  r.held = s.values + warp * kKeep;
+  r.holds = per_warp <= kKeep;
   r.inf = false;
   r.table = exp2((double)lane / kTable);
   if (tid == 0) {
@@ -505,7 +507,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   }
   ptx::griddep_wait();
   float top = -INFINITY;
-  if (per_warp <= kKeep) {
+  if (r.holds) {
     float *hold = s.values + warp * kKeep;
     for (int b = lane; b - lane < r.w1 - r.w0; b += 256) {
       float v[8];
@@ -522,7 +524,6 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
       }
     }
     __syncwarp();
-    r.held = hold;
   } else {
     r.each(lane, [&](int, float v) { top = fmaxf(top, v); });
   }
@@ -570,7 +571,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
     r.inf = true;
     r.max = 0.0f;
     float *hold = s.values + warp * kKeep;
-    if (r.held)
+    if (r.holds)
       for (int i = lane; i < kKeep; i += 32) hold[i] = r.counted(hold[i]);
     __syncwarp();
   }
@@ -621,7 +622,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
     return c.keeps(v, i) && (double)w >= least ? w : 0;
   };
   u64 mine = 0;
-  if (r.held) {
+  if (r.holds) {
     // what the cuts keep, often few, moves to the front of the warp's slice
     float *hold = s.values + warp * kKeep;
     int n = 0;
