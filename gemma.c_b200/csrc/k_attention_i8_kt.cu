@@ -269,11 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       return t < n ? __ldg(src + kbeg + t) : 1.0f;
     };
     const float inv_cap = CAP ? 1.0f / a.sc_att : 0.0f, unit = CAP ? a.sc_att * kLog2e : kLog2e;
-    float rf[RQ], l[RQ];
+    float rf[RQ], l[RQ], lim[RQ];  // lim: the largest exponent that fits, m + kSlack
 #pragma unroll
     for (int r = 0; r < RQ; ++r) {
       rf[r] = nt > 0 ? s_rf[r0 + r] : 0.0f;
       l[r] = 0.0f;
+      lim[r] = -INFINITY;
     }
     // the output column of this thread, a lane of O^T, and its rows of it (hdim 256:
     // two blocks of columns, half of the rows each; else a quarter)
@@ -343,10 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       }
       bool over = !ok;
 #pragma unroll
-      for (int r = 0; r < RQ; ++r) {
-        const float m = s_m[r0 + r];
-        over |= x[r] > m + kSlack || (m == -INFINITY && x[r] > m);
-      }
+      for (int r = 0; r < RQ; ++r) over |= x[r] > lim[r];
       bool fresh = j == 0;
       if (ptx::named_bar_or(1, kSoftmax, over)) {
         // some row's weights would run over: move every row's m to its largest
@@ -376,7 +374,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
         for (int r = 0; r < C::OR; ++r) acc[r] *= s_f[orow + r];
 #pragma unroll
-        for (int r = 0; r < RQ; ++r) l[r] *= s_f[r0 + r];
+        for (int r = 0; r < RQ; ++r) {
+          l[r] *= s_f[r0 + r];
+          lim[r] = s_m[r0 + r] + kSlack;
+        }
         fresh = true;
       }
       // this buffer's last reader is the product of tile j - 2
@@ -384,8 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       uint32_t w[RQ];
 #pragma unroll
       for (int r = 0; r < RQ; ++r) {
-        const float m = s_m[r0 + r];
-        const float v = ex2(x[r] - (m == -INFINITY ? 0.0f : m - kTop));
+        const float v = ex2(x[r] - (lim[r] == -INFINITY ? 0.0f : lim[r] - (kSlack + kTop)));
         l[r] = __fmaf_rn(v, rvs, l[r]);
         w[r] = __float2uint_rn(v);
       }
