@@ -25,6 +25,13 @@ a chunk of tokens the same way, with one GEMM over wq|wk|wv (the values of
 gemma.c's per-head GEMMs), the tensor-core GEMMs for the projections, and
 the causal attention kernel.
 
+With kv_bits=8 the KV cache holds int8 codes and a scale per row (a quarter of
+the memory; gcu_kv_i8): the step and the prefill then use
+gcu_dev_qkv_norm_rope_cache_i8 and the attention over that cache.  `fork`
+starts several sequences from the prompt in the cache, which they share, and
+`step_seqs` decodes one token of each; `sample` draws the next tokens from the
+logits of the last step.
+
 Weights follow gemma.c's TextDecoder (gemma.c:1174-1301); torch only holds
 the device memory and the stream.  The RoPE tables are computed on the host
 per position as rope_freqs does (gemma.c:4178-4216) unless the caller passes
@@ -61,9 +68,11 @@ class Decoder:
     eps, sc_att, sc_log.  layers: per layer a dict of (q, scales) numpy pairs
     wq, wk, wv, wo, w1 (up), w2 (gate), w3 (down) and norm vectors n1..n4, nq,
     nk.  emb: the tied embedding (q, scales) used as lm_head; fnorm: the final
-    norm.  clen: KV-cache positions."""
+    norm.  clen: KV-cache positions.  kv_bits: 32 (fp32 cache) or 8."""
 
-    def __init__(self, cfg: dict, layers: list, emb, fnorm, clen: int, device="cuda"):
+    def __init__(self, cfg: dict, layers: list, emb, fnorm, clen: int, device="cuda", kv_bits: int = 32):
+        if kv_bits not in (8, 32):
+            raise ValueError(f"a KV cache of 8 or 32 bits, not {kv_bits}")
         import torch
         self.torch = torch
         self.cfg = cfg
@@ -82,13 +91,22 @@ class Decoder:
         q_sz = c["n_heads"] * c["hdim"]
         f32 = dict(dtype=torch.float32, device=device)
         i8 = dict(dtype=torch.int8, device=device)
-        self.kv = torch.zeros((c["nl"], 2, c["nkv"], clen, c["hdim"]), **f32)
+        self.kv_bits = kv_bits
+        if kv_bits == 8:
+            self.kv8 = [gcu.KvCacheI8.empty(1, c["nkv"], clen, c["hdim"], device) for _ in range(c["nl"])]
+        else:
+            self.kv = torch.zeros((c["nl"], 2, c["nkv"], clen, c["hdim"]), **f32)
+        self.nseq = 0
         self.x = torch.empty((1, c["dim"]), **f32)
         self.x2 = torch.empty((1, c["dim"]), **f32)  # the residual stream alternates between x and x2
         self.out = torch.empty((1, c["dim"]), **f32)
-        self.xq = torch.empty((c["n_heads"], 1, c["hdim"]), **f32)
-        self.xk = torch.empty((c["nkv"], 1, c["hdim"]), **f32)
-        self.xv = torch.empty((c["nkv"], 1, c["hdim"]), **f32)
+        # the projections of one token, q|k|v in one row
+        kv_sz = c["nkv"] * c["hdim"]
+        self.qkv = torch.empty((1, q_sz + 2 * kv_sz), **f32)
+        self.xq = self.qkv[0, :q_sz].view(c["n_heads"], 1, c["hdim"])
+        self.xk = self.qkv[0, q_sz:q_sz + kv_sz].view(c["nkv"], 1, c["hdim"])
+        self.xv = self.qkv[0, q_sz + kv_sz:].view(c["nkv"], 1, c["hdim"])
+        self.xqr = torch.empty((c["n_heads"], 1, c["hdim"]), **f32)  # rotated queries (8-bit cache)
         self.xo = torch.empty((1, q_sz), **f32)
         self.xg = torch.empty((1, c["mlp_dim"]), **f32)
         self.xu = torch.empty((1, c["mlp_dim"]), **f32)
@@ -129,14 +147,20 @@ class Decoder:
         for l, w in enumerate(self.L):
             # gemma.c:4775-4848: QK norm, RoPE and the cache write of position
             # pos, then attention over [spos, pos] -- one launch
-            kc, vc = self.kv[l, 0], self.kv[l, 1]
             sliding = bool(c["swa"][l])
-            spos = pos + 1 - c["slide"] if sliding and pos >= c["slide"] else 0
-            gcu.dev_attention_decode_rope(self.xo.view(nh, hdim), self.xq.view(nh, hdim), self.xk.view(nkv, hdim),
-                                          self.xv.view(nkv, hdim), kc, vc, self.freqs[0 if sliding else 1], spos,
-                                          pos + 1 - spos, asc, c["sc_att"],
-                                          nq=w["nq"] if c["qk_norm"] else None,
-                                          nk=w["nk"] if c["qk_norm"] else None, eps=eps, stream=stream)
+            norms = dict(nq=w["nq"] if c["qk_norm"] else None, nk=w["nk"] if c["qk_norm"] else None, eps=eps,
+                         stream=stream)
+            if self.kv_bits == 8:  # two launches: the row's scale is known when the whole row is
+                gcu.dev_qkv_norm_rope_cache_i8(self.xqr, self.qkv, self.kv8[l],
+                                               self.freqs[0:1] if sliding else self.freqs[1:2], pos, **norms)
+                gcu.dev_attention_decode_i8(self.xo.view(1, nh, hdim), self.xqr.view(1, nh, hdim), self.kv8[l], None,
+                                            pos + 1, asc, c["sc_att"], c["slide"] if sliding else 0, stream=stream)
+            else:
+                kc, vc = self.kv[l, 0], self.kv[l, 1]
+                spos = pos + 1 - c["slide"] if sliding and pos >= c["slide"] else 0
+                gcu.dev_attention_decode_rope(self.xo.view(nh, hdim), self.xq.view(nh, hdim), self.xk.view(nkv, hdim),
+                                              self.xv.view(nkv, hdim), kc, vc, self.freqs[0 if sliding else 1], spos,
+                                              pos + 1 - spos, asc, c["sc_att"], **norms)
             # gemma.c:4855-4860: O projection (quantize_act of the attention
             # output in the same launch)
             gcu.dev_quantize_gemm_int8_multi([(w["wo"][0], w["wo"][1], self.out)], q, self.s, self.xo, 1, q_sz,
@@ -231,14 +255,19 @@ class Decoder:
             gcu.dev_gemm_int8(self.pqkv[:n], self.wqkv[l][0], self.wqkv[l][1], q_dim, ps, n, q_sz + 2 * kv_sz, dim,
                               stream=stream)
             # gemma.c:5095-5145: QK norm, RoPE (queries scaled), cache write
-            kc, vc = self.kv[l, 0], self.kv[l, 1]
             sliding = bool(c["swa"][l])
-            gcu.dev_qkv_norm_rope_cache(xq, self.pqkv[:n], kc, vc, self.pfreq[0 if sliding else 1, :n], spos, nh,
-                                        asc, w["nq"] if c["qk_norm"] else None, w["nk"] if c["qk_norm"] else None,
-                                        eps, stream=stream)
-            # gemma.c:5160-5295: causal attention, sliding window on local layers
-            gcu.dev_attention_prefill(self.pxo[:n], xq, kc, vc, spos, c["slide"] if sliding else 0, c["sc_att"],
-                                      True, stream=stream)
+            freq, slide = self.pfreq[0 if sliding else 1, :n], c["slide"] if sliding else 0
+            nq, nk = (w["nq"], w["nk"]) if c["qk_norm"] else (None, None)
+            # and causal attention, sliding window on local layers (gemma.c:5160-5295)
+            if self.kv_bits == 8:
+                gcu.dev_qkv_norm_rope_cache_i8(xq, self.pqkv[:n], self.kv8[l], freq, spos, asc, nq, nk, eps,
+                                               stream=stream)
+                gcu.dev_attention_prefill_i8(self.pxo[:n], xq, self.kv8[l], spos, slide, c["sc_att"], True,
+                                             stream=stream)
+            else:
+                kc, vc = self.kv[l, 0], self.kv[l, 1]
+                gcu.dev_qkv_norm_rope_cache(xq, self.pqkv[:n], kc, vc, freq, spos, nh, asc, nq, nk, eps, stream=stream)
+                gcu.dev_attention_prefill(self.pxo[:n], xq, kc, vc, spos, slide, c["sc_att"], True, stream=stream)
             # gemma.c:5296-5340: O projection, post-attention norm + residual,
             # pre-FFN norm + quantize
             gcu.dev_quantize_gemm_int8_multi([(w["wo"][0], w["wo"][1], pout)], q_qsz, ps, self.pxo[:n], n, q_sz,
@@ -264,6 +293,101 @@ class Decoder:
         if c["sc_log"]:
             gcu.dev_softcap(self.logits, c["sc_log"], stream=stream)
 
+    # ---- several sequences from one prompt (8-bit cache) ------------------------
+    def fork(self, nseq: int, plen: int, tail: int):
+        """Start nseq sequences from the first plen positions of the cache, which they
+        share, each with a cache of its own for `tail` further tokens."""
+        if self.kv_bits != 8:
+            raise ValueError("fork: sequences share an 8-bit KV cache (kv_bits=8)")
+        if nseq < 1 or tail < 1 or not 0 <= plen <= self.clen:
+            raise ValueError(f"fork of {nseq} sequences with {tail} tokens from {plen} of {self.clen} positions")
+        torch, c = self.torch, self.cfg
+        f32 = dict(dtype=torch.float32, device=self.dev)
+        i8 = dict(dtype=torch.int8, device=self.dev)
+        dim, mlp, hd = c["dim"], c["mlp_dim"], c["hdim"]
+        q_sz, kv_sz = c["n_heads"] * hd, c["nkv"] * hd
+        self.nseq, self.plen, self.tail = nseq, plen, tail
+        self.own8 = [gcu.KvCacheI8.empty(nseq, c["nkv"], tail, hd, self.dev) for _ in range(c["nl"])]
+        self.slen = torch.zeros(nseq, dtype=torch.int32, device=self.dev)  # tokens of each sequence's own
+        self.sx = torch.empty((nseq, dim), **f32)
+        self.sqkv = torch.empty((nseq, q_sz + 2 * kv_sz), **f32)
+        self.sxq = torch.empty((nseq, c["n_heads"], hd), **f32)
+        self.sxo = torch.zeros((nseq, q_sz), **f32)
+        self.sout = torch.empty((nseq, dim), **f32)
+        self.sxg = torch.empty((nseq, mlp), **f32)
+        self.sxu = torch.empty((nseq, mlp), **f32)
+        self.sq = [torch.empty((nseq, n), **i8) for n in (dim, q_sz, mlp)]
+        self.ss = torch.empty(nseq, **f32)
+        self.slogits = torch.empty((nseq, c["nvocab"]), **f32)
+        self.sfreq = torch.empty((2, nseq, hd), **f32)  # sliding, full
+        if not hasattr(self, "wqkv"):
+            self.wqkv = [(torch.cat([w["wq"][0], w["wk"][0], w["wv"][0]]).contiguous(),
+                          torch.cat([w["wq"][1], w["wk"][1], w["wv"][1]]).contiguous()) for w in self.L]
+
+    def set_seq_freqs(self, slid, full):
+        """Upload the RoPE tables (nseq, hdim) of the positions about to be decoded: plen +
+        the sequence's own tokens so far."""
+        torch = self.torch
+        self.sfreq.copy_(torch.from_numpy(np.stack([np.asarray(slid, np.float32), np.asarray(full, np.float32)])))
+
+    def step_seqs(self, stream=None):
+        """Decode one token of every forked sequence from the embeddings in self.sx
+        (nseq, dim): the step of forward_text_decode for all of them at once, the
+        attention over the shared prompt computed once for all.  Leaves the logits
+        in self.slogits and the final hidden states in self.sx, and counts the
+        tokens in self.slen; a sequence whose self.slen is negative stands still
+        (its logits mean nothing).  Set the tables with set_seq_freqs beforehand."""
+        if not self.nseq:
+            raise ValueError("step_seqs: fork first")
+        c, n = self.cfg, self.nseq
+        dim, mlp, hd, nh = c["dim"], c["mlp_dim"], c["hdim"], c["n_heads"]
+        q_sz, kv_sz = nh * hd, c["nkv"] * hd
+        asc = float(np.float32(1.0) / np.sqrt(np.float32(c["q_scale"])))
+        eps, x, ps, out = c["eps"], self.sx, self.ss, self.sout
+        q_dim, q_qsz, q_mlp = self.sq
+        with self.torch.cuda.stream(stream) if stream is not None else _null():
+            self.slen.add_((self.slen >= 0).to(self.slen.dtype))
+        gcu.dev_rmsnorm_quantize(q_dim, ps, x, self.L[0]["n1"], eps, n, dim, stream=stream)
+        for l, w in enumerate(self.L):
+            gcu.dev_gemm_int8(self.sqkv, self.wqkv[l][0], self.wqkv[l][1], q_dim, ps, n, q_sz + 2 * kv_sz, dim,
+                              stream=stream)
+            sliding = bool(c["swa"][l])
+            nq, nk = (w["nq"], w["nk"]) if c["qk_norm"] else (None, None)
+            gcu.dev_qkv_norm_rope_cache_i8_seqs(self.sxq, self.sqkv, self.own8[l], self.slen,
+                                                self.sfreq[0 if sliding else 1], 1.0, nq, nk, eps, stream=stream)
+            gcu.dev_attention_decode_i8(self.sxo.view(n, nh, hd), self.sxq, self.own8[l], self.slen, self.tail, asc,
+                                        c["sc_att"], c["slide"] if sliding else 0, self.kv8[l], self.plen,
+                                        stream=stream)
+            gcu.dev_quantize_gemm_int8_multi([(w["wo"][0], w["wo"][1], out)], q_qsz, ps, self.sxo, n, q_sz,
+                                             stream=stream)
+            gcu.dev_residual_norm_quantize(x, q_dim, ps, out, x, w["n2"] if c["mlp_pre"] else None,
+                                           w["n3"] if c["mlp_pre"] else w["n2"], eps, n, dim, stream=stream)
+            gcu.dev_gemm_int8(self.sxg, w["w2"][0], w["w2"][1], q_dim, ps, n, mlp, dim, stream=stream)
+            gcu.dev_gemm_int8(self.sxu, w["w1"][0], w["w1"][1], q_dim, ps, n, mlp, dim, stream=stream)
+            gcu.dev_geglu_quantize(q_mlp, ps, self.sxg, self.sxu, n, mlp, stream=stream)
+            gcu.dev_gemm_int8(out, w["w3"][0], w["w3"][1], q_mlp, ps, n, dim, mlp, stream=stream)
+            post = w["n4"] if c["mlp_pst"] else None
+            if l + 1 < len(self.L):
+                gcu.dev_residual_norm_quantize(x, q_dim, ps, out, x, post, self.L[l + 1]["n1"], eps, n, dim,
+                                               stream=stream)
+            else:
+                gcu.dev_rmsnorm_residual(x, out, x, post, eps, n, dim, stream=stream)
+        gcu.dev_rmsnorm_quantize(q_dim, ps, x, self.fnorm, eps, n, dim, out=x, stream=stream)
+        gcu.dev_gemm_int8(self.slogits, self.emb[0], self.emb[1], q_dim, ps, n, c["nvocab"], dim, stream=stream)
+        if c["sc_log"]:
+            gcu.dev_softcap(self.slogits, c["sc_log"], stream=stream)
+
+    def sample(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seqs=False, prob=None, stream=None):
+        """The next token of each row of the last step's logits (of step_seqs when
+        seqs, else of step or prefill) from the random numbers u (rows,) float32
+        on the device; int32 (rows,).  See gcu.dev_sample."""
+        logits = self.slogits if seqs else self.logits
+        token = self.torch.empty(logits.shape[0], dtype=self.torch.int32, device=self.dev)
+        if stream is not None:
+            token.record_stream(stream)
+        gcu.dev_sample(token, logits, u, temperature, top_k, top_p, min_p, prob=prob, stream=stream)
+        return token
+
     def launches_per_step(self, prefill: bool = False) -> int:
         """Kernel launches of one decode step (5 per layer: the residual
         updates, norms, GeGLU and quantize steps run in front of the GEMVs
@@ -271,10 +395,11 @@ class Decoder:
         the first layer's norm and Q/K/V) or one prefill chunk (11 per layer:
         the chunk merge of the attention and the separate quantize of the O
         projection's input at m > 8); an attention window split over CTAs adds
-        its merge launch to the decode count."""
+        its merge launch to the decode count, and an 8-bit cache the launch
+        that writes it."""
         if prefill:
             return 11 * self.cfg["nl"] + 3 + (1 if self.cfg["sc_log"] else 0)
-        return 5 * self.cfg["nl"] + 4 + (1 if self.cfg["sc_log"] else 0)
+        return (6 if self.kv_bits == 8 else 5) * self.cfg["nl"] + 4 + (1 if self.cfg["sc_log"] else 0)
 
 
 class _null:
