@@ -89,9 +89,16 @@ struct Plan {
   int chunk, splits;
 };
 
+// Splits of n keys in tiles for `units` CTAs a split, of `ctas` in all.  However many
+// units there are, a CTA takes at most kMaxKeys: decode's sums of byte products are
+// 32-bit (66,312 keys of 255*127 fit), and a thread's fp32 sum of weights then has
+// at most 128 terms in a row.  At 128 tiles the set-up of a further CTA is 1.5%.
+constexpr long kMaxKeys = 16384;
+
 Plan plan_range(long n, long units, long ctas, int tile) {
   if (n < 1) n = 1;
-  const long tiles = (n + tile - 1) / tile, want = std::min(tiles, std::max(1l, ctas / units));
+  const long tiles = (n + tile - 1) / tile, least = (n + kMaxKeys - 1) / kMaxKeys;
+  const long want = std::min(tiles, std::max(least, ctas / units));
   Plan p;
   p.chunk = (int)((tiles + want - 1) / want * tile);
   p.splits = (int)((n + p.chunk - 1) / p.chunk);

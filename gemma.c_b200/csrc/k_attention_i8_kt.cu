@@ -11,9 +11,9 @@
 //                             MN-major: V's tile as it lies is V^T)
 // Weights are 32-bit fixed point, W = round(2^(s + log2 vs - m)), m placed so that
 // the row's largest weight so far is 2^24 at least and 2^31.5 at most; rounding
-// is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 65536
-// keys fits), so nothing is lost however long the range, and only moves to fp32
-// registers when a row's m has to move.
+// is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 66,312
+// keys fits, and the plan gives a CTA fewer), so nothing is lost, and only moves
+// to fp32 registers when a row's m has to move.
 //
 // Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
 // against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM.

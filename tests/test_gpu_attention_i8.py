@@ -269,3 +269,61 @@ def test_side_stream():
     s.synchronize()
     want, tol = R.decode(xq, c, [3000], 0.125, 0.0, 0)
     check(xo, want, tol)
+
+
+def same_rows(nseq, nkv, clen, hd):
+    """A cache whose rows are all alike, codes at 127, but for a first key a little larger: every
+    other weight is 0.997 of the largest, so that its leading byte is 255."""
+    c = gcu.KvCacheI8.empty(nseq, nkv, clen, hd, "cuda")
+    c.k.fill_(127)
+    c.v.fill_(127)
+    c.ks.fill_(1.5 / 127)
+    c.ks[:, :, 0] = 1.503 / 127
+    c.vs.fill_(0.5)
+    return c
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_decode_sums_of_very_long_ranges(shared):
+    """More rows than there are SMs, so that one CTA could take a whole range, over a cache
+    longer than a 32-bit sum of byte products holds (66,312 keys of 255*127)."""
+    hd, n = 64, 70001
+    if shared:
+        nseq, nh, nkv = 592, 8, 1
+        pre, own = same_rows(1, nkv, n, hd), same_rows(nseq, nkv, 4, hd)
+        length = torch.zeros(nseq, dtype=torch.int32, device="cuda")
+    else:
+        nseq, nh, nkv = 149, 1, 1
+        pre, own, length = None, same_rows(nseq, nkv, n, hd), torch.full((nseq,), n, dtype=torch.int32, device="cuda")
+    xq = torch.full((nseq, nh, hd), 1.0 / hd, device="cuda")
+    xo = torch.empty_like(xq)
+    gcu.dev_attention_decode_i8(xo, xq, own, length, own.k.shape[2], 1.0, 0.0, 0, pre, n if shared else 0)
+    # The mean of equal rows.  fp32 sums of at most 128 equal weights in a row, each step off by half a
+    # step of the sum so far: 64 * 2^-24 of the total; 20 for the few sums that join them and the division.
+    check(xo, np.full(xq.shape, 63.5), 63.5 * 84 * 2.0 ** -24)
+
+
+def test_two_streams_at_once():
+    """Decode and prefill of two streams, each with scratch of its own."""
+    rng = np.random.default_rng(12)
+    c = R.cache(rng, 2, 2, 5000, 128)
+    xq = rng.standard_normal((2, 8, 128), dtype=np.float32)
+    xp = rng.standard_normal((8, 40, 128), dtype=np.float32)
+    kv, q, p = handle(c), dev(xq), dev(xp)
+    want, tol = R.decode(xq, c, [4999, 3000], 128 ** -0.5, 0.0, 0)
+    wantp, tolp = R.prefill(xp, [t[:1] for t in c], 4960, 0, 0.0, True)
+    length = dev(np.asarray([4999, 3000], np.int32))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                xo, po = torch.empty_like(q), torch.empty((40, 8 * 128), device="cuda")
+                gcu.dev_attention_decode_i8(xo, q, kv, length, 5000, 128 ** -0.5)
+                gcu.dev_attention_prefill_i8(po, p, kv.seq(0), 4960)
+                outs.append((xo, po))
+    torch.cuda.synchronize()
+    for xo, po in outs:
+        check(xo, want, tol)
+        check(po, wantp, tolp)
