@@ -27,6 +27,7 @@
 #include <cooperative_groups.h>
 
 #include <mutex>
+#include <utility>
 
 #define GCU_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -489,6 +490,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   Shared &s = *reinterpret_cast<Shared *>(raw);
   ptx::griddep_launch();
   cg::cluster_group cl = cg::this_cluster();
+  auto started = cl.barrier_arrive();  // waited for before the first access to another CTA
   const int rank = cl.block_rank(), row = blockIdx.x / kCluster;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // contiguous slices of CTAs and warps, in index order, multiples of 128
@@ -535,6 +537,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   top = warp_max[lane];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  cl.barrier_wait(std::move(started));
   if (tid < kCluster) cl.map_shared_rank(&s, tid)->maxes[rank] = top;
   cl.sync();
   r.max = s.maxes[0];
@@ -577,8 +580,8 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   }
   r.scale = 1.4426950408889634 / (double)a.temperature;
   r.max_d = (double)r.max;
-  r.least = (float)(r.max_d - 63.0 / r.scale);
-  r.bin_scale = kBinsPerNat / a.temperature;
+  r.least = fmaxf((float)(r.max_d - 63.0 / r.scale), -3.4028235e38f);  // -inf lies below it
+  r.bin_scale = fminf(kBinsPerNat / a.temperature, 3.4028235e38f);     // 0 times it is 0
   r.one = a.one;
   Cut c;
   const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
@@ -699,8 +702,6 @@ GCU_EXPORT int gcu_dev_sample(int *token, float *prob, const float *logits, long
       !(min_p >= 0.0f && min_p <= 1.0f))
     return set_error("sample: temperature %g, top_k %d, top_p %g, min_p %g (finite and >= 0; >= 0; > 0; 0 to 1)",
                      temperature, top_k, top_p, min_p);
-  // largest weight exponent: (max - x) / T must not leave fp32 as 0 / 0
-  if (temperature > 0.0f && temperature < 1e-30f) temperature = 1e-30f;
   double one = 9223372036854775808.0;  // 2^63, halved until nvocab of them fit
   for (long n = 1; n < nvocab; n <<= 1) one *= 0.5;
   one = one > 2251799813685248.0 ? 2251799813685248.0 : one;  // and 2^51 at most, a whole number of a double

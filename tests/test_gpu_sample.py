@@ -120,3 +120,49 @@ def test_same_answer_in_every_call_and_graph():
     u.fill_(0.0)
     g.replay()
     assert token.tolist() == [R.sample(r, 0.0, 1.0, 0, 0.9, 0.0)[0] for r in x.cpu().numpy()]
+
+
+@pytest.mark.parametrize("t,k,p,minp", SETTINGS)
+@pytest.mark.parametrize("n", [262145, 400001, 1 << 20])
+def test_rows_longer_than_shared_memory(n, t, k, p, minp):
+    rng = np.random.default_rng(n)
+    x = (rng.standard_normal((3, n)) * 3).astype(np.float32)
+    x[1] = rng.integers(0, 2, n)  # ties
+    x[2, ::3] = np.nan
+    x[2, [n - 5, 70]] = np.inf
+    check(x, np.array([0.3, 0.6, 0.7], np.float32), t, k, p, minp)
+
+
+@pytest.mark.parametrize("t", [1e-45, 1e-38, 1e-20, 1e20, 3e38])
+@pytest.mark.parametrize("k,p,minp", [(0, 1.0, 0.0), (20, 1.0, 0.0), (0, 0.9, 0.0), (900, 0.4, 0.3)])
+def test_extreme_temperatures(t, k, p, minp):
+    rng = np.random.default_rng(16)
+    x = rng.standard_normal((5, 3001)).astype(np.float32)
+    x[1, 100:] = -np.inf
+    x[2] = np.float32(1e-45) * rng.integers(0, 4, 3001).astype(np.float32)  # steps of the smallest float
+    x[3] = np.where(rng.random(3001) < 0.5, -3.4028235e38, 3.4028235e38)
+    x[4, 1::2] = np.nan
+    check(x, np.array([0.2, 0.9, 0.5, 0.7, 0.999], np.float32), t, k, p, minp)
+
+
+def test_many_rows():
+    rng = np.random.default_rng(17)
+    x, u = (rng.standard_normal((700, 517)) * 2).astype(np.float32), rng.random(700, dtype=np.float32)
+    check(x, u, 0.8, 30, 0.9, 0.02)
+    check(x, u)
+
+
+def test_two_streams_at_once():
+    rng = np.random.default_rng(18)
+    x, u = (rng.standard_normal((40, 20001)) * 2).astype(np.float32), rng.random(40, dtype=np.float32)
+    want = [R.sample(r, v, 0.9, 0, 0.9, 0.0)[0] for r, v in zip(x, u)]
+    dx, du = torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda()
+    torch.cuda.synchronize()
+    outs, streams = [], [torch.cuda.Stream() for _ in range(3)]
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            token = torch.empty(40, dtype=torch.int32, device="cuda")
+            gcu.dev_sample(token, dx, du, 0.9, 0, 0.9)
+            outs.append(token)
+    torch.cuda.synchronize()
+    assert all(t.tolist() == want for t in outs)
