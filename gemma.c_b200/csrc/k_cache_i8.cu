@@ -11,11 +11,14 @@
 // sum of squares is taken in 64 bits (its order cannot show in 32) and every
 // fp32 step is rounded by itself.
 //
-// One warp per head row; lane l holds elements [l*E, l*E + E) of each half
-// (E = hdim/64), so both elements of a RoPE pair sit in one lane, loads and
-// stores are coalesced and only the two row reductions cross lanes.
+// A warp takes four heads of a token, lane l elements [l*E, l*E + E) of each half of
+// each row (E = hdim/64), so both elements of a RoPE pair sit in one lane, loads
+// and stores are coalesced, the tables and norm weights are read once for four
+// rows, and only the two row reductions cross lanes, for four rows at once.
 // HBM-bound: per token 4*(nh + 2*nkv)*hdim bytes in, 4*nh*hdim + nkv*(2*hdim +
-// 8) out.
+// 8) out.  4096 tokens of 16 + 8 + 8 heads of 256: 45 us for 222 MB (4.9 TB/s,
+// with an L2 full of another kernel's output to write back); one row per warp took
+// 55, with 285 instructions a row against 120.  Reading them back: 20 us, 84 MB.
 #include "gcu_internal.cuh"
 
 #define GCU_EXPORT extern "C" __attribute__((visibility("default")))
@@ -23,7 +26,11 @@
 namespace gcu {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;       // of k_read
+constexpr int kWriteThreads = 128;  // of k_write
+constexpr int kRows = 4;            // head rows of a warp
+
+__host__ __device__ __forceinline__ int groups(int heads) { return (heads + kRows - 1) / kRows; }
 
 struct WriteArgs {
   float *xq;
@@ -61,6 +68,14 @@ template <int E>
 __device__ __forceinline__ void load(float (&v)[E], const float *p) {
   *reinterpret_cast<typename Vec<E>::F *>(v) = __ldg(reinterpret_cast<const typename Vec<E>::F *>(p));
 }
+// a lane's 2*E floats of a RoPE table row
+template <int E>
+__device__ __forceinline__ void load_table(float (&v)[2 * E], const float *p) {
+  using F = typename Vec<E == 1 ? 2 : 4>::F;
+#pragma unroll
+  for (int i = 0; i < 2 * E; i += sizeof(F) / 4)
+    *reinterpret_cast<F *>(v + i) = __ldg(reinterpret_cast<const F *>(p + i));
+}
 template <int E>
 __device__ __forceinline__ void store(float *p, const float (&v)[E]) {
   *reinterpret_cast<typename Vec<E>::F *>(p) = *reinterpret_cast<const typename Vec<E>::F *>(v);
@@ -77,35 +92,63 @@ __device__ __forceinline__ double rsqrt64(double x) {
   return y * (1.5 - 0.5 * x * y * y);
 }
 
-// a, b: the lane's elements of the first and second half; fr: the lane's table
-// entries (cos, sin per element)
+// Lane l of 32 gets row l / 8's total of v[row] over the lanes: the first two
+// steps halve the rows that a lane carries, so four rows take 6 exchanges, not 20.
+template <typename T, typename F>
+__device__ __forceinline__ T reduce_rows(const T (&v)[kRows], int lane, F op) {
+  const bool up = lane & 16, odd = lane & 8;
+  T a = up ? v[2] : v[0], b = up ? v[3] : v[1];
+  a = op(a, __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16));
+  b = op(b, __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16));
+  T c = odd ? b : a;
+  c = op(c, __shfl_xor_sync(0xffffffffu, odd ? a : b, 8));
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) c = op(c, __shfl_xor_sync(0xffffffffu, c, o));
+  return c;
+}
+
+// a, b: the lane's elements of the first and second half of each row; w: the norm's
+// weights, or null; t: the lane's table entries (cos, sin per element)
 template <int E>
-__device__ __forceinline__ void norm_rope(float (&a)[E], float (&b)[E], const float *w, float eps, const float *fr,
-                                          float scale, int lane) {
+__device__ __forceinline__ void norm_rope(float (&a)[kRows][E], float (&b)[kRows][E], const float *w, float eps,
+                                          const float (&t)[2 * E], float scale, int lane) {
   constexpr int HD = 64 * E;
   if (w) {
-    double sq = 0.0;
-#pragma unroll
-    for (int i = 0; i < E; ++i) sq += (double)a[i] * a[i] + (double)b[i] * b[i];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-    const float rms = (float)rsqrt64(sq / HD + (double)eps);
     float wa[E], wb[E];
     load<E>(wa, w + lane * E);
     load<E>(wb, w + HD / 2 + lane * E);
+    double sq[kRows];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      a[i] = __fmul_rn(__fmul_rn(a[i], rms), __fadd_rn(wa[i], 1.0f));
-      b[i] = __fmul_rn(__fmul_rn(b[i], rms), __fadd_rn(wb[i], 1.0f));
+    for (int r = 0; r < kRows; ++r) {
+      sq[r] = 0.0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const double x = a[r][i], y = b[r][i];
+        sq[r] = fma(x, x, fma(y, y, sq[r]));
+      }
+    }
+    const double sum = reduce_rows(sq, lane, [](double x, double y) { return x + y; });
+    const float mine = (float)rsqrt64(sum * (1.0 / HD) + (double)eps);
+#pragma unroll
+    for (int i = 0; i < E; ++i) wa[i] = __fadd_rn(wa[i], 1.0f), wb[i] = __fadd_rn(wb[i], 1.0f);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      const float rms = __shfl_sync(0xffffffffu, mine, 8 * r);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        a[r][i] = __fmul_rn(__fmul_rn(a[r][i], rms), wa[i]);
+        b[r][i] = __fmul_rn(__fmul_rn(b[r][i], rms), wb[i]);
+      }
     }
   }
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const float2 t = __ldg(reinterpret_cast<const float2 *>(fr) + lane * E + i);
-    const float x = a[i], y = b[i];
-    a[i] = __fmul_rn(__fsub_rn(__fmul_rn(x, t.x), __fmul_rn(y, t.y)), scale);
-    b[i] = __fmul_rn(__fadd_rn(__fmul_rn(x, t.y), __fmul_rn(y, t.x)), scale);
-  }
+  for (int r = 0; r < kRows; ++r)
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float x = a[r][i], y = b[r][i];
+      a[r][i] = __fmul_rn(__fsub_rn(__fmul_rn(x, t[2 * i]), __fmul_rn(y, t[2 * i + 1])), scale);
+      b[r][i] = __fmul_rn(__fadd_rn(__fmul_rn(x, t[2 * i + 1]), __fmul_rn(y, t[2 * i])), scale);
+    }
 }
 
 template <int E>
@@ -117,15 +160,18 @@ __device__ __forceinline__ typename Vec<E>::C codes(const float (&v)[E], float i
 }
 
 template <int E>
-__global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
+__global__ void __launch_bounds__(kWriteThreads) k_write(WriteArgs a) {
   constexpr int HD = 64 * E;
   ptx::griddep_launch();
   const int lane = threadIdx.x & 31;
-  const long row = (long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const int heads = a.n_heads + 2 * a.kv.nkv;
+  // x is the token, y some of its groups of heads: query, key, then value heads
+  const int t = blockIdx.x, qg = groups(a.n_heads), kg = groups(a.kv.nkv);
+  const int g = blockIdx.y * (kWriteThreads / 32) + (threadIdx.x >> 5);
   ptx::griddep_wait();
-  if (row >= (long)a.rows * heads) return;  // whole warp
-  const int t = (int)(row / heads), h = (int)(row - (long)t * heads);
+  if (g >= qg + 2 * kg) return;  // whole warp
+  const bool isq = g < qg, isk = !isq && g < qg + kg;
+  const int h0 = (isq ? g : isk ? g - qg : g - qg - kg) * kRows;
+  const int nr = min(kRows, (isq ? a.n_heads : a.kv.nkv) - h0);
   int seq = 0, pos = a.spos + t;
   if (a.len) {
     seq = t;
@@ -137,66 +183,98 @@ __global__ void __launch_bounds__(kThreads) k_write(WriteArgs a) {
     }
     pos = n - 1;
   }
-  float lo[E], hi[E];
-  const float *src = a.qkv + t * a.ld + (long)h * HD + lane * E;
-  load<E>(lo, src);
-  load<E>(hi, src + HD / 2);
-  const bool isq = h < a.n_heads, isk = !isq && h < a.n_heads + a.kv.nkv;
-  if (isq || isk)
-    norm_rope<E>(lo, hi, isq ? a.nq : a.nk, a.eps, a.freqs + (long)t * HD, isq ? a.q_scale : 1.0f, lane);
+  float lo[kRows][E], hi[kRows][E];
+  const float *src =
+      a.qkv + t * a.ld + ((long)h0 + (isq ? 0 : isk ? a.n_heads : a.n_heads + a.kv.nkv)) * HD + lane * E;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    if (r < nr) {
+      load<E>(lo[r], src + r * HD);
+      load<E>(hi[r], src + r * HD + HD / 2);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) lo[r][i] = hi[r][i] = 0.0f;
+    }
+  }
+  if (isq || isk) {
+    float fr[2 * E];
+    load_table<E>(fr, a.freqs + (long)t * HD + lane * 2 * E);
+    norm_rope<E>(lo, hi, isq ? a.nq : a.nk, a.eps, fr, isq ? a.q_scale : 1.0f, lane);
+  }
   if (isq) {
-    float *dst = a.xq + (a.len ? ((long)t * a.n_heads + h) * HD : ((long)h * a.rows + t) * HD) + lane * E;
-    store<E>(dst, lo);
-    store<E>(dst + HD / 2, hi);
+    const long step = a.len ? HD : (long)a.rows * HD;
+    float *dst = a.xq + (a.len ? (long)t * a.n_heads * HD : (long)t * HD) + h0 * step + lane * E;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (r >= nr) break;
+      store<E>(dst + r * step, lo[r]);
+      store<E>(dst + r * step + HD / 2, hi[r]);
+    }
     return;
   }
-  float amax = 0.0f;
+  float amax[kRows];
 #pragma unroll
-  for (int i = 0; i < E; ++i) amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+  for (int r = 0; r < kRows; ++r) {
+    amax[r] = 0.0f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int i = 0; i < E; ++i) amax[r] = fmaxf(amax[r], fmaxf(fabsf(lo[r][i]), fabsf(hi[r][i])));
+  }
   float scale, inv;
-  ptx::quant_scale(amax, scale, inv);
-  const int hk = h - a.n_heads - (isk ? 0 : a.kv.nkv);
-  int8_t *q = (isk ? a.kv.k : a.kv.v) + seq * a.kv.seq_stride + hk * a.kv.kv_stride + (long)pos * HD + lane * E;
-  *reinterpret_cast<typename Vec<E>::C *>(q) = codes<E>(lo, inv);
-  *reinterpret_cast<typename Vec<E>::C *>(q + HD / 2) = codes<E>(hi, inv);
-  if (lane == 0) (isk ? a.kv.ks : a.kv.vs)[seq * a.kv.sc_seq_stride + hk * a.kv.sc_stride + pos] = scale;
+  ptx::quant_scale(reduce_rows(amax, lane, [](float x, float y) { return fmaxf(x, y); }), scale, inv);
+  int8_t *q = (isk ? a.kv.k : a.kv.v) + seq * a.kv.seq_stride + h0 * a.kv.kv_stride + (long)pos * HD + lane * E;
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const float f = __shfl_sync(0xffffffffu, inv, 8 * r);
+    if (r >= nr) break;
+    *reinterpret_cast<typename Vec<E>::C *>(q + r * a.kv.kv_stride) = codes<E>(lo[r], f);
+    *reinterpret_cast<typename Vec<E>::C *>(q + r * a.kv.kv_stride + HD / 2) = codes<E>(hi[r], f);
+  }
+  if (lane % 8 == 0 && lane / 8 < nr)
+    (isk ? a.kv.ks : a.kv.vs)[seq * a.kv.sc_seq_stride + (h0 + lane / 8) * a.kv.sc_stride + pos] = scale;
 }
 
-// 16 lanes x 4 codes a step over a row of the cache, 16-byte stores
+// 4 codes a thread, kReadRows rows at a time so that their loads overlap; a CTA
+// reads kReadRows * 1024 / HD positions of one head, K or V (y).
+constexpr int kReadRows = 4;
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads) k_read(float *k, float *v, long out_seq_stride, long out_stride,
-                                                   gcu_kv_i8 kv, int spos, int ntok) {
+                                                   gcu_kv_i8 kv, int spos, int ntok, int blocks) {
   ptx::griddep_launch();
-  constexpr int L = HD / 4;  // threads per row
-  const long i = (long)blockIdx.x * kThreads + threadIdx.x;
+  constexpr int L = HD / 4, R = kThreads / L;  // threads per row, rows at once
+  const int bh = blockIdx.x / blocks, b = bh / kv.nkv, h = bh - b * kv.nkv;
+  const int t0 = (blockIdx.x - bh * blocks) * (kReadRows * R) + threadIdx.x / L, c = threadIdx.x % L * 4;
+  const int8_t *src = (blockIdx.y ? kv.v : kv.k) + b * kv.seq_stride + h * kv.kv_stride + (long)spos * HD + c;
+  const float *sc = (blockIdx.y ? kv.vs : kv.ks) + b * kv.sc_seq_stride + h * kv.sc_stride + spos;
+  float *dst = (blockIdx.y ? v : k) + b * out_seq_stride + h * out_stride + c;
   ptx::griddep_wait();
-  const int c = (int)(i % L);
-  long r = i / L;
-  const int t = (int)(r % ntok);
-  r /= ntok;
-  const int h = (int)(r % kv.nkv);
-  const long b = r / kv.nkv;
-  if (b >= kv.nseq) return;
-  const bool isv = blockIdx.y;
-  const char4 q = *reinterpret_cast<const char4 *>((isv ? kv.v : kv.k) + b * kv.seq_stride + h * kv.kv_stride +
-                                                   (long)(spos + t) * HD + c * 4);
-  const float s = (isv ? kv.vs : kv.ks)[b * kv.sc_seq_stride + h * kv.sc_stride + spos + t];
-  *reinterpret_cast<float4 *>((isv ? v : k) + b * out_seq_stride + h * out_stride + (long)t * HD + c * 4) =
-      make_float4(q.x * s, q.y * s, q.z * s, q.w * s);
+  char4 q[kReadRows];
+  float s[kReadRows];
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    const int t = min(t0 + i * R, ntok - 1);
+    q[i] = *reinterpret_cast<const char4 *>(src + (long)t * HD);
+    s[i] = sc[t];
+  }
+#pragma unroll
+  for (int i = 0; i < kReadRows; ++i) {
+    const int t = t0 + i * R;
+    if (t < ntok)
+      *reinterpret_cast<float4 *>(dst + (long)t * HD) =
+          make_float4(q[i].x * s[i], q[i].y * s[i], q[i].z * s[i], q[i].w * s[i]);
+  }
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 int launch_write(const WriteArgs &a, cudaStream_t st) {
-  const long rows = (long)a.rows * (a.n_heads + 2 * a.kv.nkv);
-  const long ctas = (rows + kThreads / 32 - 1) / (kThreads / 32);
-  if (ctas > 0x7fffffffL) return set_error("qkv_norm_rope_cache_i8: %ld head rows", rows);
-  const dim3 grid((unsigned)ctas);
-  cudaError_t e = a.kv.hdim == 256   ? launch_k(k_write<4>, grid, dim3(kThreads), 0, st, a)
-                  : a.kv.hdim == 128 ? launch_k(k_write<2>, grid, dim3(kThreads), 0, st, a)
-                                     : launch_k(k_write<1>, grid, dim3(kThreads), 0, st, a);
+  constexpr int kWarps = kWriteThreads / 32;
+  const int y = (groups(a.n_heads) + 2 * groups(a.kv.nkv) + kWarps - 1) / kWarps;
+  if (y > 65535) return set_error("qkv_norm_rope_cache_i8: %d query and %d kv heads", a.n_heads, a.kv.nkv);
+  const dim3 grid(a.rows, y);
+  cudaError_t e = a.kv.hdim == 256   ? launch_k(k_write<4>, grid, dim3(kWriteThreads), 0, st, a)
+                  : a.kv.hdim == 128 ? launch_k(k_write<2>, grid, dim3(kWriteThreads), 0, st, a)
+                                     : launch_k(k_write<1>, grid, dim3(kWriteThreads), 0, st, a);
   GCU_CUDA(e);
   return 0;
 }
@@ -275,11 +353,13 @@ GCU_EXPORT int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, lo
   if ((kv->nkv > 1 && out_stride < (long)ntok * kv->hdim) ||
       (kv->nseq > 1 && out_seq_stride < (kv->nkv - 1) * out_stride + (long)ntok * kv->hdim))
     return set_error("%s: output strides overlap rows of %d positions x %d", what, ntok, kv->hdim);
-  const long items = (long)kv->nseq * kv->nkv * ntok * (kv->hdim / 4), ctas = (items + kThreads - 1) / kThreads;
-  if (ctas > 0x7fffffffL) return set_error("%s: %ld rows", what, items);
+  const int per = kReadRows * kThreads * 4 / kv->hdim;  // positions of a CTA
+  const int blocks = (int)(((long)ntok + per - 1) / per);
+  const long ctas = (long)kv->nseq * kv->nkv * blocks;
+  if (ctas > 0x7fffffffL) return set_error("%s: %ld CTAs", what, ctas);
   const dim3 grid((unsigned)ctas, 2);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto kern = kv->hdim == 256 ? k_read<256> : kv->hdim == 128 ? k_read<128> : k_read<64>;
-  GCU_CUDA(launch_k(kern, grid, dim3(kThreads), 0, st, k, v, out_seq_stride, out_stride, *kv, spos, ntok));
+  GCU_CUDA(launch_k(kern, grid, dim3(kThreads), 0, st, k, v, out_seq_stride, out_stride, *kv, spos, ntok, blocks));
   return 0;
 }
