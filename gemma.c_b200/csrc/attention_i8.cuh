@@ -47,7 +47,8 @@ struct Args {
   // Key ranges are cut into `splits` chunks; a launch writes slots [slot0,
   // slot0 + splits) of `slots` per row: unnormalised sums part[slot][row][hdim]
   // and (m, l) stat[slot][row] with row = i*n_heads + h, weights 2^(log2e*s - m).
-  // slots == 1: the rows go straight to xo.
+  // slots == 1: the rows go straight to xo, from the chunks' CTAs together (a
+  // cluster) when there are several.
   int chunk, splits, slot0, slots;
   float *part;
   float2 *stat;
@@ -241,6 +242,7 @@ constexpr int kTcRows = 128, kTcKeys = 64;
 // for one or two sets of rows (a shared prefix, the sequences' own caches)
 int launch_kt(const Args *sets, int n, int rows, cudaStream_t st);
 constexpr int kKtKeys = 128;
+constexpr int kKtCluster = 8;  // chunks that one launch joins
 int launch_merge(const Args &a, cudaStream_t st);
 
 }  // namespace attn8

@@ -110,13 +110,20 @@ int visible(int n, int slide) { return slide > 0 ? std::min(n, slide) : n; }
 struct DecodePlan {
   int rows;  // query rows per CTA
   Plan own, pre;
-  int slots() const { return own.splits + pre.splits; }
+  bool cluster;  // the chunks' CTAs join their sums themselves
+  int slots() const { return cluster ? 1 : own.splits + pre.splits; }
 };
 
 // Splits of the prefix: a CTA costs about kSetup tiles' time before and after its
 // tiles, and CTAs run one per SM, the prefix's first.  Of the splits that give
 // at most one wave of prefix CTAs the one whose last CTA ends first.
 constexpr long kSetup = 3;
+
+// Up to kKtCluster chunks are joined in the kernel that makes them, which saves the
+// scratch and the merge's launch (5 us of the caller's time) and is worth kJoin
+// further tiles a CTA: 2048 keys of one head take 8.6 us either way, 512 keys 7.6
+// against 7.7; with three further tiles (4096 keys) 10.6 against 9.4.
+constexpr long kJoin = 1;
 
 DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads, int slide) {
   const long G = max_group(n_heads, own.nkv), sms = std::max(1, num_sms());
@@ -125,6 +132,12 @@ DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads,
   const long units = (long)own.nkv * own.nseq;
   p.own = plan_range(visible(max_len, slide), units, plen > 0 ? sms / 2 : sms, kKtKeys);
   p.pre = Plan{1, 0};
+  p.cluster = false;
+  if (plen == 0) {
+    const Plan few = plan_range(visible(max_len, slide), units, std::min(sms, kKtCluster * units), kKtKeys);
+    p.cluster = few.splits > 1 && few.splits <= kKtCluster && few.chunk <= p.own.chunk + kJoin * kKtKeys;
+    if (p.cluster) p.own = few;
+  }
   if (plen > 0) {
     const long n = visible(plen, slide), tiles = (n + kKtKeys - 1) / kKtKeys;
     const long pre = (own.nseq * G + p.rows - 1) / p.rows * own.nkv;

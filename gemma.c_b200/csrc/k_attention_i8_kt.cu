@@ -21,7 +21,8 @@
 // Warps 0-15: softmax, thread = (key, a quarter of the rows); 16: products; 17: loads.
 #include "attention_i8.cuh"
 
-#include <algorithm>
+#include <cooperative_groups.h>
+
 #include <mutex>
 
 namespace gcu {
@@ -75,9 +76,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R];
-  __shared__ float s_rf[R], s_m[R], s_f[R], s_red[16][R / 4];
+  __shared__ float s_rf[R], s_m[R], s_f[R], s_sum[R], s_red[16][R / 4];
   // aligned by an offset: the accesses stay in the shared address space
   uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+  float *part = reinterpret_cast<float *>(smem + C::K_OFF);  // a fused merge's sums, over K's first tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int set = (int)blockIdx.x >= p.first1;
   const Args &a = p.a[set];
@@ -88,6 +90,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   const int first = a.mode == OWN ? group * G : group * R;
   const int nr = max(0, a.mode == OWN ? G : min(R, a.ni * G - first));
   const RowSplit rows(first, G);
+  const bool fused = a.slots == 1 && a.splits > 1;  // the splits are a cluster
   // The loads start before anything else: their warp sets up their barriers.
   if (warp == kLoadWarp && lane == 0) {
     ptx::prefetch_tmap(&p.k[set]);
@@ -435,7 +438,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         const int hh = rr / RQ, i = rows.i(rr), h = h0 + rows.g(rr);
         const float sum = (s_red[hh * 4][rr % RQ] + s_red[hh * 4 + 1][rr % RQ]) +
                           (s_red[hh * 4 + 2][rr % RQ] + s_red[hh * 4 + 3][rr % RQ]);
-        if (a.slots == 1) {  // a row that sees nothing: zeros
+        if (fused) {
+          part[rr * HD + ocol] = acc[r];
+          if (ocol == 0) s_sum[rr] = sum;
+        } else if (a.slots == 1) {  // a row that sees nothing: zeros
           if (row_live(a, i)) a.xo[(long)i * a.o_i + (long)h * HD + ocol] = acc[r] / (sum == 0.0f ? 1.0f : sum);
         } else {
           const size_t at = ((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h;
@@ -450,6 +456,28 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   __syncthreads();
   ptx::tc_fence_after();
   if (warp == kMmaWarp) ptx::tmem_dealloc(tmem, C::COLS);
+  if (fused) {
+    // o = sum_s e_s O_s / sum_s e_s l_s, e_s = 2^(m_s - max m), in chunk order from the
+    // CTAs' shared memory, each CTA a share of the elements
+    auto cl = cooperative_groups::this_cluster();
+    cl.sync();
+    for (int e = split * kThreads + threadIdx.x; e < nr * HD; e += a.splits * kThreads) {
+      const int rr = e / HD;
+      float m = -INFINITY, o = 0.0f, l = 0.0f;
+      for (int s = 0; s < a.splits; ++s) m = fmaxf(m, cl.map_shared_rank(s_m, s)[rr]);
+      for (int s = 0; s < a.splits; ++s) {
+        const float ms = cl.map_shared_rank(s_m, s)[rr], ls = cl.map_shared_rank(s_sum, s)[rr];
+        if (ms == -INFINITY && ls == 0.0f) continue;  // sees none of the chunk
+        const float f = ex2(ms - m);
+        l += f * ls;
+        o += f * cl.map_shared_rank(part, s)[e];
+      }
+      const int i = rows.i(rr);
+      if (row_live(a, i))
+        a.xo[(long)i * a.o_i + (long)(h0 + rows.g(rr)) * HD + e % HD] = o / (l == 0.0f ? 1.0f : l);
+    }
+    cl.sync();  // read by all
+  }
 }
 
 template <int HD, int R, bool CAP>
@@ -479,7 +507,9 @@ int launch_kt_r(const Args *sets, int n, cudaStream_t st) {
       done |= 1ull << (dev & 63);
     }
   }
-  GCU_CUDA(launch_k(k_kt<HD, R, CAP>, dim3((unsigned)blocks, sets[0].kv.nkv), dim3(kThreads), C::SMEM, st, p));
+  const unsigned cluster = sets[0].slots == 1 ? sets[0].splits : 1;
+  GCU_CUDA(launch_cluster_k(k_kt<HD, R, CAP>, dim3((unsigned)blocks, sets[0].kv.nkv), dim3(kThreads), cluster, C::SMEM,
+                            st, p));
   return 0;
 }
 

@@ -651,18 +651,28 @@ def _want(what, ok, *msg):
         raise GcuError(f"{what}: " + " ".join(str(m) for m in msg))
 
 
-def _device(what, t):
-    """The current device's index, which t has to be on."""
+def _torch():
+    """torch, imported by the first call that takes its tensors."""
+    global torch
     import torch
-    d = torch._C._cuda_getDevice() if t.is_cuda else -2
-    if t.get_device() != d:
-        raise GcuError(f"{what}: a tensor is on {t.device} and the current device is another")
+    return torch
+
+
+torch = None
+
+
+def _device(what, index):
+    """The current device's index, which must be `index`."""
+    d = (torch or _torch())._C._cuda_getDevice() if index >= 0 else -2
+    if index != d:
+        raise GcuError(f"{what}: a tensor is on {f'cuda:{index}' if index >= 0 else 'the CPU'} and the current device "
+                       "is another")
     return d
 
 
 def _rows(what, name, t, dtype, shape, dev):
     """t is a contiguous tensor of this dtype and shape (a tuple) on CUDA device dev."""
-    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+    if t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
         return
     raise GcuError(f"{what}: {name} must be a contiguous {dtype} tensor of {shape} on the current device, "
                    f"not {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -673,11 +683,15 @@ def _work(nbytes, device, stream):
     call's own: in a captured graph it lives in the graph's pool."""
     if not nbytes:
         return None, 0, None
-    import torch
     w = torch.empty(nbytes, dtype=torch.uint8, device=device)
     if stream is not None:
         w.record_stream(stream)  # the block is not handed out again before the call is done
     return w.data_ptr(), nbytes, w
+
+
+def _on(stream, dev):
+    """The handle of stream, or of device dev's current one."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(dev)
 
 
 class KvCacheI8:
@@ -698,7 +712,7 @@ class KvCacheI8:
               "a head's positions must be contiguous")
         self.k, self.v, self.ks, self.vs = k, v, ks, vs
         self.nseq, self.nkv, self.clen, self.hdim = k.shape
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.c = _KvI8(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), k.stride(0), k.stride(1),
                        ks.stride(0), ks.stride(1), *k.shape)
         self.ref = ctypes.byref(self.c)
@@ -721,19 +735,20 @@ def _ptr(t):
 
 
 def _check_write(what, xq, shape, qkv, kv, freqs, nq, nk, rows, n_heads):
-    import torch
-    dev, f32 = _device(what, kv.k), torch.float32
+    """The device and qkv's row stride."""
+    dev = _device(what, kv.index)
+    f32, hdim, ld = torch.float32, kv.hdim, qkv.stride()
     _rows(what, "xq", xq, f32, shape, dev)
-    if not (qkv.dtype is f32 and qkv.dim() == 2 and qkv.shape[0] == rows and qkv.stride(1) == 1 and
-            qkv.shape[1] >= (n_heads + 2 * kv.nkv) * kv.hdim and qkv.get_device() == dev):
+    if not (qkv.dtype is f32 and len(ld) == 2 and ld[1] == 1 and qkv.shape[0] == rows and
+            qkv.shape[1] >= (n_heads + 2 * kv.nkv) * hdim and qkv.get_device() == dev):
         raise GcuError(f"{what}: qkv must be float32 rows of the fused q|k|v projection, one per token, "
                        f"not {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
-    _rows(what, "freqs", freqs, f32, (rows, kv.hdim), dev)
+    _rows(what, "freqs", freqs, f32, (rows, hdim), dev)
     if nq is not None:
-        _rows(what, "nq", nq, f32, (kv.hdim,), dev)
+        _rows(what, "nq", nq, f32, (hdim,), dev)
     if nk is not None:
-        _rows(what, "nk", nk, f32, (kv.hdim,), dev)
-    return dev
+        _rows(what, "nk", nk, f32, (hdim,), dev)
+    return dev, ld[0]
 
 
 def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
@@ -741,41 +756,38 @@ def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, n
     (n_heads+2*nkv)*hdim) rows, rotated queries to xq (n_heads, ntok, hdim),
     codes and scales to kv (KvCacheI8) at [spos, spos+ntok); freqs (ntok, hdim)."""
     what = "dev_qkv_norm_rope_cache_i8"
-    n_heads, ntok = xq.shape[0], xq.shape[1]
-    _check_write(what, xq, (n_heads, ntok, kv.hdim), qkv, kv, freqs, nq, nk, ntok, n_heads)
-    _check(lib().gcu_dev_qkv_norm_rope_cache_i8(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref, _ptr(nq), _ptr(nk),
-                                                eps, freqs.data_ptr(), q_scale, n_heads, spos, ntok, _stream(stream)),
-           what)
+    n_heads, ntok = xq.shape[:2]
+    dev, ld = _check_write(what, xq, (n_heads, ntok, kv.hdim), qkv, kv, freqs, nq, nk, ntok, n_heads)
+    _check(lib().gcu_dev_qkv_norm_rope_cache_i8(xq.data_ptr(), qkv.data_ptr(), ld, kv.ref, _ptr(nq), _ptr(nk), eps,
+                                                freqs.data_ptr(), q_scale, n_heads, spos, ntok, _on(stream, dev)), what)
 
 
 def dev_qkv_norm_rope_cache_i8_seqs(xq, qkv, kv, length, freqs, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
     """One token of each of kv.nseq sequences: row b of qkv to position length[b] - 1
     of sequence b (length int32 (nseq,) counts the new token; below 1: skipped),
     queries to xq (nseq, n_heads, hdim); freqs (nseq, hdim)."""
-    import torch
     what = "dev_qkv_norm_rope_cache_i8_seqs"
     n_heads = xq.shape[1]
-    dev = _check_write(what, xq, (kv.nseq, n_heads, kv.hdim), qkv, kv, freqs, nq, nk, kv.nseq, n_heads)
+    dev, ld = _check_write(what, xq, (kv.nseq, n_heads, kv.hdim), qkv, kv, freqs, nq, nk, kv.nseq, n_heads)
     _rows(what, "length", length, torch.int32, (kv.nseq,), dev)
-    _check(lib().gcu_dev_qkv_norm_rope_cache_i8_seqs(xq.data_ptr(), qkv.data_ptr(), qkv.stride(0), kv.ref,
+    _check(lib().gcu_dev_qkv_norm_rope_cache_i8_seqs(xq.data_ptr(), qkv.data_ptr(), ld, kv.ref,
                                                      length.data_ptr(), _ptr(nq), _ptr(nk), eps, freqs.data_ptr(),
-                                                     q_scale, n_heads, _stream(stream)), what)
+                                                     q_scale, n_heads, _on(stream, dev)), what)
 
 
 def dev_cache_i8_read(k, v, kv, spos, stream=None):
     """Positions [spos, spos+ntok) of kv as fp32 rows in k, v (nseq, nkv, ntok, hdim),
     views of a longer fp32 cache among them."""
-    import torch
     what = "dev_cache_i8_read"
-    dev = _device(what, kv.k)
-    st = k.stride()
-    if not (k.dtype is torch.float32 and v.dtype is torch.float32 and k.dim() == 4 and v.shape == k.shape and
-            v.stride() == st and k.shape[0] == kv.nseq and k.shape[1] == kv.nkv and k.shape[3] == kv.hdim and
-            st[3] == 1 and (st[2] == kv.hdim or k.shape[2] < 2) and k.get_device() == dev and v.get_device() == dev):
+    dev = _device(what, kv.index)
+    st, sh, f32 = k.stride(), k.shape, torch.float32
+    if not (k.dtype is f32 and v.dtype is f32 and len(sh) == 4 and v.shape == sh and v.stride() == st and
+            sh[0] == kv.nseq and sh[1] == kv.nkv and sh[3] == kv.hdim and st[3] == 1 and
+            (st[2] == kv.hdim or sh[2] < 2) and k.get_device() == dev and v.get_device() == dev):
         raise GcuError(f"{what}: k and v must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, alike, on the "
                        f"cache's device, not {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
-    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0], st[1], kv.ref, spos, k.shape[2],
-                                       _stream(stream)), what)
+    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0], st[1], kv.ref, spos, sh[2],
+                                       _on(stream, dev)), what)
 
 
 def dev_attention_decode_i8(xo, xq, kv, length, max_len, asc, sc_att=0.0, slide=0, prefix=None, plen=0, stream=None):
@@ -783,31 +795,29 @@ def dev_attention_decode_i8(xo, xq, kv, length, max_len, asc, sc_att=0.0, slide=
     sees the plen positions of prefix (a KvCacheI8 of one sequence, shared) and
     the first length[b] of its own cache (int32 (nseq,); None: max_len each), of
     these the last `slide` when slide > 0.  length[b] < 0: skipped."""
-    import torch
     what = "dev_attention_decode_i8"
-    dev, n_heads = _device(what, kv.k), xq.shape[1]
-    shape = (kv.nseq, n_heads, kv.hdim)
-    _rows(what, "xq", xq, torch.float32, shape, dev)
-    _rows(what, "xo", xo, torch.float32, shape, dev)
+    dev, n_heads = _device(what, kv.index), xq.shape[1]
+    shape, f32 = (kv.nseq, n_heads, kv.hdim), torch.float32
+    _rows(what, "xq", xq, f32, shape, dev)
+    _rows(what, "xo", xo, f32, shape, dev)
     if length is not None:
         _rows(what, "length", length, torch.int32, (kv.nseq,), dev)
     pref = None
     if prefix is not None:
-        _device(what, prefix.k)
+        _device(what, prefix.index)
         pref = prefix.ref
     l = lib()
     work, nbytes, keep = _work(l.gcu_attention_decode_i8_work(pref, plen, kv.ref, max_len, n_heads, slide), kv.device, stream)
     _check(l.gcu_dev_attention_decode_i8(xo.data_ptr(), xq.data_ptr(), pref, plen, kv.ref, _ptr(length), max_len, n_heads,
-                                         slide, asc, sc_att, work, nbytes, _stream(stream)), what)
+                                         slide, asc, sc_att, work, nbytes, _on(stream, dev)), what)
 
 
 def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, stream=None):
     """dev_attention_prefill over an 8-bit cache of one sequence: xq (n_heads, ntok, hdim)
     rotated and scaled, kv holding the chunk at [spos, spos+ntok); writes xo
     rows (ntok, >= n_heads*hdim)."""
-    import torch
     what = "dev_attention_prefill_i8"
-    dev, n_heads, ntok = _device(what, kv.k), xq.shape[0], xq.shape[1]
+    dev, (n_heads, ntok) = _device(what, kv.index), xq.shape[:2]
     _rows(what, "xq", xq, torch.float32, (n_heads, ntok, kv.hdim), dev)
     if not (xo.dtype is torch.float32 and xo.dim() == 2 and xo.shape[0] == ntok and xo.stride(1) == 1 and
             xo.shape[1] >= n_heads * kv.hdim and xo.get_device() == dev):
@@ -816,22 +826,21 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
     work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, int(mask)), kv.device,
                                stream)
     _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0), xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
-                                          sc_att, int(mask), work, nbytes, _stream(stream)), what)
+                                          sc_att, int(mask), work, nbytes, _on(stream, dev)), what)
 
 
 def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
     """The next token of each row of logits (m, nvocab): token int32 (m,), from u (m,)
     float32 random numbers in [0, 1); prob (m,) float32 (optional) receives the
     tokens' shares of the kept weights.  See gcu_dev_sample in include/gcu.h."""
-    import torch
     what = "dev_sample"
-    dev = _device(what, logits)
-    if not (logits.dtype is torch.float32 and logits.dim() == 2 and logits.stride(1) == 1):
+    dev, ld = _device(what, logits.get_device()), logits.stride()
+    if not (logits.dtype is torch.float32 and len(ld) == 2 and ld[1] == 1):
         raise GcuError(f"{what}: logits must be float32 (m, nvocab) rows, not {logits.dtype} {tuple(logits.shape)}")
     m, n = logits.shape
     _rows(what, "token", token, torch.int32, (m,), dev)
     _rows(what, "u", u, torch.float32, (m,), dev)
     if prob is not None:
         _rows(what, "prob", prob, torch.float32, (m,), dev)
-    _check(lib().gcu_dev_sample(token.data_ptr(), _ptr(prob), logits.data_ptr(), logits.stride(0) if m > 1 else 0,
-                                u.data_ptr(), temperature, top_k, top_p, min_p, m, n, _stream(stream)), what)
+    _check(lib().gcu_dev_sample(token.data_ptr(), _ptr(prob), logits.data_ptr(), ld[0] if m > 1 else 0,
+                                u.data_ptr(), temperature, top_k, top_p, min_p, m, n, _on(stream, dev)), what)

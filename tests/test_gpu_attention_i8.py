@@ -327,3 +327,20 @@ def test_two_streams_at_once():
     for xo, po in outs:
         check(xo, want, tol)
         check(po, wantp, tolp)
+
+
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 1, 256), (6, 4, 64), (4, 2, 128)])
+@pytest.mark.parametrize("max_len", [130, 513, 900, 1024])
+def test_decode_few_chunks(nh, nkv, hd, max_len):
+    """Two to eight chunks, joined in the launch that makes them: lengths that end in the first
+    chunk, between chunks, and in the last; skipped sequences; empty ones."""
+    rng = np.random.default_rng(max_len)
+    lens = [max_len, 0, -1, 1, 128, 129, max_len - 1, 7]
+    c = R.cache(rng, len(lens), nkv, max_len, hd)
+    xq = rng.standard_normal((len(lens), nh, hd), dtype=np.float32)
+    live = np.asarray(lens) >= 0
+    for slide, cap in ((0, 0.0), (140, 0.0), (0, 8.0)):
+        want, tol = R.decode(xq, c, lens, hd ** -0.5, cap, slide)
+        got = run_decode(xq, handle(c), lens, max_len, cap, slide).cpu().numpy()
+        assert np.all(got[~live] == 9.0) and np.all(got[np.asarray(lens) == 0] == 0.0)
+        check(got[live], want[live], tol)
