@@ -17,11 +17,13 @@
 // too many elements is split by its float keys until they fit or are all equal,
 // and then the cut is an index.
 //
-// One cluster of eight CTAs per row: every CTA keeps its contiguous slice in shared
-// memory (rows up to 262144; longer ones are read again from L2), histograms and
+// One cluster of 2 to 16 CTAs per row: every CTA scans its contiguous slice, from
+// shared memory where it fits (n / CTAs up to 32768) or again from L2, histograms and
 // lists meet in distributed shared memory, and the whole search is one launch
-// with one read of HBM.  Bound by latency for a few rows, each pass a scan of 32 K
-// logits and a cluster barrier, and by the 64-bit weights for many.
+// with one read of HBM.  Bound by the 64-bit weights, 12 instructions of the FP64
+// units each, and by the latency of the passes and their cluster barriers.
+// 262144 logits, top-p 0.9 and min-p: 31 us for a row (16 CTAs), 41 for 15 rows (8), 82 for
+// 32 (4; clusters of 8, of which 15 run at once, take 116), 143 for 64 (2; 194 with 8).
 #include "gcu_internal.cuh"
 
 #include <cooperative_groups.h>
@@ -38,7 +40,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
-constexpr int kCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kBins = 2048;
 constexpr float kBinsPerNat = 128.0f;
 constexpr int kCap = 1024;                // elements that are sorted
@@ -75,8 +77,8 @@ struct Shared {
   u64 list[kCap];                     // rank 0: all that is gathered, sorted ascending
   u64 weight[kCap];
   unsigned int order[kCap];
-  u64 warp_sum[kWarps], totals[kCluster];
-  float maxes[kCluster];
+  u64 warp_sum[kWarps], totals[kMaxCluster];
+  float maxes[kMaxCluster];
   u64 cta_sum, before;
   u64 upto;
   unsigned int nfound, klo, khi;
@@ -133,20 +135,29 @@ struct Row {
   // that their arithmetic overlaps.
   template <typename F>
   __device__ __forceinline__ void each4(int lane, F f) const {
-    for (int b = w0; b < w1; b += 128) {
-      float v[4];
-      if (holds) {
+    if (holds) {
+      for (int b = w0; b < w1; b += 128) {
+        float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = held[b - w0 + 32 * j + lane];
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = b + 32 * j + lane;
-          v[j] = i < w1 ? __ldg(x + i) : -INFINITY;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = counted(v[j]);
+        f(b + lane, v);
       }
+      return;
+    }
+    float next[4];
+    auto fetch = [&](int b) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = b + 32 * j + lane;
+        next[j] = i < w1 ? __ldg(x + i) : -INFINITY;
+      }
+    };
+    fetch(w0);
+    for (int b = w0; b < w1; b += 128) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = counted(next[j]);
+      fetch(b + 128);
       f(b + lane, v);
     }
   }
@@ -234,7 +245,7 @@ __device__ __forceinline__ float list_value(u64 e) { return value_of(~(uint32_t)
 
 // The row's histogram of the elements that bin_of(index, value) gives a bin (not
 // -1), of their number or (MASS) their weights, in every CTA's sum.
-template <bool MASS, typename B>
+template <int C, bool MASS, typename B>
 __device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, B bin_of) {
   const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
   for (int b = tid; b < kBins; b += kThreads) {
@@ -259,18 +270,18 @@ __device__ void histogram(cg::cluster_group &cl, Shared &s, const Row &r, B bin_
   });
   cl.sync();
   // each CTA sums its share of the bins over the cluster and hands it to all
-  constexpr int kShare = kBins / kCluster;
+  constexpr int kShare = kBins / C;
   if (tid < kShare) {
     const int b = rank * kShare + tid;
     u64 n = 0;
 #pragma unroll
-    for (int p = 0; p < kCluster; ++p) {
+    for (int p = 0; p < C; ++p) {
       const Shared &o = *cl.map_shared_rank(&s, p);
       n += o.lo[b];
       if (MASS) n += (u64)o.hi[b] << 32;
     }
 #pragma unroll
-    for (int p = 0; p < kCluster; ++p) cl.map_shared_rank(&s, p)->sum[b] = n;
+    for (int p = 0; p < C; ++p) cl.map_shared_rank(&s, p)->sum[b] = n;
   }
   cl.sync();
 }
@@ -304,7 +315,7 @@ __device__ void find_bin(Shared &s, u64 before, double target, int warp, int lan
 
 // Elements that pass `in`, to rank 0's list; their number, in every CTA.  More than
 // kCap: the list is not made.
-template <typename P>
+template <int C, typename P>
 __device__ int gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
   const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
   if (tid == 0) s.nfound = 0;
@@ -319,10 +330,10 @@ __device__ int gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
     if (hit && at < kCap) s.found[at] = ((u64)~key_of(v) << 32) | (unsigned int)i;
   });
   __syncthreads();
-  if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.nfound;
+  if (tid < C) cl.map_shared_rank(&s, tid)->totals[rank] = s.nfound;
   cl.sync();
   u64 before = 0, all = 0;
-  for (int q = 0; q < kCluster; ++q) {
+  for (int q = 0; q < C; ++q) {
     if (q < rank) before += s.totals[q];
     all += s.totals[q];
   }
@@ -357,7 +368,7 @@ __device__ void sort_list(Shared &s, const Row &r, int nl) {
 // The search for one cut among the elements that `c` keeps, whatever its size.
 // Starts from find_bin's answer over the linear bins.  c is left as it is when the
 // elements never reach the target.
-template <bool MASS>
+template <int C, bool MASS>
 __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c, double target) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = cl.block_rank();
   Shared &s0 = *cl.map_shared_rank(&s, 0);
@@ -370,12 +381,12 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
     const int bin = s.bin;
     const u64 before = s.before;
     auto here = [&](int i, float v) { return level == 0 ? c.keeps(v, i) && r.bin(v) == bin : key_bin(i, v) == bin; };
-    const int nbin = gather(cl, s, r, here);
+    const int nbin = gather<C>(cl, s, r, here);
     if (nbin <= kCap) {
       if (rank == 0) {
         sort_list(s, r, nbin);
         const int at = cut_list<MASS>(s, nbin, before, target, warp, lane);
-        if (tid < kCluster) {
+        if (tid < C) {
           Shared &o = *cl.map_shared_rank(&s, tid);
           o.cut_key = ~(uint32_t)(s.list[at] >> 32);
           o.need = (u64)(uint32_t)s.list[at];
@@ -424,7 +435,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
       r.each(lane, [&](int i, float v) { mine += c.keeps(v, i) && v == tie; });
       mine = warp_total(mine);
       u64 p = cta_prefix(s, mine, warp, lane);
-      if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
+      if (tid < C) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
       cl.sync();
       for (int q = 0; q < rank; ++q) p += s.totals[q];
       if (p < need && need <= p + mine) {  // this warp holds it
@@ -432,7 +443,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
           const bool hit = c.keeps(v, i) && v == tie;
           const unsigned int b = __ballot_sync(0xffffffffu, hit);
           if (hit && p + __popc(b & ((2u << lane) - 1)) == need)
-            for (int q = 0; q < kCluster; ++q) cl.map_shared_rank(&s, q)->cut_idx = i;
+            for (int q = 0; q < C; ++q) cl.map_shared_rank(&s, q)->cut_idx = i;
           p += __popc(b);
         });
       }
@@ -442,7 +453,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
       return;
     }
     step = (khi - klo) / kBins + 1;
-    histogram<MASS>(cl, s, r, key_bin);
+    histogram<C, MASS>(cl, s, r, key_bin);
     find_bin(s, before, target, warp, lane);
   }
 }
@@ -485,16 +496,17 @@ __device__ void choose_from_list(Shared &s, const SampleArgs &a, const Row &r, i
   }
 }
 
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
+template <int C>
+__global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   extern __shared__ __align__(16) uint8_t raw[];
   Shared &s = *reinterpret_cast<Shared *>(raw);
   ptx::griddep_launch();
   cg::cluster_group cl = cg::this_cluster();
   auto started = cl.barrier_arrive();  // waited for before the first access to another CTA
-  const int rank = cl.block_rank(), row = blockIdx.x / kCluster;
+  const int rank = cl.block_rank(), row = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // contiguous slices of CTAs and warps, in index order, multiples of 128
-  const int per_warp = ((a.n + kCluster * kWarps - 1) / (kCluster * kWarps) + 127) & ~127;
+  const int per_warp = ((a.n + C * kWarps - 1) / (C * kWarps) + 127) & ~127;
   Row r;
   r.x = a.logits + (long)row * a.ld;
   r.w0 = min(a.n, (rank * kWarps + warp) * per_warp);
@@ -538,10 +550,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   cl.barrier_wait(std::move(started));
-  if (tid < kCluster) cl.map_shared_rank(&s, tid)->maxes[rank] = top;
+  if (tid < C) cl.map_shared_rank(&s, tid)->maxes[rank] = top;
   cl.sync();
   r.max = s.maxes[0];
-  for (int p = 1; p < kCluster; ++p) r.max = fmaxf(r.max, s.maxes[p]);
+  for (int p = 1; p < C; ++p) r.max = fmaxf(r.max, s.maxes[p]);
   if (r.max == -INFINITY) {  // nothing to choose from
     if (rank == 0 && tid == 0) {
       a.token[row] = -1;
@@ -587,23 +599,23 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
   // all that lies up to the end of the bin, as one list
   auto list_upto = [&](int bin) {
-    return gather(cl, s, r, [&](int, float v) { return v > -INFINITY && r.bin(v) <= bin; });
+    return gather<C>(cl, s, r, [&](int, float v) { return v > -INFINITY && r.bin(v) <= bin; });
   };
   if (by_k) {
-    histogram<false>(cl, s, r, [&](int, float v) { return v > -INFINITY ? r.bin(v) : -1; });
+    histogram<C, false>(cl, s, r, [&](int, float v) { return v > -INFINITY ? r.bin(v) : -1; });
     find_bin(s, 0, (double)a.top_k, warp, lane);
     if (s.bin >= 0 && s.upto <= kCap) {
       const int nl = list_upto(s.bin);
       if (rank == 0) choose_from_list(s, a, r, row, nl, 0);
       return;
     }
-    find_cut<false>(cl, s, r, c, (double)a.top_k);
+    find_cut<C, false>(cl, s, r, c, (double)a.top_k);
   }
   if (by_p) {
     if (by_k) {
-      histogram<true>(cl, s, r, [&](int i, float v) { return c.keeps(v, i) ? r.bin(v) : -1; });
+      histogram<C, true>(cl, s, r, [&](int i, float v) { return c.keeps(v, i) ? r.bin(v) : -1; });
     } else {
-      histogram<true>(cl, s, r, [&](int, float v) { return r.bin(v); });
+      histogram<C, true>(cl, s, r, [&](int, float v) { return r.bin(v); });
     }
     u64 all = s.sum[tid * 2] + s.sum[tid * 2 + 1];
     cta_scan(s, all, warp, lane);
@@ -617,7 +629,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
       if (rank == 0) choose_from_list(s, a, r, row, nl, all);
       return;
     }
-    find_cut<true>(cl, s, r, c, target);
+    find_cut<C, true>(cl, s, r, c, target);
   }
   const double least = (double)a.min_p * r.one;
   auto kept = [&](int i, float v) -> u64 {
@@ -650,10 +662,10 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   }
   mine = warp_total(mine);
   u64 p = cta_prefix(s, mine, warp, lane);
-  if (tid < kCluster) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
+  if (tid < C) cl.map_shared_rank(&s, tid)->totals[rank] = s.cta_sum;
   cl.sync();
   u64 total = 0;
-  for (int q = 0; q < kCluster; ++q) {
+  for (int q = 0; q < C; ++q) {
     if (q < rank) p += s.totals[q];
     total += s.totals[q];
   }
@@ -685,6 +697,59 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) k_s
   }
 }
 
+// Clusters of C CTAs that run at once on the current device (0: the size is not
+// to be had), after the kernel's opt-ins; both once per device.
+template <int C>
+int resident(int *n) {
+  constexpr int kDevices = 64;
+  static std::mutex mu;
+  static int known[kDevices];  // their number + 1
+  int dev = 0;
+  GCU_CUDA(cudaGetDevice(&dev));
+  if (dev >= kDevices) return set_error("sample: device %d", dev);
+  std::lock_guard<std::mutex> lk(mu);
+  if (!known[dev]) {
+    GCU_CUDA(cudaFuncSetAttribute(k_sample<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
+    if (C > 8) GCU_CUDA(cudaFuncSetAttribute(k_sample<C>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = dim3(C);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = sizeof(Shared);
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    int c = 0;
+    GCU_CUDA(cudaOccupancyMaxActiveClusters(&c, k_sample<C>, &cfg));
+    known[dev] = c + 1;
+  }
+  *n = known[dev] - 1;
+  return 0;
+}
+
+template <int C>
+int launch(const SampleArgs &a, cudaStream_t st) {
+  GCU_CUDA(launch_cluster_k(k_sample<C>, dim3((unsigned)a.m * C), dim3(kThreads), C, sizeof(Shared), st, a));
+  return 0;
+}
+
+// Few rows are cut finely, many coarsely: a row's time is about that of kFixed
+// logits in every CTA (barriers, the histogram's sums, the list) and of its slice, and
+// rows beyond the resident clusters wait.
+constexpr long kFixed = 16384;
+
+template <int C>
+int consider(const SampleArgs &a, long &best, int &size) {
+  int n = 0;
+  if (resident<C>(&n)) return 1;
+  if (n == 0) return 0;
+  const long time = ((long)a.m + n - 1) / n * (kFixed + a.n / C);
+  if (time < best) best = time, size = C;
+  return 0;
+}
+
 }  // namespace
 }  // namespace gcu
 
@@ -706,19 +771,17 @@ GCU_EXPORT int gcu_dev_sample(int *token, float *prob, const float *logits, long
   for (long n = 1; n < nvocab; n <<= 1) one *= 0.5;
   one = one > 2251799813685248.0 ? 2251799813685248.0 : one;  // and 2^51 at most, a whole number of a double
   SampleArgs a{token, prob, logits, ld, u, temperature, top_p, min_p, top_k, m, nvocab, one};
-  {
-    // the shared-memory opt-in is per device: once for each device this runs on
-    static std::mutex mu;
-    static unsigned long long done = 0;
-    int dev = 0;
-    GCU_CUDA(cudaGetDevice(&dev));
-    std::lock_guard<std::mutex> lk(mu);
-    if (!(done & (1ull << (dev & 63)))) {
-      GCU_CUDA(cudaFuncSetAttribute(k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
-      done |= 1ull << (dev & 63);
-    }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  long best = 0x7fffffffffffffffl;
+  int size = 0;
+  if (consider<2>(a, best, size) || consider<4>(a, best, size) || consider<8>(a, best, size) ||
+      consider<16>(a, best, size))
+    return 1;
+  switch (size) {
+    case 2: return launch<2>(a, st);
+    case 4: return launch<4>(a, st);
+    case 8: return launch<8>(a, st);
+    case 16: return launch<16>(a, st);
   }
-  GCU_CUDA(launch_k(k_sample, dim3((unsigned)m * kCluster), dim3(kThreads), sizeof(Shared),
-                    static_cast<cudaStream_t>(stream), a));
-  return 0;
+  return set_error("sample: no cluster of %d bytes of shared memory a CTA fits", (int)sizeof(Shared));
 }
