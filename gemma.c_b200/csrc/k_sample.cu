@@ -22,8 +22,8 @@
 // lists meet in distributed shared memory, and the whole search is one launch
 // with one read of HBM.  Bound by the 64-bit weights, 12 instructions of the FP64
 // units each, and by the latency of the passes and their cluster barriers.
-// 262144 logits, top-p 0.9 and min-p: 31 us for a row (16 CTAs), 41 for 15 rows (8), 82 for
-// 32 (4; clusters of 8, of which 15 run at once, take 116), 143 for 64 (2; 194 with 8).
+// 262144 logits, top-p 0.9 and min-p: 30 us for a row (16 CTAs), 40 for 15 rows (8), 74 for
+// 32 (4; clusters of 8, of which 15 run at once, took 116), 124 for 64 (2; with 8, 194).
 #include "gcu_internal.cuh"
 
 #include <cooperative_groups.h>
@@ -124,6 +124,15 @@ struct Row {
   // steps of 1/128 below the largest; monotone in v
   __device__ __forceinline__ int bin(float v) const {
     return min((int)((max - v) * bin_scale), kBins - 1);
+  }
+  // About the logit `off` bins above the start of a bin: with 0.01 above all of the
+  // bin, with -1.01 below all of it (the last has no end).  bin()'s roundings are
+  // 2^-22 of 2048 bins at most, and those of the logits' own size are allowed for.
+  __device__ __forceinline__ float edge(int bin, double off) const {
+    if (off < 0.0 && bin == kBins - 1) return -INFINITY;
+    const double x = max_d - (bin - off) / (double)bin_scale;
+    const double slack = (fabs(max_d) + fabs(x)) * 2.4e-7;
+    return (float)(off < 0.0 ? x - slack : x + slack);
   }
   // a logit as it counts: NaN as -inf, -0 as +0
   __device__ __forceinline__ float counted(float v) const {
@@ -314,20 +323,28 @@ __device__ void find_bin(Shared &s, u64 before, double target, int warp, int lan
 }
 
 // Elements that pass `in`, to rank 0's list; their number, in every CTA.  More than
-// kCap: the list is not made.
+// kCap: the list is not made.  None lies outside [lo, hi]: a cheaper test that most
+// groups of 128 elements end with.
 template <int C, typename P>
-__device__ int gather(cg::cluster_group &cl, Shared &s, const Row &r, P in) {
+__device__ int gather(cg::cluster_group &cl, Shared &s, const Row &r, float lo, float hi, P in) {
   const int tid = threadIdx.x, lane = tid & 31, rank = cl.block_rank();
   if (tid == 0) s.nfound = 0;
   __syncthreads();
-  r.each(lane, [&](int i, float v) {
-    const bool hit = in(i, v);
-    const unsigned int b = __ballot_sync(0xffffffffu, hit);
-    if (!b) return;  // the whole warp
-    unsigned int at = 0;
-    if (lane == 0) at = atomicAdd(&s.nfound, (unsigned int)__popc(b));
-    at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
-    if (hit && at < kCap) s.found[at] = ((u64)~key_of(v) << 32) | (unsigned int)i;
+  r.each4(lane, [&](int i, const float (&v)[4]) {
+    bool may = false;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) may |= v[j] >= lo && v[j] <= hi;
+    if (!__any_sync(0xffffffffu, may)) return;  // the whole warp
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool hit = v[j] >= lo && v[j] <= hi && in(i + 32 * j, v[j]);
+      const unsigned int b = __ballot_sync(0xffffffffu, hit);
+      if (!b) continue;
+      unsigned int at = 0;
+      if (lane == 0) at = atomicAdd(&s.nfound, (unsigned int)__popc(b));
+      at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
+      if (hit && at < kCap) s.found[at] = ((u64)~key_of(v[j]) << 32) | (unsigned int)(i + 32 * j);
+    }
   });
   __syncthreads();
   if (tid < C) cl.map_shared_rank(&s, tid)->totals[rank] = s.nfound;
@@ -381,7 +398,8 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
     const int bin = s.bin;
     const u64 before = s.before;
     auto here = [&](int i, float v) { return level == 0 ? c.keeps(v, i) && r.bin(v) == bin : key_bin(i, v) == bin; };
-    const int nbin = gather<C>(cl, s, r, here);
+    const float top = level == 0 ? r.edge(bin, 0.01) : value_of(khi - bin * step);
+    const int nbin = gather<C>(cl, s, r, level == 0 ? r.edge(bin, -1.01) : -INFINITY, top, here);
     if (nbin <= kCap) {
       if (rank == 0) {
         sort_list(s, r, nbin);
@@ -599,7 +617,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
   // all that lies up to the end of the bin, as one list
   auto list_upto = [&](int bin) {
-    return gather<C>(cl, s, r, [&](int, float v) { return v > -INFINITY && r.bin(v) <= bin; });
+    return gather<C>(cl, s, r, r.edge(bin, -1.01), INFINITY,
+                     [&](int, float v) { return v > -INFINITY && r.bin(v) <= bin; });
   };
   if (by_k) {
     histogram<C, false>(cl, s, r, [&](int, float v) { return v > -INFINITY ? r.bin(v) : -1; });
@@ -636,11 +655,29 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
     const u64 w = r.weight(v);
     return c.keeps(v, i) && (double)w >= least ? w : 0;
   };
+  // what the cuts keep, often few, moves to the front of the warp's shared memory
   u64 mine = 0;
-  if (r.holds) {
-    // what the cuts keep, often few, moves to the front of the warp's slice
-    float *hold = s.values + warp * kKeep;
-    int n = 0;
+  float *hold = s.values + warp * kKeep;
+  int n = 0;
+  auto weigh = [&]() {
+    __syncwarp();
+#pragma unroll 4
+    for (int b = 0; b < n; b += 32) {
+      const u64 w = r.weight(b + lane < n ? hold[b + lane] : -INFINITY);
+      mine += (double)w >= least ? w : 0;
+    }
+    __syncwarp();
+    n = 0;
+  };
+  if (!by_k && !by_p) {  // all but -inf, which weighs nothing
+    r.each4(lane, [&](int, const float (&v)[4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u64 w = r.weight(v[j]);
+        mine += (double)w >= least ? w : 0;
+      }
+    });
+  } else {
     r.each4(lane, [&](int i, const float (&v)[4]) {
       __syncwarp();
 #pragma unroll
@@ -650,15 +687,9 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
         if (in) hold[n + __popc(b & ((1u << lane) - 1))] = v[j];
         n += __popc(b);
       }
-      __syncwarp();
+      if (!r.holds && n > kKeep - 128) weigh();
     });
-#pragma unroll 4
-    for (int b = 0; b < n; b += 32) {
-      const u64 w = r.weight(b + lane < n ? hold[b + lane] : -INFINITY);
-      mine += (double)w >= least ? w : 0;
-    }
-  } else {
-    r.each(lane, [&](int i, float v) { mine += kept(i, v); });
+    weigh();
   }
   mine = warp_total(mine);
   u64 p = cta_prefix(s, mine, warp, lane);
