@@ -7,8 +7,9 @@
 //   S^T  [128 keys x 3R]    = K [128 x hdim] * Q^T, the R rows' three digits side
 //                             by side (kind::i8, exact)
 //   O^T  [hdim x 4R]       += V^T [hdim x 128 keys] * W, the R rows' weights as four
-//                             unsigned digits (kind::i8 with both operands
-//                             MN-major: V's tile as it lies is V^T)
+//                             unsigned digits each, the bytes of an integer as they
+//                             lie (kind::i8 with both operands MN-major: V's tile
+//                             as it lies is V^T)
 // Weights are 32-bit fixed point, W = round(2^(s + log2 vs - m)), m placed so that
 // the row's largest weight so far is 2^24 at least and 2^31.5 at most; rounding
 // is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 66,312
@@ -61,11 +62,13 @@ struct Cfg {
   static_assert(STAGES >= 2 && O_COL + MB * NP <= 512, "budget");
 };
 
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[4]) { ptx::tmem_ld_32x4(at, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[8]) { ptx::tmem_ld_32x8(at, r); }
+
 struct alignas(64) KtArgs {
   CUtensorMap k[2], v[2];
   Args a[2];
-  int groups[2];  // row groups of each set
-  int first1;     // blocks of set 0
+  int first1;  // CTAs of set 0: the longer set's come first
 };
 
 template <int HD, int R, bool CAP>
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   const int set = (int)blockIdx.x >= p.first1;
   const Args &a = p.a[set];
   const int block = (int)blockIdx.x - (set ? p.first1 : 0);
-  const int split = block % a.splits, group = block / a.splits, hk = blockIdx.y;
+  const int split = block % a.splits, unit = block / a.splits, group = unit / a.kv.nkv, hk = unit - group * a.kv.nkv;
   const int h0 = head0(hk, a.n_heads, a.kv.nkv), G = head0(hk + 1, a.n_heads, a.kv.nkv) - h0;
   // rows of this CTA: OWN one sequence's group, else R of the (i, g) rows
   const int first = a.mode == OWN ? group * G : group * R;
@@ -271,13 +274,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       const int t = j * kKeys + key;
       return t < n ? __ldg(src + kbeg + t) : 1.0f;
     };
-    const float inv_cap = CAP ? 1.0f / a.sc_att : 0.0f, unit = CAP ? a.sc_att * kLog2e : kLog2e;
-    float rf[RQ], l[RQ], lim[RQ];  // lim: the largest exponent that fits, m + kSlack
+    const float to_unit = CAP ? 1.0f / a.sc_att : kLog2e, unit = a.sc_att * kLog2e;
+    // up: what takes an exponent to that of the weight, kTop - m; while m is -inf,
+    // whatever is seen at all is too large
+    constexpr float kUnseen = 1e30f;
+    float rf[RQ], l[RQ], up[RQ];
 #pragma unroll
     for (int r = 0; r < RQ; ++r) {
-      rf[r] = nt > 0 ? s_rf[r0 + r] : 0.0f;
+      rf[r] = nt > 0 ? s_rf[r0 + r] * to_unit : 0.0f;
       l[r] = 0.0f;
-      lim[r] = -INFINITY;
+      up[r] = kUnseen;
     }
     // the output column of this thread, a lane of O^T, and its rows of it (hdim 256:
     // two blocks of columns, half of the rows each; else a quarter)
@@ -286,22 +292,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     float acc[C::OR];
 #pragma unroll
     for (int r = 0; r < C::OR; ++r) acc[r] = 0.0f;
-    const uint32_t olane = lanes + C::O_COL + oblock * C::NP + orow;
+    const uint32_t olane = lanes + C::O_COL + oblock * C::NP + 4 * orow;
     // add O^T's digit sums (complete) to the column's sums, then scale them
     auto flush = [&]() {
       ptx::tc_fence_after();
 #pragma unroll
       for (int r = 0; r < C::OR; r += 4) {
-        uint32_t d3[4], d2[4], d1[4], d0[4];
-        ptx::tmem_ld_32x4(olane + r, d0);
-        ptx::tmem_ld_32x4(olane + R + r, d1);
-        ptx::tmem_ld_32x4(olane + 2 * R + r, d2);
-        ptx::tmem_ld_32x4(olane + 3 * R + r, d3);
+        uint32_t d[16];
+        ptx::tmem_ld_32x16(olane + 4 * r, d);
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = (float)(int)d3[e] * 16777216.0f + (float)(int)d2[e] * 65536.0f;
-          v += (float)(int)d1[e] * 256.0f + (float)(int)d0[e];
+          float v = (float)(int)d[4 * e + 3] * 16777216.0f + (float)(int)d[4 * e + 2] * 65536.0f;
+          v += (float)(int)d[4 * e + 1] * 256.0f + (float)(int)d[4 * e];
           acc[r + e] += v;
         }
       }
@@ -317,23 +320,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       ptx::tc_fence_after();
       // exponents: the score in log2 units plus log2 of the value row's scale
       float x[RQ];
-#pragma unroll
-      for (int c = 0; c < RQ; c += 4) {
-        uint32_t s2[4], s1[4], s0[4];
-        const uint32_t at = lanes + C::S_COL + (j & 1) * C::NS + r0 + c;
-        ptx::tmem_ld_32x4(at, s0);
-        ptx::tmem_ld_32x4(at + R, s1);
-        ptx::tmem_ld_32x4(at + 2 * R, s2);
+      {
+        uint32_t s2[RQ], s1[RQ], s0[RQ];
+        const uint32_t at = lanes + C::S_COL + (j & 1) * C::NS + r0;
+        tmem_ld(at, s0);
+        tmem_ld(at + R, s1);
+        tmem_ld(at + 2 * R, s2);
         ptx::tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const float2 y = high_digit(s2 + e, low_digits(s1 + e, s0 + e));
-          float s[2] = {y.x * ks * rf[c + e], y.y * ks * rf[c + e + 1]};
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            if (CAP) s[q] = tanh_fast(s[q] * inv_cap);
-            x[c + e + q] = __fmaf_rn(s[q], unit, lvs);
+        for (int r = 0; r < RQ; r += 2) {
+          const float2 y = __fmul2_rn(high_digit(s2 + r, low_digits(s1 + r, s0 + r)), make_float2(ks, ks));
+          float2 e;
+          if constexpr (CAP) {
+            e = __fmul2_rn(y, make_float2(rf[r], rf[r + 1]));
+            e = __ffma2_rn(make_float2(tanh_fast(e.x), tanh_fast(e.y)), make_float2(unit, unit), make_float2(lvs, lvs));
+          } else {
+            e = __ffma2_rn(y, make_float2(rf[r], rf[r + 1]), make_float2(lvs, lvs));
           }
+          x[r] = e.x;
+          x[r + 1] = e.y;
         }
       }
       ptx::tc_fence_before();
@@ -345,11 +350,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         for (int r = 0; r < RQ; ++r)
           if (t < s_lo[r0 + r] || t >= min(s_hi[r0 + r], kend)) x[r] = -INFINITY;
       }
-      bool over = !ok;
+      float e[RQ];  // the weights' exponents
+      auto exponents = [&]() {
 #pragma unroll
-      for (int r = 0; r < RQ; ++r) over |= x[r] > lim[r];
+        for (int r = 0; r < RQ; r += 2) {
+          const float2 t = __fadd2_rn(make_float2(x[r], x[r + 1]), make_float2(up[r], up[r + 1]));
+          e[r] = t.x;
+          e[r + 1] = t.y;
+        }
+      };
+      exponents();
+      float most = e[0];
+#pragma unroll
+      for (int r = 1; r < RQ; ++r) most = fmaxf(most, e[r]);
       bool fresh = j == 0;
-      if (ptx::named_bar_or(1, kSoftmax, over)) {
+      if (ptx::named_bar_or(1, kSoftmax, !ok || most > kTop + kSlack)) {
         // some row's weights would run over: move every row's m to its largest
         // exponent so far, and take O^T's sums at the old one
         if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
@@ -379,38 +394,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
         for (int r = 0; r < RQ; ++r) {
           l[r] *= s_f[r0 + r];
-          lim[r] = s_m[r0 + r] + kSlack;
+          const float m = s_m[r0 + r];
+          up[r] = m == -INFINITY ? kUnseen : kTop - m;
         }
+        exponents();
         fresh = true;
       }
       // this buffer's last reader is the product of tile j - 2
       if (j > 1) ok = wait(&pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       uint32_t w[RQ];
 #pragma unroll
-      for (int r = 0; r < RQ; ++r) {
-        const float v = ex2(x[r] - (lim[r] == -INFINITY ? 0.0f : lim[r] - (kSlack + kTop)));
-        l[r] = __fmaf_rn(v, rvs, l[r]);
-        w[r] = __float2uint_rn(v);
+      for (int r = 0; r < RQ; r += 2) {
+        const float2 v = make_float2(ex2(e[r]), ex2(e[r + 1]));
+        const float2 t = __ffma2_rn(v, make_float2(rvs, rvs), make_float2(l[r], l[r + 1]));
+        l[r] = t.x;
+        l[r + 1] = t.y;
+        w[r] = __float2uint_rn(v.x);
+        w[r + 1] = __float2uint_rn(v.y);
       }
       uint8_t *dst = smem + C::P_OFF + (j & 1) * C::P_BYTES + key * C::P_ROW;
       const int sw = C::P_ROW == 128 ? key & 7 : (key >> 1) & 3;
 #pragma unroll
-      for (int d = 0; d < 4; ++d) {
-        const int col = d * R + r0;
-        uint32_t b[RQ / 4];
-#pragma unroll
-        for (int e = 0; e < RQ / 4; ++e) {
-          const uint32_t lo = __byte_perm(w[4 * e], w[4 * e + 1], d | (d + 4) << 4);
-          const uint32_t hi = __byte_perm(w[4 * e + 2], w[4 * e + 3], d | (d + 4) << 4);
-          b[e] = __byte_perm(lo, hi, 0x5410);
-        }
-        uint8_t *q = dst + (((col >> 4) ^ sw) << 4) + (col & 15);
-        if constexpr (RQ == 8) {
-          *reinterpret_cast<uint2 *>(q) = make_uint2(b[0], b[1]);
-        } else {
-          *reinterpret_cast<uint32_t *>(q) = b[0];
-        }
-      }
+      for (int r = 0; r < RQ; r += 4)
+        *reinterpret_cast<uint4 *>(dst + (((r0 + r) >> 2 ^ sw) << 4)) = make_uint4(w[r], w[r + 1], w[r + 2], w[r + 3]);
       if (threadIdx.x == 0) *(volatile int *)&s_fresh[j & 1] = fresh;
       ptx::fence_proxy_async_smem();
       ptx::mbar_arrive(&pfull[j & 1]);
@@ -491,7 +497,7 @@ int launch_kt_r(const Args *sets, int n, cudaStream_t st) {
     p.a[s] = a;
     if (s == 1) p.first1 = (int)(n > 1 ? blocks : 0x7fffffff);
     if (s >= n) continue;
-    blocks += (a.mode == OWN ? (long)a.ni : ((long)a.ni * G + R - 1) / R) * a.splits;
+    blocks += (a.mode == OWN ? (long)a.ni : ((long)a.ni * G + R - 1) / R) * a.kv.nkv * a.splits;
     if (blocks > 0x7fffffffL - 1) return set_error("attention_i8: %ld CTAs", blocks);
     if (gemm_tmap_heads_i8(&p.k[s], a.kv.k, a.kv, kKeys) || gemm_tmap_heads_i8(&p.v[s], a.kv.v, a.kv, kKeys)) return 1;
   }
@@ -508,7 +514,7 @@ int launch_kt_r(const Args *sets, int n, cudaStream_t st) {
     }
   }
   const unsigned cluster = sets[0].slots == 1 ? sets[0].splits : 1;
-  GCU_CUDA(launch_cluster_k(k_kt<HD, R, CAP>, dim3((unsigned)blocks, sets[0].kv.nkv), dim3(kThreads), cluster, C::SMEM,
+  GCU_CUDA(launch_cluster_k(k_kt<HD, R, CAP>, dim3((unsigned)blocks), dim3(kThreads), cluster, C::SMEM,
                             st, p));
   return 0;
 }
