@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R];
+  __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R], s_row[R];
   __shared__ float s_rf[R], s_m[R], s_f[R], s_sum[R], s_red[16][R / 4];
   // aligned by an offset: the accesses stay in the shared address space
   uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -121,9 +121,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 
   // The rows' windows, lane r of every warp: the CTA's key range, and the keys that
   // every row sees.
-  int lo = 0, hi = 0;
-  if (lane < nr) row_window(a, rows.i(lane), lo, hi);
+  int lo = 0, hi = 0, row = 0;  // row: its place among the i * n_heads + h
+  if (lane < nr) {
+    const int i = rows.i(lane);
+    row = i * a.n_heads + h0 + rows.g(lane);
+    row_window(a, i, lo, hi);
+    if (!row_live(a, i)) row = -1;
+  }
   if (threadIdx.x < R) {
+    s_row[threadIdx.x] = row;
     s_lo[threadIdx.x] = lo;
     s_hi[threadIdx.x] = hi;
     s_m[threadIdx.x] = -INFINITY;
@@ -161,11 +167,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   }
   // the query rows' digits, row n = d * R + r; rows past the end are zeros
   if (nt > 0) {
-    constexpr int E = HD / 32;
-    for (int r = warp; r < R; r += kThreads / 32) {
-      float v[E], amax;
+    constexpr int E = HD / 32, W = kThreads / 32, N = (R + W - 1) / W;  // rows of a warp
+    float vs[N][E];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = warp + n * W, at = __shfl_sync(0xffffffffu, row, r & 31);
+      load_floats<E>(vs[n], a.xq + (long)at * HD + lane * E, r < nr && at >= 0);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = warp + n * W;
+      if (r >= R) break;
+      float (&v)[E] = vs[n];
+      float amax;
       uint32_t w[3][(E + 3) / 4];
-      load_floats<E>(v, a.xq + (long)rows.i(r) * a.q_i + (long)(h0 + rows.g(r)) * a.q_h + lane * E, r < nr);
       row_digits<E>(v, w, amax);
       const int col = lane * E, in = col % C::SW;
 #pragma unroll
@@ -432,28 +447,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       if (lane == 0) s_red[warp][r] = v;
     }
     ptx::named_bar_sync(1, kSoftmax);
+    const size_t rows_all = (size_t)a.ni * a.n_heads;
+    const int slot = a.slot0 + split;
+    if (threadIdx.x < nr) {
+      const int r = threadIdx.x, q = r / RQ * 4, at = s_row[r];
+      const float sum = (s_red[q][r % RQ] + s_red[q + 1][r % RQ]) + (s_red[q + 2][r % RQ] + s_red[q + 3][r % RQ]);
+      const float m = s_m[r];
+      s_sum[r] = sum;
+      if (a.slots > 1 && at >= 0) a.stat[slot * rows_all + at] = make_float2(m == -INFINITY ? m : m - kTop, sum);
+    }
     if (nt > 0) {
       ok = wait(&pvdone[(nt - 1) & 1], ((nt - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       flush();
     }
+    // OWN and PREFIX rows lie one after another: row * HD
+    ptx::named_bar_sync(1, kSoftmax);
     if (ok && ocol < HD) {
+      float *to = fused ? part + ocol : a.slots == 1 ? a.xo + ocol : a.part + (size_t)slot * rows_all * HD + ocol;
 #pragma unroll
       for (int r = 0; r < C::OR; ++r) {
         const int rr = orow + r;
         if (rr >= nr) break;
-        const int hh = rr / RQ, i = rows.i(rr), h = h0 + rows.g(rr);
-        const float sum = (s_red[hh * 4][rr % RQ] + s_red[hh * 4 + 1][rr % RQ]) +
-                          (s_red[hh * 4 + 2][rr % RQ] + s_red[hh * 4 + 3][rr % RQ]);
+        const int at = s_row[rr];
         if (fused) {
-          part[rr * HD + ocol] = acc[r];
-          if (ocol == 0) s_sum[rr] = sum;
-        } else if (a.slots == 1) {  // a row that sees nothing: zeros
-          if (row_live(a, i)) a.xo[(long)i * a.o_i + (long)h * HD + ocol] = acc[r] / (sum == 0.0f ? 1.0f : sum);
-        } else {
-          const size_t at = ((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h;
-          const float m = s_m[rr];
-          a.part[at * HD + ocol] = acc[r];
-          if (ocol == 0) a.stat[at] = make_float2(m == -INFINITY ? m : m - kTop, sum);
+          to[rr * HD] = acc[r];
+        } else if (at >= 0) {  // a row that sees nothing: zeros
+          const float sum = s_sum[rr];
+          to[(size_t)at * HD] = a.slots == 1 ? acc[r] / (sum == 0.0f ? 1.0f : sum) : acc[r];
         }
       }
     }
@@ -478,9 +498,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         l += f * ls;
         o += f * cl.map_shared_rank(part, s)[e];
       }
-      const int i = rows.i(rr);
-      if (row_live(a, i))
-        a.xo[(long)i * a.o_i + (long)(h0 + rows.g(rr)) * HD + e % HD] = o / (l == 0.0f ? 1.0f : l);
+      if (s_row[rr] >= 0) a.xo[(long)s_row[rr] * HD + e % HD] = o / (l == 0.0f ? 1.0f : l);
     }
     cl.sync();  // read by all
   }
