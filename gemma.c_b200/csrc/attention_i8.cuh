@@ -149,28 +149,36 @@ __device__ __forceinline__ void load_floats(float (&v)[E], const float *src, boo
     v[1] = f.y;
   }
 }
-// a warp's row: its largest |element| (NaN if there is one) and the digits of this
-// lane's elements, packed bytes of d0, d1, d2
-template <int E>
-__device__ __forceinline__ void row_digits(const float (&v)[E], uint32_t (&w)[3][(E + 3) / 4], float &amax) {
-  amax = 0.0f;
+// N rows of a warp: their largest |elements| (NaN if there is one) and the digits of
+// this lane's elements, packed bytes of d0, d1, d2
+template <int E, int N>
+__device__ __forceinline__ void row_digits(const float (&v)[N][E], uint32_t (&w)[N][3][(E + 3) / 4], float (&amax)[N]) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) amax = max_nan(amax, fabsf(v[e]));
+  for (int n = 0; n < N; ++n) {
+    amax[n] = 0.0f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float inv = amax > 0.0f ? kQMax / amax : 0.0f;
-  // n + 0x808080 has the digits, each plus 128, as its bytes
-  uint32_t u[(E + 3) / 4 * 4] = {};
+    for (int e = 0; e < E; ++e) amax[n] = max_nan(amax[n], fabsf(v[n][e]));
+  }
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    u[e] = __float_as_uint(__fmaf_rn(v[e], inv, 12582912.0f)) - 0x4B400000u + 0x808080u;
+  for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-  for (int i = 0; i < (E + 3) / 4; ++i) {
-    const uint32_t *x = u + 4 * i;
-    const uint32_t a = __byte_perm(x[0], x[1], 0x5140), b = __byte_perm(x[2], x[3], 0x5140);
-    w[0][i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
-    w[1][i] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
-    w[2][i] = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410) ^ 0x80808080u;
+    for (int n = 0; n < N; ++n) amax[n] = max_nan(amax[n], __shfl_xor_sync(0xffffffffu, amax[n], o));
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float inv = amax[n] > 0.0f ? kQMax / amax[n] : 0.0f;
+    // n + 0x808080 has the digits, each plus 128, as its bytes
+    uint32_t u[(E + 3) / 4 * 4] = {};
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      u[e] = __float_as_uint(__fmaf_rn(v[n][e], inv, 12582912.0f)) - 0x4B400000u + 0x808080u;
+#pragma unroll
+    for (int i = 0; i < (E + 3) / 4; ++i) {
+      const uint32_t *x = u + 4 * i;
+      const uint32_t a = __byte_perm(x[0], x[1], 0x5140), b = __byte_perm(x[2], x[3], 0x5140);
+      w[n][0][i] = __byte_perm(a, b, 0x5410) ^ 0x80808080u;
+      w[n][1][i] = __byte_perm(a, b, 0x7632) ^ 0x80808080u;
+      w[n][2][i] = __byte_perm(__byte_perm(x[0], x[1], 0x0062), __byte_perm(x[2], x[3], 0x0062), 0x5410) ^ 0x80808080u;
+    }
   }
 }
 template <int E>

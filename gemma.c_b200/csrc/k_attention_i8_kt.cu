@@ -168,28 +168,27 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   // the query rows' digits, row n = d * R + r; rows past the end are zeros
   if (nt > 0) {
     constexpr int E = HD / 32, W = kThreads / 32, N = (R + W - 1) / W;  // rows of a warp
-    float vs[N][E];
+    float vs[N][E];  // of all its rows in flight at once
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int r = warp + n * W, at = __shfl_sync(0xffffffffu, row, r & 31);
       load_floats<E>(vs[n], a.xq + (long)at * HD + lane * E, r < nr && at >= 0);
     }
+    float amax[N];
+    uint32_t w[N][3][(E + 3) / 4];
+    row_digits<E, N>(vs, w, amax);
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int r = warp + n * W;
       if (r >= R) break;
-      float (&v)[E] = vs[n];
-      float amax;
-      uint32_t w[3][(E + 3) / 4];
-      row_digits<E>(v, w, amax);
       const int col = lane * E, in = col % C::SW;
 #pragma unroll
       for (int d = 0; d < 3; ++d) {
-        const int row = d * R + r, sw = C::SW == 128 ? row & 7 : (row >> 1) & 3;
-        uint8_t *q = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + row * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
-        put_digits<E>(q, w[d]);
+        const int line = d * R + r, sw = C::SW == 128 ? line & 7 : (line >> 1) & 3;
+        uint8_t *q = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + line * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
+        put_digits<E>(q, w[n][d]);
       }
-      if (lane == 0) s_rf[r] = amax / kQMax * a.asc;
+      if (lane == 0) s_rf[r] = amax[n] / kQMax * a.asc;
     }
   }
   ptx::fence_proxy_async_smem();
@@ -471,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         const int at = s_row[rr];
         if (fused) {
           to[rr * HD] = acc[r];
-        } else if (at >= 0) {  // a row that sees nothing: zeros
+        } else if (at >= 0 && (nt > 0 || a.slots == 1)) {  // a row that sees nothing: zeros
           const float sum = s_sum[rr];
           to[(size_t)at * HD] = a.slots == 1 ? acc[r] / (sum == 0.0f ? 1.0f : sum) : acc[r];
         }

@@ -132,10 +132,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
   const Args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.y;
+  // heavy CTAs first: the first chunks, and of each the last query rows, which see
+  // the most keys; the heads side by side
+  const int hk = blockIdx.x % a.kv.nkv, unit = blockIdx.x / a.kv.nkv, split = unit / p.tiles;
+  const int tile = p.tiles - 1 - (unit - split * p.tiles);
   const int h0 = head0(hk, a.n_heads, a.kv.nkv), G = head0(hk + 1, a.n_heads, a.kv.nkv) - h0;
-  // heavy tiles first: the last query rows of a prompt see the most keys
-  const int tile = p.tiles - 1 - (int)(blockIdx.x / a.splits), split = blockIdx.x % a.splits;
   const int first = tile * kRows, nrows = min(kRows, a.ni * G - first);
   const RowSplit rows(first, G);
   if (threadIdx.x == 0) {
@@ -222,22 +223,31 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     auto load_row = [&](float (&v)[E], int r) {
       load_floats<E>(v, a.xq + (long)rows.i(r) * a.q_i + (long)(h0 + rows.g(r)) * a.q_h + lane * E, r < nrows);
     };
-    float v[E], ahead[E];
-    load_row(v, warp);
+    float v[2][E], ahead[2][E];  // two rows at a time: their reductions overlap
+    load_row(v[0], warp);
+    load_row(v[1], warp + W);
 #pragma unroll 1
-    for (int r = warp; r < kRows; r += W) {
-      load_row(ahead, r + W);
-      float amax;
-      uint32_t w[3][(E + 3) / 4];
-      row_digits<E>(v, w, amax);
-      const int col = lane * E, in = col % C::SW;
-      const int sw = C::SW == 128 ? r & 7 : (r >> 1) & 3;
-      uint8_t *dst = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + r * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
+    for (int r0 = warp; r0 < kRows; r0 += 2 * W) {
+      load_row(ahead[0], r0 + 2 * W);
+      load_row(ahead[1], r0 + 3 * W);
+      float amax[2];
+      uint32_t w[2][3][(E + 3) / 4];
+      row_digits<E, 2>(v, w, amax);
 #pragma unroll
-      for (int d = 0; d < 3; ++d) put_digits<E>(dst + d * C::KB * C::Q_BLOCK, w[d]);
-      if (lane == 0) s_rf[r] = amax / kQMax * a.asc;
+      for (int t = 0; t < 2; ++t) {
+        const int r = r0 + t * W, col = lane * E, in = col % C::SW;
+        if (r >= kRows) break;
+        const int sw = C::SW == 128 ? r & 7 : (r >> 1) & 3;
+        uint8_t *dst = smem + C::Q_OFF + (col / C::SW) * C::Q_BLOCK + r * C::SW + (((in >> 4) ^ sw) << 4) + (in & 15);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = ahead[e];
+        for (int d = 0; d < 3; ++d) put_digits<E>(dst + d * C::KB * C::Q_BLOCK, w[t][d]);
+        if (lane == 0) s_rf[r] = amax[t] / kQMax * a.asc;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[0][e] = ahead[0][e];
+        v[1][e] = ahead[1][e];
+      }
     }
     // tile 0's scales
     if ((int)threadIdx.x < 2 * NK) {
@@ -574,7 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       a.stat[((size_t)(a.slot0 + split) * a.ni + rows.i(row)) * a.n_heads + h0 + rows.g(row)] =
           make_float2(m == -INFINITY ? m : m - kTop, l);
     ptx::named_bar_sync(3, kSoftmax);
-    for (int r = warp; r < nrows && ok; r += kSoftmax / 32) {
+    const bool none = nt == 0 && a.slots > 1;  // (-inf, 0) says that there is nothing to add
+    for (int r = warp; r < nrows && ok && !none; r += kSoftmax / 32) {
       const int i = rows.i(r), h = h0 + rows.g(r);
       float *out = a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD
                                 : a.part + (((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h) * HD;
@@ -595,7 +606,8 @@ int launch_tc_hd(const Args &a, cudaStream_t st) {
   p.a = a;
   const int gmax = (a.n_heads + a.kv.nkv - 1) / a.kv.nkv;
   p.tiles = (int)(((long)a.ni * gmax + kRows - 1) / kRows);
-  if ((long)p.tiles * a.splits > 0x7fffffffL) return set_error("attention_i8: %d x %d CTAs", p.tiles, a.splits);
+  const long ctas = (long)p.tiles * a.splits * a.kv.nkv;
+  if (ctas > 0x7fffffffL) return set_error("attention_i8: %ld CTAs", ctas);
   if (gemm_tmap_heads_i8(&p.tmK, a.kv.k, a.kv, NK)) return 1;
   {
     // the shared-memory opt-in is per device: once for each device this runs on
@@ -609,7 +621,7 @@ int launch_tc_hd(const Args &a, cudaStream_t st) {
       done |= 1ull << (dev & 63);
     }
   }
-  GCU_CUDA(launch_k(k_tc<HD, CAP>, dim3((unsigned)(p.tiles * a.splits), a.kv.nkv), dim3(kThreads), C::SMEM, st, p));
+  GCU_CUDA(launch_k(k_tc<HD, CAP>, dim3((unsigned)ctas), dim3(kThreads), C::SMEM, st, p));
   return 0;
 }
 
