@@ -125,6 +125,13 @@ constexpr long kSetup = 3;
 // against 7.7; with three further tiles (4096 keys) 10.6 against 9.4.
 constexpr long kJoin = 1;
 
+bool join(Plan &p, long n, long units) {
+  const Plan few = plan_range(n, units, std::min((long)num_sms(), kKtCluster * units), kKtKeys);
+  if (few.splits < 2 || few.splits > kKtCluster || few.chunk > p.chunk + kJoin * kKtKeys) return false;
+  p = few;
+  return true;
+}
+
 DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads, int slide) {
   const long G = max_group(n_heads, own.nkv), sms = std::max(1, num_sms());
   DecodePlan p;
@@ -132,12 +139,7 @@ DecodePlan plan_decode(const gcu_kv_i8 &own, int plen, int max_len, int n_heads,
   const long units = (long)own.nkv * own.nseq;
   p.own = plan_range(visible(max_len, slide), units, plen > 0 ? sms / 2 : sms, kKtKeys);
   p.pre = Plan{1, 0};
-  p.cluster = false;
-  if (plen == 0) {
-    const Plan few = plan_range(visible(max_len, slide), units, std::min(sms, kKtCluster * units), kKtKeys);
-    p.cluster = few.splits > 1 && few.splits <= kKtCluster && few.chunk <= p.own.chunk + kJoin * kKtKeys;
-    if (p.cluster) p.own = few;
-  }
+  p.cluster = plen == 0 && join(p.own, visible(max_len, slide), units);
   if (plen > 0) {
     const long n = visible(plen, slide), tiles = (n + kKtKeys - 1) / kKtKeys;
     const long pre = (own.nseq * G + p.rows - 1) / p.rows * own.nkv;
@@ -229,24 +231,66 @@ GCU_EXPORT int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu
 
 namespace {
 
-Plan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, int slide, int mask) {
-  // a window's width, and the tokens of one CTA's rows past its first
-  const long n = mask && slide > 0 ? std::min((long)spos + ntok, (long)slide + kTcRows) : (long)spos + ntok;
-  const long units = ((long)ntok * max_group(n_heads, kv.nkv) + kTcRows - 1) / kTcRows * kv.nkv;
-  return plan_range(n, units, num_sms(), kTcKeys);
+// Which kernel takes a prompt chunk, and how its keys are split.  k_kt (32 rows a
+// CTA) starts and ends quickly and joins its chunks itself, k_tc (128 rows) moves a
+// quarter of the keys per product: 512 tokens of 4 + 1 heads of 256 take 12.8 us
+// against 21.5, 2048 of 16 + 8 heads 136 against 93.  The times come from a model
+// fitted to both at 64 to 4096 tokens, heads 4 + 1, 8 + 4 and 16 + 8 of 64, 128 and 256:
+// `fixed` us a CTA and `tile` us a tile of keys, the longest CTA or the average load
+// of an SM, and a merge.
+struct PrefillPlan {
+  bool kt, cluster;
+  int rows;
+  Plan p;
+  int slots() const { return cluster ? 1 : p.splits; }
+};
+
+// kernel: 0 the faster of the two, 1 k_kt, 2 k_tc
+PrefillPlan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, int slide, int mask, bool cap,
+                         int kernel = 0) {
+  const long G = max_group(n_heads, kv.nkv), sms = std::max(1, num_sms()), end = (long)spos + ntok;
+  const bool window = mask && slide > 0;
+  auto plan = [&](bool kt, double &time) {
+    PrefillPlan p;
+    p.kt = kt;
+    p.rows = !kt ? kTcRows : ntok * G > 16 ? 32 : 16;
+    const int keys = kt ? kKtKeys : kTcKeys;
+    const long units = (ntok * G + p.rows - 1) / p.rows * kv.nkv;
+    // keys that a CTA's rows see when the last of them is at position at - 1: a window
+    // and the tokens of the rows past the first
+    auto seen = [&](long at) { return !mask ? end : window ? std::min(at, (long)slide + p.rows) : at; };
+    const long n = seen(end);
+    p.p = plan_range(n, units, sms, keys);
+    p.cluster = kt && join(p.p, n, units);
+    const double fixed = kt ? (kv.hdim == 256 ? 7.5 : 6.5) : kv.hdim == 256 ? 12.0 : kv.hdim == 128 ? 9.0 : 8.0;
+    double tile = kt ? (kv.hdim == 256 ? 1.4 : 1.25) : kv.hdim == 256 ? 2.4 : kv.hdim == 128 ? 1.6 : 1.45;
+    if (cap) tile *= kt ? 1.4 : 1.6;
+    const long ctas = units * p.p.splits, waves = (ctas + sms - 1) / sms;
+    const double mean = (seen(spos + 1) + 2 * seen(spos + ntok / 2 + 1) + n) / 4.0 / keys + 0.5;
+    time = std::max(fixed + tile * (p.p.chunk / keys),
+                    (kt ? (double)waves : (double)ctas / sms) * fixed + units * mean * tile / sms);
+    if (p.p.splits > 1 && !p.cluster) time += 5.0;
+    return p;
+  };
+  double few, many;
+  const PrefillPlan kt = plan(true, few), tc = plan(false, many);
+  return kernel ? (kernel == 1 ? kt : tc) : few < many ? kt : tc;
 }
 
 }  // namespace
 
 GCU_EXPORT size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide,
-                                                int mask) {
+                                                float sc_att, int mask) {
   if (!kv || kv->nkv < 1 || n_heads < 1 || ntok < 1 || spos < 0) return 0;
-  return slot_bytes(plan_prefill(*kv, n_heads, spos, ntok, slide, mask).splits, (long)ntok * n_heads, kv->hdim);
+  return slot_bytes(plan_prefill(*kv, n_heads, spos, ntok, slide, mask, sc_att != 0.0f).slots(), (long)ntok * n_heads,
+                    kv->hdim);
 }
 
-GCU_EXPORT int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,
-                                            int spos, int ntok, int slide, float sc_att, int mask, void *work,
-                                            size_t work_bytes, void *stream) {
+// The public call, and with the kernel given (for tests and measurements; not in the
+// public header).
+GCU_EXPORT int gcu_dev_attention_prefill_i8_tuned(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv,
+                                                  int n_heads, int spos, int ntok, int slide, float sc_att, int mask,
+                                                  void *work, size_t work_bytes, int kernel, void *stream) {
   if (ntok == 0) return 0;
   const char *what = "attention_prefill_i8";
   if (check_kv_i8(what, kv, 1) || check_heads(what, n_heads, kv->nkv)) return 1;
@@ -256,13 +300,20 @@ GCU_EXPORT int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *x
   if (xostr == 0) xostr = n_heads * kv->hdim;
   if (!aligned16(xo) || !aligned16(xq) || xostr % 4 || xostr < n_heads * kv->hdim)
     return set_error("%s: buffers must be 16-byte aligned, xostr a multiple of 4 floats, at least n_heads*hdim", what);
-  const Plan p = plan_prefill(*kv, n_heads, spos, ntok, slide, mask);
+  const PrefillPlan p = plan_prefill(*kv, n_heads, spos, ntok, slide, mask, sc_att != 0.0f, kernel);
   const long rows = (long)ntok * n_heads;
-  if (check_work(what, slot_bytes(p.splits, rows, kv->hdim), work, work_bytes)) return 1;
+  if (check_work(what, slot_bytes(p.slots(), rows, kv->hdim), work, work_bytes)) return 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Args a{xq, kv->hdim, (long)ntok * kv->hdim, xo, xostr, *kv, PREFILL, n_heads, ntok, spos, slide, mask ? 1 : 0, 0, 0,
-         nullptr, 1.0f, sc_att, p.chunk, p.splits, 0, p.splits, nullptr, nullptr, dev_error_word()};
+         nullptr, 1.0f, sc_att, p.p.chunk, p.p.splits, 0, p.slots(), nullptr, nullptr, dev_error_word()};
   use_work(a, work, rows);
-  if (launch_tc(a, st)) return 1;
+  if (p.kt ? launch_kt(&a, 1, p.rows, st) : launch_tc(a, st)) return 1;
   return a.slots > 1 ? launch_merge(a, st) : 0;
+}
+
+GCU_EXPORT int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,
+                                            int spos, int ntok, int slide, float sc_att, int mask, void *work,
+                                            size_t work_bytes, void *stream) {
+  return gcu_dev_attention_prefill_i8_tuned(xo, xostr, xq, kv, n_heads, spos, ntok, slide, sc_att, mask, work,
+                                            work_bytes, 0, stream);
 }

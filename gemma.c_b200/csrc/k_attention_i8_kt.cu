@@ -79,6 +79,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R], s_row[R];
+  __shared__ long s_out[R];
+  __shared__ float s_part[kKtCluster][R];  // a fused merge's factors
   __shared__ float s_rf[R], s_m[R], s_f[R], s_sum[R], s_red[16][R / 4];
   // aligned by an offset: the accesses stay in the shared address space
   uint8_t *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
@@ -87,7 +89,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   const int set = (int)blockIdx.x >= p.first1;
   const Args &a = p.a[set];
   const int block = (int)blockIdx.x - (set ? p.first1 : 0);
-  const int split = block % a.splits, unit = block / a.splits, group = unit / a.kv.nkv, hk = unit - group * a.kv.nkv;
+  const int split = block % a.splits, unit = block / a.splits;
+  int group = unit / a.kv.nkv;
+  const int hk = unit - group * a.kv.nkv;
+  // a prompt's last rows see the most keys: they come first
+  if (a.mode == PREFILL) group = (int)gridDim.x / (a.splits * a.kv.nkv) - 1 - group;
   const int h0 = head0(hk, a.n_heads, a.kv.nkv), G = head0(hk + 1, a.n_heads, a.kv.nkv) - h0;
   // rows of this CTA: OWN one sequence's group, else R of the (i, g) rows
   const int first = a.mode == OWN ? group * G : group * R;
@@ -122,14 +128,18 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   // The rows' windows, lane r of every warp: the CTA's key range, and the keys that
   // every row sees.
   int lo = 0, hi = 0, row = 0;  // row: its place among the i * n_heads + h
+  long from = 0, to = 0;        // in xq and xo
   if (lane < nr) {
-    const int i = rows.i(lane);
-    row = i * a.n_heads + h0 + rows.g(lane);
+    const int i = rows.i(lane), h = h0 + rows.g(lane);
+    row = i * a.n_heads + h;
+    from = i * a.q_i + h * a.q_h;
+    to = i * a.o_i + (long)h * HD;
     row_window(a, i, lo, hi);
     if (!row_live(a, i)) row = -1;
   }
   if (threadIdx.x < R) {
     s_row[threadIdx.x] = row;
+    s_out[threadIdx.x] = to;
     s_lo[threadIdx.x] = lo;
     s_hi[threadIdx.x] = hi;
     s_m[threadIdx.x] = -INFINITY;
@@ -172,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const int r = warp + n * W, at = __shfl_sync(0xffffffffu, row, r & 31);
-      load_floats<E>(vs[n], a.xq + (long)at * HD + lane * E, r < nr && at >= 0);
+      load_floats<E>(vs[n], a.xq + __shfl_sync(0xffffffffu, from, r & 31) + lane * E, r < nr && at >= 0);
     }
     float amax[N];
     uint32_t w[N][3][(E + 3) / 4];
@@ -459,20 +469,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       ok = wait(&pvdone[(nt - 1) & 1], ((nt - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       flush();
     }
-    // OWN and PREFIX rows lie one after another: row * HD
     ptx::named_bar_sync(1, kSoftmax);
     if (ok && ocol < HD) {
-      float *to = fused ? part + ocol : a.slots == 1 ? a.xo + ocol : a.part + (size_t)slot * rows_all * HD + ocol;
+      float *to_part = a.part + (size_t)slot * rows_all * HD + ocol;
 #pragma unroll
       for (int r = 0; r < C::OR; ++r) {
         const int rr = orow + r;
         if (rr >= nr) break;
         const int at = s_row[rr];
         if (fused) {
-          to[rr * HD] = acc[r];
-        } else if (at >= 0 && (nt > 0 || a.slots == 1)) {  // a row that sees nothing: zeros
+          part[rr * HD + ocol] = acc[r];
+        } else if (at < 0) {
+          continue;
+        } else if (a.slots == 1) {  // a row that sees nothing: zeros
           const float sum = s_sum[rr];
-          to[(size_t)at * HD] = a.slots == 1 ? acc[r] / (sum == 0.0f ? 1.0f : sum) : acc[r];
+          a.xo[s_out[rr] + ocol] = acc[r] / (sum == 0.0f ? 1.0f : sum);
+        } else if (nt > 0) {
+          to_part[(size_t)at * HD] = acc[r];
         }
       }
     }
@@ -486,18 +499,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     // CTAs' shared memory, each CTA a share of the elements
     auto cl = cooperative_groups::this_cluster();
     cl.sync();
-    for (int e = split * kThreads + threadIdx.x; e < nr * HD; e += a.splits * kThreads) {
-      const int rr = e / HD;
-      float m = -INFINITY, o = 0.0f, l = 0.0f;
-      for (int s = 0; s < a.splits; ++s) m = fmaxf(m, cl.map_shared_rank(s_m, s)[rr]);
-      for (int s = 0; s < a.splits; ++s) {
-        const float ms = cl.map_shared_rank(s_m, s)[rr], ls = cl.map_shared_rank(s_sum, s)[rr];
-        if (ms == -INFINITY && ls == 0.0f) continue;  // sees none of the chunk
-        const float f = ex2(ms - m);
-        l += f * ls;
-        o += f * cl.map_shared_rank(part, s)[e];
+    if ((int)threadIdx.x < nr) {
+      const int r = threadIdx.x;
+      float ms[kKtCluster], ls[kKtCluster], m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kKtCluster; ++s) {
+        ms[s] = s < a.splits ? cl.map_shared_rank(s_m, s)[r] : -INFINITY;
+        ls[s] = s < a.splits ? cl.map_shared_rank(s_sum, s)[r] : 0.0f;
       }
-      if (s_row[rr] >= 0) a.xo[(long)s_row[rr] * HD + e % HD] = o / (l == 0.0f ? 1.0f : l);
+#pragma unroll
+      for (int s = 0; s < kKtCluster; ++s) m = fmaxf(m, ms[s]);
+#pragma unroll
+      for (int s = 0; s < kKtCluster; ++s) {
+        const float f = ms[s] == -INFINITY && ls[s] == 0.0f ? 0.0f : ex2(ms[s] - m);  // 0: sees none of the chunk
+        s_part[s][r] = f;
+        l += f * ls[s];
+      }
+      s_lo[r] = __float_as_int(l == 0.0f ? 1.0f : l);
+    }
+    __syncthreads();
+    for (int e = split * kThreads + threadIdx.x; e < nr * (HD / 4); e += a.splits * kThreads) {
+      const int rr = e / (HD / 4);
+      float4 v[kKtCluster];
+#pragma unroll
+      for (int s = 0; s < kKtCluster; ++s)
+        v[s] = s < a.splits && s_part[s][rr] != 0.0f ? reinterpret_cast<const float4 *>(cl.map_shared_rank(part, s))[e]
+                                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int s = 0; s < kKtCluster; ++s) {
+        const float f = s_part[s][rr];
+        o.x += f * v[s].x;
+        o.y += f * v[s].y;
+        o.z += f * v[s].z;
+        o.w += f * v[s].w;
+      }
+      const float l = __int_as_float(s_lo[rr]);
+      if (s_row[rr] >= 0)
+        *reinterpret_cast<float4 *>(a.xo + s_out[rr] + e % (HD / 4) * 4) = make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
     }
     cl.sync();  // read by all
   }

@@ -124,7 +124,7 @@ SIGNATURES = {
     "gcu_attention_decode_i8_work": (ctypes.c_size_t, [_vp, _int, _vp, _int, _int, _int]),
     "gcu_dev_attention_decode_i8": (_int, [_vp, _vp, _vp, _int, _vp, _vp, _int, _int, _int, ctypes.c_float,
                                            ctypes.c_float, _vp, ctypes.c_size_t, _vp]),
-    "gcu_attention_prefill_i8_work": (ctypes.c_size_t, [_vp, _int, _int, _int, _int, _int]),
+    "gcu_attention_prefill_i8_work": (ctypes.c_size_t, [_vp, _int, _int, _int, _int, ctypes.c_float, _int]),
     "gcu_dev_attention_prefill_i8": (_int, [_vp, _int, _vp, _vp, _int, _int, _int, _int, ctypes.c_float, _int, _vp,
                                             ctypes.c_size_t, _vp]),
     "gcu_dev_sample": (_int, [_vp, _vp, _vp, ctypes.c_long, _vp, ctypes.c_float, _int, ctypes.c_float, ctypes.c_float,
@@ -135,6 +135,8 @@ SIGNATURES = {
 }
 # exported but not part of the public header (benchmark sweeps, self-test)
 EXTRA = {
+    "gcu_dev_attention_prefill_i8_tuned": (_int, [_vp, _int, _vp, _vp, _int, _int, _int, _int, ctypes.c_float, _int,
+                                                  _vp, ctypes.c_size_t, _int, _vp]),
     "gcu_selftest_bounded_wait": (_int, [_int, _int, ctypes.POINTER(ctypes.c_ulonglong), _vp]),
     "gcu_dev_gemm_int8_multi_tuned": (_int, [ctypes.POINTER(GemvJob), _int, _vp, _int, _vp, _int, _int, _int,
                                              _int, _int, _vp]),
@@ -823,8 +825,8 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
             xo.shape[1] >= n_heads * kv.hdim and xo.get_device() == dev):
         raise GcuError(f"{what}: xo must be float32 (ntok, >= n_heads*hdim) rows, not {xo.dtype} {tuple(xo.shape)}")
     l = lib()
-    work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, int(mask)), kv.device,
-                               stream)
+    work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, sc_att, int(mask)),
+                               kv.device, stream)
     _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0), xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
                                           sc_att, int(mask), work, nbytes, _on(stream, dev)), what)
 

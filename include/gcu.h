@@ -419,7 +419,8 @@ int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu_kv_i8 *pre
  * already in the cache; xq [n_heads][ntok][hdim], rotated and scaled; token i
  * of head h goes to xo + i*xostr + h*hdim (xostr 0 = n_heads*hdim).  mask,
  * slide and sc_att as there; work as above. */
-size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide, int mask);
+size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide, float sc_att,
+                                     int mask);
 int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,
                                  int spos, int ntok, int slide, float sc_att, int mask, void *work,
                                  size_t work_bytes, void *stream);
