@@ -1,9 +1,8 @@
-// k_attention_i8_tc.cu -- attention over the 8-bit KV cache on the tensor cores:
-// prompt chunks, and decode rows that share a prefix.
+// k_attention_i8_tc.cu -- attention over the 8-bit KV cache for prompt chunks of
+// many rows.
 //
-// A CTA takes 128 query rows of one kv head (token or sequence i, head of the
-// group: the heads that share keys fill the rows) and one chunk of the key
-// range, and walks it in tiles of NK keys, keeping the running maximum and sum
+// A CTA takes 128 query rows of one kv head (token i, head of the group: the heads
+// that share keys fill the rows) and one chunk of the key range, and walks it in tiles of NK keys, keeping the running maximum and sum
 // of the softmax:
 //   S   three tcgen05.mma kind::i8 products per tile, the query's three digits
 //       against the codes as TMA brings them: exact int32 sums in TMEM, put
@@ -589,7 +588,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       const int i = rows.i(r), h = h0 + rows.g(r);
       float *out = a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD
                                 : a.part + (((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h) * HD;
-      if (a.slots == 1 && !row_live(a, i)) continue;
 #pragma unroll
       for (int c = lane; c < HD / 4; c += 32) reinterpret_cast<float4 *>(out)[c] = stage[r * (HD / 4) + (c ^ (r & 7))];
     }

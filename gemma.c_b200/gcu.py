@@ -750,7 +750,7 @@ def _check_write(what, xq, shape, qkv, kv, freqs, nq, nk, rows, n_heads):
         _rows(what, "nq", nq, f32, (hdim,), dev)
     if nk is not None:
         _rows(what, "nk", nk, f32, (hdim,), dev)
-    return dev, ld[0]
+    return dev, ld[0] if rows > 1 else (n_heads + 2 * kv.nkv) * hdim  # one row: its stride is never taken
 
 
 def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, nk=None, eps=1e-6, stream=None):
@@ -788,7 +788,8 @@ def dev_cache_i8_read(k, v, kv, spos, stream=None):
             (st[2] == kv.hdim or sh[2] < 2) and k.get_device() == dev and v.get_device() == dev):
         raise GcuError(f"{what}: k and v must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, alike, on the "
                        f"cache's device, not {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
-    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0], st[1], kv.ref, spos, sh[2],
+    _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0] if sh[0] > 1 else 0,
+                                       st[1] if sh[1] > 1 else 0, kv.ref, spos, sh[2],
                                        _on(stream, dev)), what)
 
 
@@ -827,7 +828,7 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
     l = lib()
     work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, sc_att, int(mask)),
                                kv.device, stream)
-    _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0), xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
+    _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0) if ntok > 1 else 0, xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
                                           sc_att, int(mask), work, nbytes, _on(stream, dev)), what)
 
 

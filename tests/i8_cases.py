@@ -106,7 +106,9 @@ def tolerance(score, n, vmax):
     query's 23-bit form, the digits' sum, the scales, log2 e, the shift by the
     maximum): 8 half steps of 2^-24, which the exponential turns into a relative
     error of the weight; it enters the sum and, against it, the weights' total.
-    The weights are multiplied as two bf16 parts: 2^-9 * 2^-9 each way, 2^-17 in
+    The weights are multiplied as integers of 24 bits or more, or as two fp16 parts,
+    2^-22 of each; a matrix product that adds by cutting off loses 2^-23 a time, over
+    32 additions between the sums that are rounded: 2^-18, and the parts, 2^-17 in
     all.  Sums of n terms in fp32: sqrt(n) half steps, and 64 for exp2, the
     products and the final division."""
     return (2.0 ** -24 * (16.0 * score + math.sqrt(n) + 64.0) + 2.0 ** -17) * vmax

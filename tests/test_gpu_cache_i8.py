@@ -143,3 +143,57 @@ def test_capture_and_other_stream():
     gcu.dev_cache_i8_read(out, torch.empty_like(out), kv, 0, stream=s)
     s.synchronize()
     assert torch.equal(out, kv.k.float() * kv.ks.unsqueeze(-1))
+
+
+def test_odd_strides_of_single_rows():
+    """A stride along a dimension of one is never taken, whatever it is."""
+    rng = np.random.default_rng(31)
+    x = rng.standard_normal((6 * 64,), dtype=np.float32)
+    kv = gcu.KvCacheI8.empty(1, 1, 5, 64)
+    qkv = torch.as_strided(dev(x), (1, 6 * 64), (7, 1))
+    xq, fr = torch.empty((4, 1, 64), device="cuda"), R.tables([3], 64)
+    gcu.dev_qkv_norm_rope_cache_i8(xq, qkv, kv, dev(fr), 3)
+    k, ks = R.quantize_rows(R.norm_rope(x.reshape(6, 64)[4:5], None, 1e-6, fr, 1.0))
+    assert np.array_equal(kv.k[0, :, 3].cpu().numpy(), k) and np.array_equal(kv.ks[0, :, 3].cpu().numpy(), ks)
+    out = torch.zeros((2, 1 * 64), device="cuda")
+    rk, rv = (torch.as_strided(o, (1, 1, 1, 64), (5, 3, 64, 1)) for o in out)
+    gcu.dev_cache_i8_read(rk, rv, kv, 3)
+    assert np.array_equal(out[0].cpu().numpy(), k[0] * ks[0])
+    xo = torch.as_strided(torch.zeros(4 * 64, device="cuda"), (1, 4 * 64), (1, 1))
+    gcu.dev_attention_prefill_i8(xo, xq, kv, 3, slide=1)
+    v, vs = R.quantize_rows(x.reshape(6, 64)[5])
+    assert np.allclose(xo.cpu().numpy().reshape(4, 64), v * vs, rtol=2.0 ** -20, atol=0)
+
+
+def test_offsets_past_32_bits():
+    """The last head of a cache whose heads begin 4.8 GB in: write, read back, and both kinds of
+    attention over a window at its end."""
+    nkv, clen, hd, nh, n = 3, 9_400_003, 256, 3, 40
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("24 GB of device memory needed")
+    rng = np.random.default_rng(32)
+    codes = torch.empty((2, 1, nkv, clen, hd), dtype=torch.int8, device="cuda")
+    scales = torch.empty((2, 1, nkv, clen), device="cuda")
+    kv = gcu.KvCacheI8(codes[0], codes[1], scales[0], scales[1])
+    spos = clen - n
+    x = rng.standard_normal((n, (nh + 2 * nkv) * hd), dtype=np.float32)
+    fr = R.tables(np.arange(n), hd)  # angles small enough to be exact
+    xq = torch.empty((nh, n, hd), device="cuda")
+    gcu.dev_qkv_norm_rope_cache_i8(xq, dev(x), kv, dev(fr), spos, hd ** -0.5)
+    rows = x.reshape(n, -1, hd)
+    k, ks = R.quantize_rows(R.norm_rope(rows[:, nh:nh + nkv], None, 1e-6, fr[:, None], 1.0))
+    v, vs = R.quantize_rows(rows[:, nh + nkv:])
+    small = tuple(np.moveaxis(t, 0, 1)[None] for t in (k, v, ks, vs))
+    assert np.array_equal(kv.k[0, :, spos:].cpu().numpy(), small[0][0])
+    rk, rv = (torch.empty((1, nkv, n, hd), device="cuda") for _ in range(2))
+    gcu.dev_cache_i8_read(rk, rv, kv, spos)
+    assert np.array_equal(rv.cpu().numpy(), small[1] * small[3][..., None])
+    q = xq.cpu().numpy()
+    xo = torch.empty((n, nh * hd), device="cuda")
+    gcu.dev_attention_prefill_i8(xo, xq, kv, spos, slide=8)
+    want, tol = R.prefill(q[:, 8:], small, 8, 8, 0.0, True)
+    assert np.max(np.abs(xo.cpu().numpy()[8:] - want)) <= tol
+    one = torch.empty((1, nh, hd), device="cuda")
+    gcu.dev_attention_decode_i8(one, xq[:, -1][None].contiguous(), kv, None, clen, 1.0, 0.0, n)
+    want, tol = R.decode(q[None, :, -1], small, [n], 1.0, 0.0, 0)
+    assert np.max(np.abs(one.cpu().numpy() - want)) <= tol
