@@ -211,11 +211,12 @@ __device__ __forceinline__ float2 high_digit(const uint32_t *s2, float2 low) {
 }
 
 // A value row's scale as it goes into the exponent and out of the sum of weights.
-// Taken as at least 2^-100 and at most 2^100: reciprocals and sums stay finite.
+// Taken as at least 2^-64 and at most 2^100: reciprocals stay finite, and so do the
+// sums of weights over them, up to 2^24 * 2^64 a key.
 // NaN makes the weights NaN where the key is seen; where it is not, 1 / vs is
 // finite against the zero weight.
 __device__ __forceinline__ void value_scale(float v, float &log2_vs, float &inv_vs) {
-  constexpr float lo = 7.888609e-31f, hi = 1.2676506e30f;
+  constexpr float lo = 5.421011e-20f, hi = 1.2676506e30f;
   v = v < lo ? lo : v > hi ? hi : v;
   log2_vs = log2f(v);
   inv_vs = v == v ? 1.0f / v : 1.0f;

@@ -215,6 +215,10 @@ int gemm_workspace(size_t bytes, void **ws, int **counters, int ncounters,
 // 8-bit KV cache (k_cache_i8.cu): checks a descriptor's sizes, strides and
 // alignment; sets the error and returns 1 when it cannot be used.
 int check_kv_i8(const char *what, const gcu_kv_i8 *kv, int nseq = 0);
+// whether [a, a + na) and [b, b + nb) share a byte
+inline bool overlap(const void *a, long na, const void *b, long nb) {
+  return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 
 // Shared with the chain kernel (k_chain.cu): TMA tensor maps of the GEMM's
 // operand layouts (int8 [rows][k], box 128 B x box_rows, 128-byte swizzle;

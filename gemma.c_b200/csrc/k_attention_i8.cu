@@ -189,7 +189,7 @@ using namespace gcu::attn8;
 
 GCU_EXPORT size_t gcu_attention_decode_i8_work(const gcu_kv_i8 *, int plen, const gcu_kv_i8 *own, int max_len,
                                                int n_heads, int slide) {
-  if (!own || own->nkv < 1 || n_heads < 1) return 0;
+  if (!own || own->nkv < 1 || own->nseq < 1 || n_heads < 1) return 0;
   return slot_bytes(plan_decode(*own, plen, max_len, n_heads, slide).slots(), (long)own->nseq * n_heads, own->hdim);
 }
 
@@ -212,6 +212,7 @@ GCU_EXPORT int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu
   const DecodePlan p = plan_decode(*own, plen, max_len, n_heads, slide);
   const long rows = (long)own->nseq * n_heads;
   if (check_work(what, slot_bytes(p.slots(), rows, own->hdim), work, work_bytes)) return 1;
+  if (overlap(xo, rows * own->hdim * 4, xq, rows * own->hdim * 4)) return set_error("%s: xo and xq overlap", what);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long qrow = (long)n_heads * own->hdim;
   Args a{xq, qrow, own->hdim, xo, qrow, *own, OWN, n_heads, own->nseq, 0, slide, 1, plen, max_len, len, asc, sc_att,
@@ -305,6 +306,8 @@ GCU_EXPORT int gcu_dev_attention_prefill_i8_tuned(float *xo, int xostr, const fl
   const PrefillPlan p = plan_prefill(*kv, n_heads, spos, ntok, slide, mask, sc_att != 0.0f, kernel);
   const long rows = (long)ntok * n_heads;
   if (check_work(what, slot_bytes(p.slots(), rows, kv->hdim), work, work_bytes)) return 1;
+  if (overlap(xo, ((long)(ntok - 1) * xostr + (long)n_heads * kv->hdim) * 4, xq, rows * kv->hdim * 4))
+    return set_error("%s: xo and xq overlap", what);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Args a{xq, kv->hdim, (long)ntok * kv->hdim, xo, xostr, *kv, PREFILL, n_heads, ntok, spos, slide, mask ? 1 : 0, 0, 0,
          nullptr, 1.0f, sc_att, p.p.chunk, p.p.splits, 0, p.slots(), nullptr, nullptr, dev_error_word()};

@@ -268,6 +268,9 @@ __global__ void __launch_bounds__(kThreads) k_read(float *k, float *v, long out_
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 int launch_write(const WriteArgs &a, cudaStream_t st) {
+  if (overlap(a.xq, (long)a.rows * a.n_heads * a.kv.hdim * 4, a.qkv,
+              ((a.rows - 1) * a.ld + (long)(a.n_heads + 2 * a.kv.nkv) * a.kv.hdim) * 4))
+    return set_error("qkv_norm_rope_cache_i8: xq and qkv overlap");
   constexpr int kWarps = kWriteThreads / 32;
   const int y = (groups(a.n_heads) + 2 * groups(a.kv.nkv) + kWarps - 1) / kWarps;
   if (y > 65535) return set_error("qkv_norm_rope_cache_i8: %d query and %d kv heads", a.n_heads, a.kv.nkv);
@@ -353,6 +356,7 @@ GCU_EXPORT int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, lo
   if ((kv->nkv > 1 && out_stride < (long)ntok * kv->hdim) ||
       (kv->nseq > 1 && out_seq_stride < (kv->nkv - 1) * out_stride + (long)ntok * kv->hdim))
     return set_error("%s: output strides overlap rows of %d positions x %d", what, ntok, kv->hdim);
+  if (k == v) return set_error("%s: k and v overlap", what);
   const int per = kReadRows * kThreads * 4 / kv->hdim;  // positions of a CTA
   const int blocks = (int)(((long)ntok + per - 1) / per);
   const long ctas = (long)kv->nseq * kv->nkv * blocks;

@@ -376,7 +376,7 @@ typedef struct {
  * QK-norm weights [hdim] or NULL; freqs [ntok][hdim] (cos, sin interleaved).
  * The norm's sum of squares is taken in 64 bits and every fp32 step after it
  * is rounded by itself (no fused multiply-adds), so the codes follow from the
- * formulas alone.  16-byte aligned qkv, xq and freqs. */
+ * formulas alone.  16-byte aligned qkv, xq and freqs; xq and qkv apart. */
 int gcu_dev_qkv_norm_rope_cache_i8(float *xq, const float *qkv, long ld, const gcu_kv_i8 *kv,
                                    const float *nq, const float *nk, float eps, const float *freqs,
                                    float q_scale, int n_heads, int spos, int ntok, void *stream);
@@ -406,7 +406,9 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * sc_att (0 = off).  A sequence that sees nothing gets zeros; one with len[b]
  * < 0 is skipped, its xo row left as it is; one with len[b] > max_len is
  * skipped too and reported by gcu_check_device.  At most 8 query heads per
- * kv head.  work: device scratch of at least
+ * kv head.  A value scale counts as at least 2^-64 and at most 2^100; keys
+ * whose value scales are more than 2^100 below another's that the row sees may
+ * weigh nothing.  xo and xq do not overlap.  work: device scratch of at least
  * gcu_attention_decode_i8_work(...) bytes, 16-byte aligned, not shared with
  * work that may run at the same time (0 bytes: may be NULL). */
 size_t gcu_attention_decode_i8_work(const gcu_kv_i8 *prefix, int plen, const gcu_kv_i8 *own, int max_len,

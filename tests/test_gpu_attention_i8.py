@@ -344,3 +344,16 @@ def test_decode_few_chunks(nh, nkv, hd, max_len):
         got = run_decode(xq, handle(c), lens, max_len, cap, slide).cpu().numpy()
         assert np.all(got[~live] == 9.0) and np.all(got[np.asarray(lens) == 0] == 0.0)
         check(got[live], want[live], tol)
+
+
+@pytest.mark.parametrize("vs", [1e-18, 1e-12, 1e12, 1e28])
+def test_all_value_scales_small_or_large(vs):
+    rng = np.random.default_rng(21)
+    own = R.cache(rng, 1, 2, 3000, 128)
+    own[3][:] = vs * rng.uniform(0.5, 2, own[3].shape).astype(np.float32)
+    xq = rng.standard_normal((1, 4, 128), dtype=np.float32)
+    want, tol = R.decode(xq, own, [3000], 128 ** -0.5, 0.0, 0)
+    check(run_decode(xq, handle(own), None, 3000), want, tol)
+    xp = rng.standard_normal((4, 50, 128), dtype=np.float32) * np.float32(0.1)
+    want, tol = R.prefill(xp, own, 2950, 0, 0.0, True)
+    check(run_prefill(xp, handle(own), 2950), want, tol)

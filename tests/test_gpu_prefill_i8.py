@@ -95,6 +95,17 @@ def test_odd_scales(kernel):
     check(forced(kernel, xq, handle(c), 310), want, tol)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("vs", [1e-18, 1e28])
+def test_value_scales(kernel, vs):
+    rng = np.random.default_rng(22)
+    c = R.cache(rng, 1, 2, 900, 128)
+    c[3][:] = vs * rng.uniform(0.5, 2, c[3].shape).astype(np.float32)
+    xq = rng.standard_normal((4, 140, 128), dtype=np.float32) * np.float32(0.1)
+    want, tol = R.prefill(xq, c, 760, 0, 0.0, True)
+    check(forced(kernel, xq, handle(c), 760), want, tol)
+
+
 @pytest.mark.parametrize("nh,nkv,hd,spos,ntok,slide,cap", [
     (16, 8, 128, 0, 1025, 0, 0.0), (16, 8, 256, 100, 1900, 0, 0.0), (8, 4, 64, 0, 2051, 0, 30.0),
     (8, 4, 256, 0, 2048, 512, 0.0), (6, 4, 128, 7, 2500, 300, 0.0), (8, 1, 256, 2000, 700, 0, 0.0)])

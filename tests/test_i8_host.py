@@ -183,3 +183,34 @@ def test_plain_forms():
     assert R.sample([0, 0, 0, 0], 0.49, 1.0, 2, 1.0, 0.0) == (0, 0.5)
     assert R.sample([0, 0, 0, 0], 0.5, 1.0, 2, 1.0, 0.0) == (1, 0.5)
     assert R.sample([np.nan, -np.inf], 0.3, 1.0, 0, 1.0, 0.0) == (-1, 0.0)
+
+
+def test_scratch_of_unusable_caches_is_zero():
+    """The scratch queries answer 0 for what the calls refuse; they never divide by a count of zero."""
+    lib, ref = gcu.lib(), ctypes.byref
+    for over in (dict(nseq=0), dict(nkv=0), dict(nseq=-3), dict(nkv=-1)):
+        bad = kv_struct()
+        for k, v in over.items():
+            setattr(bad, k, v)
+        assert lib.gcu_attention_decode_i8_work(None, 0, ref(bad), 16, 4, 0) == 0
+        assert lib.gcu_attention_decode_i8_work(ref(bad), 8, ref(bad), 16, 4, 0) == 0
+        if "nkv" in over:
+            assert lib.gcu_attention_prefill_i8_work(ref(bad), 4, 0, 4, 0, 0.0, 1) == 0
+    kv = kv_struct()
+    assert lib.gcu_attention_decode_i8_work(None, 0, None, 16, 4, 0) == 0
+    assert lib.gcu_attention_decode_i8_work(None, 0, ref(kv), 16, 0, 0) == 0
+    assert lib.gcu_attention_decode_i8_work(None, -5, ref(kv), -7, 4, -1) == 0
+    assert lib.gcu_attention_prefill_i8_work(ref(kv), 0, 0, 4, 0, 0.0, 1) == 0
+    assert lib.gcu_attention_prefill_i8_work(ref(kv), 4, -1, 4, 0, 0.0, 1) == 0
+    assert lib.gcu_attention_prefill_i8_work(ref(kv), 4, 0, 0, 0, 0.0, 1) == 0
+
+
+def test_outputs_over_their_inputs_are_refused():
+    """Rows are read by several CTAs while others are written."""
+    kv = kv_struct()
+    lib, ref = gcu.lib(), ctypes.byref
+    refused(write(kv, xq=P + 64), "overlap")
+    for xo, xq in ((P, P), (P, P + 4 * 64 * 4 - 16), (P + 16, P)):
+        refused(lib.gcu_dev_attention_decode_i8(xo, xq, None, 0, ref(kv), None, 4, 4, 0, 1.0, 0.0, None, 0, None), "overlap")
+    refused(lib.gcu_dev_attention_prefill_i8(P, 0, P + 64, ref(kv), 4, 0, 3, 0, 0.0, 1, None, 0, None), "overlap")
+    refused(lib.gcu_dev_cache_i8_read(P, P, 0, 1024, ref(kv), 0, 1, None), "overlap")
