@@ -118,8 +118,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&sfull[s], 1);
-      ptx::mbar_init(&sfree[s], kSoftmax);
-      ptx::mbar_init(&pfull[s], kSoftmax);
+      ptx::mbar_init(&sfree[s], kSoftmax / 32);
+      ptx::mbar_init(&pfull[s], kSoftmax / 32);
       ptx::mbar_init(&pvdone[s], 1);
     }
     ptx::mbar_init(&drain, 1);
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         }
       }
       ptx::tc_fence_before();
-      ptx::mbar_arrive(&sfree[j & 1]);
+      ptx::mbar_arrive_warp(&sfree[j & 1]);
       const int t0 = kbeg + j * kKeys;
       if (t0 < all_lo || t0 + kKeys > min(all_hi, kend)) {  // a tile that some row does not see in full
         const int t = t0 + key;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         *reinterpret_cast<uint4 *>(dst + (((r0 + r) >> 2 ^ sw) << 4)) = make_uint4(w[r], w[r + 1], w[r + 2], w[r + 3]);
       if (threadIdx.x == 0) *(volatile int *)&s_fresh[j & 1] = fresh;
       ptx::fence_proxy_async_smem();
-      ptx::mbar_arrive(&pfull[j & 1]);
+      ptx::mbar_arrive_warp(&pfull[j & 1]);
       ks = ks_next;
       vs = vs_next;
     }

@@ -146,17 +146,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       ptx::mbar_init(&bars.kfull[s], 1);
       ptx::mbar_init(&bars.kempty[s], 1);
       ptx::mbar_init(&bars.v8full[s], 1);
-      ptx::mbar_init(&bars.v8empty[s], kGroup);
-      ptx::mbar_init(&bars.v16full[s], kGroup);
+      ptx::mbar_init(&bars.v8empty[s], kGroup / 32);
+      ptx::mbar_init(&bars.v16full[s], kGroup / 32);
     }
     for (int s = 0; s < 2; ++s) {
-      ptx::mbar_init(&bars.dec[s], kGroup);
+      ptx::mbar_init(&bars.dec[s], kGroup / 32);
       ptx::mbar_init(&bars.sfull[s], 1);
       ptx::mbar_init(&bars.pvdone[s], 1);
     }
-    ptx::mbar_init(&bars.sfree, kGroup);
-    ptx::mbar_init(&bars.pfull, kGroup);
-    ptx::mbar_init(&bars.tfree, 2 * kGroup);
+    ptx::mbar_init(&bars.sfree, kGroup / 32);
+    ptx::mbar_init(&bars.pfull, kGroup / 32);
+    ptx::mbar_init(&bars.tfree, 2 * kGroup / 32);
     ptx::mbar_init(&bars.drain, 1);
     ptx::fence_mbar_init();
     s_abort = 0;
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       if (j > 0 && freshp[j & 1]) {
         ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
         flush(f);
-        ptx::mbar_arrive(&bars.tfree);
+        ptx::mbar_arrive_warp(&bars.tfree);
       }
     };
     // V codes of tile j to fp16; 8 columns of a key per thread.  Keys past the range
@@ -444,8 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
           *reinterpret_cast<uint4 *>(dst + key * 128 + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
         }
         ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(&bars.v8empty[j % C::NV8]);
-        ptx::mbar_arrive(&bars.v16full[j & 1]);
+        ptx::mbar_arrive_warp(&bars.v8empty[j % C::NV8]);
+        ptx::mbar_arrive_warp(&bars.v16full[j & 1]);
       }
     };
     int j = grp;
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         }
       }
       ptx::tc_fence_before();
-      ptx::mbar_arrive(&bars.sfree);
+      ptx::mbar_arrive_warp(&bars.sfree);
       // a tile that some row does not see in full
       const int t0 = kbeg + j * NK;
       if (t0 < all_lo || t0 + NK > min(all_hi, kend)) {
@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       const bool fresh = moved || j % kFlush == 0;
       if (half == 0) refs[row] = to;
       if (tid == 0) freshp[j & 1] = fresh;
-      ptx::mbar_arrive(&bars.dec[j & 1]);
+      ptx::mbar_arrive_warp(&bars.dec[j & 1]);
       const float f = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
       l *= f;
       m = to;
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         ok = wait(&bars.pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
         if (fresh) {
           flush(f);
-          ptx::mbar_arrive(&bars.tfree);
+          ptx::mbar_arrive_warp(&bars.tfree);
         }
       }
       ptx::tc_fence_after();
@@ -560,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       ptx::tmem_st_32x16(lanes + C::P_COL + NK / 2 + half * (C::HALF / 2), pl);
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
-      ptx::mbar_arrive(&bars.pfull);
+      ptx::mbar_arrive_warp(&bars.pfull);
     }
     // the group without the last tile follows its decision too (j is the tile
     // after it); then both take what is left in T
