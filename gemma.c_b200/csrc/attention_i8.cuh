@@ -215,9 +215,9 @@ __device__ __forceinline__ float2 high_digit(const uint32_t *s2, float2 low) {
 // sums of weights over them, up to 2^24 * 2^64 a key.
 // NaN makes the weights NaN where the key is seen; where it is not, 1 / vs is
 // finite against the zero weight.
+constexpr float kScaleLo = 5.421011e-20f, kScaleHi = 1.2676506e30f;
 __device__ __forceinline__ void value_scale(float v, float &log2_vs, float &inv_vs) {
-  constexpr float lo = 5.421011e-20f, hi = 1.2676506e30f;
-  v = v < lo ? lo : v > hi ? hi : v;
+  v = v < kScaleLo ? kScaleLo : v > kScaleHi ? kScaleHi : v;
   log2_vs = log2f(v);
   inv_vs = v == v ? 1.0f / v : 1.0f;
 }

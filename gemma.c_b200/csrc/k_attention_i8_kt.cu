@@ -10,9 +10,9 @@
 //                             unsigned digits each, the bytes of an integer as they
 //                             lie (kind::i8 with both operands MN-major: V's tile
 //                             as it lies is V^T)
-// Weights are 32-bit fixed point, W = round(2^(s + log2 vs - m)), m placed so that
-// the row's largest weight so far is 2^24 at least and 2^31.5 at most; rounding
-// is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 66,312
+// Weights are 32-bit fixed point, W = round(2^(s + e - m) * f) for a value scale of
+// 2^e * f, 1 <= f < 2, m placed so that the row's largest weight so far is 2^24 at
+// least and below 2^32; rounding is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 66,312
 // keys fits, and the plan gives a CTA fewer), so nothing is lost, and only moves
 // to fp32 registers when a row's m has to move.
 //
@@ -35,7 +35,20 @@ namespace {
 
 constexpr int kSoftmax = 512, kMmaWarp = 16, kLoadWarp = 17, kThreads = 576;
 constexpr int kKeys = kKtKeys;
-constexpr float kTop = 24.0f, kSlack = 7.5f;  // log2 of the weight at m, and how far it may pass
+constexpr float kTop = 24.0f, kSlack = 6.9f;  // log2 of the weight at m (over f), and how far it may pass
+
+// A value row's scale 2^e * f, as attn8::value_scale limits it: e (NaN for NaN, which then
+// makes the weights NaN where the key is seen; elsewhere the others are finite
+// against the zero weight), f and 2^-e.  Exact, and a quarter of the instructions
+// that a logarithm and a reciprocal take (32 sequences that share 32768 keys 63.0
+// -> 60.9 us).
+__device__ __forceinline__ void split_scale(float v, float &e, float &f, float &inv) {
+  v = v < kScaleLo ? kScaleLo : v > kScaleHi ? kScaleHi : v;
+  const int b = __float_as_int(v), x = min(b & 0x7f800000, 0x71800000);  // NaN as 2^100
+  e = v == v ? (float)((x >> 23) - 127) : v;
+  f = __int_as_float((b & 0x007fffff) | 0x3f800000);
+  inv = __int_as_float(0x7f000000 - x);
+}
 
 template <int HD, int R>
 struct Cfg {
@@ -341,11 +354,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       const float ks_next = fetch(ksrc, j + 1), vs_next = fetch(vsrc, j + 1);
-      float lvs, rvs;
-      value_scale(vs, lvs, rvs);
+      float evs, fvs, rvs;
+      split_scale(vs, evs, fvs, rvs);
       ok = wait(&sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       ptx::tc_fence_after();
-      // exponents: the score in log2 units plus log2 of the value row's scale
+      // exponents: the score in log2 units plus the value scale's
       float x[RQ];
       {
         uint32_t s2[RQ], s1[RQ], s0[RQ];
@@ -360,9 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
           float2 e;
           if constexpr (CAP) {
             e = __fmul2_rn(y, make_float2(rf[r], rf[r + 1]));
-            e = __ffma2_rn(make_float2(tanh_fast(e.x), tanh_fast(e.y)), make_float2(unit, unit), make_float2(lvs, lvs));
+            e = __ffma2_rn(make_float2(tanh_fast(e.x), tanh_fast(e.y)), make_float2(unit, unit), make_float2(evs, evs));
           } else {
-            e = __ffma2_rn(y, make_float2(rf[r], rf[r + 1]), make_float2(lvs, lvs));
+            e = __ffma2_rn(y, make_float2(rf[r], rf[r + 1]), make_float2(evs, evs));
           }
           x[r] = e.x;
           x[r + 1] = e.y;
@@ -436,8 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         const float2 t = __ffma2_rn(v, make_float2(rvs, rvs), make_float2(l[r], l[r + 1]));
         l[r] = t.x;
         l[r + 1] = t.y;
-        w[r] = __float2uint_rn(v.x);
-        w[r + 1] = __float2uint_rn(v.y);
+        const float2 u = __fmul2_rn(v, make_float2(fvs, fvs));
+        w[r] = __float2uint_rn(u.x);
+        w[r + 1] = __float2uint_rn(u.y);
       }
       uint8_t *dst = smem + C::P_OFF + (j & 1) * C::P_BYTES + key * C::P_ROW;
       const int sw = C::P_ROW == 128 ? key & 7 : (key >> 1) & 3;

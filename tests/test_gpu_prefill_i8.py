@@ -96,6 +96,26 @@ def test_odd_scales(kernel):
 
 
 @pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("which,bad", [(2, np.nan), (3, np.nan), (2, np.inf)])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_what_a_row_does_not_see_may_hold_anything(kernel, which, bad, hd):
+    """A scale that is no number: the rows before it in the same tile, and those whose window has
+    left it behind, are as without it."""
+    rng = np.random.default_rng(23)
+    c = R.cache(rng, 1, 1, 300, hd)
+    xq = rng.standard_normal((2, 200, hd), dtype=np.float32) * np.float32(1 / np.sqrt(hd))
+    want, tol = R.prefill(xq, c, 100, 50, 0.0, True)
+    for at in (170, 255, 299):
+        broken = [t.copy() for t in c]
+        broken[which][0, 0, at] = bad
+        got = forced(kernel, xq, handle(broken), 100, 50)
+        sees = np.array([at <= 100 + i < at + 50 for i in range(200)])
+        check(got[~sees], want[~sees], tol)
+        if np.isnan(bad):
+            assert np.all(np.isnan(got[sees]))
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("vs", [1e-18, 1e28])
 def test_value_scales(kernel, vs):
     rng = np.random.default_rng(22)
