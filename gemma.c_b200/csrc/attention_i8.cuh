@@ -32,6 +32,8 @@ enum Mode {
   PREFIX    // row i is sequence i, the cache that all sequences share
 };
 
+constexpr float kAlone = -1.0f;  // where a sum of weights would stand
+
 struct Args {
   const float *xq;  // row (i, h) at xq + i*q_i + h*q_h
   long q_i, q_h;
@@ -47,6 +49,7 @@ struct Args {
   // Key ranges are cut into `splits` chunks; a launch writes slots [slot0,
   // slot0 + splits) of `slots` per row: unnormalised sums part[slot][row][hdim]
   // and (m, l) stat[slot][row] with row = i*n_heads + h, weights 2^(log2e*s - m).
+  // slot 0 may hold (0, kAlone): the row is in xo already.
   // slots == 1: the rows go straight to xo, from the chunks' CTAs together (a
   // cluster) when there are several.
   int chunk, splits, slot0, slots;

@@ -4,6 +4,8 @@
 #include "attention_i8.cuh"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #define GCU_EXPORT extern "C" __attribute__((visibility("default")))
 
@@ -11,19 +13,22 @@ namespace gcu {
 namespace attn8 {
 namespace {
 
+constexpr int kMergeThreads = 128;  // of k_merge_many
+constexpr long kManyRows = 512;
+
 // xo = sum_s e_s O_s / sum_s e_s l_s, e_s = 2^(m_s - max m), in slot order.
-// One CTA per row; the slots' factors are formed by all threads at once and
+// For few rows, one CTA each: the slots' factors are formed by all threads at once and
 // staged, and each thread keeps eight slots' loads in flight.  Bound by latency: 7.3 us
 // cold for the 18 slots of 32768 keys and 16 heads, most of it hidden behind the end of
 // the kernel before it.
 template <int HD>
-__global__ void __launch_bounds__(HD) k_merge(const Args a) {
+__global__ void __launch_bounds__(HD) k_merge_few(const Args a) {
   __shared__ float s_e[HD], s_l[HD], s_red[HD / 32];
   ptx::griddep_launch();
   const int i = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads, d = threadIdx.x;
   const size_t row = blockIdx.x, rows = (size_t)a.ni * a.n_heads;
   ptx::griddep_wait();
-  if (!row_live(a, i)) return;
+  if (!row_live(a, i) || a.stat[row].y == kAlone) return;
   float m = -INFINITY;
   for (int s = d; s < a.slots; s += HD) m = fmaxf(m, a.stat[s * rows + row].x);
 #pragma unroll
@@ -67,6 +72,64 @@ __global__ void __launch_bounds__(HD) k_merge(const Args a) {
   a.xo[(long)i * a.o_i + (long)h * HD + d] = o / (l == 0.0f ? 1.0f : l);
 }
 
+// The same for many rows, a warp each: lane s holds slot s's (m, l), and a lane HD/32
+// columns of kFly slots in flight.  From kManyRows rows, where a CTA for each would
+// come in waves: a prompt of 16368 rows in two slots 84.2 -> 72.7 us in all; 64 rows of
+// 13 slots 10.0 -> 10.6, 8 rows of 148 slots 16.9 -> 25.3.
+template <int HD>
+__global__ void __launch_bounds__(kMergeThreads) k_merge_many(const Args a) {
+  ptx::griddep_launch();
+  constexpr int V = HD == 64 ? 2 : 4, Q = HD / 32 / V, kFly = HD == 256 ? 6 : 8;
+  using F = typename std::conditional<V == 4, float4, float2>::type;
+  const int lane = threadIdx.x & 31;
+  const long row = (long)blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5), rows = (long)a.ni * a.n_heads;
+  ptx::griddep_wait();
+  if (row >= rows) return;
+  const int i = (int)((uint32_t)row / (uint32_t)a.n_heads), h = (int)(row - (long)i * a.n_heads);
+  if (!row_live(a, i)) return;
+  auto stat = [&](int s) { return s < a.slots ? a.stat[s * rows + row] : make_float2(-INFINITY, 0.0f); };
+  float2 st = stat(lane);
+  if (__shfl_sync(0xffffffffu, st.y, 0) == kAlone) return;
+  float m = st.x;
+  for (int s = lane + 32; s < a.slots; s += 32) m = fmaxf(m, a.stat[s * rows + row].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float o[Q * V] = {}, l = 0.0f;
+  for (int s0 = 0; s0 < a.slots; s0 += 32) {
+    if (s0 > 0) st = stat(s0 + lane);
+    // a slot whose keys the row does not see: its sums count for nothing
+    const float e = st.x == -INFINITY && st.y == 0.0f ? 0.0f : ex2(st.x - m), le = e * st.y;
+    const int ns = min(32, a.slots - s0);
+    for (int t0 = 0; t0 < ns; t0 += kFly) {
+      F v[kFly][Q];
+#pragma unroll
+      for (int t = 0; t < kFly; ++t)
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+          if (t0 + t < ns)
+            v[t][q] = *reinterpret_cast<const F *>(a.part + ((size_t)(s0 + t0 + t) * rows + row) * HD + (q * 32 + lane) * V);
+#pragma unroll
+      for (int t = 0; t < kFly; ++t) {
+        if (t0 + t >= ns) break;
+        const float f = __shfl_sync(0xffffffffu, e, t0 + t);
+        l += __shfl_sync(0xffffffffu, le, t0 + t);
+        if (f == 0.0f) continue;  // such a slot may not even be written
+#pragma unroll
+        for (int c = 0; c < Q * V; ++c) o[c] += f * reinterpret_cast<const float *>(&v[t][c / V])[c % V];
+      }
+    }
+  }
+  if (l == 0.0f) l = 1.0f;
+  float *xo = a.xo + (long)i * a.o_i + (long)h * HD;
+#pragma unroll
+  for (int q = 0; q < Q; ++q) {
+    F r;
+#pragma unroll
+    for (int c = 0; c < V; ++c) reinterpret_cast<float *>(&r)[c] = o[q * V + c] / l;
+    *reinterpret_cast<F *>(xo + (q * 32 + lane) * V) = r;
+  }
+}
+
 int max_group(int n_heads, int nkv) { return (n_heads + nkv - 1) / nkv; }
 
 }  // namespace
@@ -74,10 +137,18 @@ int max_group(int n_heads, int nkv) { return (n_heads + nkv - 1) / nkv; }
 int launch_merge(const Args &a, cudaStream_t st) {
   const long rows = (long)a.ni * a.n_heads;
   if (rows > 0x7fffffffL) return set_error("attention_i8: %ld rows", rows);
-  const dim3 grid((unsigned)rows);
-  GCU_CUDA(a.kv.hdim == 256   ? launch_k(k_merge<256>, grid, dim3(256), 0, st, a)
-           : a.kv.hdim == 128 ? launch_k(k_merge<128>, grid, dim3(128), 0, st, a)
-                              : launch_k(k_merge<64>, grid, dim3(64), 0, st, a));
+  if (rows < kManyRows) {
+    const dim3 grid((unsigned)rows);
+    GCU_CUDA(a.kv.hdim == 256   ? launch_k(k_merge_few<256>, grid, dim3(256), 0, st, a)
+             : a.kv.hdim == 128 ? launch_k(k_merge_few<128>, grid, dim3(128), 0, st, a)
+                                : launch_k(k_merge_few<64>, grid, dim3(64), 0, st, a));
+    return 0;
+  }
+  constexpr int per = kMergeThreads / 32;
+  const dim3 grid((unsigned)((rows + per - 1) / per)), block(kMergeThreads);
+  GCU_CUDA(a.kv.hdim == 256   ? launch_k(k_merge_many<256>, grid, block, 0, st, a)
+           : a.kv.hdim == 128 ? launch_k(k_merge_many<128>, grid, block, 0, st, a)
+                              : launch_k(k_merge_many<64>, grid, block, 0, st, a));
   return 0;
 }
 
@@ -240,7 +311,8 @@ namespace {
 // against 21.5, 2048 of 16 + 8 heads 136 against 93.  The times come from a model
 // fitted to both at 64 to 4096 tokens, heads 4 + 1, 8 + 4 and 16 + 8 of 64, 128 and 256:
 // `fixed` us a CTA and `tile` us a tile of keys, the longest CTA or the average load
-// of an SM, and a merge.
+// of an SM, and a merge.  1023 tokens at 777 (16 + 8 heads of 128, capped) in chunks of 20
+// tiles take 72.7 us, whole ones (of up to 29) 81.
 struct PrefillPlan {
   bool kt, cluster;
   int rows;
@@ -272,7 +344,24 @@ PrefillPlan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, i
     const double mean = (seen(spos + 1) + 2 * seen(spos + ntok / 2 + 1) + n) / 4.0 / keys + 0.5;
     time = std::max(fixed + tile * (p.p.chunk / keys),
                     (kt ? (double)waves : (double)ctas / sms) * fixed + units * mean * tile / sms);
-    if (p.p.splits > 1 && !p.cluster) time += 5.0;
+    const double merge = 4.0 + ntok * (double)n_heads / 3000;
+    if (p.p.splits > 1 && !p.cluster) time += merge;
+    // Fewer CTAs than SMs and row tiles of different lengths: a second chunk for the
+    // longest ones, where the idle SMs' time and that of the short ones' takes it.
+    const double t1 = (double)n / keys, t0 = (double)seen(spos + 1) / keys;
+    if (!kt && units < sms && t1 - t0 > 2.0)
+      for (int k = 8; k < 16; ++k) {
+        const int c = (int)std::ceil(t1 * k / 16);
+        if (c <= t0 || c >= t1) continue;
+        const double first = fixed + tile * c, over = (t1 - c) / (t1 - t0) * units;
+        const double need = over * (fixed + tile * (t1 - c) / 2);
+        const double spare = 0.85 * ((sms - units) * first + (units - over) * (c - t0) / 2 * tile);
+        const double all = first + merge + (need > spare ? (need - spare) / sms + fixed + tile : 0.0);
+        if (all >= time) continue;
+        time = all;
+        p.p.chunk = c * keys;
+        p.p.splits = (int)((n + p.p.chunk - 1) / p.p.chunk);
+      }
     return p;
   };
   double few, many;

@@ -192,6 +192,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
   const long c0 = (long)s_range[0] + (long)split * a.chunk;
   const int n = (int)max(0l, min((long)s_range[1], c0 + a.chunk) - c0);
   const int kbeg = (int)min(c0, 0x7fffffffl), kend = kbeg + n, nt = (n + NK - 1) / NK;
+  // rows whose keys fit into one chunk go straight to xo, and slot 0 tells the merge
+  const bool alone = a.slots == 1 || (long)s_range[1] - s_range[0] <= a.chunk;
   Waiter wait{&s_abort, a.err};
 
   const int8_t *vh = a.kv.v + hk * a.kv.kv_stride, *kh = a.kv.k + hk * a.kv.kv_stride;
@@ -576,21 +578,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     l = (smax[row] + smax[kRows + row]) + (smax[2 * kRows + row] + smax[3 * kRows + row]);
     // Rows go out through shared memory (the queries' and keys' is free now: every
     // product that reads them is done), a warp per row, 512 bytes at a time.
-    const float d = a.slots > 1 || l == 0.0f ? 1.0f : 1.0f / l;  // a row that sees nothing: zeros
+    const float d = !alone || l == 0.0f ? 1.0f : 1.0f / l;  // a row that sees nothing: zeros
     float4 *stage = reinterpret_cast<float4 *>(smem);
 #pragma unroll
     for (int c = 0; c < C::OC; c += 4)
       stage[row * (HD / 4) + ((quarter * C::OC + c) / 4 ^ (row & 7))] =
           make_float4(acc[c] * d, acc[c + 1] * d, acc[c + 2] * d, acc[c + 3] * d);
-    if (live && ok && a.slots > 1 && quarter == 0)
+    if (live && ok && a.slots > 1 && quarter == 0 && (!alone || split == 0))
       a.stat[((size_t)(a.slot0 + split) * a.ni + rows.i(row)) * a.n_heads + h0 + rows.g(row)] =
-          make_float2(m == -INFINITY ? m : m - kTop, l);
+          alone ? make_float2(0.0f, kAlone) : make_float2(m == -INFINITY ? m : m - kTop, l);
     ptx::named_bar_sync(3, kSoftmax);
-    const bool none = nt == 0 && a.slots > 1;  // (-inf, 0) says that there is nothing to add
+    const bool none = alone ? split > 0 : nt == 0;  // (-inf, 0) says that there is nothing to add
     for (int r = warp; r < nrows && ok && !none; r += kSoftmax / 32) {
       const int i = rows.i(r), h = h0 + rows.g(r);
-      float *out = a.slots == 1 ? a.xo + (long)i * a.o_i + (long)h * HD
-                                : a.part + (((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h) * HD;
+      float *out = alone ? a.xo + (long)i * a.o_i + (long)h * HD
+                         : a.part + (((size_t)(a.slot0 + split) * a.ni + i) * a.n_heads + h) * HD;
 #pragma unroll
       for (int c = lane; c < HD / 4; c += 32) reinterpret_cast<float4 *>(out)[c] = stage[r * (HD / 4) + (c ^ (r & 7))];
     }

@@ -156,6 +156,31 @@ def test_large_chunks(nh, nkv, hd, spos, ntok, slide, cap):
 R_SCORE = 12.0  # above any score of these inputs: |q . k| of 1.5 standard deviations by 4000 keys
 
 
+@pytest.mark.parametrize("nh,nkv,hd,spos,ntok,cap", [
+    (16, 8, 128, 777, 1023, 50.0), (8, 4, 128, 0, 2000, 0.0), (16, 8, 256, 3, 1001, 0.0), (5, 2, 64, 0, 4001, 0.0),
+    (4, 1, 64, 50, 4096, 0.0)])
+def test_chunks_of_different_lengths(nh, nkv, hd, spos, ntok, cap):
+    """Sizes whose long rows are split in two and whose short ones are not: every row of a head
+    against the few-row kernel, some against the plain form."""
+    rng = np.random.default_rng(ntok)
+    c = R.cache(rng, 1, nkv, spos + ntok, hd)
+    xq = rng.standard_normal((nh, ntok, hd), dtype=np.float32) * np.float32(1.5 / np.sqrt(hd))
+    kv = handle(c)
+    few, many = (forced(k, xq, kv, spos, 0, cap, extra=8).reshape(ntok, nh, hd) for k in KERNELS)
+    xo = torch.full((ntok, nh * hd), 9.0, device="cuda")
+    gcu.dev_attention_prefill_i8(xo, dev(xq), kv, spos, 0, cap)
+    got = xo.cpu().numpy().reshape(ntok, nh, hd)
+    vmax = np.max(np.abs(c[1]) * c[3][..., None])
+    tol = R.tolerance(R_SCORE, spos + ntok, vmax)
+    assert np.max(np.abs(few - many)) <= 2 * tol and np.max(np.abs(few - got)) <= 2 * tol
+    for i in rng.integers(0, ntok, 40):
+        h = int(rng.integers(0, nh))
+        k, v = R.rows_of(c, 0, h * nkv // nh, 0, spos + i + 1)
+        want, big = R.attend(xq[h, i], k, v, 1.0, cap)
+        for o in (few, many, got):
+            check(o[i, h], want, R.tolerance(big, spos + i + 1, vmax))
+
+
 def test_the_public_call_is_capturable():
     rng = np.random.default_rng(5)
     c = R.cache(rng, 1, 2, 700, 128)
