@@ -19,8 +19,8 @@
 // Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
 // against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM:
 // 16 rows are bound by HBM (32768 keys of 8 heads: 28.9 us for 136 MB, 4.7 TB/s), 32
-// rows by the softmax, about 2000 cycles a tile (32 sequences that share
-// 32768 keys: 63 us).  A CTA costs 5 us besides its tiles.
+// rows by the softmax, about 1900 cycles a tile (32 sequences that share
+// 32768 keys: 60 us).  A CTA costs 5 us besides its tiles.
 //
 // Warps 0-15: softmax, thread = (key, a quarter of the rows); 16: products; 17: loads.
 #include "attention_i8.cuh"
