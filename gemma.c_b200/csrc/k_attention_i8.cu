@@ -349,7 +349,7 @@ PrefillPlan plan_prefill(const gcu_kv_i8 &kv, int n_heads, int spos, int ntok, i
     // Fewer CTAs than SMs and row tiles of different lengths: a second chunk for the
     // longest ones, where the idle SMs' time and that of the short ones' takes it.
     const double t1 = (double)n / keys, t0 = (double)seen(spos + 1) / keys;
-    if (!kt && units < sms && t1 - t0 > 2.0)
+    if (!kt && !window && units < sms && t1 - t0 > 2.0)
       for (int k = 8; k < 16; ++k) {
         const int c = (int)std::ceil(t1 * k / 16);
         if (c <= t0 || c >= t1) continue;
