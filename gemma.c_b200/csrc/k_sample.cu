@@ -22,8 +22,9 @@
 // lists meet in distributed shared memory, and the whole search is one launch
 // with one read of HBM.  Bound by the 64-bit weights, 12 instructions of the FP64
 // units each, and by the latency of the passes and their cluster barriers.
-// 262144 logits, top-p 0.9 and min-p: 30 us for a row (16 CTAs), 40 for 15 rows (8), 74 for
-// 32 (4; clusters of 8, of which 15 run at once, took 116), 124 for 64 (2; with 8, 194).
+// 262144 logits, top-p 0.9 and min-p: 26 us for a row (16 CTAs), 36 for 8 rows (8), 70 for
+// 32 (4; clusters of 8, of which 15 run at once, took 116); top-k 64 and top-p 15 us for a
+// row, 19 with every list sorted by exchanges.
 #include "gcu_internal.cuh"
 
 #include <cooperative_groups.h>
@@ -44,6 +45,7 @@ constexpr int kMaxCluster = 16;
 constexpr int kBins = 2048;
 constexpr float kBinsPerNat = 128.0f;
 constexpr int kCap = 1024;                // elements that are sorted
+constexpr int kFew = 256;                 // and up to how many by counting
 constexpr int kKeep = 1024;               // logits per warp held in shared memory
 constexpr int kTable = 32;                // entries of the 2^(j/32) table, one per lane
 
@@ -77,6 +79,7 @@ struct Shared {
   u64 list[kCap];                     // rank 0: all that is gathered, sorted ascending
   u64 weight[kCap];
   unsigned int order[kCap];
+  unsigned int place[kFew];
   u64 warp_sum[kWarps], totals[kMaxCluster];
   float maxes[kMaxCluster];
   u64 cta_sum, before;
@@ -220,13 +223,33 @@ struct Cut {
   __device__ __forceinline__ bool keeps(float v, int i) const { return v > value || (v == value && i <= idx); }
 };
 
-// ascending bitonic sort of the power-of-two n2 <= kThreads elements, one per
-// thread; partners within a warp by shuffles
+__device__ __forceinline__ int pow2_at_least(int v) {
+  int p = 1;
+  while (p < v) p <<= 1;
+  return p;
+}
+// ascending sort of n <= kCap different elements.  Up to kFew: an element's place is
+// the number of smaller ones, each counted over a share of the list by 1024 / n
+// threads (broadcast reads).  More: bitonic, one element per thread, partners within a
+// warp by shuffles; the array's places up to the next power of two are filled.
 template <typename T>
-__device__ void sort(T *a, int n2) {
-  const int tid = threadIdx.x;
+__device__ void sort(T *a, int n, unsigned int *place) {
+  const int tid = threadIdx.x, n2 = max(32, pow2_at_least(n));
   __syncthreads();
-  T x = tid < n2 ? a[tid] : T(0);
+  if (n <= kFew) {
+    const int e = tid & (n2 - 1), parts = kThreads / n2, share = (n + parts - 1) / parts, from = tid / n2 * share;
+    const T x = e < n ? a[e] : T(0);
+    if (tid < kFew) place[tid] = 0;
+    unsigned int less = 0;
+    for (int j = from; j < min(n, from + share); ++j) less += a[j] < x;
+    __syncthreads();
+    if (e < n && less) atomicAdd(&place[e], less);
+    __syncthreads();
+    if (tid < n) a[place[tid]] = x;
+    __syncthreads();
+    return;
+  }
+  T x = tid < n ? a[tid] : T(~T(0));
   for (int size = 2; size <= n2; size <<= 1)
     for (int d = size >> 1; d > 0; d >>= 1) {
       T y;
@@ -244,11 +267,6 @@ __device__ void sort(T *a, int n2) {
   __syncthreads();
   if (tid < n2) a[tid] = x;
   __syncthreads();
-}
-__device__ __forceinline__ int pow2_at_least(int v) {
-  int p = 1;
-  while (p < v) p <<= 1;
-  return p;
 }
 __device__ __forceinline__ float list_value(u64 e) { return value_of(~(uint32_t)(e >> 32)); }
 
@@ -374,9 +392,8 @@ __device__ int cut_list(Shared &s, int nl, u64 before, double target, int warp, 
 
 // rank 0: sorts its list of nl elements and fills in their weights
 __device__ void sort_list(Shared &s, const Row &r, int nl) {
-  const int tid = threadIdx.x, n2 = pow2_at_least(nl);
-  if (tid >= nl && tid < n2) s.list[tid] = ~0ull;
-  sort(s.list, n2);
+  const int tid = threadIdx.x;
+  sort(s.list, nl, s.place);
   const u64 w = r.weight(tid < nl ? list_value(s.list[tid]) : r.max);
   if (tid < nl) s.weight[tid] = w;
   __syncthreads();
@@ -403,7 +420,7 @@ __device__ void find_cut(cg::cluster_group &cl, Shared &s, const Row &r, Cut &c,
     if (nbin <= kCap) {
       if (rank == 0) {
         sort_list(s, r, nbin);
-        const int at = cut_list<MASS>(s, nbin, before, target, warp, lane);
+        const int at = min(cut_list<MASS>(s, nbin, before, target, warp, lane), nbin - 1);
         if (tid < C) {
           Shared &o = *cl.map_shared_rank(&s, tid);
           o.cut_key = ~(uint32_t)(s.list[at] >> 32);
@@ -492,9 +509,8 @@ __device__ void choose_from_list(Shared &s, const SampleArgs &a, const Row &r, i
     nl = min(nl, cut_list<true>(s, nl, 0, (double)a.top_p * (double)all_mass, warp, lane) + 1);
   }
   // in index order (index, place), what min-p drops without weight
-  const int n2 = pow2_at_least(nl);
-  if (tid < n2) s.order[tid] = tid < nl ? (unsigned int)s.list[tid] << 10 | tid : 0xffffffffu;
-  sort(s.order, n2);
+  if (tid < nl) s.order[tid] = (unsigned int)s.list[tid] << 10 | tid;
+  sort(s.order, nl, s.place);
   u64 w = 0;
   if (tid < nl) {
     w = s.weight[s.order[tid] & (kCap - 1)];

@@ -166,3 +166,16 @@ def test_two_streams_at_once():
             outs.append(token)
     torch.cuda.synchronize()
     assert all(t.tolist() == want for t in outs)
+
+
+@pytest.mark.parametrize("k", [2, 31, 32, 33, 255, 256, 257, 600, 1023, 1024, 1025])
+def test_lists_of_every_length(k):
+    """Cuts whose lists are sorted by counting, by exchanges, and not at all."""
+    rng = np.random.default_rng(k)
+    x = (rng.standard_normal((3, 30000)) * 2).astype(np.float32)
+    x[1] = rng.integers(0, 200, 30000).astype(np.float32) / 8  # steps of many equal logits
+    x[2, k:] = -np.inf  # no more than k to keep
+    u = np.array([0.35, 0.77, 0.999], np.float32)
+    check(x, u, 1.0, k)
+    check(x, u, 3.0, k, 0.6, 0.01)
+    check(x, u, 0.5, 0, 1 - 1 / k)
