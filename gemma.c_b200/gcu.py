@@ -841,6 +841,8 @@ def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     if not (logits.dtype is torch.float32 and len(ld) == 2 and ld[1] == 1):
         raise GcuError(f"{what}: logits must be float32 (m, nvocab) rows, not {logits.dtype} {tuple(logits.shape)}")
     m, n = logits.shape
+    if m > 1 and ld[0] < n:  # 0 would reach the library as "one row behind the other"
+        raise GcuError(f"{what}: rows of {n} logits at stride {ld[0]} share memory (an expanded row: .contiguous())")
     _rows(what, "token", token, torch.int32, (m,), dev)
     _rows(what, "u", u, torch.float32, (m,), dev)
     if prob is not None:
