@@ -823,8 +823,10 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
     dev, (n_heads, ntok) = _device(what, kv.index), xq.shape[:2]
     _rows(what, "xq", xq, torch.float32, (n_heads, ntok, kv.hdim), dev)
     if not (xo.dtype is torch.float32 and xo.dim() == 2 and xo.shape[0] == ntok and xo.stride(1) == 1 and
-            xo.shape[1] >= n_heads * kv.hdim and xo.get_device() == dev):
-        raise GcuError(f"{what}: xo must be float32 (ntok, >= n_heads*hdim) rows, not {xo.dtype} {tuple(xo.shape)}")
+            xo.shape[1] >= n_heads * kv.hdim and xo.get_device() == dev and
+            (ntok < 2 or xo.stride(0) >= n_heads * kv.hdim)):
+        raise GcuError(f"{what}: xo must be float32 (ntok, >= n_heads*hdim) rows apart from each other, "
+                       f"not {xo.dtype} {tuple(xo.shape)}, strides {xo.stride()}")
     l = lib()
     work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, sc_att, int(mask)),
                                kv.device, stream)

@@ -47,3 +47,20 @@ def test_logits_rows_that_are_one_row(library):
         with pytest.raises(gcu.GcuError, match="rows of 40 logits"):
             sample(rows)
     assert len(library.made) == 2
+
+
+def prefill(xo, ntok, nh=2, hd=64):
+    kv = gcu.KvCacheI8.empty(1, 1, 16, hd, device="cpu")
+    gcu.dev_attention_prefill_i8(xo, torch.zeros((nh, ntok, hd)), kv, 0)
+
+
+def test_prefill_rows_that_are_one_row(library):
+    """As above for the rows that prefill attention writes."""
+    prefill(torch.zeros((3, 128)), 3)
+    prefill(torch.zeros((3, 160))[:, :128], 3)
+    prefill(torch.zeros((1, 128)).expand(1, -1), 1)
+    assert [args[1] for _, args in library.made] == [128, 160, 0]
+    for xo in (torch.zeros((1, 128)).expand(3, -1), torch.zeros(300).as_strided((3, 128), (64, 1))):
+        with pytest.raises(gcu.GcuError, match="rows"):
+            prefill(xo, 3)
+    assert len(library.made) == 3
