@@ -680,6 +680,14 @@ def _rows(what, name, t, dtype, shape, dev):
                    f"not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def _int32(what, *counts):
+    """Refuses what does not fit the library's ints, where it would wrap.  Called when the counts'
+    union, shifted by 31 bits, is not zero: one of them is negative or too large."""
+    for n in counts:
+        if not -0x80000000 <= n <= 0x7fffffff:
+            raise GcuError(f"{what}: {n} does not fit into 32 bits")
+
+
 def _work(nbytes, device, stream):
     """Scratch of one call.  It comes from torch's allocator, so it is the
     call's own: in a captured graph it lives in the graph's pool."""
@@ -760,6 +768,8 @@ def dev_qkv_norm_rope_cache_i8(xq, qkv, kv, freqs, spos, q_scale=1.0, nq=None, n
     what = "dev_qkv_norm_rope_cache_i8"
     n_heads, ntok = xq.shape[:2]
     dev, ld = _check_write(what, xq, (n_heads, ntok, kv.hdim), qkv, kv, freqs, nq, nk, ntok, n_heads)
+    if spos >> 31:
+        _int32(what, spos)
     _check(lib().gcu_dev_qkv_norm_rope_cache_i8(xq.data_ptr(), qkv.data_ptr(), ld, kv.ref, _ptr(nq), _ptr(nk), eps,
                                                 freqs.data_ptr(), q_scale, n_heads, spos, ntok, _on(stream, dev)), what)
 
@@ -788,6 +798,8 @@ def dev_cache_i8_read(k, v, kv, spos, stream=None):
             (st[2] == kv.hdim or sh[2] < 2) and k.get_device() == dev and v.get_device() == dev):
         raise GcuError(f"{what}: k and v must be float32 (nseq, nkv, ntok, hdim) with contiguous positions, alike, on the "
                        f"cache's device, not {k.dtype} {tuple(k.shape)}, {v.dtype} {tuple(v.shape)}")
+    if spos >> 31:
+        _int32(what, spos)
     _check(lib().gcu_dev_cache_i8_read(k.data_ptr(), v.data_ptr(), st[0] if sh[0] > 1 else 0,
                                        st[1] if sh[1] > 1 else 0, kv.ref, spos, sh[2],
                                        _on(stream, dev)), what)
@@ -809,6 +821,8 @@ def dev_attention_decode_i8(xo, xq, kv, length, max_len, asc, sc_att=0.0, slide=
     if prefix is not None:
         _device(what, prefix.index)
         pref = prefix.ref
+    if (max_len | slide | plen) >> 31:
+        _int32(what, max_len, slide, plen)
     l = lib()
     work, nbytes, keep = _work(l.gcu_attention_decode_i8_work(pref, plen, kv.ref, max_len, n_heads, slide), kv.device, stream)
     _check(l.gcu_dev_attention_decode_i8(xo.data_ptr(), xq.data_ptr(), pref, plen, kv.ref, _ptr(length), max_len, n_heads,
@@ -827,11 +841,14 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
             (ntok < 2 or xo.stride(0) >= n_heads * kv.hdim)):
         raise GcuError(f"{what}: xo must be float32 (ntok, >= n_heads*hdim) rows apart from each other, "
                        f"not {xo.dtype} {tuple(xo.shape)}, strides {xo.stride()}")
+    ld = xo.stride(0) if ntok > 1 else 0  # one row: its stride is never taken
+    if (spos | slide | ld) >> 31:
+        _int32(what, spos, slide, ld)
     l = lib()
     work, nbytes, keep = _work(l.gcu_attention_prefill_i8_work(kv.ref, n_heads, spos, ntok, slide, sc_att, int(mask)),
                                kv.device, stream)
-    _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), xo.stride(0) if ntok > 1 else 0, xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide,
-                                          sc_att, int(mask), work, nbytes, _on(stream, dev)), what)
+    _check(l.gcu_dev_attention_prefill_i8(xo.data_ptr(), ld, xq.data_ptr(), kv.ref, n_heads, spos, ntok, slide, sc_att,
+                                          int(mask), work, nbytes, _on(stream, dev)), what)
 
 
 def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
@@ -849,5 +866,7 @@ def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
     _rows(what, "u", u, torch.float32, (m,), dev)
     if prob is not None:
         _rows(what, "prob", prob, torch.float32, (m,), dev)
+    if top_k >> 31:
+        _int32(what, top_k)
     _check(lib().gcu_dev_sample(token.data_ptr(), _ptr(prob), logits.data_ptr(), ld[0] if m > 1 else 0,
                                 u.data_ptr(), temperature, top_k, top_p, min_p, m, n, _on(stream, dev)), what)

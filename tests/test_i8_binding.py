@@ -64,3 +64,31 @@ def test_prefill_rows_that_are_one_row(library):
         with pytest.raises(gcu.GcuError, match="rows"):
             prefill(xo, 3)
     assert len(library.made) == 3
+
+
+BIG = (1 << 32) + 3  # 3 in a C int
+
+
+def test_numbers_past_32_bits(library):
+    """The library's counts are C ints; a larger one does not wrap to another count."""
+    kv = gcu.KvCacheI8.empty(1, 1, 16, 64, device="cpu")
+    f32 = lambda *shape: torch.zeros(shape)
+    x, xq, rows = f32(1, 2, 64), f32(2, 3, 64), f32(3, 128)
+    calls = [
+        lambda n: gcu.dev_sample(torch.zeros(1, dtype=torch.int32), f32(1, 8), f32(1), top_k=n),
+        lambda n: gcu.dev_attention_decode_i8(f32(1, 2, 64), x, kv, None, n, 1.0),
+        lambda n: gcu.dev_attention_decode_i8(f32(1, 2, 64), x, kv, None, 8, 1.0, slide=n),
+        lambda n: gcu.dev_attention_decode_i8(f32(1, 2, 64), x, kv, None, 8, 1.0, prefix=kv, plen=n),
+        lambda n: gcu.dev_attention_prefill_i8(rows, xq, kv, n),
+        lambda n: gcu.dev_attention_prefill_i8(rows, xq, kv, 0, slide=n),
+        lambda n: gcu.dev_cache_i8_read(f32(1, 1, 2, 64), f32(1, 1, 2, 64), kv, n),
+        lambda n: gcu.dev_qkv_norm_rope_cache_i8(xq, f32(3, 256), kv, f32(3, 64), n),
+    ]
+    for call in calls:
+        call(3)
+        call(-1)  # in range here; the library says what it thinks of it
+        made = len(library.made)
+        for n in (BIG, 1 << 31, -BIG):
+            with pytest.raises(gcu.GcuError, match="32 bits"):
+                call(n)
+        assert len(library.made) == made
