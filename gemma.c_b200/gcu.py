@@ -690,12 +690,16 @@ def _int32(what, *counts):
 
 def _work(nbytes, device, stream):
     """Scratch of one call.  It comes from torch's allocator, so it is the
-    call's own: in a captured graph it lives in the graph's pool."""
+    call's own: in a captured graph it lives in the graph's pool.  It is taken
+    while `stream` is current, from that stream's pool: a block of another's
+    could still be in use there, by a call that has returned."""
     if not nbytes:
         return None, 0, None
-    w = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    if stream is not None:
-        w.record_stream(stream)  # the block is not handed out again before the call is done
+    if stream is None:
+        w = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        with torch.cuda.stream(stream):
+            w = torch.empty(nbytes, dtype=torch.uint8, device=device)
     return w.data_ptr(), nbytes, w
 
 

@@ -92,3 +92,41 @@ def test_numbers_past_32_bits(library):
             with pytest.raises(gcu.GcuError, match="32 bits"):
                 call(n)
         assert len(library.made) == made
+
+
+class Streams:
+    """Stands for torch.cuda.stream: which stream is the current one."""
+
+    def __init__(self, monkeypatch):
+        self.current, self.allocated = None, []
+        empty = torch.empty
+
+        def noted(*args, **kw):
+            self.allocated.append(self.current)
+            return empty(*args, **kw)
+        monkeypatch.setattr(torch, "empty", noted)
+        monkeypatch.setattr(torch.cuda, "stream", self.use)
+
+    def use(self, stream):
+        outer = self
+
+        class Context:
+            def __enter__(self):
+                self.before, outer.current = outer.current, stream
+
+            def __exit__(self, *exc):
+                outer.current = self.before
+        return Context()
+
+
+def test_scratch_belongs_to_the_stream_that_uses_it(library, monkeypatch):
+    """Taken from another stream's pool, a block could still be in use there."""
+    library.work = 1 << 12
+    kv = gcu.KvCacheI8.empty(1, 1, 16, 64, device="cpu")
+    x, xo, rows, xq = torch.zeros((1, 2, 64)), torch.zeros((1, 2, 64)), torch.zeros((3, 128)), torch.zeros((2, 3, 64))
+    side = object()
+    streams = Streams(monkeypatch)
+    for stream in (None, side):
+        gcu.dev_attention_decode_i8(xo, x, kv, None, 8, 1.0, stream=stream)
+        gcu.dev_attention_prefill_i8(rows, xq, kv, 0, stream=stream)
+    assert streams.allocated == [None, None, side, side] and streams.current is None
