@@ -380,11 +380,13 @@ class Decoder:
     def sample(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, seqs=False, prob=None, stream=None):
         """The next token of each row of the last step's logits (of step_seqs when
         seqs, else of step or prefill) from the random numbers u (rows,) float32
-        on the device; int32 (rows,).  See gcu.dev_sample."""
-        logits = self.slogits if seqs else self.logits
-        token = self.torch.empty(logits.shape[0], dtype=self.torch.int32, device=self.dev)
+        on the device; int32 (rows,), on `stream`: another stream waits for it before
+        it reads them.  See gcu.dev_sample."""
+        torch, logits = self.torch, self.slogits if seqs else self.logits
+        with torch.cuda.stream(stream) if stream is not None else _null():
+            token = torch.empty(logits.shape[0], dtype=torch.int32, device=self.dev)
         if stream is not None:
-            token.record_stream(stream)
+            token.record_stream(torch.cuda.current_stream())  # dropped tokens may still be read there
         gcu.dev_sample(token, logits, u, temperature, top_k, top_p, min_p, prob=prob, stream=stream)
         return token
 

@@ -51,3 +51,23 @@ def test_scratch_of_calls_on_two_streams(side_first):
             torch.cuda.synchronize()
             for j, out in enumerate(outs):
                 assert torch.equal(out, alone[j % 2])
+
+
+def test_tokens_sampled_on_another_stream():
+    """Tokens of a side stream beside work of the current stream that drops blocks of their size."""
+    import decode
+    dec = object.__new__(decode.Decoder)
+    g = torch.Generator(device="cuda").manual_seed(32)
+    dec.torch, dec.dev, dec.slogits = torch, "cuda", torch.randn((5, 50000), generator=g, device="cuda")
+    u, big = torch.rand(5, generator=g, device="cuda"), torch.zeros(1 << 28, device="cuda")
+    want = dec.sample(u, 0.9, 50, seqs=True)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        big.add_(1)  # some 300 us
+        torch.zeros(5, dtype=torch.int32, device="cuda")  # written after that, dropped now
+        token = dec.sample(u, 0.9, 50, seqs=True, stream=side)
+        side.synchronize()
+        early = token.tolist()
+        torch.cuda.synchronize()
+        assert early == token.tolist() == want.tolist()

@@ -130,3 +130,17 @@ def test_scratch_belongs_to_the_stream_that_uses_it(library, monkeypatch):
         gcu.dev_attention_decode_i8(xo, x, kv, None, 8, 1.0, stream=stream)
         gcu.dev_attention_prefill_i8(rows, xq, kv, 0, stream=stream)
     assert streams.allocated == [None, None, side, side] and streams.current is None
+
+
+def test_sampled_tokens_belong_to_the_stream_that_writes_them(library, monkeypatch):
+    """And are not handed out again while the stream that was current may still read them."""
+    import decode
+    dec = object.__new__(decode.Decoder)
+    dec.torch, dec.dev, dec.logits, dec.slogits = torch, "cpu", torch.zeros((1, 8)), torch.zeros((3, 8))
+    side, readers = object(), []
+    streams = Streams(monkeypatch)
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: readers.append(s))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: streams.current)
+    assert dec.sample(torch.zeros(1)).shape == (1,)
+    assert dec.sample(torch.zeros(3), seqs=True, stream=side).shape == (3,)
+    assert streams.allocated == [None, side] and readers == [None] and streams.current is None
