@@ -294,13 +294,19 @@ class Decoder:
             gcu.dev_softcap(self.logits, c["sc_log"], stream=stream)
 
     # ---- several sequences from one prompt (8-bit cache) ------------------------
-    def fork(self, nseq: int, plen: int, tail: int):
+    def fork(self, nseq: int, plen: int, tail: int, stream=None):
         """Start nseq sequences from the first plen positions of the cache, which they
-        share, each with a cache of its own for `tail` further tokens."""
+        share, each with a cache of its own for `tail` further tokens.  Their buffers
+        are made, and the last fork's dropped, in the order of `stream`, on which
+        step_seqs runs then (another stream waits for it)."""
         if self.kv_bits != 8:
             raise ValueError("fork: sequences share an 8-bit KV cache (kv_bits=8)")
         if nseq < 1 or tail < 1 or not 0 <= plen <= self.clen:
             raise ValueError(f"fork of {nseq} sequences with {tail} tokens from {plen} of {self.clen} positions")
+        with self.torch.cuda.stream(stream) if stream is not None else _null():
+            self._fork_buffers(nseq, plen, tail)
+
+    def _fork_buffers(self, nseq, plen, tail):
         torch, c = self.torch, self.cfg
         f32 = dict(dtype=torch.float32, device=self.dev)
         i8 = dict(dtype=torch.int8, device=self.dev)
@@ -324,11 +330,13 @@ class Decoder:
             self.wqkv = [(torch.cat([w["wq"][0], w["wk"][0], w["wv"][0]]).contiguous(),
                           torch.cat([w["wq"][1], w["wk"][1], w["wv"][1]]).contiguous()) for w in self.L]
 
-    def set_seq_freqs(self, slid, full):
+    def set_seq_freqs(self, slid, full, stream=None):
         """Upload the RoPE tables (nseq, hdim) of the positions about to be decoded: plen +
         the sequence's own tokens so far."""
         torch = self.torch
-        self.sfreq.copy_(torch.from_numpy(np.stack([np.asarray(slid, np.float32), np.asarray(full, np.float32)])))
+        host = torch.from_numpy(np.stack([np.asarray(slid, np.float32), np.asarray(full, np.float32)]))
+        with torch.cuda.stream(stream) if stream is not None else _null():
+            self.sfreq.copy_(host)
 
     def step_seqs(self, stream=None):
         """Decode one token of every forked sequence from the embeddings in self.sx

@@ -71,3 +71,38 @@ def test_tokens_sampled_on_another_stream():
         early = token.tolist()
         torch.cuda.synchronize()
         assert early == token.tolist() == want.tolist()
+
+
+def test_forked_sequences_on_another_stream():
+    """fork, tables, steps and samples on a side stream while the current one is busy, twice over:
+    as on the current stream."""
+    import synth
+    import test_gpu_decode_i8 as D
+    name = next(iter(D.META["cases"]))
+    cfg, emb, _ = D.model(name, 8, 12)
+    x = synth.normal(cfg["tid"] + 777, (6, cfg["dim"]))
+    u = torch.rand((3, 4), generator=torch.Generator().manual_seed(5)).cuda()
+    start = torch.from_numpy(synth.normal(92, (4, cfg["dim"]))).cuda()
+    big = torch.zeros(1 << 28, device="cuda")
+    side = torch.cuda.Stream()
+    results = []
+    for stream in (None, side):
+        dec = D.model(name, 8, 12)[2]
+        D.prefill(cfg, dec, x)
+        torch.cuda.synchronize()
+        got = []
+        for turn in range(2):
+            big.add_(1)
+            dec.fork(4, 6, 3, stream=stream)
+            for r in range(3):
+                dec.set_seq_freqs(*D.tables(cfg, [6 + r] * 4), stream=stream)
+                with torch.cuda.stream(stream) if stream is not None else torch.no_grad():
+                    dec.sx.copy_(start)
+                dec.step_seqs(stream=stream)
+                t = dec.sample(u[r], 0.9, 20, seqs=True, stream=stream)
+                with torch.cuda.stream(stream) if stream is not None else torch.no_grad():
+                    got.append((t.clone(), dec.slogits.clone(), dec.slen.clone()))
+        torch.cuda.synchronize()
+        results.append([[v.cpu() for v in g] for g in got])
+    for a, b in zip(*results):
+        assert all(torch.equal(s, t) for s, t in zip(a, b))

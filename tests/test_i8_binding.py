@@ -99,13 +99,15 @@ class Streams:
 
     def __init__(self, monkeypatch):
         self.current, self.allocated = None, []
-        empty = torch.empty
+        for name in ("empty", "zeros", "ones"):
+            monkeypatch.setattr(torch, name, self.noting(getattr(torch, name)))
+        monkeypatch.setattr(torch.cuda, "stream", self.use)
 
+    def noting(self, make):
         def noted(*args, **kw):
             self.allocated.append(self.current)
-            return empty(*args, **kw)
-        monkeypatch.setattr(torch, "empty", noted)
-        monkeypatch.setattr(torch.cuda, "stream", self.use)
+            return make(*args, **kw)
+        return noted
 
     def use(self, stream):
         outer = self
@@ -138,9 +140,31 @@ def test_sampled_tokens_belong_to_the_stream_that_writes_them(library, monkeypat
     dec = object.__new__(decode.Decoder)
     dec.torch, dec.dev, dec.logits, dec.slogits = torch, "cpu", torch.zeros((1, 8)), torch.zeros((3, 8))
     side, readers = object(), []
+    u = torch.zeros(1), torch.zeros(3)
     streams = Streams(monkeypatch)
     monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: readers.append(s))
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: streams.current)
-    assert dec.sample(torch.zeros(1)).shape == (1,)
-    assert dec.sample(torch.zeros(3), seqs=True, stream=side).shape == (3,)
+    assert dec.sample(u[0]).shape == (1,)
+    assert dec.sample(u[1], seqs=True, stream=side).shape == (3,)
     assert streams.allocated == [None, side] and readers == [None] and streams.current is None
+
+
+def test_a_fork_is_made_on_the_stream_that_steps_it(monkeypatch):
+    """Its caches are filled, and the last fork's dropped, in the order of that stream."""
+    import decode
+    dec = object.__new__(decode.Decoder)
+    dec.torch, dec.dev, dec.kv_bits, dec.clen = torch, "cpu", 8, 16
+    dec.cfg = dict(nl=2, n_heads=2, nkv=1, hdim=64, dim=32, mlp_dim=48, nvocab=10)
+    dec.L = [{w: (torch.zeros((4, 32), dtype=torch.int8), torch.zeros(4)) for w in ("wq", "wk", "wv")}] * 2
+    streams, side = Streams(monkeypatch), object()
+    dec.fork(3, 4, 5)
+    assert set(streams.allocated) == {None}
+    del streams.allocated[:]
+    dec.fork(3, 4, 5, stream=side)
+    assert set(streams.allocated) == {side} and streams.current is None
+    streams.copies = []
+    copy = torch.Tensor.copy_
+    monkeypatch.setattr(torch.Tensor, "copy_", lambda *a, **k: streams.copies.append(streams.current) or copy(*a, **k))
+    for s in (None, side):
+        dec.set_seq_freqs(torch.zeros((3, 64)).numpy(), torch.ones((3, 64)).numpy(), stream=s)
+    assert streams.copies == [None, side]
