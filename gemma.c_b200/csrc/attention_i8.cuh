@@ -55,7 +55,7 @@ struct Args {
   int chunk, splits, slot0, slots;
   float *part;
   float2 *stat;
-  unsigned int *err;
+  unsigned int *err, *bad_len;
 };
 
 // query heads [head0(hk), head0(hk + 1)) belong to kv head hk (h * nkv / n_heads)

@@ -45,7 +45,7 @@ int check_cuda(cudaError_t e, const char *what) {
 // ---------------------------------------------------------------------------
 // per-device state
 // ---------------------------------------------------------------------------
-__device__ unsigned int g_dev_err;
+__device__ unsigned int g_dev_err[2];  // what gave up waiting; a sequence length
 
 static thread_local int t_device = -1;
 
@@ -63,6 +63,9 @@ static int current_device() {
 // or a host entry point has run on the device, a word of mapped pinned host
 // memory, which kernels write directly and host calls read after their
 // stream wait without a device-to-host copy (each copy costs ~10 us here).
+// The word after it is for sequence lengths (dev_length_word): a caller's
+// mistake, which only gcu_check_device reports, so it neither fails another
+// caller's host call nor takes the place of a wait that gave up.
 struct DeviceInfo {
   int sms = 0;
   unsigned int *err_sym = nullptr;              // device variable
@@ -119,31 +122,29 @@ void forget_error_code(unsigned int code) {
   if (code < 32) g_codes_seen.fetch_and(~(1u << code));
 }
 
-// Read and clear every home of the error word (device variable by copy).
-static unsigned int take_error_code(bool read_symbol) {
+// Read and clear every home of error word `i` (device variable by copy).
+static unsigned int take_word(int i, bool read_symbol) {
   DeviceInfo &di = device_info();
   unsigned int code = 0;
   if (di.err_host) {
-    code = *di.err_host;
-    if (code) *di.err_host = 0;
+    code = di.err_host[i];
+    if (code) di.err_host[i] = 0;
   }
   if (read_symbol && di.err_sym) {
     unsigned int c2 = 0;
-    if (cudaMemcpy(&c2, di.err_sym, sizeof(c2), cudaMemcpyDeviceToHost) == cudaSuccess && c2) {
+    if (cudaMemcpy(&c2, di.err_sym + i, sizeof(c2), cudaMemcpyDeviceToHost) == cudaSuccess && c2) {
       unsigned int zero = 0;
-      cudaMemcpy(di.err_sym, &zero, sizeof(zero), cudaMemcpyHostToDevice);
+      cudaMemcpy(di.err_sym + i, &zero, sizeof(zero), cudaMemcpyHostToDevice);
       if (!code) code = c2;
     }
   }
-  if (code && code < 32) g_codes_seen.fetch_or(1u << code);
   return code;
 }
 
-// the message of a nonzero device error code; returns 1
-static int report_error_code(unsigned int code) {
-  if (code == DEV_BAD_LENGTH)
-    return set_error("a sequence length outside its 8-bit cache: that sequence was skipped (code %u)", code);
-  return set_error("device-side wait gave up (code %u)", code);
+static unsigned int take_error_code(bool read_symbol) {
+  const unsigned int code = take_word(0, read_symbol);
+  if (code && code < 32) g_codes_seen.fetch_or(1u << code);
+  return code;
 }
 
 int num_sms() { return device_info().sms; }
@@ -158,6 +159,10 @@ bool pdl_enabled() {
 unsigned int *dev_error_word() {
   DeviceInfo &di = device_info();
   return di.err_map ? di.err_map : di.err_sym;
+}
+unsigned int *dev_length_word() {
+  unsigned int *w = dev_error_word();
+  return w ? w + 1 : nullptr;
 }
 
 // ---------------------------------------------------------------------------
@@ -445,7 +450,7 @@ static int sync_and_check(ThreadCtx *c, cudaStream_t st) {
   (void)c;
   GCU_CUDA(cudaStreamSynchronize(st));
   const unsigned int code = take_error_code(false);
-  if (code) return report_error_code(code);
+  if (code) return set_error("device-side wait gave up (code %u)", code);
   return 0;
 }
 static int sync_and_check(ThreadCtx *c) { return sync_and_check(c, c->stream); }
@@ -494,8 +499,10 @@ GCU_EXPORT int gcu_init(int device) {
 
 GCU_EXPORT int gcu_check_device(void) {
   GCU_CUDA(cudaDeviceSynchronize());
-  const unsigned int code = take_error_code(true);
-  if (code) return report_error_code(code);
+  const unsigned int code = take_error_code(true), length = take_word(1, true);
+  const char *skipped = "a sequence length outside its 8-bit cache: that sequence was skipped";
+  if (code) return set_error("device-side wait gave up (code %u)%s%s", code, length ? "; and " : "", length ? skipped : "");
+  if (length) return set_error("%s (code %u)", skipped, length);
   return 0;
 }
 

@@ -80,7 +80,8 @@ enum DevErr : unsigned int {
   DEV_TIMEOUT_CHAIN = 9,     // a chain launch's grid-wide hand-off between two steps
   DEV_BAD_LENGTH = 10,       // a sequence length outside its 8-bit cache (that sequence was skipped)
 };
-unsigned int *dev_error_word();  // device address of the error word
+unsigned int *dev_error_word();   // device address of the error word
+unsigned int *dev_length_word();  // and of DEV_BAD_LENGTH's own
 // Bit mask of the device error codes the host has observed since start-up
 // (1u << code), including a code now sitting in the error word unread;
 // forget_error_code clears one (after the state it poisoned is rebuilt).

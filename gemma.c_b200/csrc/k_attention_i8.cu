@@ -287,7 +287,8 @@ GCU_EXPORT int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long qrow = (long)n_heads * own->hdim;
   Args a{xq, qrow, own->hdim, xo, qrow, *own, OWN, n_heads, own->nseq, 0, slide, 1, plen, max_len, len, asc, sc_att,
-         p.own.chunk, p.own.splits, p.pre.splits, p.slots(), nullptr, nullptr, dev_error_word()};
+         p.own.chunk, p.own.splits, p.pre.splits, p.slots(), nullptr, nullptr, dev_error_word(),
+         dev_length_word()};
   use_work(a, work, rows);
   Args sets[2] = {a, a};
   int n = 1;
@@ -399,7 +400,8 @@ GCU_EXPORT int gcu_dev_attention_prefill_i8_tuned(float *xo, int xostr, const fl
     return set_error("%s: xo and xq overlap", what);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   Args a{xq, kv->hdim, (long)ntok * kv->hdim, xo, xostr, *kv, PREFILL, n_heads, ntok, spos, slide, mask ? 1 : 0, 0, 0,
-         nullptr, 1.0f, sc_att, p.p.chunk, p.p.splits, 0, p.slots(), nullptr, nullptr, dev_error_word()};
+         nullptr, 1.0f, sc_att, p.p.chunk, p.p.splits, 0, p.slots(), nullptr, nullptr, dev_error_word(),
+         dev_length_word()};
   use_work(a, work, rows);
   if (p.kt ? launch_kt(&a, 1, p.rows, st) : launch_tc(a, st)) return 1;
   return a.slots > 1 ? launch_merge(a, st) : 0;

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   const int seq = a.mode == OWN ? group : 0;
   Waiter wait{&s_abort, a.err};
   if (a.mode == OWN && a.len && threadIdx.x == 0 && split == 0 && hk == 0 && __ldg(a.len + group) > a.max_len)
-    ptx::record_err(a.err, DEV_BAD_LENGTH);
+    ptx::record_err(a.bad_len, DEV_BAD_LENGTH);
 
   const uint64_t pol = ptx::policy_evict_first();
   auto load = [&](const CUtensorMap *m, uint64_t *full, int off, int j) {

@@ -43,7 +43,7 @@ struct WriteArgs {
   const float *freqs;
   float q_scale;
   int n_heads, spos, rows;
-  unsigned int *err;
+  unsigned int *bad_len;
 };
 
 template <int E>
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kWriteThreads) k_write(WriteArgs a) {
     const int n = __ldg(a.len + t);
     if (n < 1) return;
     if (n > a.kv.clen) {
-      if (lane == 0) ptx::record_err(a.err, DEV_BAD_LENGTH);
+      if (lane == 0) ptx::record_err(a.bad_len, DEV_BAD_LENGTH);
       return;
     }
     pos = n - 1;
@@ -328,7 +328,7 @@ GCU_EXPORT int gcu_dev_qkv_norm_rope_cache_i8(float *xq, const float *qkv, long 
   if (kv->nseq != 1) return set_error("%s: a cache of one sequence expected, not of %d", what, kv->nseq);
   if (spos < 0 || ntok < 0 || spos > kv->clen - ntok)
     return set_error("%s: %d positions from %d outside a cache of %d", what, ntok, spos, kv->clen);
-  WriteArgs a{xq, qkv, ld, *kv, nullptr, nq, nk, eps, freqs, q_scale, n_heads, spos, ntok, dev_error_word()};
+  WriteArgs a{xq, qkv, ld, *kv, nullptr, nq, nk, eps, freqs, q_scale, n_heads, spos, ntok, dev_length_word()};
   return launch_write(a, static_cast<cudaStream_t>(stream));
 }
 
@@ -339,7 +339,7 @@ GCU_EXPORT int gcu_dev_qkv_norm_rope_cache_i8_seqs(float *xq, const float *qkv, 
   const char *what = "qkv_norm_rope_cache_i8_seqs";
   if (check_write(what, xq, qkv, ld, kv, nq, nk, freqs, n_heads)) return 1;
   if (!len) return set_error("%s: null pointer", what);
-  WriteArgs a{xq, qkv, ld, *kv, len, nq, nk, eps, freqs, q_scale, n_heads, 0, kv->nseq, dev_error_word()};
+  WriteArgs a{xq, qkv, ld, *kv, len, nq, nk, eps, freqs, q_scale, n_heads, 0, kv->nseq, dev_length_word()};
   return launch_write(a, static_cast<cudaStream_t>(stream));
 }
 

@@ -44,7 +44,8 @@ int gcu_shutdown(void);
 /* Thread-local message of the last failed call ("" if none). */
 const char *gcu_last_error(void);
 /* Wait for the device and return 1 if a kernel recorded a device-side error
- * (a bounded wait that gave up), clearing it; 0 otherwise. */
+ * (a bounded wait that gave up, or a sequence length outside its 8-bit cache,
+ * which no other call reports), clearing it; 0 otherwise. */
 int gcu_check_device(void);
 /* Library version string. */
 const char *gcu_version(void);
