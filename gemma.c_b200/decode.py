@@ -313,6 +313,7 @@ class Decoder:
         dim, mlp, hd = c["dim"], c["mlp_dim"], c["hdim"]
         q_sz, kv_sz = c["n_heads"] * hd, c["nkv"] * hd
         self.nseq, self.plen, self.tail = nseq, plen, tail
+        self.steps = 0  # of the longest sequence, as far as the host has seen
         self.own8 = [gcu.KvCacheI8.empty(nseq, c["nkv"], tail, hd, self.dev) for _ in range(c["nl"])]
         self.slen = torch.zeros(nseq, dtype=torch.int32, device=self.dev)  # tokens of each sequence's own
         self.sx = torch.empty((nseq, dim), **f32)
@@ -344,7 +345,10 @@ class Decoder:
         attention over the shared prompt computed once for all.  Leaves the logits
         in self.slogits and the final hidden states in self.sx, and counts the
         tokens in self.slen; a sequence whose self.slen is negative stands still
-        (its logits mean nothing).  Set the tables with set_seq_freqs beforehand."""
+        (its logits mean nothing).  Raises when a sequence has no room left in its
+        tail; a step replayed from a graph is not counted here, and skips such a
+        sequence and leaves it to gcu.check_device.  Set the tables with
+        set_seq_freqs beforehand."""
         if not self.nseq:
             raise ValueError("step_seqs: fork first")
         c, n = self.cfg, self.nseq
@@ -354,6 +358,12 @@ class Decoder:
         eps, x, ps, out = c["eps"], self.sx, self.ss, self.sout
         q_dim, q_qsz, q_mlp = self.sq
         with self.torch.cuda.stream(stream) if stream is not None else _null():
+            if not (self.slen.is_cuda and self.torch.cuda.is_current_stream_capturing()):
+                if self.steps >= self.tail:  # the lengths may have been set since: see what they are
+                    self.steps = int(self.slen.max())
+                if self.steps >= self.tail:
+                    raise ValueError(f"step_seqs: a sequence has its {self.tail} tokens (a negative slen stands still)")
+                self.steps = max(self.steps, 0) + 1
             self.slen.add_((self.slen >= 0).to(self.slen.dtype))
         gcu.dev_rmsnorm_quantize(q_dim, ps, x, self.L[0]["n1"], eps, n, dim, stream=stream)
         for l, w in enumerate(self.L):

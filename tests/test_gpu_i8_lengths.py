@@ -40,7 +40,7 @@ def test_a_length_error_is_not_the_next_matmuls(op):
     want = oracle.gemm_int8(w, ws, x, xs)
     too_long(op)
     assert np.array_equal(gcu.gemm_int8(w, ws, x, xs), want)  # 16 rows: the GEMM kernel
-    assert np.array_equal(gcu.gemv_int8(w, ws, x[0], xs[:1]), want[0])
+    assert np.array_equal(gcu.gemv_int8(w, ws, x[0], xs[0]), want[0])
     with pytest.raises(gcu.GcuError, match="length outside"):
         gcu.check_device()
     gcu.check_device()  # reported once
@@ -56,3 +56,39 @@ def test_a_length_error_does_not_hide_a_wait(first):
     with pytest.raises(gcu.GcuError, match="wait gave up.*length outside"):
         gcu.check_device()
     gcu.check_device()
+
+
+def test_decoder_stops_at_its_tail():
+    """The steps that fit, from replays too, and then a refusal on the host or the device's report."""
+    import synth
+    import test_gpu_decode_i8 as D
+    name = next(iter(D.META["cases"]))
+    cfg, emb, dec = D.model(name, 8, 8)
+    D.prefill(cfg, dec, synth.normal(cfg["tid"] + 777, (4, cfg["dim"])))
+
+    def start():
+        dec.fork(2, 4, 3)
+        dec.set_seq_freqs(*D.tables(cfg, [4] * 2))
+        dec.sx.copy_(torch.from_numpy(synth.normal(93, (2, cfg["dim"]))))
+    start()
+    for _ in range(3):
+        dec.step_seqs()
+    with pytest.raises(ValueError, match="3 tokens"):
+        dec.step_seqs()
+    assert dec.slen.tolist() == [3, 3]
+    gcu.check_device()
+    start()
+    dec.step_seqs()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dec.step_seqs()
+    g.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    gcu.check_device()
+    assert dec.slen.tolist() == [3, 3]
+    g.replay()
+    torch.cuda.synchronize()
+    with pytest.raises(gcu.GcuError, match="length outside"):
+        gcu.check_device()

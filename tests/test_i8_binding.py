@@ -14,7 +14,7 @@ class Calls:
         self.made, self.work = [], work
 
     def __getattr__(self, name):
-        def call(*args):
+        def call(*args, **kw):
             if name.endswith("_work"):
                 return self.work
             self.made.append((name, args))
@@ -168,3 +168,38 @@ def test_a_fork_is_made_on_the_stream_that_steps_it(monkeypatch):
     for s in (None, side):
         dec.set_seq_freqs(torch.zeros((3, 64)).numpy(), torch.ones((3, 64)).numpy(), stream=s)
     assert streams.copies == [None, side]
+
+
+def test_steps_past_the_tail_are_refused(monkeypatch):
+    """Not carried out with the sequence's attention left out."""
+    import decode
+    dec = object.__new__(decode.Decoder)
+    dec.torch, dec.dev, dec.kv_bits, dec.clen = torch, "cpu", 8, 16
+    dec.cfg = dict(nl=1, n_heads=2, nkv=1, hdim=64, dim=32, mlp_dim=48, nvocab=10, q_scale=64.0, eps=1e-6, swa=[0],
+                   qk_norm=0, mlp_pre=0, mlp_pst=0, slide=0, sc_att=0.0, sc_log=0.0)
+    w = (torch.zeros((4, 32), dtype=torch.int8), torch.zeros(4))
+    dec.L = [dict({k: w for k in ("wq", "wk", "wv", "wo", "w1", "w2", "w3")}, n1=None, n2=None)]
+    dec.emb, dec.fnorm, dec.kv8 = w, None, [gcu.KvCacheI8.empty(1, 1, 16, 64, "cpu")]
+    dec.fork(3, 4, 2)
+    calls = Calls()
+    monkeypatch.setattr(decode, "gcu", calls)
+    for _ in range(2):
+        dec.step_seqs()
+    made = len(calls.made)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="2 tokens"):
+            dec.step_seqs()
+    assert len(calls.made) == made and dec.slen.tolist() == [2, 2, 2]
+    dec.slen.copy_(torch.tensor([-1, 1, 0]))  # one is done, the others go back
+    dec.step_seqs()
+    assert dec.slen.tolist() == [-1, 2, 1]
+    with pytest.raises(ValueError, match="2 tokens"):
+        dec.step_seqs()
+    dec.slen[1] = -1
+    dec.step_seqs()
+    assert dec.slen.tolist() == [-1, -1, 2]
+    monkeypatch.setattr(decode, "gcu", gcu)
+    dec.fork(1, 4, 1)
+    monkeypatch.setattr(decode, "gcu", calls)
+    dec.step_seqs()
+    assert dec.slen.tolist() == [1]
