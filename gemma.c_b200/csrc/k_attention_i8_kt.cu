@@ -10,11 +10,16 @@
 //                             unsigned digits each, the bytes of an integer as they
 //                             lie (kind::i8 with both operands MN-major: V's tile
 //                             as it lies is V^T)
-// Weights are 32-bit fixed point, W = round(2^(s + e - m) * f) for a value scale of
-// 2^e * f, 1 <= f < 2, m placed so that the row's largest weight so far is 2^24 at
-// least and below 2^32; rounding is 2^-25 of that weight.  O stays in int32 in TMEM (a digit's sum over 66,312
-// keys fits, and the plan gives a CTA fewer), so nothing is lost, and only moves
-// to fp32 registers when a row's m has to move.
+// Weights are 32-bit fixed point, W = round(2^(s + e - m) * f + d_t) for a value scale
+// of 2^e * f, 1 <= f < 2, m placed so that the row's largest weight so far is 2^25 at
+// least and below 2^32.  The offset d_t in [-1/2, 1/2) runs through the golden
+// ratio's multiples along the keys: of many small weights some gain what others lose
+// (of n equal ones a few steps are left, where plain rounding could take all of them),
+// so a sum of products is off by about sqrt(n) / 2 steps of 2^-25 of the largest weight, while
+// the sum of weights, in fp32, is of the weights as they were.
+// O stays in int32 in TMEM (a digit's sum over 66,312 keys fits, and the plan gives a
+// CTA fewer), so nothing more is lost, and only moves to fp32 registers when a row's
+// m has to move.
 //
 // Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
 // against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM:
@@ -35,7 +40,10 @@ namespace {
 
 constexpr int kSoftmax = 512, kMmaWarp = 16, kLoadWarp = 17, kThreads = 576;
 constexpr int kKeys = kKtKeys;
-constexpr float kTop = 24.0f, kSlack = 6.9f;  // log2 of the weight at m (over f), and how far it may pass
+// log2 of the weight at m (over f), and how far it may pass: what precision wants high
+// and few moves of m want low.  32 sequences that share 32768 keys, prompt of 512: 62.9 and 12.8 us
+// with 24, 63.2 and 12.9 with 25, 64.3 and 13.2 with 26, 66.5 and 13.8 with 28.
+constexpr float kTop = 25.0f, kSlack = 5.9f;
 
 // A value row's scale 2^e * f, as attn8::value_scale limits it: e (NaN for NaN, which then
 // makes the weights NaN where the key is seen; elsewhere the others are finite
@@ -351,6 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       ptx::tc_fence_before();
     };
     float ks = fetch(ksrc, 0), vs = fetch(vsrc, 0);
+    constexpr uint32_t kGolden = 2654435769u;  // 2^32 times the golden ratio's fraction
     bool ok = true;
     for (int j = 0; j < nt; ++j) {
       const float ks_next = fetch(ksrc, j + 1), vs_next = fetch(vsrc, j + 1);
@@ -443,13 +452,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       // this buffer's last reader is the product of tile j - 2
       if (j > 1) ok = wait(&pvdone[j & 1], ((j - 2) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
       uint32_t w[RQ];
+      // a weight of 0 stays 0
+      const float off = __uint_as_float((uint32_t)(kbeg + j * kKeys + key) * kGolden >> 9 | 0x3f800000u) - 1.5f;
 #pragma unroll
       for (int r = 0; r < RQ; r += 2) {
         const float2 v = make_float2(ex2(e[r]), ex2(e[r + 1]));
         const float2 t = __ffma2_rn(v, make_float2(rvs, rvs), make_float2(l[r], l[r + 1]));
         l[r] = t.x;
         l[r + 1] = t.y;
-        const float2 u = __fmul2_rn(v, make_float2(fvs, fvs));
+        const float2 u = __ffma2_rn(v, make_float2(fvs, fvs), make_float2(off, off));
         w[r] = __float2uint_rn(u.x);
         w[r + 1] = __float2uint_rn(u.y);
       }

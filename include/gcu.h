@@ -407,9 +407,12 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * sc_att (0 = off).  A sequence that sees nothing gets zeros; one with len[b]
  * < 0 is skipped, its xo row left as it is; one with len[b] > max_len is
  * skipped too and reported by gcu_check_device.  At most 8 query heads per
- * kv head.  A value scale counts as at least 2^-64 and at most 2^100; keys
- * whose value scales are more than 2^100 below another's that the row sees may
- * weigh nothing.  xo and xq do not overlap.  work: device scratch of at least
+ * kv head.  A value scale counts as at least 2^-64 and at most 2^100.  Weights
+ * times value scales are held in steps of at most 2^-25 of the row's largest
+ * such product: each is off by less than a step, up or down by its position, so
+ * that a sum over n keys is off by about sqrt(n) / 2 steps (a value row 2^-10 of the
+ * largest one's size has 15 bits under an equal weight); the sums of weights
+ * are fp32's.  xo and xq do not overlap.  work: device scratch of at least
  * gcu_attention_decode_i8_work(...) bytes, 16-byte aligned, not shared with
  * work that may run at the same time (0 bytes: may be NULL). */
 size_t gcu_attention_decode_i8_work(const gcu_kv_i8 *prefix, int plen, const gcu_kv_i8 *own, int max_len,
@@ -421,7 +424,8 @@ int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu_kv_i8 *pre
  * a chunk of ntok tokens at [spos, spos+ntok) whose keys and values are
  * already in the cache; xq [n_heads][ntok][hdim], rotated and scaled; token i
  * of head h goes to xo + i*xostr + h*hdim (xostr 0 = n_heads*hdim).  mask,
- * slide and sc_att as there; work as above. */
+ * slide and sc_att as there; work as above, and the weights too, or, in long
+ * chunks, to 2^-22 of each and 2^-35 of the row's largest. */
 size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide, float sc_att,
                                      int mask);
 int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,

@@ -1,0 +1,91 @@
+"""Precision of attention over the 8-bit cache where few keys dominate, relative to each output
+element (i8_bounds derives the tolerances)."""
+import math
+
+import numpy as np
+import pytest
+
+import i8_bounds as B
+import i8_cases as R
+from test_gpu_prefill_i8 import forced
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import gcu  # noqa: E402
+
+# steps of k_kt's weights, of the row's largest; k_tc's are two fp16 parts
+UNIT = {"few rows": 2.0 ** -25, "many rows": 2.0 ** -35}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    gcu.init(0)
+    yield
+    gcu.check_device()
+
+
+def dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def handle(c):
+    return gcu.KvCacheI8(*(dev(t) for t in c))
+
+
+def one_key_over_many(n, hd, ratio, nkv):
+    """A cache whose key 5 outweighs each of the others, all alike, by exp(ratio)."""
+    c = gcu.KvCacheI8.empty(1, nkv, n, hd)
+    c.k.fill_(127)
+    c.ks.fill_(1.0 / 127)
+    c.ks[:, :, 5] = (1.0 + ratio) / 127
+    return c, torch.full((1, nkv, hd), 1.0 / hd, device="cuda")
+
+
+@pytest.mark.parametrize("n", [1820, 3641, 16384])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_many_small_weights_of_equal_values(n, hd):
+    """Values that are all alike come out as they are: what the small weights lose in the sum of
+    products they must not keep in the sum of weights.  More heads than SMs: a CTA takes all keys."""
+    nkv = 150
+    # The exponentials are the same in both sums.  fp32 sums as in i8_bounds, and the weights' steps:
+    # less than one each, a standard deviation of a half, six times, against a largest weight of 1.
+    tol = 2.0 ** -24 * (math.sqrt(n) + 64) + 3 * math.sqrt(n) * UNIT["few rows"]
+    for ratio in (16.0, 17.4, 18.0, 20.0):
+        c, q = one_key_over_many(n, hd, ratio, nkv)
+        c.v.fill_(127)
+        c.vs.fill_(1.0 / 127)
+        xo = torch.empty_like(q)
+        gcu.dev_attention_decode_i8(xo, q, c, None, n, 1.0)
+        one = 127 * np.float64(np.float32(1.0 / 127))
+        B.check(xo, np.full((1, nkv, hd), one), np.full((1, nkv, hd), tol))
+
+
+@pytest.mark.parametrize("kernel", UNIT)
+@pytest.mark.parametrize("ratio", [10.0, 17.4])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_one_key_and_many_small_weights(kernel, ratio, hd):
+    """Random values; the heavy key's are small in half of the columns, which are the others' then."""
+    rng = np.random.default_rng(41)
+    n, ntok = 5000, 3
+    k = rng.standard_normal((1, 1, n, hd), dtype=np.float32)
+    v = rng.standard_normal((1, 1, n, hd), dtype=np.float32)
+    v[..., 2000, ::2] *= 1e-6
+    c = R.quantize_rows(k) + R.quantize_rows(v)
+    c = [c[0], c[2], c[1], c[3]]
+    xq = rng.standard_normal((2, ntok, hd), dtype=np.float32) * np.float32(1 / np.sqrt(hd))
+    c[2][0, 0, 2000] = 0
+    scores = np.einsum("htd,nd->htn", xq, c[0][0, 0].astype(np.float32) * c[2][0, 0, :, None])
+    # the heavy key: along the mean query, its scale such that it outweighs the largest by `ratio` on average
+    c[0][0, 0, 2000] = R.quantize_rows(xq.mean((0, 1)))[0]
+    base = np.einsum("htd,d->ht", xq, c[0][0, 0, 2000].astype(np.float32)).mean()
+    c[2][0, 0, 2000] = (scores.max() + ratio) / base
+    got = forced(kernel, xq, handle(c), n - ntok).reshape(ntok, 2, hd)
+    for i in range(ntok):
+        m = n - ntok + i + 1
+        for h in range(2):
+            want, tol = B.attend(xq[h, i], c[0][0, 0, :m], c[2][0, 0, :m], c[1][0, 0, :m], c[3][0, 0, :m], 1.0,
+                                 unit=UNIT[kernel], cut=kernel == "many rows")
+            B.check(got[i, h], want, tol)
