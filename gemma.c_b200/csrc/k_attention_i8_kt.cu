@@ -415,11 +415,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       bool fresh = j == 0;
       if (ptx::named_bar_or(1, kSoftmax, !ok || most > kTop + kSlack)) {
         // some row's weights would run over: move every row's m to its largest
-        // exponent so far, and take O^T's sums at the old one
+        // exponent so far, and take O^T's sums at the old one.  What runs over from a row
+        // of zeros may: its W, the largest integer then, multiplies zeros.  (fvs * rvs is
+        // 1 for a scale of 1 alone; keeping vs itself up to here cost 0.9 us of 63.4.)
+        float less = 0.0f;
+        if (fvs * rvs == 1.0f && t0 + key < kend &&
+            row_of_zeros<HD>(a.kv.v + seq * a.kv.seq_stride + hk * a.kv.kv_stride + (long)(t0 + key) * HD))
+          less = kZeros;
         if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
 #pragma unroll
         for (int r = 0; r < RQ; ++r) {
-          float top = x[r];
+          float top = x[r] - less;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           if (lane == 0) s_red[warp][r] = top;

@@ -114,11 +114,14 @@ __device__ __forceinline__ uint2 to_half4(uint32_t w) {
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[8]) { ptx::tmem_ld_32x8(at, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[16]) { ptx::tmem_ld_32x16(at, r); }
 
-// thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK]
-__device__ __forceinline__ void put_scale(float *sc, int i, float v) {
+// thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK] of a tile whose value
+// codes are at `codes`, `keys` of them in the range
+template <int HD>
+__device__ __forceinline__ void put_scale(float *sc, int i, float v, const int8_t *codes, int keys) {
   if (i < NK) {
     sc[i] = v;
   } else if (i < 2 * NK) {
+    if (v == 1.0f && i - NK < keys && row_of_zeros<HD>(codes + (i - NK) * HD)) v = kScaleZeros;
     value_scale(v, sc[i], sc[i + NK]);
   }
 }
@@ -257,7 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     if ((int)threadIdx.x < 2 * NK) {
       const int t = threadIdx.x % NK;
       const float *src = (threadIdx.x < NK ? a.kv.ks : a.kv.vs) + hk * a.kv.sc_stride;
-      put_scale(reinterpret_cast<float *>(smem + C::SC_OFF), threadIdx.x, t < n ? __ldg(src + kbeg + t) : 1.0f);
+      put_scale<HD>(reinterpret_cast<float *>(smem + C::SC_OFF), threadIdx.x, t < n ? __ldg(src + kbeg + t) : 1.0f,
+                    vh + (long)kbeg * HD, n);
     }
   }
   ptx::fence_proxy_async_smem();
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       if (j > 0) follow(j - 1);
       // while the scores are formed: the scales of the other group's next tile, which it
       // reads after this tile's decision, and the values
-      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
+      put_scale<HD>(sc + ((j + 1) & 3) * 3 * NK, tid, next, vh + (long)(kbeg + (j + 1) * NK) * HD, n - (j + 1) * NK);
       next = fetch_scale(j + 3);
       if (HD == 256) convert(j);
       ok = wait(&bars.sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;

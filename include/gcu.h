@@ -407,7 +407,8 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * sc_att (0 = off).  A sequence that sees nothing gets zeros; one with len[b]
  * < 0 is skipped, its xo row left as it is; one with len[b] > max_len is
  * skipped too and reported by gcu_check_device.  At most 8 query heads per
- * kv head.  A value scale counts as at least 2^-64 and at most 2^100.  Weights
+ * kv head.  A value scale counts as at least 2^-64 and at most 2^100, that of a
+ * row of zeros (1, as it is written) as 2^-32 in what follows.  Weights
  * times value scales are held in steps of at most 2^-25 of the row's largest
  * such product: each is off by less than a step, up or down by its position, so
  * that a sum over n keys is off by about sqrt(n) / 2 steps (a value row 2^-10 of the

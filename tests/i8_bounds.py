@@ -15,7 +15,8 @@ For one query row with weights p_t = exp(s_t) and values v_t = vs_t * vc_t, o = 
   Sums of n weights in fp32: sqrt(n) half steps of A, 64 for the sums' joining and the division.
   `unit`: the weights' products with the value scales, in steps of at most `unit` of the row's
   largest one, off by less than a step (evenly spread: a standard deviation of a half, taken six
-  times, over n keys): 3 sqrt(n) unit * max(p vs) * 127 / sum p.
+  times, over n keys): 3 sqrt(n) unit * max(p vs) * 127 / sum p.  A row of zeros, whose scale is 1,
+  counts as one of 2^-32 there.
   `cut`: matrix sums in fp32 that are cut off, 2^-23 a time for 32 times: 2^-18 of A, and of the parts."""
 import math
 
@@ -38,7 +39,7 @@ def attend(q, kc, ks, vc, vs, asc, cap=0.0, unit=0.0, cut=False):
     total = p.sum()
     size = p @ np.abs(v) / total
     tol = (2 * d + 2.0 ** -24 * (math.sqrt(n) + 64) + (2.0 ** -17 if cut else 0.0)) * size
-    tol += 3 * math.sqrt(n) * unit * np.max(p * vs) * 127 / total
+    tol += 3 * math.sqrt(n) * unit * np.max(p * np.where(vc.any(1), vs, 2.0 ** -32)) * 127 / total
     return p @ v / total, tol
 
 

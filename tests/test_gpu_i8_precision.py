@@ -89,3 +89,78 @@ def test_one_key_and_many_small_weights(kernel, ratio, hd):
             want, tol = B.attend(xq[h, i], c[0][0, 0, :m], c[2][0, 0, :m], c[1][0, 0, :m], c[3][0, 0, :m], 1.0,
                                  unit=UNIT[kernel], cut=kernel == "many rows")
             B.check(got[i, h], want, tol)
+
+
+def with_zero_rows(rng, nkv, n, hd, size):
+    """Value rows of a size, one in six of zeros as the writer leaves them (scale 1), 200 in a row too."""
+    v = rng.standard_normal((1, nkv, n, hd), dtype=np.float32) * np.float32(size)
+    v[0, :, rng.random(n) < 1 / 6] = 0
+    v[0, :, 300:500] = 0
+    k, ks = R.quantize_rows(rng.standard_normal((1, nkv, n, hd), dtype=np.float32))
+    v, vs = R.quantize_rows(v)
+    assert np.all(vs[0, :, 300:500] == 1)
+    return k, v, ks, vs
+
+
+SIZES = [1e-6, 1e-3, 0.01, 1.0, 1e4, 1e24]
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kernel", UNIT)
+def test_prefill_rows_of_zeros(kernel, hd, size):
+    """They weigh in the sum of weights and leave the other rows their precision."""
+    rng = np.random.default_rng(51)
+    n, ntok = 900, 130
+    c = with_zero_rows(rng, 1, n, hd, size)
+    xq = rng.standard_normal((2, ntok, hd), dtype=np.float32) * np.float32(1.5 / np.sqrt(hd))
+    got = forced(kernel, xq, handle(c), n - ntok).reshape(ntok, 2, hd)
+    for i in range(0, ntok, 7):
+        m = n - ntok + i + 1
+        for h in range(2):
+            row = c[0][0, 0, :m], c[2][0, 0, :m], c[1][0, 0, :m], c[3][0, 0, :m]
+            want, tol = B.attend(xq[h, i], *row, 1.0, unit=UNIT[kernel], cut=kernel == "many rows")
+            B.check(got[i, h], want, tol)
+
+
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("hd", [64, 256])
+def test_decode_rows_of_zeros(size, shared, hd):
+    """In the sequences' own caches and in a shared prefix; the heaviest key of one head among them."""
+    rng = np.random.default_rng(52)
+    nseq, nkv, G, n = 3, 2, 2, 1100
+    pre = with_zero_rows(rng, nkv, n, hd, size)
+    own = [np.repeat(t, nseq, 0) for t in with_zero_rows(rng, nkv, 600, hd, size)]
+    pre[2][0, 1, 400] *= 8
+    xq = rng.standard_normal((nseq, nkv * G, hd), dtype=np.float32) * np.float32(1.5)
+    lens = [600, 450, 290]
+    xo = torch.empty(xq.shape, device="cuda")
+    gcu.dev_attention_decode_i8(xo, dev(xq), handle(own), dev(np.asarray(lens, np.int32)), 600, hd ** -0.5,
+                                prefix=handle(pre) if shared else None, plen=n if shared else 0)
+    got = xo.cpu().numpy()
+    for b in range(nseq):
+        for h in range(nkv * G):
+            j = h // G
+            row = [own[t][b, j, :lens[b]] for t in (0, 2, 1, 3)]
+            if shared:
+                row = [np.concatenate([pre[t][0, j], r]) for t, r in zip((0, 2, 1, 3), row)]
+            want, tol = B.attend(xq[b, h], *row, hd ** -0.5, unit=UNIT["few rows"])
+            B.check(got[b, h], want, tol)
+
+
+def test_only_rows_of_zeros():
+    """Zeros come out, also when a chunk sees nothing else."""
+    hd = 128
+    c = gcu.KvCacheI8.empty(2, 1, 4000, hd)
+    c.k.fill_(3)
+    q, xo = torch.ones((2, 4, hd), device="cuda"), torch.full((2, 4, hd), 9.0, device="cuda")
+    gcu.dev_attention_decode_i8(xo, q, c, None, 4000, 1.0)
+    assert not xo.any()
+    c.v[0, 0, 3999] = 127  # one row of 127 among 4000 equal weights
+    gcu.dev_attention_decode_i8(xo, q, c, None, 4000, 1.0)
+    B.check(xo[0], np.full((4, hd), 127 / 4000), np.full((4, hd), 127 / 4000 * 2.0 ** -24 * (math.sqrt(4000) + 64)))
+    assert not xo[1].any()
+    rows, xq = torch.full((30, 4 * hd), 9.0, device="cuda"), torch.ones((4, 30, hd), device="cuda")
+    gcu.dev_attention_prefill_i8(rows, xq, c.seq(1), 3900)
+    assert not rows.any()
