@@ -40,21 +40,23 @@ namespace {
 
 constexpr int kSoftmax = 512, kMmaWarp = 16, kLoadWarp = 17, kThreads = 576;
 constexpr int kKeys = kKtKeys;
-// log2 of the weight at m (over f), and how far it may pass: what precision wants high
-// and few moves of m want low.  32 sequences that share 32768 keys, prompt of 512: 62.9 and 12.8 us
+// log2 of W at m (over f), and by how much an exponent may pass m: what precision wants
+// high and few moves of m want low.  It multiplies f, so that the exponent is x - m for
+// scores of any size.  32 sequences that share 32768 keys, prompt of 512: 62.9 and 12.8 us
 // with 24, 63.2 and 12.9 with 25, 64.3 and 13.2 with 26, 66.5 and 13.8 with 28.
-constexpr float kTop = 25.0f, kSlack = 5.9f;
+constexpr int kTop = 25;
+constexpr float kSlack = 5.9f, kOne = 1 << kTop;
 
 // A value row's scale 2^e * f, as attn8::value_scale limits it: e (NaN for NaN, which then
 // makes the weights NaN where the key is seen; elsewhere the others are finite
-// against the zero weight), f and 2^-e.  Exact, and a quarter of the instructions
+// against the zero weight), f * 2^kTop and 2^-e.  Exact, and a quarter of the instructions
 // that a logarithm and a reciprocal take (32 sequences that share 32768 keys 63.0
 // -> 60.9 us).
 __device__ __forceinline__ void split_scale(float v, float &e, float &f, float &inv) {
   v = v < kScaleLo ? kScaleLo : v > kScaleHi ? kScaleHi : v;
   const int b = __float_as_int(v), x = min(b & 0x7f800000, 0x71800000);  // NaN as 2^100
   e = v == v ? (float)((x >> 23) - 127) : v;
-  f = __int_as_float((b & 0x007fffff) | 0x3f800000);
+  f = __int_as_float((b & 0x007fffff) | (0x3f800000 + (kTop << 23)));
   inv = __int_as_float(0x7f000000 - x);
 }
 
@@ -323,9 +325,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       return t < n ? __ldg(src + kbeg + t) : 1.0f;
     };
     const float to_unit = CAP ? 1.0f / a.sc_att : kLog2e, unit = a.sc_att * kLog2e;
-    // up: what takes an exponent to that of the weight, kTop - m; while m is -inf,
+    // up: what takes an exponent to that of the weight, -m; while m is -inf,
     // whatever is seen at all is too large
-    constexpr float kUnseen = 1e30f;
+    constexpr float kUnseen = 3.4e38f;
     float rf[RQ], l[RQ], up[RQ];
 #pragma unroll
     for (int r = 0; r < RQ; ++r) {
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
     for (int r = 0; r < C::OR; ++r) acc[r] = 0.0f;
     const uint32_t olane = lanes + C::O_COL + oblock * C::NP + 4 * orow;
-    // add O^T's digit sums (complete) to the column's sums, then scale them
+    // add O^T's digit sums (complete), back at the weights' size, to the column's sums
     auto flush = [&]() {
       ptx::tc_fence_after();
 #pragma unroll
@@ -351,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float v = (float)(int)d[4 * e + 3] * 16777216.0f + (float)(int)d[4 * e + 2] * 65536.0f;
-          v += (float)(int)d[4 * e + 1] * 256.0f + (float)(int)d[4 * e];
+          float v = (float)(int)d[4 * e + 3] * (16777216.0f / kOne) + (float)(int)d[4 * e + 2] * (65536.0f / kOne);
+          v += (float)(int)d[4 * e + 1] * (256.0f / kOne) + (float)(int)d[4 * e] * (1.0f / kOne);
           acc[r + e] += v;
         }
       }
@@ -413,13 +415,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
 #pragma unroll
       for (int r = 1; r < RQ; ++r) most = fmaxf(most, e[r]);
       bool fresh = j == 0;
-      if (ptx::named_bar_or(1, kSoftmax, !ok || most > kTop + kSlack)) {
+      if (ptx::named_bar_or(1, kSoftmax, !ok || most > kSlack)) {
         // some row's weights would run over: move every row's m to its largest
         // exponent so far, and take O^T's sums at the old one.  What runs over from a row
         // of zeros may: its W, the largest integer then, multiplies zeros.  (fvs * rvs is
-        // 1 for a scale of 1 alone; keeping vs itself up to here cost 0.9 us of 63.4.)
+        // kOne for a scale of 1 alone; keeping vs itself up to here cost 0.9 us of 63.4.)
         float less = 0.0f;
-        if (fvs * rvs == 1.0f && t0 + key < kend &&
+        if (fvs * rvs == kOne && t0 + key < kend &&
             row_of_zeros<HD>(a.kv.v + seq * a.kv.seq_stride + hk * a.kv.kv_stride + (long)(t0 + key) * HD))
           less = kZeros;
         if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         for (int r = 0; r < RQ; ++r) {
           l[r] *= s_f[r0 + r];
           const float m = s_m[r0 + r];
-          up[r] = m == -INFINITY ? kUnseen : kTop - m;
+          up[r] = m == -INFINITY ? kUnseen : -m;
         }
         exponents();
         fresh = true;
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       const float sum = (s_red[q][r % RQ] + s_red[q + 1][r % RQ]) + (s_red[q + 2][r % RQ] + s_red[q + 3][r % RQ]);
       const float m = s_m[r];
       s_sum[r] = sum;
-      if (a.slots > 1 && at >= 0) a.stat[slot * rows_all + at] = make_float2(m == -INFINITY ? m : m - kTop, sum);
+      if (a.slots > 1 && at >= 0) a.stat[slot * rows_all + at] = make_float2(m, sum);
     }
     if (nt > 0) {
       ok = wait(&pvdone[(nt - 1) & 1], ((nt - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;

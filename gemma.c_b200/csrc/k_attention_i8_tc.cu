@@ -55,8 +55,9 @@ constexpr int kRegsSoftmax = 112, kRegsOther = 32;  // 4 * 112 + 32 = 5 * 96
 constexpr int kRows = 128;
 constexpr int NK = 64;     // keys per tile
 constexpr int kFlush = 4;  // tiles per T
-// Weights run up to 2^kTop at the reference point and may pass it by 2^kSlack:
-// 2^15 stays below fp16's 65504.
+// m is placed kTop below the largest exponent so far, so that weights run up to 2^10 and
+// may pass that by 2^kSlack: 2^15 stays below fp16's 65504.  Beside scores whose own
+// spacing is more than that, m is rounded up, at most to the largest exponent.
 constexpr float kTop = 10.0f, kSlack = 5.0f;
 
 template <int HD>
@@ -522,9 +523,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       }
       top = fmaxf(top, top2);
       smax[(grp * 2 + half) * kRows + row] = top;
-      const bool moved = ptx::named_bar_or(1 + grp, kGroup, top > m + kSlack || (m == -INFINITY && top > m) || !ok);
+      const bool moved = ptx::named_bar_or(1 + grp, kGroup, top > __fadd_rd(m, kTop + kSlack) || !ok);
       if (moved && ptx::named_bar_or(1 + grp, kGroup, !ok)) break;
-      const float to = moved ? fmaxf(m, fmaxf(top, smax[(grp * 2 + (half ^ 1)) * kRows + row])) : m;
+      const float to =
+          moved ? fmaxf(m, __fsub_ru(fmaxf(top, smax[(grp * 2 + (half ^ 1)) * kRows + row]), kTop)) : m;
       const bool fresh = moved || j % kFlush == 0;
       if (half == 0) refs[row] = to;
       if (tid == 0) freshp[j & 1] = fresh;
@@ -532,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       const float f = to == m ? 1.0f : ex2(m - to);  // m = -inf: 0
       l *= f;
       m = to;
-      const float ref = m == -INFINITY ? 0.0f : m - kTop;
+      const float ref = m == -INFINITY ? 0.0f : m;
       uint32_t ph[C::HALF / 2], pl[C::HALF / 2];
       float2 lt = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
           make_float4(acc[c] * d, acc[c + 1] * d, acc[c + 2] * d, acc[c + 3] * d);
     if (live && ok && a.slots > 1 && quarter == 0 && (!alone || split == 0))
       a.stat[((size_t)(a.slot0 + split) * a.ni + rows.i(row)) * a.n_heads + h0 + rows.g(row)] =
-          alone ? make_float2(0.0f, kAlone) : make_float2(m == -INFINITY ? m : m - kTop, l);
+          alone ? make_float2(0.0f, kAlone) : make_float2(m, l);
     ptx::named_bar_sync(3, kSoftmax);
     const bool none = alone ? split > 0 : nt == 0;  // (-inf, 0) says that there is nothing to add
     for (int r = warp; r < nrows && ok && !none; r += kSoftmax / 32) {

@@ -413,7 +413,8 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * such product: each is off by less than a step, up or down by its position, so
  * that a sum over n keys is off by about sqrt(n) / 2 steps (a value row 2^-10 of the
  * largest one's size has 15 bits under an equal weight); the sums of weights
- * are fp32's.  xo and xq do not overlap.  work: device scratch of at least
+ * are fp32's, without the keys whose product is below 2^-126 of the largest.
+ * xo and xq do not overlap.  work: device scratch of at least
  * gcu_attention_decode_i8_work(...) bytes, 16-byte aligned, not shared with
  * work that may run at the same time (0 bytes: may be NULL). */
 size_t gcu_attention_decode_i8_work(const gcu_kv_i8 *prefix, int plen, const gcu_kv_i8 *own, int max_len,

@@ -164,3 +164,35 @@ def test_only_rows_of_zeros():
     rows, xq = torch.full((30, 4 * hd), 9.0, device="cuda"), torch.ones((4, 30, hd), device="cuda")
     gcu.dev_attention_prefill_i8(rows, xq, c.seq(1), 3900)
     assert not rows.any()
+
+
+SCORES = [1e3, 3e5, 4e7, 3e8, 6e8, 1e10, 1e26, -1e3, -3e8, -6e8, -1e10, -1e20, -1e29]
+
+
+@pytest.mark.parametrize("score", SCORES)
+@pytest.mark.parametrize("hd", [64, 256])
+def test_scores_of_any_size(score, hd):
+    """One key wins by half of its score (3e8: past 2^28 in log2 units, whose neighbours are 32
+    apart): its values come out.  Two such keys, alike: their mean."""
+    rng = np.random.default_rng(61)
+    n, at, twin = 700, 513, 77
+    v, vs = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32))
+    vs[0, 0, twin] = vs[0, 0, at]
+    k = np.full((1, 1, n, hd), 127 if score > 0 else -127, np.int8)
+    ks = np.full((1, 1, n), abs(score) / 127 * (0.5 if score > 0 else 2), np.float32)
+    row = lambda t: v[0, 0, t] * np.float64(vs[0, 0, t])
+    xq = np.full((1, 2, hd), 1 / hd, np.float32)
+    for winners in ((at,), (twin, at)):
+        ks[0, 0, list(winners)] = abs(score) / 127
+        want = np.mean([row(t) for t in winners], 0)
+        size = np.mean([np.abs(row(t)) for t in winners], 0)
+        # a step of the weight or, of two fp16 parts, its 2^-22, the digits' sums, the division
+        tol = np.broadcast_to(size * 2.0 ** -21, (2, hd))
+        kv = handle((k, v, ks, vs))
+        xo = torch.empty((1, 2, hd), device="cuda")
+        gcu.dev_attention_decode_i8(xo, dev(xq), kv, None, n, 1.0)
+        B.check(xo[0], np.broadcast_to(want, (2, hd)), tol)
+        for kernel in UNIT:
+            got = forced(kernel, np.repeat(xq.transpose(1, 0, 2), 90, 1), kv, n - 90).reshape(90, 2, hd)
+            for i in (-1, -8):
+                B.check(got[i], np.broadcast_to(want, (2, hd)), tol)
