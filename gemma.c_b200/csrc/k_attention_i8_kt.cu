@@ -380,13 +380,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
         ptx::tmem_ld_wait();
 #pragma unroll
         for (int r = 0; r < RQ; r += 2) {
-          const float2 y = __fmul2_rn(high_digit(s2 + r, low_digits(s1 + r, s0 + r)), make_float2(ks, ks));
+          // q . kc first: digits times a scale of 1e28 would run over
+          const float2 y = __fmul2_rn(high_digit(s2 + r, low_digits(s1 + r, s0 + r)), make_float2(rf[r], rf[r + 1]));
           float2 e;
           if constexpr (CAP) {
-            e = __fmul2_rn(y, make_float2(rf[r], rf[r + 1]));
+            e = __fmul2_rn(y, make_float2(ks, ks));
             e = __ffma2_rn(make_float2(tanh_fast(e.x), tanh_fast(e.y)), make_float2(unit, unit), make_float2(evs, evs));
           } else {
-            e = __ffma2_rn(y, make_float2(rf[r], rf[r + 1]), make_float2(evs, evs));
+            e = __ffma2_rn(y, make_float2(ks, ks), make_float2(evs, evs));
           }
           x[r] = e.x;
           x[r + 1] = e.y;

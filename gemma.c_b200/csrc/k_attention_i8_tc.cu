@@ -491,14 +491,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
         for (int e = 0; e < C::RB; e += 4) {
           const float4 k = *reinterpret_cast<const float4 *>(ks + c + e);
           const float4 v = *reinterpret_cast<const float4 *>(lvs + c + e);
-          float2 y = __fmul2_rn(high_digit(s2 + e, make_float2(x[c + e], x[c + e + 1])), make_float2(k.x, k.y));
-          float2 z = __fmul2_rn(high_digit(s2 + e + 2, make_float2(x[c + e + 2], x[c + e + 3])), make_float2(k.z, k.w));
+          // q . kc first: digits times a scale of 1e28 would run over
+          const float2 f = CAP ? make_float2(rf_nat, rf_nat) : make_float2(rf, rf);
+          float2 y = __fmul2_rn(high_digit(s2 + e, make_float2(x[c + e], x[c + e + 1])), f);
+          float2 z = __fmul2_rn(high_digit(s2 + e + 2, make_float2(x[c + e + 2], x[c + e + 3])), f);
           if constexpr (CAP) {
-            y = make_float2(tanh_fast(y.x * rf_nat), tanh_fast(y.y * rf_nat));
-            z = make_float2(tanh_fast(z.x * rf_nat), tanh_fast(z.y * rf_nat));
+            y = __ffma2_rn(make_float2(tanh_fast(y.x * k.x), tanh_fast(y.y * k.y)), make_float2(rf, rf), make_float2(v.x, v.y));
+            z = __ffma2_rn(make_float2(tanh_fast(z.x * k.z), tanh_fast(z.y * k.w)), make_float2(rf, rf), make_float2(v.z, v.w));
+          } else {
+            y = __ffma2_rn(y, make_float2(k.x, k.y), make_float2(v.x, v.y));
+            z = __ffma2_rn(z, make_float2(k.z, k.w), make_float2(v.z, v.w));
           }
-          y = __ffma2_rn(y, make_float2(rf, rf), make_float2(v.x, v.y));
-          z = __ffma2_rn(z, make_float2(rf, rf), make_float2(v.z, v.w));
           x[c + e] = y.x;
           x[c + e + 1] = y.y;
           x[c + e + 2] = z.x;

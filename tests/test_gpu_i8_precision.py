@@ -166,7 +166,8 @@ def test_only_rows_of_zeros():
     assert not rows.any()
 
 
-SCORES = [1e3, 3e5, 4e7, 3e8, 6e8, 1e10, 1e26, -1e3, -3e8, -6e8, -1e10, -1e20, -1e29]
+SCORES = [1e3, 3e5, 4e7, 3e8, 6e8, 1e10, 1e26, -1e3, -3e8, -6e8, -1e10, -1e20, -1e29,
+          1e32, -1e32]
 
 
 @pytest.mark.parametrize("score", SCORES)
