@@ -24,6 +24,7 @@ namespace attn8 {
 
 constexpr int kMaxGroup = 8;        // query heads per kv head
 constexpr float kQMax = 4194000.0f;  // below 2^22: q * inv + 1.5 * 2^23 holds it as an integer
+constexpr float kQLeast = 1e-31f;    // rows of smaller elements are scaled as if by this: 1 / scale stays finite
 constexpr float kLog2e = 1.4426950408889634f;
 
 enum Mode {
@@ -152,13 +153,13 @@ __device__ __forceinline__ void load_floats(float (&v)[E], const float *src, boo
     v[1] = f.y;
   }
 }
-// N rows of a warp: their largest |elements| (NaN if there is one) and the digits of
-// this lane's elements, packed bytes of d0, d1, d2
+// N rows of a warp: their largest |elements| (NaN if there is one; kQLeast at least) and
+// the digits of this lane's elements, packed bytes of d0, d1, d2
 template <int E, int N>
 __device__ __forceinline__ void row_digits(const float (&v)[N][E], uint32_t (&w)[N][3][(E + 3) / 4], float (&amax)[N]) {
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    amax[n] = 0.0f;
+    amax[n] = kQLeast;
 #pragma unroll
     for (int e = 0; e < E; ++e) amax[n] = max_nan(amax[n], fabsf(v[n][e]));
   }
@@ -168,7 +169,7 @@ __device__ __forceinline__ void row_digits(const float (&v)[N][E], uint32_t (&w)
     for (int n = 0; n < N; ++n) amax[n] = max_nan(amax[n], __shfl_xor_sync(0xffffffffu, amax[n], o));
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    const float inv = amax[n] > 0.0f ? kQMax / amax[n] : 0.0f;
+    const float inv = kQMax / amax[n];
     // n + 0x808080 has the digits, each plus 128, as its bytes
     uint32_t u[(E + 3) / 4 * 4] = {};
 #pragma unroll

@@ -197,3 +197,22 @@ def test_scores_of_any_size(score, hd):
             got = forced(kernel, np.repeat(xq.transpose(1, 0, 2), 90, 1), kv, n - 90).reshape(90, 2, hd)
             for i in (-1, -8):
                 B.check(got[i], np.broadcast_to(want, (2, hd)), tol)
+
+
+@pytest.mark.parametrize("kernel", UNIT)
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("key,query", [(1e30, 1e-30), (1e33, 1e-33), (1e-30, 1e30)])
+def test_large_keys_and_small_queries(kernel, cap, key, query):
+    """And the other way round: their scores are ordinary ones."""
+    rng = np.random.default_rng(71)
+    n, ntok, hd = 300, 40, 256
+    k, ks = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32) * np.float32(key))
+    v, vs = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32))
+    xq = (rng.standard_normal((2, ntok, hd)) * (query / 16)).astype(np.float32)
+    got = forced(kernel, xq, handle((k, v, ks, vs)), n - ntok, cap=cap).reshape(ntok, 2, hd)
+    for i in range(0, ntok, 5):
+        m = n - ntok + i + 1
+        for h in range(2):
+            want, tol = B.attend(xq[h, i], k[0, 0, :m], ks[0, 0, :m], v[0, 0, :m], vs[0, 0, :m], 1.0, cap,
+                                 unit=UNIT[kernel], cut=kernel == "many rows")
+            B.check(got[i, h], want, tol)
