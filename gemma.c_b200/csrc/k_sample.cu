@@ -102,7 +102,7 @@ struct Row {
   double max_d, scale;  // scale: log2(e) / T
   float least;          // logits below it weigh nothing
   double one;
-  float bin_scale;
+  float half_max, bin_scale;
 
   // one * 2^((v - max) * log2(e) / T), rounded to a whole number, to 2^-39 of itself;
   // the whole warp calls it.  t = k/32 + r; 2^r by its Taylor series to r^4 (|r| <=
@@ -124,16 +124,17 @@ struct Row {
     const u64 f = (u64)__double_as_longlong(fma(fma(w * r, p, w), s, 4503599627370496.0)) & 0xfffffffffffffull;
     return v < least ? 0 : f;
   }
-  // steps of 1/128 below the largest; monotone in v
+  // steps of 1/128 below the largest; monotone in v.  Half the distance, which fits where
+  // the distance of two logits past 1.7e38 does not, times twice the scale.
   __device__ __forceinline__ int bin(float v) const {
-    return min((int)((max - v) * bin_scale), kBins - 1);
+    return min((int)(__fmaf_rn(-0.5f, v, half_max) * bin_scale), kBins - 1);
   }
   // About the logit `off` bins above the start of a bin: with 0.01 above all of the
   // bin, with -1.01 below all of it (the last has no end).  bin()'s roundings are
   // 2^-22 of 2048 bins at most, and those of the logits' own size are allowed for.
   __device__ __forceinline__ float edge(int bin, double off) const {
     if (off < 0.0 && bin == kBins - 1) return -INFINITY;
-    const double x = max_d - (bin - off) / (double)bin_scale;
+    const double x = max_d - (bin - off) * 2.0 / (double)bin_scale;
     const double slack = (fabs(max_d) + fabs(x)) * 2.4e-7;
     return (float)(off < 0.0 ? x - slack : x + slack);
   }
@@ -627,7 +628,8 @@ __global__ void __launch_bounds__(kThreads) k_sample(const SampleArgs a) {
   r.scale = 1.4426950408889634 / (double)a.temperature;
   r.max_d = (double)r.max;
   r.least = fmaxf((float)(r.max_d - 63.0 / r.scale), -3.4028235e38f);  // -inf lies below it
-  r.bin_scale = fminf(kBinsPerNat / a.temperature, 3.4028235e38f);     // 0 times it is 0
+  r.half_max = 0.5f * r.max;
+  r.bin_scale = fminf(2.0f * kBinsPerNat / a.temperature, 3.4028235e38f);  // 0 times it is 0
   r.one = a.one;
   Cut c;
   const bool by_k = a.top_k > 0 && a.top_k < a.n, by_p = a.top_p < 1.0f;
