@@ -8,10 +8,14 @@
 //
 // The codes stay integers up to the matrix products: a query row is scaled to
 // 23-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
-// products with int8 keys are int8 x int8 sums, exact in int32, and q is rounded by
-// 2^-23 of the row's largest element at most -- twice what fp32 rounds that element
-// by, and three instructions an element, as the integer comes out of a floating
-// point addition.
+// products with int8 keys are int8 x int8 sums, exact in int32.  That is fixed point: every
+// element is rounded by up to 2^-23 of the row's largest, twice what fp32 rounds that
+// one by, and one 2^-10 of its size keeps 13 bits where fp32 keeps 24.  A score moves
+// by up to 2^-23 max|q| * asc * ks * sum |kc|.  The keys' own codes are rounded by 2^-8 of
+// their row's largest, far more than that.  A fourth digit would cost a third more
+// product and 64 TMEM columns, which k_tc has not left at hdim 256 (192 of scores, 256 of
+// sums, 64 of weights); three also cost three instructions an element, as the integer
+// comes out of a floating point addition.
 //
 // Rows: the query heads of one kv head share its keys, so a row is (i, g):
 // token or sequence i, head h0 + g of the group, row index i * G + g.

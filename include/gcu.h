@@ -404,14 +404,17 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * cache, of these plen + len[b] positions the last `slide` when slide > 0.
  * len: device int32 [nseq], 0 <= len[b] <= max_len <= clen, or NULL when
  * every sequence has max_len.  Scores are scaled by asc, then soft-capped by
- * sc_att (0 = off).  A sequence that sees nothing gets zeros; one with len[b]
- * < 0 is skipped, its xo row left as it is; one with len[b] > max_len is
- * skipped too and reported by gcu_check_device.  At most 8 query heads per
- * kv head.  A value scale counts as at least 2^-64 and at most 2^100, that of a
- * row of zeros (1, as it is written) as 2^-32 in what follows.  Weights
- * times value scales are held in steps of at most 2^-25 of the row's largest
- * such product: each is off by less than a step, up or down by its position, so
- * that a sum over n keys is off by about sqrt(n) / 2 steps (a value row 2^-10 of the
+ * sc_att (0 = off; tanh to 2^-22 of itself).  A sequence that sees nothing gets
+ * zeros; one with len[b] < 0 is skipped, its xo row left as it is; one with
+ * len[b] > max_len is skipped too and reported by gcu_check_device.  At most 8
+ * query heads per kv head.
+ * Precision.  Queries are held in fixed point, each element to 2^-23 of its
+ * row's largest (one 2^-10 of that size has 13 bits); rows of less than 1e-31 as
+ * if that were their largest.  A value scale counts as at least 2^-64 and at most
+ * 2^100, that of a row of zeros (1, as it is written) as 2^-32.  Weights times
+ * value scales are held in steps of at most 2^-25 of the row's largest such
+ * product, each off by less than a step, up or down by its position, so that a
+ * sum over n keys is off by about sqrt(n) / 2 steps (a value row 2^-10 of the
  * largest one's size has 15 bits under an equal weight); the sums of weights
  * are fp32's, without the keys whose product is below 2^-126 of the largest.
  * xo and xq do not overlap.  work: device scratch of at least
@@ -426,8 +429,8 @@ int gcu_dev_attention_decode_i8(float *xo, const float *xq, const gcu_kv_i8 *pre
  * a chunk of ntok tokens at [spos, spos+ntok) whose keys and values are
  * already in the cache; xq [n_heads][ntok][hdim], rotated and scaled; token i
  * of head h goes to xo + i*xostr + h*hdim (xostr 0 = n_heads*hdim).  mask,
- * slide and sc_att as there; work as above, and the weights too, or, in long
- * chunks, to 2^-22 of each and 2^-35 of the row's largest. */
+ * slide and sc_att as there; work and precision as above, but for the weights
+ * of long chunks, which are held to 2^-22 of each and 2^-35 of the row's largest. */
 size_t gcu_attention_prefill_i8_work(const gcu_kv_i8 *kv, int n_heads, int spos, int ntok, int slide, float sc_att,
                                      int mask);
 int gcu_dev_attention_prefill_i8(float *xo, int xostr, const float *xq, const gcu_kv_i8 *kv, int n_heads,

@@ -216,3 +216,25 @@ def test_large_keys_and_small_queries(kernel, cap, key, query):
             want, tol = B.attend(xq[h, i], k[0, 0, :m], ks[0, 0, :m], v[0, 0, :m], vs[0, 0, :m], 1.0, cap,
                                  unit=UNIT[kernel], cut=kernel == "many rows")
             B.check(got[i, h], want, tol)
+
+
+@pytest.mark.parametrize("kernel", UNIT)
+@pytest.mark.parametrize("outlier", [27.0, 270.0, 2700.0])
+def test_outlier_query_channels(kernel, outlier):
+    """A query channel far above the others over a key channel that is small: the others' bits are
+    what the largest leaves them, as stated."""
+    rng = np.random.default_rng(81)
+    n, ntok, hd = 600, 24, 128
+    k = rng.standard_normal((1, 1, n, hd), dtype=np.float32)
+    k[..., 9] *= np.float32(1 / outlier)
+    k, ks = R.quantize_rows(k)
+    v, vs = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32))
+    xq = rng.standard_normal((2, ntok, hd), dtype=np.float32) * np.float32(1.5 / np.sqrt(hd))
+    xq[..., 9] *= np.float32(outlier)
+    got = forced(kernel, xq, handle((k, v, ks, vs)), n - ntok).reshape(ntok, 2, hd)
+    for i in range(ntok):
+        m = n - ntok + i + 1
+        for h in range(2):
+            want, tol = B.attend(xq[h, i], k[0, 0, :m], ks[0, 0, :m], v[0, 0, :m], vs[0, 0, :m], 1.0,
+                                 unit=UNIT[kernel], cut=kernel == "many rows")
+            B.check(got[i, h], want, tol)
