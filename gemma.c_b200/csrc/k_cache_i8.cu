@@ -271,6 +271,7 @@ int launch_write(const WriteArgs &a, cudaStream_t st) {
   if (overlap(a.xq, (long)a.rows * a.n_heads * a.kv.hdim * 4, a.qkv,
               ((a.rows - 1) * a.ld + (long)(a.n_heads + 2 * a.kv.nkv) * a.kv.hdim) * 4))
     return set_error("qkv_norm_rope_cache_i8: xq and qkv overlap");
+  if (a.kv.k == a.kv.v || a.kv.ks == a.kv.vs) return set_error("qkv_norm_rope_cache_i8: the cache's k and v overlap");
   constexpr int kWarps = kWriteThreads / 32;
   const int y = (groups(a.n_heads) + 2 * groups(a.kv.nkv) + kWarps - 1) / kWarps;
   if (y > 65535) return set_error("qkv_norm_rope_cache_i8: %d query and %d kv heads", a.n_heads, a.kv.nkv);

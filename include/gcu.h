@@ -377,7 +377,8 @@ typedef struct {
  * QK-norm weights [hdim] or NULL; freqs [ntok][hdim] (cos, sin interleaved).
  * The norm's sum of squares is taken in 64 bits and every fp32 step after it
  * is rounded by itself (no fused multiply-adds), so the codes follow from the
- * formulas alone.  16-byte aligned qkv, xq and freqs; xq and qkv apart. */
+ * formulas alone.  16-byte aligned qkv, xq and freqs; xq and qkv apart, and the
+ * cache's k and v. */
 int gcu_dev_qkv_norm_rope_cache_i8(float *xq, const float *qkv, long ld, const gcu_kv_i8 *kv,
                                    const float *nq, const float *nk, float eps, const float *freqs,
                                    float q_scale, int n_heads, int spos, int ntok, void *stream);

@@ -203,3 +203,20 @@ def test_steps_past_the_tail_are_refused(monkeypatch):
     monkeypatch.setattr(decode, "gcu", calls)
     dec.step_seqs()
     assert dec.slen.tolist() == [1]
+
+
+def test_writes_to_one_buffer_for_keys_and_values():
+    """A cache that is only read may have them in one; written, each would overwrite the other."""
+    import ctypes
+    from test_i8_host import P, kv_struct, refused
+    kv = kv_struct()
+    assert kv.k == kv.v
+    lib, ref = gcu.lib(), ctypes.byref
+    other = torch.zeros(4096, dtype=torch.int8)
+    at = (other.data_ptr() + 15) // 16 * 16
+    for over in ({}, dict(v=at), dict(vs=at)):
+        c = kv_struct(**over)
+        q = torch.zeros(2048)
+        qkv = (q.data_ptr() + 15) // 16 * 16
+        refused(lib.gcu_dev_qkv_norm_rope_cache_i8(P, qkv, 512, ref(c), None, None, 1e-6, P, 1.0, 4, 0, 1, None), "k and v")
+        refused(lib.gcu_dev_qkv_norm_rope_cache_i8_seqs(P, qkv, 512, ref(c), P, None, None, 1e-6, P, 1.0, 4, None), "k and v")
