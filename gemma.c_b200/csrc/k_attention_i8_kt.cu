@@ -22,10 +22,11 @@
 // m has to move.
 //
 // Per 128 keys at hdim 256 this is 16 products of N <= 128 (about 1100 cycles)
-// against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM:
-// 16 rows are bound by HBM (32768 keys of 8 heads: 28.9 us for 136 MB, 4.7 TB/s), 32
-// rows by the softmax, about 1900 cycles a tile (32 sequences that share
-// 32768 keys: 60 us).  A CTA costs 5 us besides its tiles.
+// against 64 KB of codes, which at the card's copy rate are 2800 cycles of one SM.  A CTA
+// costs 5.4 us besides its tiles and, with 16 rows, 1.0 us a tile whose codes are in L2;
+// from HBM 148 CTAs of 32 tiles take 50 us for 310 MB.  32768 keys of 8 heads: 29.6 us for
+// 136 MB, the merge of 18 chunks 3.6 of them.  32 rows are bound by the softmax, 1.5 us a
+// tile: 32 sequences that share 32768 keys 64 us, 52 without keys of their own.
 //
 // Warps 0-15: softmax, thread = (key, a quarter of the rows); 16: products; 17: loads.
 #include "attention_i8.cuh"

@@ -2,18 +2,18 @@
 // many rows.
 //
 // A CTA takes 128 query rows of one kv head (token i, head of the group: the heads
-// that share keys fill the rows) and one chunk of the key range, and walks it in tiles of NK keys, keeping the running maximum and sum
-// of the softmax:
+// that share keys fill the rows) and one chunk of the key range, and walks it in tiles
+// of NK keys, keeping the running maximum and sum of the softmax:
 //   S   three tcgen05.mma kind::i8 products per tile, the query's three digits
 //       against the codes as TMA brings them: exact int32 sums in TMEM, put
 //       together in fp32 (65536 s2 + 256 s1 + s0).  No conversion of K.
 //   P   w = 2^(s + log2 vs[t] - m), m a reference point of the row near the
 //       largest exponent so far, split into two fp16 parts in TMEM: w to 2^-22,
-//       and to 2^-39 of the row's largest (the weights are placed just below
-//       fp16's largest number).
+//       and to 2^-35 of the row's largest (that is 2^10 or more, just below fp16's
+//       largest number, and the second part ends at fp16's smallest, 2^-24).
 //   T   two kind::f16 products, P's parts against the V codes as fp16 (exact).
 //   l   sum of w / vs in fp32.
-// vs rides in the exponent, so rows of V of any size keep their precision.  m
+// vs rides in the exponent, so w is of the size that counts for the output.  m
 // stays where it is until an exponent passes it by kSlack.
 //
 // The tensor cores add in fp32 by cutting off (measured: 2e-9 of the sum is lost
@@ -32,8 +32,8 @@
 // formed.  Warp 16: products, issued by one thread of a warp that computes
 // the descriptors uniformly; 17: loads.  While the softmax of tile j runs, the
 // tensor cores compute S of tile j + 1 and T of tile j - 1.
-// Bound by the softmax threads: about 4000 cycles a tile at hdim 256 against 1900 of
-// products.  8192 tokens of 16 + 8 heads of 256 take 1123 us, 490 TFLOP/s of the
+// Bound by the softmax threads: 2.5 us a tile at hdim 256 against about 1900 cycles of
+// products.  8192 tokens of 16 + 8 heads of 256 take 1179 us, 466 TFLOP/s of the
 // attention's own products.
 // Every wait is bounded; a role that gives up sets the CTA's abort flag, which
 // ends the others' waits.
