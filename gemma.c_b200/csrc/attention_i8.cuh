@@ -234,19 +234,8 @@ __device__ __forceinline__ void value_scale(float v, float &log2_vs, float &inv_
 // products whatever its scale, but with 1 it could set m and take the bits of rows of
 // small values. For m it counts as a row of scale 2^-32 (k_kt), or altogether (k_tc, where
 // 2^32 times its weight goes into the sum of weights): its part of that sum then stays a
-// normal number beside scales of up to 2^90. Only scales of exactly 1 are looked at; the
-// rows that are not zeros mostly end at the first load.
+// normal number beside scales of up to 2^90. Only scales of exactly 1 are looked at.
 constexpr float kZeros = 32.0f, kScaleZeros = 2.3283064e-10f;
-template <int HD>
-__device__ __forceinline__ bool row_of_zeros(const int8_t *codes) {
-  uint32_t any = 0;
-#pragma unroll 1
-  for (int i = 0; i < HD && !any; i += 16) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4 *>(codes + i));
-    any = w.x | w.y | w.z | w.w;
-  }
-  return !any;
-}
 
 // The roles of a CTA wait with a limit.  Every wait is on the phase after the last
 // one that its waiter knows complete (a parity cannot tell two phases apart): what

@@ -92,6 +92,20 @@ struct Cfg {
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[4]) { ptx::tmem_ld_32x4(at, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[8]) { ptx::tmem_ld_32x8(at, r); }
 
+// Whether a value row is all zeros, in its tile as TMA left it: 16-byte steps of the
+// row's SW bytes in the order that spreads neighbouring keys over the banks.
+template <typename C>
+__device__ __forceinline__ bool row_of_zeros(const uint8_t *row, int key) {
+  uint32_t any = 0;
+#pragma unroll 1
+  for (int i = 0; i < C::KB * C::SW / 16 && !any; ++i) {
+    const int b = i * 16 / C::SW, at = (i ^ (C::SW == 128 ? key : key >> 1)) % (C::SW / 16);
+    const uint4 w = *reinterpret_cast<const uint4 *>(row + b * C::T_BLOCK + at * 16);
+    any = w.x | w.y | w.z | w.w;
+  }
+  return !any;
+}
+
 struct alignas(64) KtArgs {
   CUtensorMap k[2], v[2];
   Args a[2];
@@ -105,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t kfull[ST], kempty[ST], vfull[ST], vempty[ST], sfull[2], sfree[2], pfull[2], pvdone[2], drain;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_fresh[2], s_lo[R], s_hi[R], s_row[R];
+  __shared__ int s_abort, s_gone, s_fresh[2], s_lo[R], s_hi[R], s_row[R];
   __shared__ long s_out[R];
   __shared__ float s_part[kKtCluster][R];  // a fused merge's factors
   __shared__ float s_rf[R], s_m[R], s_f[R], s_sum[R], s_red[16][R / 4];
@@ -148,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
     }
     ptx::mbar_init(&drain, 1);
     ptx::fence_mbar_init();
-    s_abort = 0;
+    s_abort = s_gone = 0;
   }
   ptx::griddep_wait();
 
@@ -416,17 +430,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
       float most = e[0];
 #pragma unroll
       for (int r = 1; r < RQ; ++r) most = fmaxf(most, e[r]);
-      bool fresh = j == 0;
-      if (ptx::named_bar_or(1, kSoftmax, !ok || most > kSlack)) {
+      bool fresh = j == 0, move = ptx::named_bar_or(1, kSoftmax, !ok || most > kSlack);
+      float less = 0.0f;
+      if (move) {
+        // What runs over from a row of zeros may: its W, the largest integer then,
+        // multiplies zeros.  (fvs * rvs is kOne for a scale of 1 alone; keeping vs itself up
+        // to here cost 0.9 us of 63.4.)
+        if (fvs * rvs == kOne && t0 + key < kend) {
+          ok = wait(&vfull[j % ST], (j / ST) & 1, DEV_TIMEOUT_FULL) && ok;
+          less = row_of_zeros<C>(smem + C::V_OFF + (j % ST) * C::T_BYTES + key * C::SW, key) ? kZeros : 0.0f;
+        }
+        move = ptx::named_bar_or(1, kSoftmax, !ok || most - less > kSlack);
+      }
+      if (move) {
         // some row's weights would run over: move every row's m to its largest
-        // exponent so far, and take O^T's sums at the old one.  What runs over from a row
-        // of zeros may: its W, the largest integer then, multiplies zeros.  (fvs * rvs is
-        // kOne for a scale of 1 alone; keeping vs itself up to here cost 0.9 us of 63.4.)
-        float less = 0.0f;
-        if (fvs * rvs == kOne && t0 + key < kend &&
-            row_of_zeros<HD>(a.kv.v + seq * a.kv.seq_stride + hk * a.kv.kv_stride + (long)(t0 + key) * HD))
-          less = kZeros;
-        if (ptx::named_bar_or(1, kSoftmax, !ok)) break;
+        // exponent so far, and take O^T's sums at the old one
+        if (!ok) s_gone = 1;
 #pragma unroll
         for (int r = 0; r < RQ; ++r) {
           float top = x[r] - less;
@@ -444,6 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kt(const __grid_constant__ KtAr
           s_m[threadIdx.x] = to;
         }
         ptx::named_bar_sync(1, kSoftmax);
+        if (s_gone) break;
         if (j > 0) {
           ok = wait(&pvdone[(j - 1) & 1], ((j - 1) >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
           if (!fresh) flush();

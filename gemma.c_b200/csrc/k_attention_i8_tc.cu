@@ -115,14 +115,29 @@ __device__ __forceinline__ uint2 to_half4(uint32_t w) {
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[8]) { ptx::tmem_ld_32x8(at, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t at, uint32_t (&r)[16]) { ptx::tmem_ld_32x16(at, r); }
 
-// thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK] of a tile whose value
-// codes are at `codes`, `keys` of them in the range
+// whether a value row is all zeros; kFly loads at a time once its first 16 codes are
 template <int HD>
-__device__ __forceinline__ void put_scale(float *sc, int i, float v, const int8_t *codes, int keys) {
+__device__ __forceinline__ bool row_of_zeros(const int8_t *codes) {
+  constexpr int N = HD / 16, kFly = 5;
+  const uint4 *p = reinterpret_cast<const uint4 *>(codes);
+  const uint4 f = __ldg(p);
+  uint32_t any = f.x | f.y | f.z | f.w;
+#pragma unroll 1
+  for (int i = 1; i < N && !any; i += kFly) {
+    uint4 w[kFly];
+#pragma unroll
+    for (int t = 0; t < kFly; ++t) w[t] = __ldg(p + min(i + t, N - 1));
+#pragma unroll
+    for (int t = 0; t < kFly; ++t) any |= w[t].x | w[t].y | w[t].z | w[t].w;
+  }
+  return !any;
+}
+
+// thread i < NK puts ks[i], i < 2 NK log2 and reciprocal of vs[i - NK]
+__device__ __forceinline__ void put_scale(float *sc, int i, float v) {
   if (i < NK) {
     sc[i] = v;
   } else if (i < 2 * NK) {
-    if (v == 1.0f && i - NK < keys && row_of_zeros<HD>(codes + (i - NK) * HD)) v = kScaleZeros;
     value_scale(v, sc[i], sc[i + NK]);
   }
 }
@@ -261,8 +276,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
     if ((int)threadIdx.x < 2 * NK) {
       const int t = threadIdx.x % NK;
       const float *src = (threadIdx.x < NK ? a.kv.ks : a.kv.vs) + hk * a.kv.sc_stride;
-      put_scale<HD>(reinterpret_cast<float *>(smem + C::SC_OFF), threadIdx.x, t < n ? __ldg(src + kbeg + t) : 1.0f,
-                    vh + (long)kbeg * HD, n);
+      float v = t < n ? __ldg(src + kbeg + t) : 1.0f;
+      if (v == 1.0f && threadIdx.x >= NK && t < n && row_of_zeros<HD>(vh + (long)(kbeg + t) * HD)) v = kScaleZeros;
+      put_scale(reinterpret_cast<float *>(smem + C::SC_OFF), threadIdx.x, v);
     }
   }
   ptx::fence_proxy_async_smem();
@@ -398,6 +414,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       return tid < 2 * NK && t < n ? __ldg((tid < NK ? a.kv.ks : a.kv.vs) + hk * a.kv.sc_stride + kbeg + t) : 1.0f;
     };
     float next = fetch_scale(grp + 1);
+    // a scale of tile j that is 1: the row may be zeros.  Looked at after a tile's work, while
+    // the other group is at its own.
+    auto look = [&](int j) {
+      const int t = j * NK + (tid & (NK - 1));
+      if (next == 1.0f && tid >= NK && tid < 2 * NK && t < n && row_of_zeros<HD>(vh + (long)(kbeg + t) * HD))
+        next = kScaleZeros;
+    };
+    look(grp + 1);
     float m = -INFINITY, l = 0.0f;
     float acc[C::OC];  // the row's sums, output columns [quarter * OC, +OC)
 #pragma unroll
@@ -461,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       if (j > 0) follow(j - 1);
       // while the scores are formed: the scales of the other group's next tile, which it
       // reads after this tile's decision, and the values
-      put_scale<HD>(sc + ((j + 1) & 3) * 3 * NK, tid, next, vh + (long)(kbeg + (j + 1) * NK) * HD, n - (j + 1) * NK);
+      put_scale(sc + ((j + 1) & 3) * 3 * NK, tid, next);
       next = fetch_scale(j + 3);
       if (HD == 256) convert(j);
       ok = wait(&bars.sfull[j & 1], (j >> 1) & 1, DEV_TIMEOUT_TMEM) && ok;
@@ -572,6 +596,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_tc(const __grid_constant__ TcAr
       ptx::tmem_st_wait();
       ptx::tc_fence_before();
       ptx::mbar_arrive_warp(&bars.pfull);
+      look(j + 3);
     }
     // the group without the last tile follows its decision too (j is the tile
     // after it); then both take what is left in T
