@@ -695,7 +695,7 @@ def _work(nbytes, device, stream):
     could still be in use there, by a call that has returned."""
     if not nbytes:
         return None, 0, None
-    if stream is None:
+    if stream is None or stream.cuda_stream == _on(None, device.index):
         w = torch.empty(nbytes, dtype=torch.uint8, device=device)
     else:
         with torch.cuda.stream(stream):

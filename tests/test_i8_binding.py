@@ -1,5 +1,7 @@
 """What the Python calls of the 8-bit cache and of sampling hand to the library, without a GPU:
 the tensors are on the CPU, the library is a record of its calls."""
+import types
+
 import pytest
 
 import gcu
@@ -126,8 +128,9 @@ def test_scratch_belongs_to_the_stream_that_uses_it(library, monkeypatch):
     library.work = 1 << 12
     kv = gcu.KvCacheI8.empty(1, 1, 16, 64, device="cpu")
     x, xo, rows, xq = torch.zeros((1, 2, 64)), torch.zeros((1, 2, 64)), torch.zeros((3, 128)), torch.zeros((2, 3, 64))
-    side = object()
+    side = types.SimpleNamespace(cuda_stream=7)
     streams = Streams(monkeypatch)
+    monkeypatch.setattr(gcu, "_on", lambda stream, dev: (stream or streams.current or types.SimpleNamespace(cuda_stream=0)).cuda_stream)
     for stream in (None, side):
         gcu.dev_attention_decode_i8(xo, x, kv, None, 8, 1.0, stream=stream)
         gcu.dev_attention_prefill_i8(rows, xq, kv, 0, stream=stream)
