@@ -7,15 +7,14 @@
 //   o     = sum_t p[t] * vs[t] * vc[t] / sum_t p[t]
 //
 // The codes stay integers up to the matrix products: a query row is scaled to
-// 23-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
+// 24-bit integers (q ~ sq * (65536 d2 + 256 d1 + d0), d signed bytes), so its
 // products with int8 keys are int8 x int8 sums, exact in int32.  That is fixed point: every
-// element is rounded by up to 2^-23 of the row's largest, twice what fp32 rounds that
-// one by, and one 2^-10 of its size keeps 13 bits where fp32 keeps 24.  A score moves
-// by up to 2^-23 max|q| * asc * ks * sum |kc|.  The keys' own codes are rounded by 2^-8 of
-// their row's largest, far more than that.  A fourth digit would cost a third more
-// product and 64 TMEM columns, which k_tc has not left at hdim 256 (192 of scores, 256 of
-// sums, 64 of weights); three also cost three instructions an element, as the integer
-// comes out of a floating point addition.
+// element is rounded by up to 2^-24 of the row's largest, as fp32 rounds that one, and
+// one 2^-10 of its size keeps 14 bits where fp32 keeps 24.  A score moves by up to
+// 2^-24 max|q| * asc * ks * sum |kc|.  The keys' own codes are rounded by 2^-8 of their
+// row's largest, far more than that.  A fourth digit would cost a third more product and
+// 64 TMEM columns, which k_tc has not left at hdim 256 (192 of scores, 256 of sums, 64
+// of weights).
 //
 // Rows: the query heads of one kv head share its keys, so a row is (i, g):
 // token or sequence i, head h0 + g of the group, row index i * G + g.
@@ -27,7 +26,7 @@ namespace gcu {
 namespace attn8 {
 
 constexpr int kMaxGroup = 8;        // query heads per kv head
-constexpr float kQMax = 4194000.0f;  // below 2^22: q * inv + 1.5 * 2^23 holds it as an integer
+constexpr float kQMax = 8355000.0f;  // three signed bytes hold up to 127 * 65793 = 8355711
 constexpr float kQLeast = 1e-31f;    // rows of smaller elements are scaled as if by this: 1 / scale stays finite
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -174,11 +173,10 @@ __device__ __forceinline__ void row_digits(const float (&v)[N][E], uint32_t (&w)
 #pragma unroll
   for (int n = 0; n < N; ++n) {
     const float inv = kQMax / amax[n];
-    // n + 0x808080 has the digits, each plus 128, as its bytes
+    // n + 0x808080 (8421504) has the digits, each plus 128, as its bytes
     uint32_t u[(E + 3) / 4 * 4] = {};
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      u[e] = __float_as_uint(__fmaf_rn(v[n][e], inv, 12582912.0f)) - 0x4B400000u + 0x808080u;
+    for (int e = 0; e < E; ++e) u[e] = __float2uint_rn(__fmaf_rn(v[n][e], inv, 8421504.0f));
 #pragma unroll
     for (int i = 0; i < (E + 3) / 4; ++i) {
       const uint32_t *x = u + 4 * i;
@@ -204,7 +202,7 @@ __device__ __forceinline__ void put_digits(uint8_t *dst, const uint32_t (&w)[(E 
 // mantissa of 1.5 * 2^23 by an integer addition (a conversion instruction runs
 // at a fraction of the rate); the offsets leave with the next step.  256 s1 + s0
 // is rounded at 2^31.6 at most, to 2^8, where the largest possible product of one
-// query and key element alone is 127 * 2^22 = 2^29.
+// query and key element alone is 127 * 2^23 = 2^30.
 __device__ __forceinline__ float2 magic2(const uint32_t *s) {
   return make_float2(__uint_as_float(s[0] + 0x4B400000u), __uint_as_float(s[1] + 0x4B400000u));
 }

@@ -409,8 +409,8 @@ int gcu_dev_cache_i8_read(float *k, float *v, long out_seq_stride, long out_stri
  * zeros; one with len[b] < 0 is skipped, its xo row left as it is; one with
  * len[b] > max_len is skipped too and reported by gcu_check_device.  At most 8
  * query heads per kv head.
- * Precision.  Queries are held in fixed point, each element to 2^-23 of its
- * row's largest (one 2^-10 of that size has 13 bits); rows of less than 1e-31 as
+ * Precision.  Queries are held in fixed point, each element to 2^-24 of its
+ * row's largest (one 2^-10 of that size has 14 bits); rows of less than 1e-31 as
  * if that were their largest.  A value scale counts as at least 2^-64 and at most
  * 2^100, that of a row of zeros (1, as it is written) as 2^-32.  Weights times
  * value scales are held in steps of at most 2^-25 of the row's largest such

@@ -6,8 +6,8 @@ For one query row with weights p_t = exp(s_t) and values v_t = vs_t * vc_t, o = 
 
   A relative error d_t of the weights moves o by sum p_t (v_t - o) d_t / sum p, at most 2 d A with
   A = sum p |v| / sum p.  d has these parts:
-    - the query's elements are whole multiples of its largest one's 2^-22 (4194000 steps), each off
-      by half a step at most, evenly spread: a score moves by asc * ks * qmax * 2^-23 / sqrt(3)
+    - the query's elements are whole multiples of its largest one's 2^-23 (8355000 steps), each off
+      by half a step at most, evenly spread: a score moves by asc * ks * qmax * 2^-24 / sqrt(3)
       * |kc| (its standard deviation), taken six times; qmax counts as 1e-31 at least;
     - 8 half steps of fp32 of the score's own size (digits, scales, log2 e, the shift by the
       maximum), and of the cap's tanh, 2^-22 of the capped score;
@@ -28,7 +28,7 @@ def attend(q, kc, ks, vc, vs, asc, cap=0.0, unit=0.0, cut=False):
     q, kc, ks, vc, vs = (np.asarray(a, np.float64) for a in (q, kc, ks, vc, vs))
     n = len(ks)
     s = asc * ks * (kc @ q)
-    move = 6 * asc * np.max(ks * np.sqrt((kc * kc).sum(1))) * max(np.max(np.abs(q)), 1e-31) * 2.0 ** -23 / math.sqrt(3)
+    move = 6 * asc * np.max(ks * np.sqrt((kc * kc).sum(1))) * max(np.max(np.abs(q)), 1e-31) * 2.0 ** -24 / math.sqrt(3)
     d = move + 2.0 ** -24 * 8 * np.max(np.abs(s))
     if cap:
         s = np.tanh(s / cap) * cap

@@ -238,3 +238,26 @@ def test_outlier_query_channels(kernel, outlier):
             want, tol = B.attend(xq[h, i], k[0, 0, :m], ks[0, 0, :m], v[0, 0, :m], vs[0, 0, :m], 1.0,
                                  unit=UNIT[kernel], cut=kernel == "many rows")
             B.check(got[i, h], want, tol)
+
+
+@pytest.mark.parametrize("kernel", UNIT)
+def test_queries_keep_24_bits(kernel):
+    """Elements of three steps of the largest one's 2^-23, over keys that are zero where that one is:
+    the scores are theirs alone, and nothing of them is rounded."""
+    rng = np.random.default_rng(91)
+    n, ntok, hd = 500, 20, 128
+    k, _ = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32))
+    k[..., 0] = 0
+    ks = rng.uniform(600, 1200, (1, 1, n)).astype(np.float32)
+    v, vs = R.quantize_rows(rng.standard_normal((1, 1, n, hd), dtype=np.float32))
+    small = (rng.choice([-3, -1, 1, 3], (2, ntok, hd)) / 8355000).astype(np.float32)
+    xq = small.copy()
+    xq[..., 0] = 1
+    small[..., 0] = 0
+    got = forced(kernel, xq, handle((k, v, ks, vs)), n - ntok).reshape(ntok, 2, hd)
+    for i in range(ntok):
+        m = n - ntok + i + 1
+        for h in range(2):
+            want, tol = B.attend(small[h, i], k[0, 0, :m], ks[0, 0, :m], v[0, 0, :m], vs[0, 0, :m], 1.0,
+                                 unit=UNIT[kernel], cut=kernel == "many rows")
+            B.check(got[i, h], want, tol)
