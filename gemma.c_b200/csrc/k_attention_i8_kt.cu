@@ -26,7 +26,7 @@
 // costs 5.4 us besides its tiles and, with 16 rows, 1.0 us a tile whose codes are in L2;
 // from HBM 148 CTAs of 32 tiles take 50 us for 310 MB.  32768 keys of 8 heads: 29.6 us for
 // 136 MB, the merge of 18 chunks 3.6 of them.  32 rows are bound by the softmax, 1.5 us a
-// tile: 32 sequences that share 32768 keys 64 us, 52 without keys of their own.
+// tile: 32 sequences that share 32768 keys 63 us, 52 without keys of their own.
 //
 // Warps 0-15: softmax, thread = (key, a quarter of the rows); 16: products; 17: loads.
 #include "attention_i8.cuh"

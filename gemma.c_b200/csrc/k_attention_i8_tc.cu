@@ -33,7 +33,7 @@
 // the descriptors uniformly; 17: loads.  While the softmax of tile j runs, the
 // tensor cores compute S of tile j + 1 and T of tile j - 1.
 // Bound by the softmax threads: 2.5 us a tile at hdim 256 against about 1900 cycles of
-// products.  8192 tokens of 16 + 8 heads of 256 take 1179 us, 466 TFLOP/s of the
+// products.  8192 tokens of 16 + 8 heads of 256 take 1180 us, 466 TFLOP/s of the
 // attention's own products.
 // Every wait is bounded; a role that gives up sets the CTA's abort flag, which
 // ends the others' waits.
