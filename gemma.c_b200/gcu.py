@@ -856,7 +856,7 @@ def dev_attention_prefill_i8(xo, xq, kv, spos, slide=0, sc_att=0.0, mask=True, s
 
 
 def dev_sample(token, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, prob=None, stream=None):
-    """The next token of each row of logits (m, nvocab): token int32 (m,), from u (m,)
+    """The next token of each row of logits (m, nvocab; rows nvocab or more apart): token int32 (m,), from u (m,)
     float32 random numbers in [0, 1); prob (m,) float32 (optional) receives the
     tokens' shares of the kept weights.  See gcu_dev_sample in include/gcu.h."""
     what = "dev_sample"
